@@ -50,6 +50,10 @@ SIGNATURES = {
     "gdn_metadata_copy": [P, P, PI64, PI64, PI64, P, I32, P],
     "gdn_metadata_pad": [P, P, PI64, PI64, PI64, PI64, P, I32, P],
     "gdn_rms_norm_gated": [P, I32, I64, I64, P, I32, I64, I64, I64, I64, P, I32, F32, P, P],
+    "gdn_rms_norm": [P, I32, I64, I64, I64, P, I64, P, I32, F32, F32, P, I64, P, I64, P, I64, P, I64, I64, P],
+    "gdn_quantize_fp8": [P, I32, I64, I64, I64, P, I64, P, I64, I64, P],
+    "gdn_rms_norm_gated_fp8": [P, I32, I64, I64, I64, I64, I64, P, I64, I64, P, I32, F32, P, I64, P, I64, I64, P],
+    "gdn_fp8_linear": [P, I64, P, I64, I64, P, I64, P, I64, I64, I64, I64, I64, P, I32, I64, P],
     "gdn_conv_snapshots": [P, I64, I32, P, I32, I64, I64, I64, I32, P, I64, I64, I64, P, I32, P, I32, P, I32, I64,
                            P],
     "gdn_chunk_gated_delta_rule": [P, P, P, I32, P, P, P, I32, I64, I64, I64, I64, I64, I64, P, I32, I64, I64, I64,
@@ -156,6 +160,17 @@ def call(name: str, *args) -> None:
         if rc == 2:
             raise NotImplementedError(f"{name}: {msg}")
         raise RuntimeError(f"{name} failed ({rc}): {msg}")
+
+
+def call_on(t: torch.Tensor, name: str, *args) -> None:
+    """``call`` with the current stream of ``t``'s device as the last argument,
+    on that device."""
+    stream = stream_of(t)
+    if t.get_device() == torch.cuda.current_device():
+        call(name, *args, stream)
+    else:
+        with torch.cuda.device(t.device):
+            call(name, *args, stream)
 
 
 def workspace(name: str, device, *sizes) -> tuple[torch.Tensor | None, int]:

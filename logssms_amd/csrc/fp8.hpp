@@ -1,0 +1,117 @@
+// Block-scaled 8-bit values (OCP e4m3) shared by the row kernels that write
+// them and the product that reads them: a block of 128 consecutive values of a
+// row carries one fp32 scale s = max|y| / 448, and q = e4m3(y / s).
+#pragma once
+
+#include "common.hpp"
+
+namespace gdn {
+
+constexpr int kFp8Block = 128;
+constexpr float kFp8Top = 448.0f;               // the largest e4m3 value
+constexpr float kFp8LeastScale = 0x1p-126f;     // a block of zeros; its reciprocal is finite
+
+// Largest magnitude over the aligned 16 lanes that hold one block, as the bits
+// of |y|: ordered as integers NaN > infinity > every finite value, so a block
+// with a NaN gets a NaN scale and never one of its finite values'.
+__device__ __forceinline__ uint32_t block_amax(uint32_t m) {
+  auto dpp = [](uint32_t x, auto ctrl) __attribute__((always_inline)) {
+    return static_cast<uint32_t>(__builtin_amdgcn_update_dpp(0, static_cast<int>(x), decltype(ctrl)::value, 0xf, 0xf,
+                                                             false));
+  };
+  m = max(m, dpp(m, std::integral_constant<int, 0xB1>{}));   // quad_perm [1,0,3,2]
+  m = max(m, dpp(m, std::integral_constant<int, 0x4E>{}));   // quad_perm [2,3,0,1]
+  m = max(m, dpp(m, std::integral_constant<int, 0x141>{}));  // row_half_mirror
+  m = max(m, dpp(m, std::integral_constant<int, 0x128>{}));  // row_ror:8
+  return m;
+}
+__device__ __forceinline__ uint32_t abs_bits(float y) { return __float_as_uint(y) & 0x7fffffffu; }
+
+// The scale of a block from its amax bits.  An infinity gives an infinite
+// scale (q = NaN for it and 0 for its neighbours, all of which read back as
+// NaN); fmaxf would turn a NaN into the least scale, hence the comparison.
+__device__ __forceinline__ float block_scale(uint32_t amax_bits) {
+  const float s = __uint_as_float(amax_bits) / kFp8Top;
+  return s < kFp8LeastScale ? kFp8LeastScale : s;
+}
+
+// Eight values times 1 / s as e4m3 (round to nearest even; |y| / s <= 448 but
+// for the rounding of 1 / s, which cannot reach the next code's border).
+__device__ __forceinline__ uint2 pack8_fp8(const float (&y)[8], float inv) {
+  int lo = 0, hi = 0;
+  lo = __builtin_amdgcn_cvt_pk_fp8_f32(y[0] * inv, y[1] * inv, lo, false);
+  lo = __builtin_amdgcn_cvt_pk_fp8_f32(y[2] * inv, y[3] * inv, lo, true);
+  hi = __builtin_amdgcn_cvt_pk_fp8_f32(y[4] * inv, y[5] * inv, hi, false);
+  hi = __builtin_amdgcn_cvt_pk_fp8_f32(y[6] * inv, y[7] * inv, hi, true);
+  return make_uint2(static_cast<uint32_t>(lo), static_cast<uint32_t>(hi));
+}
+
+// Destination of quantised rows: values [rows, cols] at a row stride that is a
+// multiple of 16 bytes (the bytes from cols up to the next multiple of 16 are
+// written as zeros), scales [rows, ceil(cols / 128)] at any strides.
+struct Fp8Rows {
+  uint8_t* values;
+  int64_t row_stride;
+  float* scales;
+  int64_t scale_row_stride, scale_block_stride;
+};
+
+// Quantise the 8 values y of row r, columns 8 vec .. 8 vec + 7 (zeros from
+// cols on), held by lane vec % 16 of the aligned 16-lane group of its block.
+__device__ __forceinline__ void store_fp8(const Fp8Rows& q, int64_t r, int64_t vec, int64_t cols,
+                                          const float (&y)[8]) {
+  uint32_t m = 0;
+#pragma unroll
+  for (int e = 0; e < 8; ++e) m = max(m, abs_bits(y[e]));
+  m = block_amax(m);
+  const float s = block_scale(m);
+  const int64_t padded = (cols + 15) & ~int64_t{15};
+  if (8 * vec < padded) *reinterpret_cast<uint2*>(q.values + r * q.row_stride + 8 * vec) = pack8_fp8(y, 1.0f / s);
+  if ((vec & 15) == 0 && 8 * vec < cols)
+    q.scales[r * q.scale_row_stride + (vec >> 4) * q.scale_block_stride] = s;
+}
+
+// Eight elements of a row from column c on as floats; zeros from cols on.
+// VEC: cols is a multiple of 8 and the address of 16 bytes.
+template <class T, bool VEC>
+__device__ __forceinline__ void load8(const T* row, int64_t c, int64_t cols, float (&x)[8]) {
+  if constexpr (VEC) {
+    if (c < cols) {
+      if constexpr (std::is_same_v<T, float>) {
+        const float4 a = *reinterpret_cast<const float4*>(row + c), b = *reinterpret_cast<const float4*>(row + c + 4);
+        x[0] = a.x, x[1] = a.y, x[2] = a.z, x[3] = a.w, x[4] = b.x, x[5] = b.y, x[6] = b.z, x[7] = b.w;
+      } else {
+        unpack8<T>(*reinterpret_cast<const uint4*>(row + c), x);
+      }
+    } else {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) x[e] = 0.f;
+    }
+  } else {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) x[e] = c + e < cols ? to_f32(row[c + e]) : 0.f;
+  }
+}
+template <class T, bool VEC>
+__device__ __forceinline__ void store8(T* row, int64_t c, int64_t cols, const float (&y)[8]) {
+  if constexpr (VEC) {
+    if (c >= cols) return;
+    if constexpr (std::is_same_v<T, float>) {
+      *reinterpret_cast<float4*>(row + c) = make_float4(y[0], y[1], y[2], y[3]);
+      *reinterpret_cast<float4*>(row + c + 4) = make_float4(y[4], y[5], y[6], y[7]);
+    } else {
+      *reinterpret_cast<uint4*>(row + c) = pack8_io<T>(y);
+    }
+  } else {
+#pragma unroll
+    for (int e = 0; e < 8; ++e)
+      if (c + e < cols) row[c + e] = from_f32<T>(y[e]);
+  }
+}
+
+// Whether load8 / store8 may take their 16-byte form on rows at this stride.
+inline bool rows_vec(const void* p, int64_t row_stride, int64_t rows) {
+  return aligned16(p) && (rows == 1 || row_stride % 8 == 0);
+}
+
+}  // namespace gdn

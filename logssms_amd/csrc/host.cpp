@@ -42,7 +42,11 @@ namespace {
   X(gdn_fused_recurrent)                  \
   X(gdn_fused_conv_recurrent)             \
   X(gdn_logstate_restore)                 \
-  X(gdn_rms_norm_gated)
+  X(gdn_rms_norm_gated)                   \
+  X(gdn_rms_norm)                         \
+  X(gdn_quantize_fp8)                     \
+  X(gdn_rms_norm_gated_fp8)               \
+  X(gdn_fp8_linear)
 namespace lib {
 #define GDN_POINTER(name) decltype(&::name) name = nullptr;
 GDN_TYPED(GDN_POINTER)

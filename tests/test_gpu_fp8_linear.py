@@ -1,0 +1,207 @@
+"""The block-scaled 8-bit product (``gdn_fp8_linear``, ``csrc/fp8_linear.hip``)
+against ``oracle/fp8.py`` in float64 on the same quantised operands.  The bound
+is the oracle's (``linear_bound``: what the 8-bit matrix instructions and fp32
+sums may lose) plus half a step of the output's type."""
+
+import pytest
+import torch
+
+from oracle import fp8 as ref
+from tests.gpu_util import DEV, gen, randn
+
+pytestmark = pytest.mark.gpu
+
+FP8 = torch.float8_e4m3fn
+HALF = {torch.bfloat16: 2.0 ** -8, torch.float16: 2.0 ** -11}
+FLOOR = {torch.bfloat16: 2.0 ** -134, torch.float16: 2.0 ** -25}
+
+#         M, N, K
+SHAPES = [(1, 1, 1), (1, 16, 128), (2, 17, 130), (1, 2048, 4096), (16, 48, 256), (17, 100, 1000), (33, 128, 16),
+          (64, 333, 272), (31, 200, 2048), (65, 129, 131), (129, 257, 384), (300, 1111, 1000), (256, 256, 128),
+          (100, 64, 5000), (513, 130, 640), (200, 1, 33)]
+ids = [f"{m}x{n}x{k}" for m, n, k in SHAPES]
+
+
+def operands(m, n, k, g, wild=0.0):
+    """Quantised operands whose blocks differ in size, with garbage (NaN codes)
+    in the bytes behind each row's end."""
+    wide = (k + 15) // 16 * 16
+
+    def rows(count, scale_rows):
+        v = randn(count, k, g=g, std=60.0) * torch.exp(wild * randn(count, k, g=g))
+        codes = torch.full((count, wide), 0x7F, dtype=torch.uint8)
+        codes[:, :k] = v.clamp(-448, 448).to(FP8).view(torch.uint8)
+        scales = 0.01 * torch.exp(randn(scale_rows, -(-k // 128), g=g))
+        return codes.view(FP8)[:, :k], scales
+
+    return rows(m, m), rows(n, -(-n // 128))
+
+
+def to_dev(pair):
+    from logssms_amd.kernel import Fp8Tensor
+    values, scales = pair
+    count, k = values.shape
+    wide = values.as_strided((count, values.stride(0)), (values.stride(0), 1))
+    return Fp8Tensor(wide.to(DEV)[:, :k], scales.to(DEV))
+
+
+def check(got, x, w, dtype, rows=None, cols=None):
+    """got against the oracle on some rows and columns (all by default)."""
+    rows = torch.arange(x[0].shape[0]) if rows is None else rows
+    cols = torch.arange(w[0].shape[0]) if cols is None else cols
+    k = x[0].shape[1]
+    a = ref.dequantize(x[0], x[1])[rows].to(DEV)
+    b = ref.dequantize(w[0], w[1])[cols].to(DEV)
+    one = torch.ones(1, -(-k // 128), dtype=torch.float64, device=DEV)
+    want = a @ b.t()
+    loss = ref.linear_bound(a, one.expand(len(rows), -1), b, one.expand(len(cols), -1))
+    assert got.dtype == dtype
+    err = (got[rows.to(DEV)][:, cols.to(DEV)].double() - want).abs()
+    bound = loss + (want.abs() + loss) * HALF[dtype] + FLOOR[dtype]
+    assert (err <= bound).all(), f"{float((err / bound).max())} times the bound"
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16], ids=str)
+@pytest.mark.parametrize("shape", SHAPES, ids=ids)
+def test_product_matches_oracle(shape, dtype):
+    from logssms_amd.kernel import Fp8Tensor, fp8_linear
+    m, n, k = shape
+    print(f"fp8_linear {shape} {dtype}", flush=True)
+    for wild in (0.0, 1.5):
+        x, w = operands(m, n, k, gen(m + n + k), wild)
+        dx, dw = to_dev(x), to_dev(w)
+        got = fp8_linear(dx, dw, dtype)
+        assert got.shape == (m, n)
+        check(got, x, w, dtype)
+        # the scales of the tokens block by block, as the quantisers lay them out
+        again = fp8_linear(Fp8Tensor(dx.values, dx.scales.t().contiguous().t()), dw, dtype)
+        assert torch.equal(again, got)
+
+
+@pytest.mark.parametrize("shape", [(4096, 4097, 160), (5000, 4000, 1040), (700, 6000, 2050), (16, 12288, 2048)],
+                         ids=str)
+def test_large_products_on_sampled_rows(shape):
+    from logssms_amd.kernel import fp8_linear
+    m, n, k = shape
+    print(f"fp8_linear large {shape}", flush=True)
+    g = gen(m)
+    x, w = operands(m, n, k, g, 0.5)
+    got = fp8_linear(to_dev(x), to_dev(w))
+    rows = torch.unique(torch.cat([torch.arange(min(m, 40)), torch.randint(0, m, (160,), generator=g),
+                                   torch.arange(max(0, m - 40), m)]))
+    cols = torch.unique(torch.cat([torch.arange(40), torch.randint(0, n, (160,), generator=g), torch.arange(n - 40, n)]))
+    check(got, x, w, torch.bfloat16, rows, cols)
+    # every element, against the fp32 product of the dequantised operands
+    want = (ref.dequantize(*x).to(DEV) @ ref.dequantize(*w).to(DEV).t()).float()
+    rms = want.square().mean().sqrt()
+    assert ((got.float() - want).abs() <= 2.0 ** -7 * (want.abs() + rms)).all()
+
+
+@pytest.mark.parametrize("m", [1, 40, 300])
+def test_strides_and_untouched_surroundings(m):
+    """Operands and output inside larger buffers; what lies around the output stays."""
+    from logssms_amd.kernel import Fp8Tensor, fp8_linear
+    n, k = 200, 272
+    print(f"fp8_linear strides m={m}", flush=True)
+    g = gen(m)
+    x, w = operands(m, n, k, g)
+    dx, dw = to_dev(x), to_dev(w)
+    plain = fp8_linear(dx, dw)
+    wide = torch.full((m + 2, 512), 0x7F, dtype=torch.uint8, device=DEV).view(FP8)
+    wide.view(torch.uint8)[1:m + 1, 64:64 + k] = dx.values.view(torch.uint8)
+    scales = torch.full((m + 2, 8), float("nan"), device=DEV)
+    scales[1:m + 1, 1:7:2] = dx.scales
+    weight = torch.full((n + 2, 304), 0x7F, dtype=torch.uint8, device=DEV).view(FP8)
+    weight.view(torch.uint8)[2:, 16:16 + k] = dw.values.view(torch.uint8)
+    for pad in (3, 8):  # rows of the output at odd addresses and at multiples of 16 bytes
+        out = torch.full((m + 2, n + 2 * pad), 7.0, dtype=torch.bfloat16, device=DEV)
+        view = out[1:m + 1, pad:pad + n]
+        got = fp8_linear(Fp8Tensor(wide[1:m + 1, 64:64 + k], scales[1:m + 1, 1:7:2]),
+                         Fp8Tensor(weight[2:, 16:16 + k], dw.scales.t().contiguous().t()), out=view)
+        assert got is view and torch.equal(view, plain)
+        view.fill_(7.0)
+        assert (out == 7.0).all()
+
+
+@pytest.mark.parametrize("m", [3, 50, 200])
+def test_what_is_not_finite_stays_in_its_row_or_column(m):
+    from logssms_amd.kernel import fp8_linear
+    n, k = 150, 300
+    print(f"fp8_linear nan m={m}", flush=True)
+    x, w = operands(m, n, k, gen(m))
+    x[0].view(torch.uint8)[1, 299] = 0x7F
+    x[1][2, 0] = float("inf")
+    w[0].view(torch.uint8)[149, 0] = 0xFF
+    got = fp8_linear(to_dev(x), to_dev(w)).cpu()
+    assert got[1].isnan().all() and not got[2, :149].isfinite().any() and got[:, 149].isnan().all()
+    rest = torch.ones(m, n, dtype=torch.bool)
+    rest[1], rest[2], rest[:, 149] = False, False, False
+    assert got[rest].isfinite().all()
+
+
+@pytest.mark.parametrize("m", [5, 90, 600])
+def test_same_bits_every_time_and_for_every_batch(m):
+    """A row's result does not depend on the call, on other work, or (within a
+    form of the kernel) on the rows beside it."""
+    from logssms_amd.kernel import Fp8Tensor, fp8_linear
+    x, w = operands(m, 700, 1000, gen(m))
+    dx, dw = to_dev(x), to_dev(w)
+    first = fp8_linear(dx, dw)
+    for _ in range(3):
+        assert torch.equal(fp8_linear(dx, dw), first)
+    perm = torch.randperm(m, generator=gen(1)).to(DEV)
+    shuffled = Fp8Tensor(to_dev((x[0].as_strided((m, 1008), (1008, 1)), x[1])).values.view(torch.uint8)[perm].view(FP8)[:, :1000],
+                         dx.scales[perm])
+    assert torch.equal(fp8_linear(shuffled, dw), first[perm])
+
+
+@pytest.mark.parametrize("m", [1, 48, 300])
+def test_norms_and_products_in_one_graph(m):
+    """The run of a layer: residual norm in 8 bits, product, gated norm in 8
+    bits, product; captured and replayed on new inputs beside eager work."""
+    from logssms_amd.kernel import add_rms_norm_fp8, fp8_linear, quantize_fp8_weight, rms_norm_gated_fp8
+    g = gen(m)
+    hidden, heads = 256, 4
+    x, res = (randn(m, hidden, g=g, dtype=torch.bfloat16).to(DEV) for _ in range(2))
+    weight = (1 + 0.1 * randn(hidden, g=g)).to(DEV)
+    head_weight = (1 + 0.1 * randn(128, g=g)).to(DEV)
+    w_in = quantize_fp8_weight(randn(2 * heads * 128, hidden, g=g, std=0.06).to(DEV))
+    w_out = quantize_fp8_weight(randn(hidden, heads * 128, g=g, std=0.04).to(DEV))
+
+    def layer():
+        q, total = add_rms_norm_fp8(x, res, weight, 1e-6)
+        core, z = fp8_linear(q, w_in).view(m, 2 * heads, 128).split(heads, 1)
+        p = rms_norm_gated_fp8(core, z, head_weight, 1e-6)
+        return q, core, z, p, fp8_linear(p, w_out), total
+
+    def expected(q, core, z, p):
+        _, y = ref.rms_norm(x.cpu(), weight.cpu(), 1e-6, residual=res.cpu())
+        first = ref.linear(q.values.cpu(), q.scales.cpu(), w_in.values.cpu(), w_in.scales.cpu())
+        gated = ref.rms_norm_gated(core.cpu(), z.cpu(), head_weight.cpu(), 1e-6)
+        last = ref.linear(p.values.cpu(), p.scales.cpu(), w_out.values.cpu(), w_out.scales.cpu())
+        return y, first, gated, last
+
+    stream = torch.cuda.Stream()
+    stream.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(stream):
+        layer()
+    torch.cuda.current_stream().wait_stream(stream)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        graphed = layer()
+    for _ in range(3):
+        x.copy_(randn(m, hidden, g=g, dtype=torch.bfloat16).to(DEV))
+        q, core, z, p, out, total = layer()
+        torch.cuda.synchronize()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(graphed[4], out) and torch.equal(graphed[5], total)
+        y, first, gated, last = expected(q, core, z, p)
+        # each step against the oracle on the step's own inputs: a code's half step,
+        # and 2^-7 of the row's size for a product rounded to bf16
+        assert ((q.dequantize().double().cpu() - y).abs() <= 2.0 ** -4 * 1.01 * y.abs() + 2.0 ** -10 * 0.02).all()
+        both = torch.cat([core, z], 1).flatten(1).double().cpu()
+        for got, want in ((both, first), (out.double().cpu(), last)):
+            assert ((got - want).abs() <= 2.0 ** -8 * want.abs() + 2.0 ** -12 * want.square().mean().sqrt() * 8).all()
+        assert ((p.dequantize().double().cpu() - gated).abs()
+                <= 2.0 ** -4 * 1.01 * gated.abs() + 2.0 ** -10 * 0.02).all()
