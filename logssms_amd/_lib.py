@@ -162,17 +162,6 @@ def call(name: str, *args) -> None:
         raise RuntimeError(f"{name} failed ({rc}): {msg}")
 
 
-def call_on(t: torch.Tensor, name: str, *args) -> None:
-    """``call`` with the current stream of ``t``'s device as the last argument,
-    on that device."""
-    stream = stream_of(t)
-    if t.get_device() == torch.cuda.current_device():
-        call(name, *args, stream)
-    else:
-        with torch.cuda.device(t.device):
-            call(name, *args, stream)
-
-
 def workspace(name: str, device, *sizes) -> tuple[torch.Tensor | None, int]:
     """The workspace the ``name`` query asks for (scratch of the current
     stream's work), and its bytes: ``(None, 0)`` where none is used, and where

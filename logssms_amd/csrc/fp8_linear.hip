@@ -128,9 +128,11 @@ __global__ __launch_bounds__(64 * kFewWaves) void few_rows_kernel(Linear p) {
 // A block of WN x WM waves owns a tile of BN = 32 FN WN columns and BM = 32 FM
 // WM tokens at a time.  Both operands of a block of K go straight to LDS, one
 // step ahead of the products, rows of 128 bytes with the 16-byte chunk c of
-// row r at c ^ (r & 7): the fragment reads take the same chunk of eight
-// consecutive rows at a time, which this spreads over all banks.  The direct
-// loads land in lane order, so the lanes' source chunks are permuted instead.
+// row r at c ^ (r / 2 % 8): a fragment read takes the same chunk of 16
+// consecutive rows at a time, two rows of which fill the 64 banks, so this
+// spreads them over all of the banks (c ^ (r % 8) cost 4 conflict cycles on
+// each 4).  The direct loads land in lane order, so the lanes' source chunks
+// are permuted instead.
 template <int WN, int WM, int FN, int FM>
 struct Tile {
   static constexpr int kWaves = WN * WM, kThreads = 64 * kWaves;
@@ -150,7 +152,8 @@ __global__ __launch_bounds__(64 * WN * WM) void tile_kernel(Linear p) {
   const int wn = wave % WN, wm = wave / WN;
   const int blocks = (p.K + kFp8Block - 1) / kFp8Block;
   const int padded = (p.K + 15) & ~15;
-  const int chunk = (lane & 7) ^ (lane >> 3);  // of the 8 rows that a load covers, lane l brings row l / 8
+  // of the 8 rows that a load covers, lane l brings chunk l % 8 of row l / 8, in odd groups of 8 rows the one 4 across
+  const int chunk = (lane & 7) ^ (lane >> 4);
 
   // blocks with the same index modulo 8 share an XCD and its L2: each XCD takes
   // a contiguous range of the tiles, whose order runs over 8 token tiles first
@@ -159,40 +162,58 @@ __global__ __launch_bounds__(64 * WN * WM) void tile_kernel(Linear p) {
   const int first = static_cast<int>(static_cast<int64_t>(tiles) * xcd / 8) + (blockIdx.x >> 3);
   const int last = static_cast<int>(static_cast<int64_t>(tiles) * (xcd + 1) / 8);
   if (first >= last) return;  // whole block
-  auto place = [&](int t, int& m0, int& n0) {
+  // What a step's loads need of tile t: its corner, and where the loads of the
+  // next block of K start.
+  struct Cursor {
+    int t, b, m0, n0;
+    const uint8_t *x, *w;
+    const float* xs;
+  };
+  auto enter = [&](int t) {
     const int group = t / (8 * p.tiles_n), in = t - group * 8 * p.tiles_n;
     const int height = min(8, p.tiles_m - 8 * group);
-    m0 = (8 * group + in % height) * T::BM;
-    n0 = in / height * T::BN;
+    Cursor c;
+    c.t = t, c.b = 0;
+    c.m0 = (8 * group + in % height) * T::BM;
+    c.n0 = in / height * T::BN;
+    c.x = p.x + c.m0 * p.x_stride;
+    c.w = p.w + c.n0 * p.w_stride;
+    c.xs = p.xs + c.m0 * p.xs_row;
+    return c;
+  };
+  auto advance = [&](Cursor& c) {
+    if (c.b + 1 == blocks) {
+      if (c.t + per_xcd >= last) return false;
+      c = enter(c.t + per_xcd);
+    } else {
+      c.b += 1, c.x += kFp8Block, c.w += kFp8Block, c.xs += p.xs_block;
+    }
+    return true;
   };
 
-  auto fill = [&](int t, int b, int stage) {
-    int m0, n0;
-    place(t, m0, n0);
-    const int k = b * kFp8Block, width = min(kFp8Block, padded - k);
-    uint8_t* base = lds + stage * T::kStage;
-    const bool past = 16 * chunk >= width;
-    auto rows = [&](const uint8_t* src, int64_t stride, int64_t row0, int count, int group0, auto Jc, uint8_t* dst) {
+  auto fill = [&](const Cursor& c, uint8_t* base) {
+    const int width = min(kFp8Block, padded - c.b * kFp8Block);
+    auto rows = [&](const uint8_t* src, int64_t stride, int count, int group0, auto Jc, uint8_t* dst) {
       constexpr int J = decltype(Jc)::value;
       const uint32_t bytes = static_cast<uint32_t>((count - 1) * stride + width);
       const __amdgpu_buffer_rsrc_t rsrc =
-          __builtin_amdgcn_make_buffer_rsrc(const_cast<uint8_t*>(src + row0 * stride + k), 0, bytes, 0x00020000);
-      const uint32_t at = static_cast<uint32_t>((lane >> 3) * stride + 16 * chunk);
+          __builtin_amdgcn_make_buffer_rsrc(const_cast<uint8_t*>(src), 0, bytes, 0x00020000);
+      const uint32_t row = static_cast<uint32_t>((lane >> 3) * stride);
 #pragma unroll
       for (int j = 0; j < J; ++j) {
-        const uint32_t off = at + static_cast<uint32_t>((group0 + j) * 8 * stride);
+        const int from = 16 * (chunk ^ (4 * ((group0 + j) & 1)));
+        const uint32_t off = row + from + static_cast<uint32_t>((group0 + j) * 8 * stride);
         __builtin_amdgcn_raw_ptr_buffer_load_lds(rsrc, (lds_void*)(dst + (group0 + j) * 1024), 16,
-                                                 past ? 0xffffff00u : off, 0, 0, 0);
+                                                 from >= width ? 0xffffff00u : off, 0, 0, 0);
       }
     };
-    rows(p.w, p.w_stride, n0, min(T::BN, p.N - n0), wave * T::JN, std::integral_constant<int, T::JN>{}, base);
-    rows(p.x, p.x_stride, m0, min(T::BM, p.M - m0), wave * T::JM, std::integral_constant<int, T::JM>{},
+    rows(c.w, p.w_stride, min(T::BN, p.N - c.n0), wave * T::JN, std::integral_constant<int, T::JN>{}, base);
+    rows(c.x, p.x_stride, min(T::BM, p.M - c.m0), wave * T::JM, std::integral_constant<int, T::JM>{},
          base + T::BN * kFp8Block);
     if (wave * 64 < T::BM && (T::BM % 64 == 0 || wave * 64 + lane < T::BM)) {
-      const int count = min(T::BM, p.M - m0);
       const __amdgpu_buffer_rsrc_t rsrc = __builtin_amdgcn_make_buffer_rsrc(
-          const_cast<float*>(p.xs + m0 * p.xs_row + b * p.xs_block), 0,
-          static_cast<uint32_t>(((count - 1) * p.xs_row + 1) * 4), 0x00020000);
+          const_cast<float*>(c.xs), 0, static_cast<uint32_t>(((min(T::BM, p.M - c.m0) - 1) * p.xs_row + 1) * 4),
+          0x00020000);
       __builtin_amdgcn_raw_ptr_buffer_load_lds(rsrc, (lds_void*)(base + T::kRows * kFp8Block + wave * 256), 4,
                                                static_cast<uint32_t>((wave * 64 + lane) * p.xs_row * 4), 0, 0, 0);
     }
@@ -207,30 +228,29 @@ __global__ __launch_bounds__(64 * WN * WM) void tile_kernel(Linear p) {
 #pragma unroll
       for (int e = 0; e < 16; ++e) acc[i][j][e] = 0.f;
 
-  int t = first, b = 0, stage = 0;
-  fill(t, 0, 0);
+  int stage = 0;
+  Cursor ahead = enter(first);
+  fill(ahead, lds);
   while (true) {
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
     __syncthreads();  // the stage is filled, and nobody reads the other one any more
-    const bool ends = b + 1 == blocks;
-    const int next = ends ? t + per_xcd : t;
-    if (next < last) fill(next, ends ? 0 : b + 1, stage ^ 1);
+    const int b = ahead.b, m0 = ahead.m0, n0 = ahead.n0;
+    const bool ends = b + 1 == blocks, more = advance(ahead);
+    if (more) fill(ahead, lds + (stage ^ 1) * T::kStage);
     uint8_t* base = lds + stage * T::kStage;
     if (ends && (p.K & 15)) {  // bytes past K inside the last 16 of each row
       const int left = p.K & 15, at = (p.K & (kFp8Block - 1)) >> 4;
       for (int row = threadIdx.x; row < T::kRows; row += T::kThreads) {
-        i32x4* v = reinterpret_cast<i32x4*>(base + row * kFp8Block + 16 * (at ^ (row & 7)));
+        i32x4* v = reinterpret_cast<i32x4*>(base + row * kFp8Block + 16 * (at ^ (row >> 1 & 7)));
         *v = mask_tail(*v, left);
       }
       __syncthreads();
     }
-    int m0, n0;
-    place(t, m0, n0);
     auto frag = [&](int row, int half) {  // lanes (r, g): row r, bytes 64 half + 32 g .. + 31
       const uint8_t* at = base + (row + r) * kFp8Block;
       const int c = 4 * half + 2 * g;
-      return join(*reinterpret_cast<const i32x4*>(at + 16 * (c ^ (r & 7))),
-                  *reinterpret_cast<const i32x4*>(at + 16 * ((c + 1) ^ (r & 7))));
+      return join(*reinterpret_cast<const i32x4*>(at + 16 * (c ^ (r >> 1 & 7))),
+                  *reinterpret_cast<const i32x4*>(at + 16 * ((c + 1) ^ (r >> 1 & 7))));
     };
     i32x8 bx[FM][2];
     float s[FM];
@@ -295,9 +315,7 @@ __global__ __launch_bounds__(64 * WN * WM) void tile_kernel(Linear p) {
           for (int e = 0; e < 16; ++e) acc[i][j][e] = 0.f;
         }
     }
-    if (next >= last) break;
-    t = next;
-    b = ends ? 0 : b + 1;
+    if (!more) break;
     stage ^= 1;
   }
 }

@@ -3,7 +3,9 @@
 //     arguments in a loop over their C types (ctypes took 2.5 us for the 46
 //     arguments of a decode step);
 //   * conv_recurrent, the checks and the call of one decode or verify step
-//     with tensors in hand.
+//     with tensors in hand;
+//   * rms_norm, quantize_fp8, rms_norm_gated_fp8 and fp8_linear, the same for
+//     the 8-bit projections.
 // A decode step of one sequence is an 8 us kernel behind what the host does
 // to launch it: 15.8 us in Python and ctypes, 5.8 us through this module.
 #include <Python.h>
@@ -12,7 +14,9 @@
 #include <utility>
 
 #include <ATen/ATen.h>
+#include <c10/core/DeviceGuard.h>
 #include <c10/hip/HIPStream.h>
+#include <torch/csrc/Dtype.h>
 #include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/python_variable.h>
 
@@ -238,10 +242,251 @@ PyObject* conv_recurrent(PyObject*, PyObject* const* args, Py_ssize_t n) {
   END_HANDLE_TH_ERRORS
 }
 
+// ---------------------------------------------------------------- 8-bit projections
+constexpr int64_t kFp8Block = 128;
+int64_t blocks_of(int64_t n) { return (n + kFp8Block - 1) / kFp8Block; }
+int64_t padded16(int64_t n) { return (n + 15) / 16 * 16; }
+
+void require_device(const at::Tensor& t) {
+  if (t.is_cuda()) return;
+  PyErr_SetString(PyExc_RuntimeError, "libgdn_mi355x kernels need tensors on a ROCm device");
+  throw Failed();
+}
+
+// f(args..., the current stream of t's device) on that device.
+template <class R, class... P, class... A>
+void launch(const char* name, R (*f)(P...), const at::Tensor& t, A... args) {
+  if (!bound(f != nullptr)) throw Failed();
+  const c10::DeviceGuard guard(t.device());
+  const int rc =
+      unlocked(f, args..., static_cast<void*>(c10::hip::getCurrentHIPStream(t.device().index()).stream()));
+  if (rc == GDN_OK) return;
+  PyErr_Format(rc == GDN_ERR_UNSUPPORTED ? PyExc_NotImplementedError : PyExc_RuntimeError, "%s failed (%d): %s", name, rc,
+               lib::gdn_last_error());
+  throw Failed();
+}
+
+// t as [rows, cols] with unit column stride; a copy where it has no such view.
+at::Tensor rows_of(const at::Tensor& t) {
+  const int64_t cols = t.size(-1);
+  const at::Tensor r = t.dim() == 2 ? t : t.reshape({t.numel() / cols, cols});
+  return cols == 1 || r.stride(1) == 1 ? r : r.contiguous();
+}
+
+// Uninitialised quantised rows: values at a stride that is a multiple of 16
+// bytes, scales block by block (strides 1, rows), as the product reads them.
+struct Fp8Out {
+  at::Tensor values, scales;
+};
+Fp8Out fp8_out(int64_t rows, int64_t cols, const at::Tensor& like) {
+  const auto options = like.options();
+  Fp8Out out{at::empty({rows, padded16(cols)}, options.dtype(at::kFloat8_e4m3fn)),
+             at::empty_strided({rows, blocks_of(cols)}, {1, std::max<int64_t>(rows, 1)}, options.dtype(at::kFloat))};
+  if (out.values.size(1) != cols) out.values = out.values.narrow(1, 0, cols);
+  return out;
+}
+
+PyObject* wrap(const at::Tensor& t) {
+  if (t.defined()) return THPVariable_Wrap(t);
+  Py_RETURN_NONE;
+}
+template <class... T>
+PyObject* tuple_of(const T&... tensors) {
+  PyObject* made[] = {wrap(tensors)...};
+  PyObject* result = PyTuple_New(sizeof...(T));
+  for (size_t i = 0; i < sizeof...(T); ++i) {
+    if (!result || !made[i]) {
+      for (size_t j = i; j < sizeof...(T); ++j) Py_XDECREF(made[j]);
+      Py_XDECREF(result);
+      return nullptr;
+    }
+    PyTuple_SET_ITEM(result, i, made[i]);
+  }
+  return result;
+}
+
+float real(PyObject* o) {
+  float v;
+  if (!convert(o, v)) throw Failed();
+  return v;
+}
+bool truth(PyObject* o) {
+  const int v = PyObject_IsTrue(o);
+  if (v < 0) throw Failed();
+  return v;
+}
+
+// rms_norm(x, residual or None, weight, eps, weight_offset, residual_out or None,
+//   quantize, keep) -> (values, scales, y, residual_out), None for what is not wanted
+PyObject* rms_norm(PyObject*, PyObject* const* args, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  try {
+    require(n == 8, "rms_norm: 8 arguments expected");
+    const at::Tensor& x = tensor(args[0]);
+    const at::Tensor weight = tensor(args[2]).contiguous();
+    const float eps = real(args[3]), offset = real(args[4]);
+    const bool quantize = truth(args[6]), keep = truth(args[7]);
+    require(x.dim() >= 1 && x.size(-1) > 0, "rows of at least one value");
+    const int64_t cols = x.size(-1);
+    require(weight.dim() == 1 && weight.size(0) == cols, "weight must be [x.shape[-1]]");
+    require(weight.device() == x.device(), "all operands on one device");
+    const at::Tensor x2 = rows_of(x);
+    const int64_t rows = x2.size(0);
+    at::Tensor res2, sum, sum2;
+    const bool add = args[1] != Py_None;
+    if (add) {
+      const at::Tensor& residual = tensor(args[1]);
+      auto like_x = [&](const at::Tensor& t) {
+        return t.sizes() == x.sizes() && t.scalar_type() == x.scalar_type() && t.device() == x.device();
+      };
+      require(like_x(residual), "the residual must be like x");
+      res2 = rows_of(residual);
+      if (args[5] != Py_None) {
+        sum = tensor(args[5]);
+        require(like_x(sum), "residual_out must be like x");
+        sum2 = sum.dim() == 2 ? sum : sum.view({rows, cols});
+        require((cols == 1 || sum2.stride(1) == 1) && (rows <= 1 || sum2.stride(0) >= cols),
+                "residual_out needs rows of unit stride");
+      }
+    } else {
+      require(args[5] == Py_None, "residual_out without a residual");
+    }
+    require_device(x);
+    const int code = dtype_code(x), weight_code = dtype_code(weight);
+    if (add && !sum.defined()) {
+      sum = at::empty(x.sizes(), x.options());
+      sum2 = sum;
+    }
+    Fp8Out q;
+    at::Tensor y;
+    if (quantize) q = fp8_out(rows, cols, x);
+    if (keep) y = at::empty(x.sizes(), x.options());
+    auto at_of = [](const at::Tensor& t) { return t.defined() ? t.data_ptr() : nullptr; };
+    const int64_t sum_stride = !sum2.defined() ? 0 : sum2.is_contiguous() ? cols : sum2.stride(0);
+    launch("gdn_rms_norm", lib::gdn_rms_norm, x, x2.data_ptr(), code, rows, cols, x2.stride(0), at_of(res2),
+           add ? res2.stride(0) : 0, weight.data_ptr(), weight_code, offset, eps, at_of(sum2), sum_stride, at_of(y), cols,
+           at_of(q.values), quantize ? q.values.stride(0) : 0, static_cast<float*>(at_of(q.scales)),
+           quantize ? q.scales.stride(0) : 0, quantize ? q.scales.stride(1) : 0);
+    return tuple_of(q.values, q.scales, y, sum);
+  } catch (const Failed&) {
+    return nullptr;
+  }
+  END_HANDLE_TH_ERRORS
+}
+
+// quantize_fp8(x) -> (values, scales)
+PyObject* quantize_fp8(PyObject*, PyObject* arg) {
+  HANDLE_TH_ERRORS
+  try {
+    const at::Tensor& x = tensor(arg);
+    require(x.dim() >= 1 && x.size(-1) > 0, "rows of at least one value");
+    const int code = dtype_code(x);
+    require_device(x);
+    const at::Tensor x2 = rows_of(x);
+    const int64_t rows = x2.size(0), cols = x2.size(1);
+    const Fp8Out q = fp8_out(rows, cols, x);
+    launch("gdn_quantize_fp8", lib::gdn_quantize_fp8, x, x2.data_ptr(), code, rows, cols, x2.stride(0),
+           q.values.data_ptr(), q.values.stride(0), q.scales.data_ptr<float>(), q.scales.stride(0), q.scales.stride(1));
+    return tuple_of(q.values, q.scales);
+  } catch (const Failed&) {
+    return nullptr;
+  }
+  END_HANDLE_TH_ERRORS
+}
+
+// rms_norm_gated_fp8(hidden, gate, weight, eps) -> (values, scales)
+PyObject* rms_norm_gated_fp8(PyObject*, PyObject* const* args, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  try {
+    require(n == 4, "rms_norm_gated_fp8: 4 arguments expected");
+    const at::Tensor &given = tensor(args[0]), &given_gate = tensor(args[1]);
+    const at::Tensor weight = tensor(args[2]).contiguous();
+    const float eps = real(args[3]);
+    require(given.dim() == 3 && given.sizes() == given_gate.sizes(), "[tokens, heads, dim] expected");
+    require(given.scalar_type() == given_gate.scalar_type(), "hidden states and gate of one dtype");
+    require(given.device() == given_gate.device() && given.device() == weight.device(), "all operands on one device");
+    const int64_t tokens = given.size(0), heads = given.size(1), dim = given.size(2);
+    require(heads > 0 && dim > 0 && weight.dim() == 1 && weight.size(0) == dim, "weight must be [dim]");
+    const int code = dtype_code(given), weight_code = dtype_code(weight);
+    require_device(given);
+    auto unit = [&](const at::Tensor& t) { return dim == 1 || t.stride(2) == 1 ? t : t.contiguous(); };
+    const at::Tensor x = unit(given), gate = unit(given_gate);
+    const Fp8Out q = fp8_out(tokens, heads * dim, x);
+    launch("gdn_rms_norm_gated_fp8", lib::gdn_rms_norm_gated_fp8, x, x.data_ptr(), code, tokens, heads, dim, x.stride(0),
+           x.stride(1), gate.data_ptr(), gate.stride(0), gate.stride(1), weight.data_ptr(), weight_code, eps,
+           q.values.data_ptr(), q.values.stride(0), q.scales.data_ptr<float>(), q.scales.stride(0), q.scales.stride(1));
+    return tuple_of(q.values, q.scales);
+  } catch (const Failed&) {
+    return nullptr;
+  }
+  END_HANDLE_TH_ERRORS
+}
+
+// 8-bit rows as the product takes them: 16-byte aligned, apart, and readable
+// up to the next multiple of 16 bytes.
+void check_fp8_rows(const at::Tensor& t, bool weight) {
+  require(t.dim() == 2 && t.scalar_type() == at::kFloat8_e4m3fn,
+          weight ? "weight values must be a 2-D float8_e4m3fn tensor" : "x values must be a 2-D float8_e4m3fn tensor");
+  const int64_t rows = t.size(0), cols = t.size(1);
+  require(cols > 0 && (cols == 1 || t.stride(1) == 1), "8-bit values need unit column stride");
+  if (rows == 0) return;
+  require(reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 == 0 &&
+              (rows == 1 || (t.stride(0) % 16 == 0 && t.stride(0) >= cols)),
+          "8-bit rows must start at multiples of 16 bytes and not overlap");
+  require(cols % 16 == 0 || t.storage_offset() + (rows - 1) * t.stride(0) + padded16(cols) <=
+                                static_cast<int64_t>(t.storage().nbytes()),
+          "the last 8-bit row must be readable up to a multiple of 16 bytes");
+}
+
+// fp8_linear(x values, x scales, weight values, weight scales, out_dtype, out or None)
+PyObject* fp8_linear(PyObject*, PyObject* const* args, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  try {
+    require(n == 6, "fp8_linear: 6 arguments expected");
+    const at::Tensor &x = tensor(args[0]), &xs = tensor(args[1]), &w = tensor(args[2]), &ws = tensor(args[3]);
+    check_fp8_rows(x, false);
+    check_fp8_rows(w, true);
+    const int64_t M = x.size(0), K = x.size(1), N = w.size(0), blocks = blocks_of(K);
+    require(N > 0 && w.size(1) == K, "x [M, K] and weight [N, K] must share K");
+    require(xs.scalar_type() == at::kFloat && xs.dim() == 2 && xs.size(0) == M && xs.size(1) == blocks,
+            "x scales must be fp32 [M, ceil(K / 128)]");
+    require(ws.scalar_type() == at::kFloat && ws.dim() == 2 && ws.size(0) == blocks_of(N) && ws.size(1) == blocks,
+            "weight scales must be fp32 [ceil(N / 128), ceil(K / 128)]");
+    require(THPDtype_Check(args[4]), "out_dtype must be a dtype");
+    const at::ScalarType type = reinterpret_cast<THPDtype*>(args[4])->scalar_type;
+    require(type == at::kBFloat16 || type == at::kHalf, "out_dtype must be bfloat16 or float16");
+    at::Tensor out;
+    if (args[5] != Py_None) {
+      out = tensor(args[5]);
+      require(out.dim() == 2 && out.size(0) == M && out.size(1) == N && out.scalar_type() == type,
+              "out must be [M, N] of out_dtype");
+      require((N == 1 || out.stride(1) == 1) && (M <= 1 || out.stride(0) >= N), "out needs rows of unit stride");
+      require(out.device() == x.device(), "all operands on one device");
+    }
+    require(xs.device() == x.device() && w.device() == x.device() && ws.device() == x.device(),
+            "all operands on one device");
+    if (!out.defined()) out = at::empty({M, N}, x.options().dtype(type));
+    if (M > 0) {
+      require_device(x);
+      launch("gdn_fp8_linear", lib::gdn_fp8_linear, x, x.data_ptr(), x.stride(0), xs.data_ptr<float>(), xs.stride(0),
+             xs.stride(1), w.data_ptr(), w.stride(0), ws.data_ptr<float>(), ws.stride(0), ws.stride(1), M, N, K,
+             out.data_ptr(), dtype_code(out), out.stride(0));
+    }
+    return THPVariable_Wrap(out);
+  } catch (const Failed&) {
+    return nullptr;
+  }
+  END_HANDLE_TH_ERRORS
+}
+
 #define GDN_METHOD(name) {#name, reinterpret_cast<PyCFunction>(&Entry<&lib::name>::call), METH_FASTCALL, nullptr},
 PyMethodDef kMethods[] = {
     {"bind", &bind, METH_O, nullptr},
     {"conv_recurrent", reinterpret_cast<PyCFunction>(&conv_recurrent), METH_FASTCALL, nullptr},
+    {"rms_norm", reinterpret_cast<PyCFunction>(&rms_norm), METH_FASTCALL, nullptr},
+    {"quantize_fp8", &quantize_fp8, METH_O, nullptr},
+    {"rms_norm_gated_fp8", reinterpret_cast<PyCFunction>(&rms_norm_gated_fp8), METH_FASTCALL, nullptr},
+    {"fp8_linear", reinterpret_cast<PyCFunction>(&fp8_linear), METH_FASTCALL, nullptr},
     GDN_TYPED(GDN_METHOD)
     {nullptr, nullptr, 0, nullptr}};
 PyModuleDef kModule = {PyModuleDef_HEAD_INIT, "_host", nullptr, -1, kMethods, nullptr, nullptr, nullptr, nullptr};

@@ -46,37 +46,12 @@ def _padded(cols: int) -> int:
     return (cols + 15) // 16 * 16
 
 
-def empty_rows(rows: int, cols: int, device) -> Fp8Tensor:
-    """An uninitialised destination of quantised rows.  The scales are laid out
-    block by block (strides 1, rows): the product reads one block of many rows
-    at a time."""
-    values = torch.empty(rows, _padded(cols), dtype=FP8, device=device)
-    scales = torch.empty(-(-cols // BLOCK), rows, dtype=torch.float32, device=device)
-    return Fp8Tensor(values if values.shape[1] == cols else values[:, :cols], scales.t())
-
-
-def rows_of(x: torch.Tensor) -> torch.Tensor:
-    """``x`` as [rows, cols] with unit column stride (a copy where it has no such view)."""
-    x = x if x.ndim == 2 else x.reshape(-1, x.shape[-1])
-    return x if x.stride(1) == 1 or x.shape[1] == 1 else x.contiguous()
-
-
 def quantize_fp8(x: torch.Tensor) -> Fp8Tensor:
     """The rows of ``x`` (fp32, bf16 or f16, leading dimensions flattened) in
-    8 bits.  A block that holds a NaN or an infinity reads back as NaN."""
-    assert x.ndim >= 1 and x.shape[-1] > 0, "rows of at least one value"
-    x2 = rows_of(x)
-    out = empty_rows(x2.shape[0], x2.shape[1], x2.device)
-    _lib.call_on(
-        x2, "gdn_quantize_fp8",
-        x2.data_ptr(), _lib.dtype_code(x2.dtype), x2.shape[0], x2.shape[1], x2.stride(0), *fp8_args(out),
-    )
-    return out
-
-
-def fp8_args(t: Fp8Tensor) -> tuple:
-    values, scales = t
-    return values.data_ptr(), values.stride(0), scales.data_ptr(), scales.stride(0), scales.stride(1)
+    8 bits.  A block that holds a NaN or an infinity reads back as NaN.  The
+    scales are laid out block by block (strides 1, rows): the product reads one
+    block of many rows at a time."""
+    return Fp8Tensor(*_lib.host().quantize_fp8(x))
 
 
 def quantize_fp8_weight(weight: torch.Tensor) -> Fp8Tensor:
@@ -94,48 +69,12 @@ def quantize_fp8_weight(weight: torch.Tensor) -> Fp8Tensor:
     return Fp8Tensor(w.view(torch.uint8)[:n, :_padded(k)].contiguous().view(FP8)[:, :k], scales)
 
 
-def _check_values(t: torch.Tensor, name: str) -> None:
-    assert t.ndim == 2 and t.dtype == FP8, f"{name} values must be a 2-D float8_e4m3fn tensor"
-    rows, cols = t.shape
-    assert cols > 0 and (cols == 1 or t.stride(1) == 1), f"{name} values need unit column stride"
-    if rows == 0:
-        return
-    assert t.data_ptr() % 16 == 0 and (rows == 1 or (t.stride(0) % 16 == 0 and t.stride(0) >= cols)), \
-        f"the rows of {name} must start at multiples of 16 bytes and not overlap"
-    if cols % 16:  # the kernel reads whole 16 bytes
-        last = t.storage_offset() + (rows - 1) * t.stride(0) + _padded(cols)
-        assert last <= t.untyped_storage().nbytes(), f"the last row of {name} must be readable up to a multiple of 16"
-
-
 def fp8_linear(x: Fp8Tensor, weight: Fp8Tensor, out_dtype: torch.dtype = torch.bfloat16, *,
                out: torch.Tensor | None = None) -> torch.Tensor:
     """``x [M, K] @ weight [N, K].T`` of quantised operands, accumulated in
     fp32 and rounded once to ``out_dtype`` (bf16 or f16).  ``out`` [M, N] may be
     a view with unit column stride; it is allocated when None."""
-    xv, xs = x
-    wv, ws = weight
-    _check_values(xv, "x")
-    _check_values(wv, "weight")
-    M, K = xv.shape
-    N = wv.shape[0]
-    blocks = -(-K // BLOCK)
-    assert N > 0 and wv.shape[1] == K, "x [M, K] and weight [N, K] must share K"
-    assert xs.dtype == torch.float32 and xs.shape == (M, blocks), "x scales must be fp32 [M, ceil(K / 128)]"
-    assert ws.dtype == torch.float32 and ws.shape == (-(-N // BLOCK), blocks), \
-        "weight scales must be fp32 [ceil(N / 128), ceil(K / 128)]"
-    if out is None:
-        out = torch.empty(M, N, dtype=out_dtype, device=xv.device)
-    else:
-        assert out.shape == (M, N) and out.dtype == out_dtype, "out must be [M, N] of out_dtype"
-        assert (N == 1 or out.stride(1) == 1) and (M <= 1 or out.stride(0) >= N), "out needs rows of unit stride"
-    assert out_dtype in (torch.bfloat16, torch.float16), "out_dtype must be bfloat16 or float16"
-    assert xv.device == xs.device == wv.device == ws.device == out.device, "all operands on one device"
-    if M:
-        _lib.call_on(
-            xv, "gdn_fp8_linear",
-            *fp8_args(x), *fp8_args(weight), M, N, K, out.data_ptr(), _lib.dtype_code(out_dtype), out.stride(0),
-        )
-    return out
+    return _lib.host().fp8_linear(x[0], x[1], weight[0], weight[1], out_dtype, out)
 
 
 __all__ = ["Fp8Tensor", "fp8_linear", "quantize_fp8", "quantize_fp8_weight"]

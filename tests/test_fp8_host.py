@@ -89,6 +89,7 @@ def _pair(rows, cols, scale_rows=None):
 def test_fp8_linear_refuses_what_does_not_fit():
     """Operands that do not fit each other or the kernel, before anything is launched."""
     from logssms_amd.kernel import Fp8Tensor, fp8_linear
+    _built()
     x, w = _pair(3, 256), _pair(200, 256, 2)
     bad = [
         (_pair(3, 128), w),  # another K
@@ -125,6 +126,7 @@ def test_fp8_linear_refuses_what_does_not_fit():
 def test_row_operators_refuse_what_does_not_fit():
     from logssms_amd.kernel import (add_rms_norm, add_rms_norm_fp8, quantize_fp8, rms_norm, rms_norm_fp8,
                                     rms_norm_gated_fp8)
+    _built()
     x, w = torch.zeros(4, 64), torch.ones(64)
     for call in (
         lambda: rms_norm(x, torch.ones(63), 1e-6),
