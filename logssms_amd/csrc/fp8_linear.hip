@@ -39,6 +39,16 @@ struct Linear {
   int wide_out;  // rows of out start at multiples of 16 bytes
 };
 
+__device__ __forceinline__ __amdgpu_buffer_rsrc_t rsrc_of(const void* from, uint32_t bytes) {
+  return __builtin_amdgcn_make_buffer_rsrc(const_cast<void*>(from), 0, bytes, 0x00020000);
+}
+// Direct-to-LDS loads of 16 or 4 bytes per active lane: lane l lands at lds + 16 l (4 l), zeros where off is past bytes.
+__device__ __forceinline__ void dma16(const void* src, uint32_t bytes, uint32_t off, void* lds) {
+  __builtin_amdgcn_raw_ptr_buffer_load_lds(rsrc_of(src, bytes), (lds_void*)lds, 16, off, 0, 0, 0);
+}
+__device__ __forceinline__ void dma4(const void* src, uint32_t bytes, uint32_t off, void* lds) {
+  __builtin_amdgcn_raw_ptr_buffer_load_lds(rsrc_of(src, bytes), (lds_void*)lds, 4, off, 0, 0, 0);
+}
 __device__ __forceinline__ i32x8 join(i32x4 a, i32x4 b) { return __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7); }
 
 // 16 bytes of a row from column k on, zeros from K on (K tails of the last
@@ -140,7 +150,7 @@ struct Tile {
   static constexpr int kStage = kRows * kFp8Block + 4 * BM;  // operands, then the tokens' scales
   static constexpr int JN = BN / 8 / kWaves, JM = BM / 8 / kWaves;
   static_assert(JN * 8 * kWaves == BN && JM * 8 * kWaves == BM, "whole loads per wave");
-  static_assert(kFp8Block % (32 * FN) == 0 || (32 * FN) % kFp8Block == 0, "one row of weight scales per fragment");
+  static_assert(kFp8Block % (32 * FN) == 0, "one row of weight scales per wave");
 };
 
 template <class OUT, int WN, int WM, int FN, int FM>
@@ -191,31 +201,36 @@ __global__ __launch_bounds__(64 * WN * WM) void tile_kernel(Linear p) {
     return true;
   };
 
-  auto fill = [&](const Cursor& c, uint8_t* base) {
+  // The loads of one step, issued piece by piece: piece i < JN + JM brings 8
+  // rows per wave, the last piece the tokens' scales.
+  struct Loads {
+    const void *x, *w, *xs;
+    uint32_t x_bytes, w_bytes, xs_bytes;
+    int width;
+    uint8_t* base;
+  };
+  auto loads_of = [&](const Cursor& c, bool any, uint8_t* base) {  // any == false: nothing is in range
     const int width = min(kFp8Block, padded - c.b * kFp8Block);
-    auto rows = [&](const uint8_t* src, int64_t stride, int count, int group0, auto Jc, uint8_t* dst) {
-      constexpr int J = decltype(Jc)::value;
-      const uint32_t bytes = static_cast<uint32_t>((count - 1) * stride + width);
-      const __amdgpu_buffer_rsrc_t rsrc =
-          __builtin_amdgcn_make_buffer_rsrc(const_cast<uint8_t*>(src), 0, bytes, 0x00020000);
-      const uint32_t row = static_cast<uint32_t>((lane >> 3) * stride);
-#pragma unroll
-      for (int j = 0; j < J; ++j) {
-        const int from = 16 * (chunk ^ (4 * ((group0 + j) & 1)));
-        const uint32_t off = row + from + static_cast<uint32_t>((group0 + j) * 8 * stride);
-        __builtin_amdgcn_raw_ptr_buffer_load_lds(rsrc, (lds_void*)(dst + (group0 + j) * 1024), 16,
-                                                 from >= width ? 0xffffff00u : off, 0, 0, 0);
-      }
+    const int rows_n = min(T::BN, p.N - c.n0), rows_m = min(T::BM, p.M - c.m0);
+    auto bytes = [&](int64_t n) { return any ? static_cast<uint32_t>(n) : 0u; };
+    return Loads{c.x, c.w, c.xs, bytes((rows_m - 1) * p.x_stride + width), bytes((rows_n - 1) * p.w_stride + width),
+                 bytes(((rows_m - 1) * p.xs_row + 1) * 4), width, base};
+  };
+  const uint32_t w_row = static_cast<uint32_t>((lane >> 3) * p.w_stride);
+  const uint32_t x_row = static_cast<uint32_t>((lane >> 3) * p.x_stride);
+  const uint32_t xs_at = static_cast<uint32_t>((wave * 64 + lane) * p.xs_row * 4);
+  auto issue = [&](const Loads& l, int piece) {
+    auto rows = [&](const void* src, uint32_t bytes, uint32_t row, int64_t stride, int group, uint8_t* dst) {
+      const int from = 16 * (chunk ^ (4 * (group & 1)));
+      const uint32_t off = row + from + static_cast<uint32_t>(group * 8 * stride);
+      dma16(src, bytes, from >= l.width ? 0xffffff00u : off, dst + group * 1024);
     };
-    rows(c.w, p.w_stride, min(T::BN, p.N - c.n0), wave * T::JN, std::integral_constant<int, T::JN>{}, base);
-    rows(c.x, p.x_stride, min(T::BM, p.M - c.m0), wave * T::JM, std::integral_constant<int, T::JM>{},
-         base + T::BN * kFp8Block);
-    if (wave * 64 < T::BM && (T::BM % 64 == 0 || wave * 64 + lane < T::BM)) {
-      const __amdgpu_buffer_rsrc_t rsrc = __builtin_amdgcn_make_buffer_rsrc(
-          const_cast<float*>(c.xs), 0, static_cast<uint32_t>(((min(T::BM, p.M - c.m0) - 1) * p.xs_row + 1) * 4),
-          0x00020000);
-      __builtin_amdgcn_raw_ptr_buffer_load_lds(rsrc, (lds_void*)(base + T::kRows * kFp8Block + wave * 256), 4,
-                                               static_cast<uint32_t>((wave * 64 + lane) * p.xs_row * 4), 0, 0, 0);
+    if (piece < T::JN) {
+      rows(l.w, l.w_bytes, w_row, p.w_stride, wave * T::JN + piece, l.base);
+    } else if (piece < T::JN + T::JM) {
+      rows(l.x, l.x_bytes, x_row, p.x_stride, wave * T::JM + piece - T::JN, l.base + T::BN * kFp8Block);
+    } else if (wave * 64 < T::BM && (T::BM % 64 == 0 || wave * 64 + lane < T::BM)) {
+      dma4(l.xs, l.xs_bytes, xs_at, l.base + T::kRows * kFp8Block + wave * 256);
     }
   };
 
@@ -230,13 +245,18 @@ __global__ __launch_bounds__(64 * WN * WM) void tile_kernel(Linear p) {
 
   int stage = 0;
   Cursor ahead = enter(first);
-  fill(ahead, lds);
+  {
+    const Loads l = loads_of(ahead, true, lds);
+#pragma unroll
+    for (int i = 0; i <= T::JN + T::JM; ++i) issue(l, i);
+  }
   while (true) {
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
     __syncthreads();  // the stage is filled, and nobody reads the other one any more
     const int b = ahead.b, m0 = ahead.m0, n0 = ahead.n0;
     const bool ends = b + 1 == blocks, more = advance(ahead);
-    if (more) fill(ahead, lds + (stage ^ 1) * T::kStage);
+    const Loads next = loads_of(ahead, more, lds + (stage ^ 1) * T::kStage);
+    issue(next, T::JN + T::JM);
     uint8_t* base = lds + stage * T::kStage;
     if (ends && (p.K & 15)) {  // bytes past K inside the last 16 of each row
       const int left = p.K & 15, at = (p.K & (kFp8Block - 1)) >> 4;
@@ -252,6 +272,8 @@ __global__ __launch_bounds__(64 * WN * WM) void tile_kernel(Linear p) {
       return join(*reinterpret_cast<const i32x4*>(at + 16 * (c ^ (r >> 1 & 7))),
                   *reinterpret_cast<const i32x4*>(at + 16 * ((c + 1) ^ (r >> 1 & 7))));
     };
+    const float sw = ((const_float*)p.ws)[min((n0 + wn * FN * 32) / kFp8Block, (p.N - 1) / kFp8Block) * p.ws_row +
+                                          b * p.ws_block];
     i32x8 bx[FM][2];
     float s[FM];
 #pragma unroll
@@ -259,24 +281,43 @@ __global__ __launch_bounds__(64 * WN * WM) void tile_kernel(Linear p) {
       const int row = (wm * FM + j) * 32;
       bx[j][0] = frag(T::BN + row, 0);
       bx[j][1] = frag(T::BN + row, 1);
-      s[j] = reinterpret_cast<const float*>(base + T::kRows * kFp8Block)[row + r];
+      s[j] = reinterpret_cast<const float*>(base + T::kRows * kFp8Block)[row + r] * sw;
     }
+    // One fragment and one product ahead: the next columns' fragments are read
+    // and the next product runs while the last one's is scaled and added.
+    auto promote = [&](const f32x16& d, int i, int j, int half) {
+#pragma unroll
+      for (int e = half; e < half + 8; ++e) acc[i][j][e] = fmaf(d[e], s[j], acc[i][j][e]);
+    };
+    i32x8 a[2][2];
+    f32x16 d[2];
+    a[0][0] = frag(wn * FN * 32, 0);
+    a[0][1] = frag(wn * FN * 32, 1);
 #pragma unroll
     for (int i = 0; i < FN; ++i) {
-      const int row = (wn * FN + i) * 32;
-      const float sw = ((const_float*)p.ws)[min((n0 + row) / kFp8Block, (p.N - 1) / kFp8Block) * p.ws_row +
-                                                            b * p.ws_block];
-      const i32x8 a0 = frag(row, 0), a1 = frag(row, 1);
+      if (i + 1 < FN) {
+        a[(i + 1) & 1][0] = frag((wn * FN + i + 1) * 32, 0);
+        a[(i + 1) & 1][1] = frag((wn * FN + i + 1) * 32, 1);
+      }
+      // the next step's loads between the products: issued at once they fill the queue and every wave waits behind it
+#pragma unroll
+      for (int piece = i * (T::JN + T::JM) / FN; piece < (i + 1) * (T::JN + T::JM) / FN; ++piece) issue(next, piece);
 #pragma unroll
       for (int j = 0; j < FM; ++j) {
-        f32x16 d = {};
-        d = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(a0, bx[j][0], d, 0, 0, 0, 0, 0, 0);
-        d = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(a1, bx[j][1], d, 0, 0, 0, 0, 0, 0);
-        const float sc = s[j] * sw;
-#pragma unroll
-        for (int e = 0; e < 16; ++e) acc[i][j][e] = fmaf(d[e], sc, acc[i][j][e]);
+        const int at = i * FM + j;
+        f32x16 zero = {};
+        d[at & 1] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(a[i & 1][0], bx[j][0], zero, 0, 0, 0, 0, 0, 0);
+        __builtin_amdgcn_sched_barrier(0);
+        if (at > 0) promote(d[(at - 1) & 1], (at - 1) / FM, (at - 1) % FM, 0);
+        __builtin_amdgcn_sched_barrier(0);
+        d[at & 1] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(a[i & 1][1], bx[j][1], d[at & 1], 0, 0, 0, 0, 0, 0);
+        __builtin_amdgcn_sched_barrier(0);
+        if (at > 0) promote(d[(at - 1) & 1], (at - 1) / FM, (at - 1) % FM, 8);
+        __builtin_amdgcn_sched_barrier(0);
       }
     }
+    promote(d[(FN * FM - 1) & 1], FN - 1, FM - 1, 0);
+    promote(d[(FN * FM - 1) & 1], FN - 1, FM - 1, 8);
     if (ends) {
       // registers 4 q .. 4 q + 3 hold columns 8 q + 4 g .. + 3 of token r; the halves of
       // the wave trade theirs, so that a lane stores 8 consecutive columns
@@ -318,6 +359,7 @@ __global__ __launch_bounds__(64 * WN * WM) void tile_kernel(Linear p) {
     if (!more) break;
     stage ^= 1;
   }
+  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // no load may land in LDS that is somebody else's by then
 }
 
 template <class OUT>
