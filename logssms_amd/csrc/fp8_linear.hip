@@ -32,8 +32,8 @@ struct Linear {
   const float* xs;
   const float* ws;
   void* out;
-  int64_t x_stride, w_stride, out_stride;       // of rows, elements
-  int64_t xs_row, xs_block, ws_row, ws_block;   // of the scales, elements
+  int x_stride, w_stride, out_stride, xs_row;    // of rows, elements
+  int64_t xs_block, ws_row, ws_block;            // of the scales, elements
   int M, N, K;
   int tiles_m, tiles_n;
   int wide_out;  // rows of out start at multiples of 16 bytes
@@ -49,8 +49,23 @@ __device__ __forceinline__ void dma16(const void* src, uint32_t bytes, uint32_t 
 __device__ __forceinline__ void dma4(const void* src, uint32_t bytes, uint32_t off, void* lds) {
   __builtin_amdgcn_raw_ptr_buffer_load_lds(rsrc_of(src, bytes), (lds_void*)lds, 4, off, 0, 0, 0);
 }
+// v, computed where it is used: not kept in a register across the loop around it.
+__device__ __forceinline__ int here(int v) {
+  asm volatile("" : "+v"(v));
+  return v;
+}
 __device__ __forceinline__ i32x8 join(i32x4 a, i32x4 b) { return __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7); }
 
+// Up to 8 columns of an output row at any even address.
+__device__ __forceinline__ void store_any(uint16_t* to, i32x4 v, int columns) {
+  if (columns >= 8) {
+    __builtin_memcpy(to, &v, 16);
+  } else {
+#pragma unroll
+    for (int e = 0; e < 8; ++e)
+      if (e < columns) to[e] = static_cast<uint16_t>(static_cast<uint32_t>(v[e / 2]) >> (16 * (e & 1)));
+  }
+}
 // 16 bytes of a row from column k on, zeros from K on (K tails of the last
 // block alone; the row is readable up to the next multiple of 16).
 __device__ __forceinline__ i32x4 mask_tail(i32x4 v, int left) {
@@ -123,7 +138,7 @@ __global__ __launch_bounds__(64 * kFewWaves) void few_rows_kernel(Linear p) {
     for (int i = 0; i < kFewWaves; ++i) sum += *reinterpret_cast<const f32x4*>(part[i][t][lane]);
     const int m = m0 + 16 * t + r, n = n0 + 4 * g;
     if (m >= p.M) continue;
-    OUT* out = static_cast<OUT*>(p.out) + m * p.out_stride + n;
+    OUT* out = static_cast<OUT*>(p.out) + static_cast<int64_t>(m) * p.out_stride + n;
     if (p.wide_out && n + 4 <= p.N) {
       *reinterpret_cast<uint2*>(out) = make_uint2(out_pack2<OUT>(sum[0], sum[1]), out_pack2<OUT>(sum[2], sum[3]));
     } else {
@@ -147,20 +162,27 @@ template <int WN, int WM, int FN, int FM>
 struct Tile {
   static constexpr int kWaves = WN * WM, kThreads = 64 * kWaves;
   static constexpr int BN = 32 * FN * WN, BM = 32 * FM * WM, kRows = BN + BM;
-  static constexpr int kStage = kRows * kFp8Block + 4 * BM;  // operands, then the tokens' scales
-  static constexpr int JN = BN / 8 / kWaves, JM = BM / 8 / kWaves;
-  static_assert(JN * 8 * kWaves == BN && JM * 8 * kWaves == BM, "whole loads per wave");
-  static_assert(kFp8Block % (32 * FN) == 0, "one row of weight scales per wave");
+  static constexpr int kW = BN * kFp8Block, kX = BM * kFp8Block, kS = 256 * kWaves;  // bytes of a step's operands and scales
+  static constexpr int kOut = 2048;  // per wave: 16 tokens of 64 columns on their way out
+  static constexpr int kLds = 2 * (kW + kX + kS) + kOut * kWaves;
+  static constexpr int JN = BN / 8 / kWaves, JM = BM / 8 / kWaves, kScales = BM / kWaves;  // loads and scales per wave
+  static constexpr int kStores = 2 * FN * FM;
+  static_assert(JN * 8 * kWaves == BN && JM * 8 * kWaves == BM && kScales <= 64, "whole loads per wave");
+  static_assert(kFp8Block % (32 * FN) == 0 && FN % 2 == 0, "one row of weight scales per wave");
 };
+
+template <int N> __device__ __forceinline__ void wait_loads() { asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory"); }
+// LDS traffic between the lanes of one wave: in order in hardware, so only the compiler has to be told.
+__device__ __forceinline__ void wave_fence() { asm volatile("" ::: "memory"); }
+__device__ __forceinline__ void lds_barrier() { asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory"); }
 
 template <class OUT, int WN, int WM, int FN, int FM>
 __global__ __launch_bounds__(64 * WN * WM) void tile_kernel(Linear p) {
   using T = Tile<WN, WM, FN, FM>;
-  __shared__ __align__(16) uint8_t lds[2 * T::kStage];
+  __shared__ __align__(16) uint8_t lds[T::kLds];
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int wn = wave % WN, wm = wave / WN;
-  const int blocks = (p.K + kFp8Block - 1) / kFp8Block;
   const int padded = (p.K + 15) & ~15;
   // of the 8 rows that a load covers, lane l brings chunk l % 8 of row l / 8, in odd groups of 8 rows the one 4 across
   const int chunk = (lane & 7) ^ (lane >> 4);
@@ -172,66 +194,72 @@ __global__ __launch_bounds__(64 * WN * WM) void tile_kernel(Linear p) {
   const int first = static_cast<int>(static_cast<int64_t>(tiles) * xcd / 8) + (blockIdx.x >> 3);
   const int last = static_cast<int>(static_cast<int64_t>(tiles) * (xcd + 1) / 8);
   if (first >= last) return;  // whole block
-  // What a step's loads need of tile t: its corner, and where the loads of the
-  // next block of K start.
-  struct Cursor {
-    int t, b, m0, n0;
-    const uint8_t *x, *w;
-    const float* xs;
-  };
-  auto enter = [&](int t) {
+  auto corner = [&](int t, int& m0, int& n0) {
     const int group = t / (8 * p.tiles_n), in = t - group * 8 * p.tiles_n;
     const int height = min(8, p.tiles_m - 8 * group);
-    Cursor c;
-    c.t = t, c.b = 0;
-    c.m0 = (8 * group + in % height) * T::BM;
-    c.n0 = in / height * T::BN;
-    c.x = p.x + c.m0 * p.x_stride;
-    c.w = p.w + c.n0 * p.w_stride;
-    c.xs = p.xs + c.m0 * p.xs_row;
-    return c;
+    m0 = (8 * group + in % height) * T::BM;
+    n0 = in / height * T::BN;
   };
-  auto advance = [&](Cursor& c) {
-    if (c.b + 1 == blocks) {
-      if (c.t + per_xcd >= last) return false;
-      c = enter(c.t + per_xcd);
-    } else {
-      c.b += 1, c.x += kFp8Block, c.w += kFp8Block, c.xs += p.xs_block;
-    }
-    return true;
+  // One operand's place in the walk over the tiles and, inside a tile, over the
+  // blocks of K: what its next loads need, kept in scalars that a step only adds to.
+  struct Walk {
+    int t, left;          // tile; columns of K from here on
+    const uint8_t* rows;  // of the tile, at the block of K
+    uint32_t span;        // bytes from the first of them to the last
+    const float* scales;  // weights: the wave's scale of the block; tokens: the first token's
+    uint32_t scale_span;
   };
-
-  // The loads of one step, issued piece by piece: piece i < JN + JM brings 8
-  // rows per wave, the last piece the tokens' scales.
-  struct Loads {
-    const void *x, *w, *xs;
-    uint32_t x_bytes, w_bytes, xs_bytes;
-    int width;
-    uint8_t* base;
+  auto enter_w = [&](Walk& c) {
+    int m0, n0;
+    corner(c.t, m0, n0);
+    c.left = padded;
+    c.rows = p.w + static_cast<int64_t>(n0) * p.w_stride;
+    c.span = static_cast<uint32_t>((min(T::BN, p.N - n0) - 1) * p.w_stride);
+    c.scales = p.ws + min((n0 + wn * FN * 32) / kFp8Block, (p.N - 1) / kFp8Block) * p.ws_row;
   };
-  auto loads_of = [&](const Cursor& c, bool any, uint8_t* base) {  // any == false: nothing is in range
-    const int width = min(kFp8Block, padded - c.b * kFp8Block);
-    const int rows_n = min(T::BN, p.N - c.n0), rows_m = min(T::BM, p.M - c.m0);
-    auto bytes = [&](int64_t n) { return any ? static_cast<uint32_t>(n) : 0u; };
-    return Loads{c.x, c.w, c.xs, bytes((rows_m - 1) * p.x_stride + width), bytes((rows_n - 1) * p.w_stride + width),
-                 bytes(((rows_m - 1) * p.xs_row + 1) * 4), width, base};
+  auto enter_x = [&](Walk& c) {
+    int m0, n0;
+    corner(c.t, m0, n0);
+    c.left = padded;
+    c.rows = p.x + static_cast<int64_t>(m0) * p.x_stride;
+    c.span = static_cast<uint32_t>((min(T::BM, p.M - m0) - 1) * p.x_stride);
+    c.scales = p.xs + static_cast<int64_t>(m0) * p.xs_row;
+    c.scale_span = static_cast<uint32_t>(((min(T::BM, p.M - m0) - 1) * p.xs_row + 1) * 4);
   };
-  const uint32_t w_row = static_cast<uint32_t>((lane >> 3) * p.w_stride);
-  const uint32_t x_row = static_cast<uint32_t>((lane >> 3) * p.x_stride);
-  const uint32_t xs_at = static_cast<uint32_t>((wave * 64 + lane) * p.xs_row * 4);
-  auto issue = [&](const Loads& l, int piece) {
-    auto rows = [&](const void* src, uint32_t bytes, uint32_t row, int64_t stride, int group, uint8_t* dst) {
-      const int from = 16 * (chunk ^ (4 * (group & 1)));
-      const uint32_t off = row + from + static_cast<uint32_t>(group * 8 * stride);
-      dma16(src, bytes, from >= l.width ? 0xffffff00u : off, dst + group * 1024);
-    };
-    if (piece < T::JN) {
-      rows(l.w, l.w_bytes, w_row, p.w_stride, wave * T::JN + piece, l.base);
-    } else if (piece < T::JN + T::JM) {
-      rows(l.x, l.x_bytes, x_row, p.x_stride, wave * T::JM + piece - T::JN, l.base + T::BN * kFp8Block);
-    } else if (wave * 64 < T::BM && (T::BM % 64 == 0 || wave * 64 + lane < T::BM)) {
-      dma4(l.xs, l.xs_bytes, xs_at, l.base + T::kRows * kFp8Block + wave * 256);
-    }
+  // to the next block of K, or the next tile; after the last one (t >= last) the
+  // loads are still issued, with nothing in range, so that every step counts the same
+  auto advance = [&](Walk& c, int64_t scale_step, auto enter) {
+    c.rows += kFp8Block;
+    c.scales += scale_step;
+    c.left -= kFp8Block;
+    if (c.left <= 0 && (c.t += per_xcd) < last) enter(c);
+  };
+  // The lanes' offsets of each load: 8 rows, a chunk of each per lane.
+  uint32_t w_at[T::JN], x_at[T::JM];
+#pragma unroll
+  for (int j = 0; j < T::JN; ++j)
+    w_at[j] = static_cast<uint32_t>(((wave * T::JN + j) * 8 + (lane >> 3)) * p.w_stride) +
+              16 * (chunk ^ (4 * ((wave * T::JN + j) & 1)));
+#pragma unroll
+  for (int j = 0; j < T::JM; ++j)
+    x_at[j] = static_cast<uint32_t>(((wave * T::JM + j) * 8 + (lane >> 3)) * p.x_stride) +
+              16 * (chunk ^ (4 * ((wave * T::JM + j) & 1)));
+  // each wave brings kScales of the tokens' scales into 256 bytes of its own (no branch: a branch here lets the
+  // compiler move the scaling behind it, for which there are no registers)
+  const uint32_t xs_at = lane < T::kScales ? static_cast<uint32_t>((wave * T::kScales + lane) * p.xs_row * 4) : 0xffffff00u;
+  auto load_rows = [&](const Walk& c, uint32_t at, int group, uint8_t* dst) {
+    const int width = min(kFp8Block, c.left);
+    const bool past = 16 * (chunk ^ (4 * (group & 1))) >= width;
+    dma16(c.rows, c.t < last ? c.span + width : 0u, past ? 0xffffff00u : at, dst + group * 1024);
+  };
+  auto load_w = [&](const Walk& c, int j, int stage) {
+    load_rows(c, w_at[j], wave * T::JN + j, lds + stage * T::kW);
+  };
+  auto load_x = [&](const Walk& c, int j, int stage) {  // the last one brings the tokens' scales
+    if (j < T::JM)
+      load_rows(c, x_at[j], wave * T::JM + j, lds + 2 * T::kW + stage * T::kX);
+    else
+      dma4(c.scales, c.t < last ? c.scale_span : 0u, xs_at, lds + 2 * (T::kW + T::kX) + stage * T::kS + wave * 256);
   };
 
   const int r = lane & 31, g = lane >> 5;
@@ -243,45 +271,57 @@ __global__ __launch_bounds__(64 * WN * WM) void tile_kernel(Linear p) {
 #pragma unroll
       for (int e = 0; e < 16; ++e) acc[i][j][e] = 0.f;
 
+  // The weights' loads run one step ahead, the tokens' nearly two: their
+  // fragments are all in registers after a wave's first products, and a second
+  // barrier there frees their place for the step after the next.
   int stage = 0;
-  Cursor ahead = enter(first);
-  {
-    const Loads l = loads_of(ahead, true, lds);
+  bool stored = false;
+  Walk ahead_w{first}, ahead_x{first};
+  enter_w(ahead_w);
+  enter_x(ahead_x);
 #pragma unroll
-    for (int i = 0; i <= T::JN + T::JM; ++i) issue(l, i);
-  }
+  for (int i = 0; i < T::JN; ++i) load_w(ahead_w, i, 0);
+#pragma unroll
+  for (int i = 0; i <= T::JM; ++i) load_x(ahead_x, i, 0);
+  advance(ahead_x, p.xs_block, enter_x);
+#pragma unroll
+  for (int i = 0; i <= T::JM; ++i) load_x(ahead_x, i, 1);
   while (true) {
-    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-    __syncthreads();  // the stage is filled, and nobody reads the other one any more
-    const int b = ahead.b, m0 = ahead.m0, n0 = ahead.n0;
-    const bool ends = b + 1 == blocks, more = advance(ahead);
-    const Loads next = loads_of(ahead, more, lds + (stage ^ 1) * T::kStage);
-    issue(next, T::JN + T::JM);
-    uint8_t* base = lds + stage * T::kStage;
+    // all but the next step's JM + 1 loads of tokens, and what the last tile stored behind them, have landed
+    if (stored) wait_loads<T::JM + 1 + T::kStores>(); else wait_loads<T::JM + 1>();
+    stored = false;
+    lds_barrier();
+    const int t = ahead_w.t;
+    const bool ends = ahead_w.left <= kFp8Block;
+    const float sw = *(const_float*)ahead_w.scales;
+    advance(ahead_w, p.ws_block, enter_w);
+    advance(ahead_x, p.xs_block, enter_x);
+    uint8_t* w_lds = lds + stage * T::kW;
+    uint8_t* x_lds = lds + 2 * T::kW + stage * T::kX;
     if (ends && (p.K & 15)) {  // bytes past K inside the last 16 of each row
-      const int left = p.K & 15, at = (p.K & (kFp8Block - 1)) >> 4;
+      const int left = p.K & 15, in = (p.K & (kFp8Block - 1)) >> 4;
       for (int row = threadIdx.x; row < T::kRows; row += T::kThreads) {
-        i32x4* v = reinterpret_cast<i32x4*>(base + row * kFp8Block + 16 * (at ^ (row >> 1 & 7)));
+        uint8_t* of = row < T::BN ? w_lds + row * kFp8Block : x_lds + (row - T::BN) * kFp8Block;
+        i32x4* v = reinterpret_cast<i32x4*>(of + 16 * (in ^ (row >> 1 & 7)));
         *v = mask_tail(*v, left);
       }
-      __syncthreads();
+      lds_barrier();
     }
-    auto frag = [&](int row, int half) {  // lanes (r, g): row r, bytes 64 half + 32 g .. + 31
-      const uint8_t* at = base + (row + r) * kFp8Block;
+    auto frag = [&](const uint8_t* base, int row, int half) {  // lanes (r, g): row r, bytes 64 half + 32 g .. + 31
+      const uint8_t* of = base + (row + r) * kFp8Block;
       const int c = 4 * half + 2 * g;
-      return join(*reinterpret_cast<const i32x4*>(at + 16 * (c ^ (r >> 1 & 7))),
-                  *reinterpret_cast<const i32x4*>(at + 16 * ((c + 1) ^ (r >> 1 & 7))));
+      return join(*reinterpret_cast<const i32x4*>(of + 16 * (c ^ (r >> 1 & 7))),
+                  *reinterpret_cast<const i32x4*>(of + 16 * ((c + 1) ^ (r >> 1 & 7))));
     };
-    const float sw = ((const_float*)p.ws)[min((n0 + wn * FN * 32) / kFp8Block, (p.N - 1) / kFp8Block) * p.ws_row +
-                                          b * p.ws_block];
     i32x8 bx[FM][2];
     float s[FM];
 #pragma unroll
     for (int j = 0; j < FM; ++j) {
       const int row = (wm * FM + j) * 32;
-      bx[j][0] = frag(T::BN + row, 0);
-      bx[j][1] = frag(T::BN + row, 1);
-      s[j] = reinterpret_cast<const float*>(base + T::kRows * kFp8Block)[row + r] * sw;
+      bx[j][0] = frag(x_lds, row, 0);
+      bx[j][1] = frag(x_lds, row, 1);
+      s[j] = *reinterpret_cast<const float*>(lds + 2 * (T::kW + T::kX) + stage * T::kS +
+                                             (row + r) / T::kScales * 256 + (row + r) % T::kScales * 4) * sw;
     }
     // One fragment and one product ahead: the next columns' fragments are read
     // and the next product runs while the last one's is scaled and added.
@@ -291,75 +331,107 @@ __global__ __launch_bounds__(64 * WN * WM) void tile_kernel(Linear p) {
     };
     i32x8 a[2][2];
     f32x16 d[2];
-    a[0][0] = frag(wn * FN * 32, 0);
-    a[0][1] = frag(wn * FN * 32, 1);
+    a[0][0] = frag(w_lds, wn * FN * 32, 0);
+    a[0][1] = frag(w_lds, wn * FN * 32, 1);
 #pragma unroll
     for (int i = 0; i < FN; ++i) {
+      if (i == 1) lds_barrier();  // every wave holds its tokens' fragments
       if (i + 1 < FN) {
-        a[(i + 1) & 1][0] = frag((wn * FN + i + 1) * 32, 0);
-        a[(i + 1) & 1][1] = frag((wn * FN + i + 1) * 32, 1);
+        a[(i + 1) & 1][0] = frag(w_lds, (wn * FN + i + 1) * 32, 0);
+        a[(i + 1) & 1][1] = frag(w_lds, (wn * FN + i + 1) * 32, 1);
       }
-      // the next step's loads between the products: issued at once they fill the queue and every wave waits behind it
+      // between the products: loads issued all at once fill the queue, and every wave waits behind it
+      if (i == 0) {
 #pragma unroll
-      for (int piece = i * (T::JN + T::JM) / FN; piece < (i + 1) * (T::JN + T::JM) / FN; ++piece) issue(next, piece);
+        for (int piece = 0; piece < T::JN; ++piece) load_w(ahead_w, piece, stage ^ 1);
+      } else {
+        constexpr int kPer = (T::JM + 1 + FN - 2) / (FN - 1);
+#pragma unroll
+        for (int piece = (i - 1) * kPer; piece < min(i * kPer, T::JM + 1); ++piece) load_x(ahead_x, piece, stage);
+      }
 #pragma unroll
       for (int j = 0; j < FM; ++j) {
-        const int at = i * FM + j;
+        const int now = i * FM + j;
         f32x16 zero = {};
-        d[at & 1] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(a[i & 1][0], bx[j][0], zero, 0, 0, 0, 0, 0, 0);
+        d[now & 1] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(a[i & 1][0], bx[j][0], zero, 0, 0, 0, 0, 0, 0);
         __builtin_amdgcn_sched_barrier(0);
-        if (at > 0) promote(d[(at - 1) & 1], (at - 1) / FM, (at - 1) % FM, 0);
+        if (now > 0) promote(d[(now - 1) & 1], (now - 1) / FM, (now - 1) % FM, 0);
         __builtin_amdgcn_sched_barrier(0);
-        d[at & 1] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(a[i & 1][1], bx[j][1], d[at & 1], 0, 0, 0, 0, 0, 0);
+        d[now & 1] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(a[i & 1][1], bx[j][1], d[now & 1], 0, 0, 0, 0, 0, 0);
         __builtin_amdgcn_sched_barrier(0);
-        if (at > 0) promote(d[(at - 1) & 1], (at - 1) / FM, (at - 1) % FM, 8);
+        if (now > 0) promote(d[(now - 1) & 1], (now - 1) / FM, (now - 1) % FM, 8);
         __builtin_amdgcn_sched_barrier(0);
       }
     }
     promote(d[(FN * FM - 1) & 1], FN - 1, FM - 1, 0);
     promote(d[(FN * FM - 1) & 1], FN - 1, FM - 1, 8);
     if (ends) {
-      // registers 4 q .. 4 q + 3 hold columns 8 q + 4 g .. + 3 of token r; the halves of
-      // the wave trade theirs, so that a lane stores 8 consecutive columns
+      // Registers 4 q .. 4 q + 3 hold columns 8 q + 4 g .. + 3 of token r.  The
+      // halves of the wave trade theirs, so that a lane has 8 consecutive columns;
+      // then 16 tokens of 64 columns at a time go through LDS and out as rows of
+      // 128 bytes (stored as they lie, in pieces of 32 bytes, the last product of
+      // 16384 x 12288 x 2048 took 437 us, without any stores 361).
+      int m0, n0;
+      corner(t, m0, n0);
+      const bool wide = p.wide_out && (p.N % 8 == 0 || n0 + T::BN <= p.N);
+      const int rows = min(T::BM, p.M - m0);
+      const int l = here(lane), r = l & 31, g = l >> 5;
+      uint8_t* mine = lds + 2 * (T::kW + T::kX + T::kS) + wave * T::kOut;
+      OUT* tile = static_cast<OUT*>(p.out) + static_cast<int64_t>(m0) * p.out_stride + n0;
+      const auto rsrc = rsrc_of(tile, (static_cast<uint32_t>(rows - 1) * p.out_stride + min(T::BN, p.N - n0)) * 2u);
 #pragma unroll
-      for (int i = 0; i < FN; ++i)
+      for (int i = 0; i < FN; i += 2)
 #pragma unroll
         for (int j = 0; j < FM; ++j) {
-          const int m = m0 + (wm * FM + j) * 32 + r;
-          const int n = n0 + (wn * FN + i) * 32;
-          OUT* out = static_cast<OUT*>(p.out) + m * p.out_stride + n;
+          i32x4 v[4];
 #pragma unroll
-          for (int q = 0; q < 4; q += 2) {
+          for (int q = 0; q < 8; q += 2) {
+            const f32x16& from = acc[i + q / 4][j];
             uint32_t lo[2], hi[2];
 #pragma unroll
             for (int e = 0; e < 2; ++e) {
-              lo[e] = out_pack2<OUT>(acc[i][j][4 * q + 2 * e], acc[i][j][4 * q + 2 * e + 1]);
-              hi[e] = out_pack2<OUT>(acc[i][j][4 * q + 4 + 2 * e], acc[i][j][4 * q + 5 + 2 * e]);
+              const int x = 4 * (q % 4) + 2 * e;
+              lo[e] = out_pack2<OUT>(from[x], from[x + 1]);
+              hi[e] = out_pack2<OUT>(from[x + 4], from[x + 5]);
               const auto swapped = __builtin_amdgcn_permlane32_swap(lo[e], hi[e], false, false);
               lo[e] = swapped[0], hi[e] = swapped[1];
             }
-            const uint4 v = make_uint4(lo[0], lo[1], hi[0], hi[1]);
-            const int c = 8 * (q + g);
-            if (m < p.M) {
-              if (p.wide_out && n + c + 8 <= p.N) {
-                *reinterpret_cast<uint4*>(out + c) = v;
-              } else {
-                const uint32_t words[4] = {v.x, v.y, v.z, v.w};
-#pragma unroll
-                for (int e = 0; e < 8; ++e)
-                  if (n + c + e < p.N)
-                    reinterpret_cast<uint16_t*>(out)[c + e] = static_cast<uint16_t>(words[e / 2] >> (16 * (e & 1)));
-              }
-            }
+            v[q / 2] = i32x4{static_cast<int>(lo[0]), static_cast<int>(lo[1]), static_cast<int>(hi[0]),
+                             static_cast<int>(hi[1])};  // columns 8 (q + g) .. + 7
           }
 #pragma unroll
-          for (int e = 0; e < 16; ++e) acc[i][j][e] = 0.f;
+          for (int half = 0; half < 2; ++half) {
+            if (r / 16 == half) {
+#pragma unroll
+              for (int q = 0; q < 8; q += 2)
+                *reinterpret_cast<i32x4*>(mine + r % 16 * 128 + 16 * ((q + g) ^ (r >> 1 & 7))) = v[q / 2];
+            }
+            wave_fence();
+#pragma unroll
+            for (int k = 0; k < 2; ++k) {  // lane l: 8 columns of row 8 k + l / 8
+              const int row = 8 * k + (l >> 3), c = l & 7;
+              const i32x4 out = *reinterpret_cast<const i32x4*>(mine + row * 128 + 16 * (c ^ (row >> 1 & 7)));
+              const int m = (wm * FM + j) * 32 + 16 * half + row, n = (wn * FN + i) * 32 + 8 * c;
+              if (wide) {  // always kStores stores: rows and columns that are not there fall out of range
+                const bool there = m < rows && n0 + n < p.N;
+                __builtin_amdgcn_raw_buffer_store_b128(
+                    out, rsrc, there ? (static_cast<uint32_t>(m) * p.out_stride + n) * 2u : 0xffffff00u, 0, 0);
+              } else if (m < rows) {
+                store_any(reinterpret_cast<uint16_t*>(tile) + static_cast<int64_t>(m) * p.out_stride + n, out,
+                          p.N - n0 - n);
+              }
+            }
+            wave_fence();
+          }
+#pragma unroll
+          for (int e = 0; e < 16; ++e) acc[i][j][e] = acc[i + 1][j][e] = 0.f;
         }
+      stored = wide;
     }
-    if (!more) break;
+    if (ahead_w.t >= last) break;
     stage ^= 1;
   }
-  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // no load may land in LDS that is somebody else's by then
+  wait_loads<0>();  // no load may land in LDS that is somebody else's by then
 }
 
 template <class OUT>
@@ -384,7 +456,7 @@ int launch_linear(Linear p, hipStream_t s) {
     p.tiles_n = (p.N + T::BN - 1) / T::BN;
     const int64_t tiles = static_cast<int64_t>(p.tiles_m) * p.tiles_n;
     GDN_REQUIRE(tiles <= 0x7fffffff / 8, "gdn_fp8_linear: too many tiles");
-    constexpr int kPerCu = (160 * 1024) / (2 * T::kStage);
+    constexpr int kPerCu = (160 * 1024) / T::kLds;
     const int grid = static_cast<int>(tiles < 256 * kPerCu ? (tiles + 7) / 8 * 8 : 256 * kPerCu);
     hipLaunchKernelGGL((tile_kernel<OUT, WN, WM, FN, FM>), dim3(grid), dim3(T::kThreads), 0, s, p);
     return GDN_LAUNCH_CHECK("gdn_fp8_linear launch");
@@ -424,13 +496,13 @@ extern "C" int gdn_fp8_linear(const void* x, int64_t x_row_stride, const float* 
   // offsets inside a tile of up to 256 rows are 32-bit
   constexpr int64_t kMostStride = int64_t{1} << 23;
   if (M > 0x7fffff00 || N > 0x7fffff00 || K > 0x7fffff00 || x_row_stride > kMostStride ||
-      weight_row_stride > kMostStride || xs_row_stride > kMostStride / 4) {
+      weight_row_stride > kMostStride || out_row_stride > kMostStride / 2 || xs_row_stride > kMostStride / 4) {
     set_error("gdn_fp8_linear: sizes or row strides beyond 2^23 are not covered");
     return GDN_ERR_UNSUPPORTED;
   }
   Linear p{static_cast<const uint8_t*>(x), static_cast<const uint8_t*>(weight), x_scales, weight_scales, out,
-           x_row_stride, weight_row_stride, out_row_stride, xs_row_stride, xs_block_stride, ws_row_stride,
-           ws_block_stride, static_cast<int>(M), static_cast<int>(N), static_cast<int>(K), 0, 0, 0};
+           static_cast<int>(x_row_stride), static_cast<int>(weight_row_stride), static_cast<int>(out_row_stride),
+           static_cast<int>(xs_row_stride), xs_block_stride, ws_row_stride, ws_block_stride, static_cast<int>(M), static_cast<int>(N), static_cast<int>(K), 0, 0, 0};
   p.wide_out = aligned16(out) && (M == 1 || out_row_stride % 8 == 0);
   hipStream_t s = static_cast<hipStream_t>(stream);
   return out_dtype == GDN_BF16 ? launch_linear<bf16>(p, s) : launch_linear<f16>(p, s);
