@@ -54,6 +54,10 @@ __device__ __forceinline__ int here(int v) {
   asm volatile("" : "+v"(v));
   return v;
 }
+__device__ __forceinline__ int here_s(int v) {  // the same for a value that all lanes share
+  asm volatile("" : "+s"(v));
+  return v;
+}
 __device__ __forceinline__ i32x8 join(i32x4 a, i32x4 b) { return __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7); }
 
 // Up to 8 columns of an output row at any even address.
@@ -158,15 +162,18 @@ __global__ __launch_bounds__(64 * kFewWaves) void few_rows_kernel(Linear p) {
 // spreads them over all of the banks (c ^ (r % 8) cost 4 conflict cycles on
 // each 4).  The direct loads land in lane order, so the lanes' source chunks
 // are permuted instead.
-template <int WN, int WM, int FN, int FM>
+template <int WN, int WM, int FN, int FM, int S>
 struct Tile {
   static constexpr int kWaves = WN * WM, kThreads = 64 * kWaves;
   static constexpr int BN = 32 * FN * WN, BM = 32 * FM * WM, kRows = BN + BM;
   static constexpr int kW = BN * kFp8Block, kX = BM * kFp8Block, kS = 256 * kWaves;  // bytes of a step's operands and scales
-  static constexpr int kOut = 2048;  // per wave: 16 tokens of 64 columns on their way out
-  static constexpr int kLds = 2 * (kW + kX + kS) + kOut * kWaves;
+  static constexpr int kLds = S * (kW + kX + kS);
   static constexpr int JN = BN / 8 / kWaves, JM = BM / 8 / kWaves, kScales = BM / kWaves;  // loads and scales per wave
   static constexpr int kStores = 2 * FN * FM;
+  static constexpr int kOut = 2048;  // per wave: 16 tokens of 64 columns on their way out, in place of a step's weights
+  // loads that are newer than a step's own when it begins
+  static constexpr int kAhead = S == 2 ? JM + 1 : (S - 2) * (JN + JM + 1);
+  static_assert(kOut * kWaves <= kW && kLds <= 160 * 1024 && kAhead + kStores < 64, "fits");
   static_assert(JN * 8 * kWaves == BN && JM * 8 * kWaves == BM && kScales <= 64, "whole loads per wave");
   static_assert(kFp8Block % (32 * FN) == 0 && FN % 2 == 0, "one row of weight scales per wave");
 };
@@ -176,9 +183,9 @@ template <int N> __device__ __forceinline__ void wait_loads() { asm volatile("s_
 __device__ __forceinline__ void wave_fence() { asm volatile("" ::: "memory"); }
 __device__ __forceinline__ void lds_barrier() { asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory"); }
 
-template <class OUT, int WN, int WM, int FN, int FM>
-__global__ __launch_bounds__(64 * WN * WM) void tile_kernel(Linear p) {
-  using T = Tile<WN, WM, FN, FM>;
+template <class OUT, int WN, int WM, int FN, int FM, int S>
+__global__ __launch_bounds__(64 * WN * WM, 2) void tile_kernel(Linear p) {
+  using T = Tile<WN, WM, FN, FM, S>;
   __shared__ __align__(16) uint8_t lds[T::kLds];
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -194,45 +201,43 @@ __global__ __launch_bounds__(64 * WN * WM) void tile_kernel(Linear p) {
   const int first = static_cast<int>(static_cast<int64_t>(tiles) * xcd / 8) + (blockIdx.x >> 3);
   const int last = static_cast<int>(static_cast<int64_t>(tiles) * (xcd + 1) / 8);
   if (first >= last) return;  // whole block
-  auto corner = [&](int t, int& m0, int& n0) {
-    const int group = t / (8 * p.tiles_n), in = t - group * 8 * p.tiles_n;
-    const int height = min(8, p.tiles_m - 8 * group);
+  auto corner = [&](int t, int& m0, int& n0) __attribute__((always_inline)) {
+    const int across = here_s(p.tiles_n), down = here_s(p.tiles_m);
+    const int group = t / (8 * across), in = t - group * 8 * across;
+    const int height = min(8, down - 8 * group);
     m0 = (8 * group + in % height) * T::BM;
     n0 = in / height * T::BN;
   };
-  // One operand's place in the walk over the tiles and, inside a tile, over the
-  // blocks of K: what its next loads need, kept in scalars that a step only adds to.
+  // A place in the walk over the tiles and, inside a tile, over the blocks of K:
+  // what the next loads need, kept in scalars that a step only adds to.
   struct Walk {
-    int t, left;          // tile; columns of K from here on
-    const uint8_t* rows;  // of the tile, at the block of K
-    uint32_t span;        // bytes from the first of them to the last
-    const float* scales;  // weights: the wave's scale of the block; tokens: the first token's
-    uint32_t scale_span;
+    int t, left;               // tile; columns of K from here on
+    const uint8_t *w, *x;      // the tile's first rows, at the block of K
+    uint32_t w_span, x_span;   // bytes from the first of them to the last
+    const float *ws, *xs;      // the wave's scale of the block; the first token's
+    uint32_t xs_span;
   };
-  auto enter_w = [&](Walk& c) {
+  auto enter = [&](int t) __attribute__((always_inline)) {
     int m0, n0;
-    corner(c.t, m0, n0);
-    c.left = padded;
-    c.rows = p.w + static_cast<int64_t>(n0) * p.w_stride;
-    c.span = static_cast<uint32_t>((min(T::BN, p.N - n0) - 1) * p.w_stride);
-    c.scales = p.ws + min((n0 + wn * FN * 32) / kFp8Block, (p.N - 1) / kFp8Block) * p.ws_row;
+    corner(t, m0, n0);
+    const int below = here_s(p.M) - m0, beside = here_s(p.N) - n0;
+    const int rows_n = beside < T::BN ? beside : T::BN, rows_m = below < T::BM ? below : T::BM;
+    return Walk{t, padded, p.w + static_cast<int64_t>(n0) * p.w_stride, p.x + static_cast<int64_t>(m0) * p.x_stride,
+                static_cast<uint32_t>((rows_n - 1) * p.w_stride), static_cast<uint32_t>((rows_m - 1) * p.x_stride),
+                p.ws + min((n0 + wn * FN * 32) / kFp8Block, (here_s(p.N) - 1) / kFp8Block) * p.ws_row,
+                p.xs + static_cast<int64_t>(m0) * p.xs_row, static_cast<uint32_t>(((rows_m - 1) * p.xs_row + 1) * 4)};
   };
-  auto enter_x = [&](Walk& c) {
-    int m0, n0;
-    corner(c.t, m0, n0);
-    c.left = padded;
-    c.rows = p.x + static_cast<int64_t>(m0) * p.x_stride;
-    c.span = static_cast<uint32_t>((min(T::BM, p.M - m0) - 1) * p.x_stride);
-    c.scales = p.xs + static_cast<int64_t>(m0) * p.xs_row;
-    c.scale_span = static_cast<uint32_t>(((min(T::BM, p.M - m0) - 1) * p.xs_row + 1) * 4);
-  };
-  // to the next block of K, or the next tile; after the last one (t >= last) the
-  // loads are still issued, with nothing in range, so that every step counts the same
-  auto advance = [&](Walk& c, int64_t scale_step, auto enter) {
-    c.rows += kFp8Block;
-    c.scales += scale_step;
+  auto step = [&](Walk& c) __attribute__((always_inline)) {
     c.left -= kFp8Block;
-    if (c.left <= 0 && (c.t += per_xcd) < last) enter(c);
+    c.w += kFp8Block, c.x += kFp8Block;
+    c.ws += p.ws_block, c.xs += p.xs_block;
+  };
+  // past the end of K: to the next tile; after the last one (t >= last) the loads
+  // are still issued, with nothing in range, so that every step counts the same
+  auto turn = [&](Walk& c) __attribute__((always_inline)) {
+    if (c.left > 0) return;
+    const int t = c.t + per_xcd;
+    if (t < last) c = enter(t); else c = Walk{t, 0, c.w, c.x, 0, 0, c.ws, c.xs, 0};
   };
   // The lanes' offsets of each load: 8 rows, a chunk of each per lane.
   uint32_t w_at[T::JN], x_at[T::JM];
@@ -247,19 +252,22 @@ __global__ __launch_bounds__(64 * WN * WM) void tile_kernel(Linear p) {
   // each wave brings kScales of the tokens' scales into 256 bytes of its own (no branch: a branch here lets the
   // compiler move the scaling behind it, for which there are no registers)
   const uint32_t xs_at = lane < T::kScales ? static_cast<uint32_t>((wave * T::kScales + lane) * p.xs_row * 4) : 0xffffff00u;
-  auto load_rows = [&](const Walk& c, uint32_t at, int group, uint8_t* dst) {
-    const int width = min(kFp8Block, c.left);
+  auto load_rows = [&](const uint8_t* src, uint32_t span, int left, uint32_t at, int group, uint8_t* dst) __attribute__((always_inline)) {
+    const int width = min(kFp8Block, left);
     const bool past = 16 * (chunk ^ (4 * (group & 1))) >= width;
-    dma16(c.rows, c.t < last ? c.span + width : 0u, past ? 0xffffff00u : at, dst + group * 1024);
+    dma16(src, span + width, past ? 0xffffff00u : at, dst + group * 1024);
   };
-  auto load_w = [&](const Walk& c, int j, int stage) {
-    load_rows(c, w_at[j], wave * T::JN + j, lds + stage * T::kW);
+  auto w_of = [&](int stage) __attribute__((always_inline)) { return lds + stage * T::kW; };
+  auto x_of = [&](int stage) __attribute__((always_inline)) { return lds + S * T::kW + stage * T::kX; };
+  auto scales_of = [&](int stage) __attribute__((always_inline)) { return lds + S * (T::kW + T::kX) + stage * T::kS; };
+  auto load_w = [&](const Walk& c, int j, int stage) __attribute__((always_inline)) {
+    load_rows(c.w, c.w_span, c.left, w_at[j], wave * T::JN + j, w_of(stage));
   };
-  auto load_x = [&](const Walk& c, int j, int stage) {  // the last one brings the tokens' scales
+  auto load_x = [&](const Walk& c, int j, int stage) __attribute__((always_inline)) {  // the last one brings the tokens' scales
     if (j < T::JM)
-      load_rows(c, x_at[j], wave * T::JM + j, lds + 2 * T::kW + stage * T::kX);
+      load_rows(c.x, c.x_span, c.left, x_at[j], wave * T::JM + j, x_of(stage));
     else
-      dma4(c.scales, c.t < last ? c.scale_span : 0u, xs_at, lds + 2 * (T::kW + T::kX) + stage * T::kS + wave * 256);
+      dma4(c.xs, c.xs_span, xs_at, scales_of(stage) + wave * 256);
   };
 
   const int r = lane & 31, g = lane >> 5;
@@ -271,35 +279,43 @@ __global__ __launch_bounds__(64 * WN * WM) void tile_kernel(Linear p) {
 #pragma unroll
       for (int e = 0; e < 16; ++e) acc[i][j][e] = 0.f;
 
-  // The weights' loads run one step ahead, the tokens' nearly two: their
-  // fragments are all in registers after a wave's first products, and a second
-  // barrier there frees their place for the step after the next.
+  // Loads run S - 1 steps ahead.  Of the two stages that the largest tile has
+  // room for, the tokens' is free again after a wave's first products, when
+  // their fragments are all in registers: a second barrier there lets the
+  // tokens' loads run nearly two steps ahead.
   int stage = 0;
   bool stored = false;
-  Walk ahead_w{first}, ahead_x{first};
-  enter_w(ahead_w);
-  enter_x(ahead_x);
+  Walk now = enter(first), ahead = now, ahead_x = now;  // ahead_x: the tokens' own place where S is 2
+  auto next = [&](Walk& c) __attribute__((always_inline)) {
+    step(c);
+    turn(c);
+  };
 #pragma unroll
-  for (int i = 0; i < T::JN; ++i) load_w(ahead_w, i, 0);
+  for (int i = 0; i < S - 1; ++i) {
 #pragma unroll
-  for (int i = 0; i <= T::JM; ++i) load_x(ahead_x, i, 0);
-  advance(ahead_x, p.xs_block, enter_x);
+    for (int j = 0; j < T::JN; ++j) load_w(ahead, j, i);
 #pragma unroll
-  for (int i = 0; i <= T::JM; ++i) load_x(ahead_x, i, 1);
+    for (int j = 0; j <= T::JM; ++j) load_x(ahead, j, i);
+    next(ahead);
+    next(ahead_x);
+  }
+  if (S == 2) {
+#pragma unroll
+    for (int j = 0; j <= T::JM; ++j) load_x(ahead_x, j, 1);
+    next(ahead_x);
+  }
+  float sw = *(const_float*)now.ws;
   while (true) {
-    // all but the next step's JM + 1 loads of tokens, and what the last tile stored behind them, have landed
-    if (stored) wait_loads<T::JM + 1 + T::kStores>(); else wait_loads<T::JM + 1>();
+    // all but the newer loads, and what the last tile stored behind them, have landed
+    if (stored) wait_loads<T::kAhead + T::kStores>(); else wait_loads<T::kAhead>();
     stored = false;
     lds_barrier();
-    const int t = ahead_w.t;
-    const bool ends = ahead_w.left <= kFp8Block;
-    const float sw = *(const_float*)ahead_w.scales;
-    advance(ahead_w, p.ws_block, enter_w);
-    advance(ahead_x, p.xs_block, enter_x);
-    uint8_t* w_lds = lds + stage * T::kW;
-    uint8_t* x_lds = lds + 2 * T::kW + stage * T::kX;
+    const bool ends = now.left <= kFp8Block;
+    const int into = stage == 0 ? S - 1 : stage - 1;  // the stage that the last step has left
+    uint8_t* w_lds = w_of(stage);
+    uint8_t* x_lds = x_of(stage);
     if (ends && (p.K & 15)) {  // bytes past K inside the last 16 of each row
-      const int left = p.K & 15, in = (p.K & (kFp8Block - 1)) >> 4;
+      const int K = here_s(p.K), left = K & 15, in = (K & (kFp8Block - 1)) >> 4;
       for (int row = threadIdx.x; row < T::kRows; row += T::kThreads) {
         uint8_t* of = row < T::BN ? w_lds + row * kFp8Block : x_lds + (row - T::BN) * kFp8Block;
         i32x4* v = reinterpret_cast<i32x4*>(of + 16 * (in ^ (row >> 1 & 7)));
@@ -307,7 +323,7 @@ __global__ __launch_bounds__(64 * WN * WM) void tile_kernel(Linear p) {
       }
       lds_barrier();
     }
-    auto frag = [&](const uint8_t* base, int row, int half) {  // lanes (r, g): row r, bytes 64 half + 32 g .. + 31
+    auto frag = [&](const uint8_t* base, int row, int half) __attribute__((always_inline)) {  // lanes (r, g): row r, bytes 64 half + 32 g .. + 31
       const uint8_t* of = base + (row + r) * kFp8Block;
       const int c = 4 * half + 2 * g;
       return join(*reinterpret_cast<const i32x4*>(of + 16 * (c ^ (r >> 1 & 7))),
@@ -320,14 +336,30 @@ __global__ __launch_bounds__(64 * WN * WM) void tile_kernel(Linear p) {
       const int row = (wm * FM + j) * 32;
       bx[j][0] = frag(x_lds, row, 0);
       bx[j][1] = frag(x_lds, row, 1);
-      s[j] = *reinterpret_cast<const float*>(lds + 2 * (T::kW + T::kX) + stage * T::kS +
-                                             (row + r) / T::kScales * 256 + (row + r) % T::kScales * 4) * sw;
+      s[j] = *reinterpret_cast<const float*>(scales_of(stage) + (row + r) / T::kScales * 256 + (row + r) % T::kScales * 4);
     }
     // One fragment and one product ahead: the next columns' fragments are read
     // and the next product runs while the last one's is scaled and added.
-    auto promote = [&](const f32x16& d, int i, int j, int half) {
+    auto promote = [&](const f32x16& d, int i, int j, int half) __attribute__((always_inline)) {
 #pragma unroll
       for (int e = half; e < half + 8; ++e) acc[i][j][e] = fmaf(d[e], s[j], acc[i][j][e]);
+    };
+    // The loads go between the products: issued all at once they fill the queue, and every wave waits behind it.
+    auto load_between = [&](int product) __attribute__((always_inline)) {
+      if (S == 2) {  // weights beside the first column fragment, tokens behind the second barrier
+        constexpr int kLater = (FN - 1) * FM;
+        if (product < FM) {
+          for (int k = product * T::JN / FM; k < (product + 1) * T::JN / FM; ++k) load_w(ahead, k, into);
+        } else {
+          for (int k = (product - FM) * (T::JM + 1) / kLater; k < (product - FM + 1) * (T::JM + 1) / kLater; ++k)
+            load_x(ahead_x, k, stage);
+        }
+      } else {
+        constexpr int kAll = T::JN + T::JM + 1;
+        for (int k = product * kAll / (FN * FM); k < (product + 1) * kAll / (FN * FM); ++k) {
+          if (k < T::JN) load_w(ahead, k, into); else load_x(ahead, k - T::JN, into);
+        }
+      }
     };
     i32x8 a[2][2];
     f32x16 d[2];
@@ -335,31 +367,28 @@ __global__ __launch_bounds__(64 * WN * WM) void tile_kernel(Linear p) {
     a[0][1] = frag(w_lds, wn * FN * 32, 1);
 #pragma unroll
     for (int i = 0; i < FN; ++i) {
-      if (i == 1) lds_barrier();  // every wave holds its tokens' fragments
+      if (S == 2 && i == 1) lds_barrier();  // every wave holds its tokens' fragments
       if (i + 1 < FN) {
         a[(i + 1) & 1][0] = frag(w_lds, (wn * FN + i + 1) * 32, 0);
         a[(i + 1) & 1][1] = frag(w_lds, (wn * FN + i + 1) * 32, 1);
       }
-      // between the products: loads issued all at once fill the queue, and every wave waits behind it
-      if (i == 0) {
-#pragma unroll
-        for (int piece = 0; piece < T::JN; ++piece) load_w(ahead_w, piece, stage ^ 1);
-      } else {
-        constexpr int kPer = (T::JM + 1 + FN - 2) / (FN - 1);
-#pragma unroll
-        for (int piece = (i - 1) * kPer; piece < min(i * kPer, T::JM + 1); ++piece) load_x(ahead_x, piece, stage);
-      }
 #pragma unroll
       for (int j = 0; j < FM; ++j) {
-        const int now = i * FM + j;
+        const int at = i * FM + j;
         f32x16 zero = {};
-        d[now & 1] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(a[i & 1][0], bx[j][0], zero, 0, 0, 0, 0, 0, 0);
+        d[at & 1] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(a[i & 1][0], bx[j][0], zero, 0, 0, 0, 0, 0, 0);
         __builtin_amdgcn_sched_barrier(0);
-        if (now > 0) promote(d[(now - 1) & 1], (now - 1) / FM, (now - 1) % FM, 0);
+        if (at == 0) {  // the scales are needed from here on; the next block's weight scale starts on its way
+#pragma unroll
+          for (int k = 0; k < FM; ++k) s[k] *= sw;
+          sw = *(const_float*)(now.ws + (ends ? 0 : p.ws_block));
+        }
+        load_between(at);
+        if (at > 0) promote(d[(at - 1) & 1], (at - 1) / FM, (at - 1) % FM, 0);
         __builtin_amdgcn_sched_barrier(0);
-        d[now & 1] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(a[i & 1][1], bx[j][1], d[now & 1], 0, 0, 0, 0, 0, 0);
+        d[at & 1] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(a[i & 1][1], bx[j][1], d[at & 1], 0, 0, 0, 0, 0, 0);
         __builtin_amdgcn_sched_barrier(0);
-        if (now > 0) promote(d[(now - 1) & 1], (now - 1) / FM, (now - 1) % FM, 8);
+        if (at > 0) promote(d[(at - 1) & 1], (at - 1) / FM, (at - 1) % FM, 8);
         __builtin_amdgcn_sched_barrier(0);
       }
     }
@@ -372,13 +401,15 @@ __global__ __launch_bounds__(64 * WN * WM) void tile_kernel(Linear p) {
       // 128 bytes (stored as they lie, in pieces of 32 bytes, the last product of
       // 16384 x 12288 x 2048 took 437 us, without any stores 361).
       int m0, n0;
-      corner(t, m0, n0);
-      const bool wide = p.wide_out && (p.N % 8 == 0 || n0 + T::BN <= p.N);
-      const int rows = min(T::BM, p.M - m0);
+      corner(now.t, m0, n0);
+      const int below = here_s(p.M) - m0, beside = here_s(p.N) - n0, stride = here_s(p.out_stride);
+      const int rows = below < T::BM ? below : T::BM;
+      const bool wide = here_s(p.wide_out) && (beside % 8 == 0 || beside >= T::BN);
       const int l = here(lane), r = l & 31, g = l >> 5;
-      uint8_t* mine = lds + 2 * (T::kW + T::kX + T::kS) + wave * T::kOut;
-      OUT* tile = static_cast<OUT*>(p.out) + static_cast<int64_t>(m0) * p.out_stride + n0;
-      const auto rsrc = rsrc_of(tile, (static_cast<uint32_t>(rows - 1) * p.out_stride + min(T::BN, p.N - n0)) * 2u);
+      lds_barrier();  // nobody reads this step's weights any more, and no load goes there before the next barrier
+      uint8_t* mine = w_lds + wave * T::kOut;
+      OUT* tile = static_cast<OUT*>(p.out) + static_cast<int64_t>(m0) * stride + n0;
+      const auto rsrc = rsrc_of(tile, (static_cast<uint32_t>(rows - 1) * stride + (beside < T::BN ? beside : T::BN)) * 2u);
 #pragma unroll
       for (int i = 0; i < FN; i += 2)
 #pragma unroll
@@ -413,12 +444,11 @@ __global__ __launch_bounds__(64 * WN * WM) void tile_kernel(Linear p) {
               const i32x4 out = *reinterpret_cast<const i32x4*>(mine + row * 128 + 16 * (c ^ (row >> 1 & 7)));
               const int m = (wm * FM + j) * 32 + 16 * half + row, n = (wn * FN + i) * 32 + 8 * c;
               if (wide) {  // always kStores stores: rows and columns that are not there fall out of range
-                const bool there = m < rows && n0 + n < p.N;
+                const bool there = m < rows && n < beside;
                 __builtin_amdgcn_raw_buffer_store_b128(
-                    out, rsrc, there ? (static_cast<uint32_t>(m) * p.out_stride + n) * 2u : 0xffffff00u, 0, 0);
+                    out, rsrc, there ? (static_cast<uint32_t>(m) * stride + n) * 2u : 0xffffff00u, 0, 0);
               } else if (m < rows) {
-                store_any(reinterpret_cast<uint16_t*>(tile) + static_cast<int64_t>(m) * p.out_stride + n, out,
-                          p.N - n0 - n);
+                store_any(reinterpret_cast<uint16_t*>(tile) + static_cast<int64_t>(m) * stride + n, out, beside - n);
               }
             }
             wave_fence();
@@ -428,8 +458,17 @@ __global__ __launch_bounds__(64 * WN * WM) void tile_kernel(Linear p) {
         }
       stored = wide;
     }
-    if (ahead_w.t >= last) break;
-    stage ^= 1;
+    step(now);
+    step(ahead);
+    step(ahead_x);
+    if (min(now.left, min(ahead.left, S == 2 ? ahead_x.left : 1)) <= 0) {
+      turn(now);
+      if (now.t >= last) break;
+      turn(ahead);
+      turn(ahead_x);
+      if (ends) sw = *(const_float*)now.ws;
+    }
+    stage = stage + 1 == S ? 0 : stage + 1;
   }
   wait_loads<0>();  // no load may land in LDS that is somebody else's by then
 }
@@ -448,23 +487,23 @@ int launch_linear(Linear p, hipStream_t s) {
     else go(std::integral_constant<int, 4>{});
     return GDN_LAUNCH_CHECK("gdn_fp8_linear launch");
   }
-  auto go = [&](auto WNc, auto WMc, auto FNc, auto FMc) -> int {
+  auto go = [&](auto WNc, auto WMc, auto FNc, auto FMc, auto Sc) -> int {
     constexpr int WN = decltype(WNc)::value, WM = decltype(WMc)::value, FN = decltype(FNc)::value,
-                  FM = decltype(FMc)::value;
-    using T = Tile<WN, WM, FN, FM>;
+                  FM = decltype(FMc)::value, S = decltype(Sc)::value;
+    using T = Tile<WN, WM, FN, FM, S>;
     p.tiles_m = (p.M + T::BM - 1) / T::BM;
     p.tiles_n = (p.N + T::BN - 1) / T::BN;
     const int64_t tiles = static_cast<int64_t>(p.tiles_m) * p.tiles_n;
     GDN_REQUIRE(tiles <= 0x7fffffff / 8, "gdn_fp8_linear: too many tiles");
     constexpr int kPerCu = (160 * 1024) / T::kLds;
     const int grid = static_cast<int>(tiles < 256 * kPerCu ? (tiles + 7) / 8 * 8 : 256 * kPerCu);
-    hipLaunchKernelGGL((tile_kernel<OUT, WN, WM, FN, FM>), dim3(grid), dim3(T::kThreads), 0, s, p);
+    hipLaunchKernelGGL((tile_kernel<OUT, WN, WM, FN, FM, S>), dim3(grid), dim3(T::kThreads), 0, s, p);
     return GDN_LAUNCH_CHECK("gdn_fp8_linear launch");
   };
 #define GDN_INT(v) std::integral_constant<int, v>{}
   const int64_t big = static_cast<int64_t>((p.M + 255) / 256) * ((p.N + 255) / 256);
-  if (big >= 256) return go(GDN_INT(2), GDN_INT(4), GDN_INT(4), GDN_INT(2));
-  return go(GDN_INT(2), GDN_INT(2), GDN_INT(2), GDN_INT(2));
+  if (big >= 256) return go(GDN_INT(2), GDN_INT(4), GDN_INT(4), GDN_INT(2), GDN_INT(2));
+  return go(GDN_INT(2), GDN_INT(2), GDN_INT(2), GDN_INT(2), GDN_INT(2));
 #undef GDN_INT
 }
 
