@@ -70,8 +70,7 @@ __device__ __forceinline__ void store_any(uint16_t* to, i32x4 v, int columns) {
       if (e < columns) to[e] = static_cast<uint16_t>(static_cast<uint32_t>(v[e / 2]) >> (16 * (e & 1)));
   }
 }
-// 16 bytes of a row from column k on, zeros from K on (K tails of the last
-// block alone; the row is readable up to the next multiple of 16).
+// The first `left` of 16 bytes, zeros behind them.
 __device__ __forceinline__ i32x4 mask_tail(i32x4 v, int left) {
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
@@ -80,75 +79,143 @@ __device__ __forceinline__ i32x4 mask_tail(i32x4 v, int left) {
   }
   return v;
 }
-__device__ __forceinline__ i32x4 load_tail(const uint8_t* row, int k, int K) {
-  const int left = K - k;
-  if (left <= 0) return i32x4{0, 0, 0, 0};
-  return mask_tail(*reinterpret_cast<const i32x4*>(row + k), left);
-}
+
+template <int N> __device__ __forceinline__ void wait_loads() { asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory"); }
+// LDS traffic between the lanes of one wave: in order in hardware, so only the compiler has to be told.
+__device__ __forceinline__ void wave_fence() { asm volatile("" ::: "memory"); }
+__device__ __forceinline__ void lds_barrier() { asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory"); }
 
 // ------------------------------------------------------------------ few rows
-// Few tokens: the weights' bytes bound the call.  A block owns 16 columns of
-// the output for 16 MT tokens; its waves split K block by block, load both
-// operands straight into registers and join their sums through LDS in the
-// order of the waves.
-constexpr int kFewWaves = 8;
+// Few tokens, or few tiles: what bounds the call is how fast its bytes come in,
+// not the matrix cores.  A block owns 16 NT columns of the output for 16 MT
+// tokens.  Its W waves split K block by block, each with S stages of LDS of its
+// own, so that no barrier stands between their loads, and join their sums
+// through LDS in the order of the waves.  (Loaded straight into the registers
+// of the matrix instructions, 16 lanes would touch 16 rows at a time: 512 x
+// 2048 x 4096 took 36 us.)  Blocks with the same index modulo 8 share an XCD
+// and its L2: they are the token tiles of the same columns.
+template <int MT, int NT, int W, int S>
+struct Few {
+  static constexpr int kStage = (NT + MT) * 16 * kFp8Block + 256;  // operands, then the tokens' scales
+  static constexpr int kStages = W * S * kStage, kSums = W * MT * NT * 1024;
+  static constexpr int kLds = kStages > kSums ? kStages : kSums;
+  static constexpr int kLoads = 2 * (NT + MT) + 1;  // per step
+  static_assert(kLds <= 160 * 1024 && (S - 1) * kLoads < 64 && MT <= 4, "fits");
+};
 
-template <class OUT, int MT>
-__global__ __launch_bounds__(64 * kFewWaves) void few_rows_kernel(Linear p) {
-  __shared__ float part[kFewWaves][MT][64][4];
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+template <class OUT, int MT, int NT, int W, int S>
+__global__ __launch_bounds__(64 * W, 2) void few_rows_kernel(Linear p) {
+  using F = Few<MT, NT, W, S>;
+  __shared__ __align__(16) uint8_t lds[F::kLds];
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int in = blockIdx.x >> 3;
+  const int n0 = (in / p.tiles_m * 8 + (blockIdx.x & 7)) * 16 * NT, m0 = in % p.tiles_m * 16 * MT;
+  if (n0 >= p.N) return;  // whole block
+  const int blocks = (p.K + kFp8Block - 1) / kFp8Block, padded = (p.K + 15) & ~15;
+  const int rows_n = min(16 * NT, p.N - n0), rows_m = min(16 * MT, p.M - m0);
+  uint8_t* mine = lds + wave * S * F::kStage;
+  const uint8_t* w = p.w + static_cast<int64_t>(n0) * p.w_stride;
+  const uint8_t* x = p.x + static_cast<int64_t>(m0) * p.x_stride;
+  const float* xs = p.xs + static_cast<int64_t>(m0) * p.xs_row;
+  const float* ws = p.ws + n0 / kFp8Block * p.ws_row;
+  const int ws_next = (n0 / kFp8Block + 1) * kFp8Block - n0;  // columns before the next row of weight scales
+  const bool ws_more = n0 / kFp8Block < (p.N - 1) / kFp8Block;
+
+  // A load brings 8 rows, chunk c of row r to c ^ (r / 2 % 8) (the tile kernel says why).
+  const int chunk = (lane & 7) ^ (lane >> 4);
+  uint32_t w_at[2 * NT], x_at[2 * MT];
+#pragma unroll
+  for (int j = 0; j < 2 * NT; ++j) w_at[j] = static_cast<uint32_t>((8 * j + (lane >> 3)) * p.w_stride) + 16 * (chunk ^ (4 * (j & 1)));
+#pragma unroll
+  for (int j = 0; j < 2 * MT; ++j) x_at[j] = static_cast<uint32_t>((8 * j + (lane >> 3)) * p.x_stride) + 16 * (chunk ^ (4 * (j & 1)));
+  const uint32_t xs_at = lane < 16 * MT ? static_cast<uint32_t>(lane * p.xs_row * 4) : 0xffffff00u;
+  auto load = [&](int b, int stage) __attribute__((always_inline)) {  // past the last block: counted, but nothing in range
+    const int width = b < blocks ? min(kFp8Block, padded - b * kFp8Block) : 0;
+    const uint32_t w_bytes = width ? static_cast<uint32_t>((rows_n - 1) * p.w_stride + width) : 0u;
+    const uint32_t x_bytes = width ? static_cast<uint32_t>((rows_m - 1) * p.x_stride + width) : 0u;
+    uint8_t* to = mine + stage * F::kStage;
+    const bool past[2] = {16 * chunk >= width, 16 * (chunk ^ 4) >= width};
+#pragma unroll
+    for (int j = 0; j < 2 * NT; ++j) dma16(w + b * kFp8Block, w_bytes, past[j & 1] ? 0xffffff00u : w_at[j], to + j * 1024);
+#pragma unroll
+    for (int j = 0; j < 2 * MT; ++j)
+      dma16(x + b * kFp8Block, x_bytes, past[j & 1] ? 0xffffff00u : x_at[j], to + (2 * NT + j) * 1024);
+    dma4(xs + b * p.xs_block, width ? static_cast<uint32_t>(((rows_m - 1) * p.xs_row + 1) * 4) : 0u, xs_at,
+         to + (NT + MT) * 2048);
+  };
+
   const int r = lane & 15, g = lane >> 4;
-  const int n0 = blockIdx.x * 16, m0 = blockIdx.y * 16 * MT;
-  const uint8_t* w = p.w + static_cast<int64_t>(min(n0 + r, p.N - 1)) * p.w_stride;
-  const uint8_t* x[MT];
-  const float* xs[MT];
+  f32x4 acc[NT][MT];
 #pragma unroll
-  for (int t = 0; t < MT; ++t) {
-    const int64_t m = min(m0 + 16 * t + r, p.M - 1);
-    x[t] = p.x + m * p.x_stride;
-    xs[t] = p.xs + m * p.xs_row;
-  }
-  const float* ws = p.ws + (n0 / kFp8Block) * p.ws_row;
-  const int blocks = (p.K + kFp8Block - 1) / kFp8Block;
-  f32x4 acc[MT];
+  for (int i = 0; i < NT; ++i)
 #pragma unroll
-  for (int t = 0; t < MT; ++t) acc[t] = f32x4{0.f, 0.f, 0.f, 0.f};
-  for (int b = wave; b < blocks; b += kFewWaves) {
-    const int k = b * kFp8Block + 16 * g;
-    const bool whole = (b + 1) * kFp8Block <= p.K;
-    auto frag = [&](const uint8_t* row) {
-      if (whole)
-        return join(*reinterpret_cast<const i32x4*>(row + k), *reinterpret_cast<const i32x4*>(row + k + 64));
-      return join(load_tail(row, k, p.K), load_tail(row, k + 64, p.K));
+    for (int j = 0; j < MT; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+  for (int i = 0; i < S - 1; ++i) load(wave + i * W, i);
+  int stage = 0;
+  for (int b = wave; b < blocks; b += W) {
+    load(b + (S - 1) * W, stage == 0 ? S - 1 : stage - 1);
+    const float scale[2] = {*(const_float*)(ws + b * p.ws_block),
+                            *(const_float*)(ws + (ws_more ? p.ws_row : 0) + b * p.ws_block)};
+    wait_loads<(S - 1) * F::kLoads>();
+    const uint8_t* from = mine + stage * F::kStage;
+    const bool tail = (p.K & 15) && b + 1 == blocks;
+    auto frag = [&](int row) __attribute__((always_inline)) {  // lanes (r, g): row r, bytes 32 g .. + 31
+      const uint8_t* of = from + (row + r) * kFp8Block;
+      i32x4 lo = *reinterpret_cast<const i32x4*>(of + 16 * ((2 * g) ^ (r >> 1)));
+      i32x4 hi = *reinterpret_cast<const i32x4*>(of + 16 * ((2 * g + 1) ^ (r >> 1)));
+      if (tail) {  // bytes past K inside the last 16
+        const int left = p.K - b * kFp8Block - 32 * g;
+        lo = mask_tail(lo, left), hi = mask_tail(hi, left - 16);
+      }
+      return join(lo, hi);
     };
-    const i32x8 a = frag(w);
-    const float sw = ws[b * p.ws_block];
+    i32x8 bx[MT];
+    float sx[MT];
 #pragma unroll
-    for (int t = 0; t < MT; ++t) {
-      const i32x8 bx = frag(x[t]);
-      const float s = xs[t][b * p.xs_block] * sw;
-      const f32x4 d = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(a, bx, f32x4{0.f, 0.f, 0.f, 0.f}, 0, 0, 0, 0, 0, 0);
-#pragma unroll
-      for (int j = 0; j < 4; ++j) acc[t][j] = fmaf(d[j], s, acc[t][j]);
+    for (int j = 0; j < MT; ++j) {
+      bx[j] = frag(16 * (NT + j));
+      sx[j] = *reinterpret_cast<const float*>(from + (NT + MT) * 2048 + 4 * (16 * j + r));
     }
-  }
 #pragma unroll
-  for (int t = 0; t < MT; ++t) *reinterpret_cast<f32x4*>(part[wave][t][lane]) = acc[t];
-  __syncthreads();
-  // wave t joins token tile t: lane (r, g) holds columns n0 + 4 g .. + 3 of token m0 + 16 t + r
-  for (int t = wave; t < MT; t += kFewWaves) {
+    for (int i = 0; i < NT; ++i) {
+      const i32x8 a = frag(16 * i);
+      const float sw = 16 * i < ws_next ? scale[0] : scale[1];
+#pragma unroll
+      for (int j = 0; j < MT; ++j) {
+        const f32x4 zero = {0.f, 0.f, 0.f, 0.f};
+        const f32x4 d = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(a, bx[j], zero, 0, 0, 0, 0, 0, 0);
+        const float s = sx[j] * sw;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) acc[i][j][e] = fmaf(d[e], s, acc[i][j][e]);
+      }
+    }
+    // the fragments are in registers before a load may overwrite their place
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+    stage = stage + 1 == S ? 0 : stage + 1;
+  }
+  wait_loads<0>();  // those past the last block too
+  lds_barrier();    // the stages are free
+#pragma unroll
+  for (int i = 0; i < NT; ++i)
+#pragma unroll
+    for (int j = 0; j < MT; ++j)
+      *reinterpret_cast<f32x4*>(lds + ((wave * NT + i) * MT + j) * 1024 + 16 * lane) = acc[i][j];
+  lds_barrier();
+  // lane (r, g) of a 16 x 16 piece holds columns 4 g .. + 3 of token r
+  for (int t = wave; t < NT * MT; t += W) {
     f32x4 sum = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-    for (int i = 0; i < kFewWaves; ++i) sum += *reinterpret_cast<const f32x4*>(part[i][t][lane]);
-    const int m = m0 + 16 * t + r, n = n0 + 4 * g;
+    for (int i = 0; i < W; ++i) sum += *reinterpret_cast<const f32x4*>(lds + (i * NT * MT + t) * 1024 + 16 * lane);
+    const int m = m0 + 16 * (t % MT) + r, n = n0 + 16 * (t / MT) + 4 * g;
     if (m >= p.M) continue;
     OUT* out = static_cast<OUT*>(p.out) + static_cast<int64_t>(m) * p.out_stride + n;
     if (p.wide_out && n + 4 <= p.N) {
       *reinterpret_cast<uint2*>(out) = make_uint2(out_pack2<OUT>(sum[0], sum[1]), out_pack2<OUT>(sum[2], sum[3]));
     } else {
 #pragma unroll
-      for (int j = 0; j < 4; ++j)
-        if (n + j < p.N) out[j] = from_f32<OUT>(sum[j]);
+      for (int e = 0; e < 4; ++e)
+        if (n + e < p.N) out[e] = from_f32<OUT>(sum[e]);
     }
   }
 }
@@ -177,11 +244,6 @@ struct Tile {
   static_assert(JN * 8 * kWaves == BN && JM * 8 * kWaves == BM && kScales <= 64, "whole loads per wave");
   static_assert(kFp8Block % (32 * FN) == 0 && FN % 2 == 0, "one row of weight scales per wave");
 };
-
-template <int N> __device__ __forceinline__ void wait_loads() { asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory"); }
-// LDS traffic between the lanes of one wave: in order in hardware, so only the compiler has to be told.
-__device__ __forceinline__ void wave_fence() { asm volatile("" ::: "memory"); }
-__device__ __forceinline__ void lds_barrier() { asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory"); }
 
 template <class OUT, int WN, int WM, int FN, int FM, int S>
 __global__ __launch_bounds__(64 * WN * WM, 2) void tile_kernel(Linear p) {
@@ -475,17 +537,20 @@ __global__ __launch_bounds__(64 * WN * WM, 2) void tile_kernel(Linear p) {
 
 template <class OUT>
 int launch_linear(Linear p, hipStream_t s) {
-  if (p.M <= 64) {
-    const dim3 threads(64 * kFewWaves);
-    auto go = [&](auto MTc) {
-      constexpr int MT = decltype(MTc)::value;
-      hipLaunchKernelGGL((few_rows_kernel<OUT, MT>), dim3((p.N + 15) / 16, (p.M + 16 * MT - 1) / (16 * MT)), threads, 0,
-                         s, p);
-    };
-    if (p.M <= 16) go(std::integral_constant<int, 1>{});
-    else if (p.M <= 32) go(std::integral_constant<int, 2>{});
-    else go(std::integral_constant<int, 4>{});
+#define GDN_INT(v) std::integral_constant<int, v>{}
+  auto few = [&](auto MTc, auto NTc, auto Wc, auto Sc) -> int {
+    constexpr int MT = decltype(MTc)::value, NT = decltype(NTc)::value, W = decltype(Wc)::value, S = decltype(Sc)::value;
+    p.tiles_m = (p.M + 16 * MT - 1) / (16 * MT);
+    p.tiles_n = (p.N + 16 * NT - 1) / (16 * NT);
+    const int64_t grid = static_cast<int64_t>((p.tiles_n + 7) / 8 * 8) * p.tiles_m;
+    GDN_REQUIRE(grid <= 0xffffffffll / (64 * W), "gdn_fp8_linear: too many tiles");
+    hipLaunchKernelGGL((few_rows_kernel<OUT, MT, NT, W, S>), dim3(static_cast<unsigned>(grid)), dim3(64 * W), 0, s, p);
     return GDN_LAUNCH_CHECK("gdn_fp8_linear launch");
+  };
+  if (p.M <= 64) {
+    if (p.M <= 16) return few(GDN_INT(1), GDN_INT(1), GDN_INT(8), GDN_INT(2));
+    if (p.M <= 32) return few(GDN_INT(2), GDN_INT(2), GDN_INT(8), GDN_INT(2));
+    return few(GDN_INT(4), GDN_INT(2), GDN_INT(4), GDN_INT(3));
   }
   auto go = [&](auto WNc, auto WMc, auto FNc, auto FMc, auto Sc) -> int {
     constexpr int WN = decltype(WNc)::value, WM = decltype(WMc)::value, FN = decltype(FNc)::value,
@@ -500,7 +565,6 @@ int launch_linear(Linear p, hipStream_t s) {
     hipLaunchKernelGGL((tile_kernel<OUT, WN, WM, FN, FM, S>), dim3(grid), dim3(T::kThreads), 0, s, p);
     return GDN_LAUNCH_CHECK("gdn_fp8_linear launch");
   };
-#define GDN_INT(v) std::integral_constant<int, v>{}
   const int64_t big = static_cast<int64_t>((p.M + 255) / 256) * ((p.N + 255) / 256);
   if (big >= 256) return go(GDN_INT(2), GDN_INT(4), GDN_INT(4), GDN_INT(2), GDN_INT(2));
   return go(GDN_INT(2), GDN_INT(2), GDN_INT(2), GDN_INT(2), GDN_INT(2));
