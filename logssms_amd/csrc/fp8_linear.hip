@@ -238,9 +238,9 @@ struct Tile {
   static constexpr int JN = BN / 8 / kWaves, JM = BM / 8 / kWaves, kScales = BM / kWaves;  // loads and scales per wave
   static constexpr int kStores = 2 * FN * FM;
   static constexpr int kOut = 2048;  // per wave: 16 tokens of 64 columns on their way out, in place of a step's weights
-  // loads that are newer than a step's own when it begins
-  static constexpr int kAhead = S == 2 ? JM + 1 : (S - 2) * (JN + JM + 1);
-  static_assert(kOut * kWaves <= kW && kLds <= 160 * 1024 && kAhead + kStores < 64, "fits");
+  // loads that are newer than those that have to be there when a step begins
+  static constexpr int kAhead = S == 2 ? JM + 1 : (S - 3) * (JN + JM + 1);
+  static_assert(kOut * kWaves <= kW && kLds <= 160 * 1024 && kAhead + kStores < 64 && S != 3, "fits");
   static_assert(JN * 8 * kWaves == BN && JM * 8 * kWaves == BM && kScales <= 64, "whole loads per wave");
   static_assert(kFp8Block % (32 * FN) == 0 && FN % 2 == 0, "one row of weight scales per wave");
 };
@@ -341,10 +341,14 @@ __global__ __launch_bounds__(64 * WN * WM, 2) void tile_kernel(Linear p) {
 #pragma unroll
       for (int e = 0; e < 16; ++e) acc[i][j][e] = 0.f;
 
-  // Loads run S - 1 steps ahead.  Of the two stages that the largest tile has
-  // room for, the tokens' is free again after a wave's first products, when
-  // their fragments are all in registers: a second barrier there lets the
-  // tokens' loads run nearly two steps ahead.
+  // Loads run S - 1 steps ahead.  Where there are four stages or more, the next
+  // step's operands have landed by the time a step begins: their first fragments
+  // are read behind the step's last products, whose scaling is left to the next
+  // step, so that the matrix cores do not wait at the barrier between them.  Of
+  // the two stages that the largest tile has room for, the tokens' is free again
+  // after a wave's first products, when their fragments are all in registers: a
+  // second barrier there lets the tokens' loads run nearly two steps ahead.
+  constexpr bool kDeep = S > 2;
   int stage = 0;
   bool stored = false;
   Walk now = enter(first), ahead = now, ahead_x = now;  // ahead_x: the tokens' own place where S is 2
@@ -367,45 +371,69 @@ __global__ __launch_bounds__(64 * WN * WM, 2) void tile_kernel(Linear p) {
     next(ahead_x);
   }
   float sw = *(const_float*)now.ws;
-  while (true) {
-    // all but the newer loads, and what the last tile stored behind them, have landed
-    if (stored) wait_loads<T::kAhead + T::kStores>(); else wait_loads<T::kAhead>();
-    stored = false;
+  i32x8 bx[FM][2], a[2][2];
+  f32x16 d[2];
+  float s[FM], sx[FM], s_last = 0.f;  // s_last: of the product whose scaling is left
+  auto frag = [&](const uint8_t* base, int row, int half) __attribute__((always_inline)) {
+    // lanes (r, g): row r, bytes 64 half + 32 g .. + 31
+    const uint8_t* of = base + (row + r) * kFp8Block;
+    const int c = 4 * half + 2 * g;
+    return join(*reinterpret_cast<const i32x4*>(of + 16 * (c ^ (r >> 1 & 7))),
+                *reinterpret_cast<const i32x4*>(of + 16 * ((c + 1) ^ (r >> 1 & 7))));
+  };
+  auto read_x = [&](int stage, int j) __attribute__((always_inline)) {
+    const int row = (wm * FM + j) * 32;
+    bx[j][0] = frag(x_of(stage), row, 0);
+    bx[j][1] = frag(x_of(stage), row, 1);
+    sx[j] = *reinterpret_cast<const float*>(scales_of(stage) + (row + r) / T::kScales * 256 + (row + r) % T::kScales * 4);
+  };
+  auto read_w = [&](int stage, int i, int to) __attribute__((always_inline)) {
+    a[to][0] = frag(w_of(stage), (wn * FN + i) * 32, 0);
+    a[to][1] = frag(w_of(stage), (wn * FN + i) * 32, 1);
+  };
+  auto patch = [&](int stage) __attribute__((always_inline)) {  // bytes past K inside the last 16 of each row
+    const int K = here_s(p.K), left = K & 15, in = (K & (kFp8Block - 1)) >> 4;
+    for (int row = threadIdx.x; row < T::kRows; row += T::kThreads) {
+      uint8_t* of = row < T::BN ? w_of(stage) + row * kFp8Block : x_of(stage) + (row - T::BN) * kFp8Block;
+      i32x4* v = reinterpret_cast<i32x4*>(of + 16 * (in ^ (row >> 1 & 7)));
+      *v = mask_tail(*v, left);
+    }
     lds_barrier();
-    const bool ends = now.left <= kFp8Block;
+  };
+  auto promote = [&](const f32x16& d, float s, int i, int j, int half) __attribute__((always_inline)) {
+#pragma unroll
+    for (int e = half; e < half + 8; ++e) acc[i][j][e] = fmaf(d[e], s, acc[i][j][e]);
+  };
+  constexpr int kLast = FN * FM - 1;
+  if (kDeep) {
+    wait_loads<T::kAhead + T::JN + T::JM + 1>();
+    lds_barrier();
+    if (padded <= kFp8Block && (p.K & 15)) patch(0);
+#pragma unroll
+    for (int j = 0; j < FM; ++j) read_x(0, j);
+    read_w(0, 0, 0);
+#pragma unroll
+    for (int e = 0; e < 16; ++e) d[kLast & 1][e] = 0.f;
+  }
+  // One step.  Plain: not a tile's last one nor the one before, and no place turns to another tile behind it.
+  auto one_step = [&](auto plainc) __attribute__((always_inline)) {
+    constexpr bool kPlain = decltype(plainc)::value;
+    // all but the newer loads, and what the last tile stored behind them, have landed
+    if (!kPlain && stored) wait_loads<T::kAhead + T::kStores>(); else wait_loads<T::kAhead>();
+    stored = false;
+    const bool ends = !kPlain && now.left <= kFp8Block;
     const int into = stage == 0 ? S - 1 : stage - 1;  // the stage that the last step has left
-    uint8_t* w_lds = w_of(stage);
-    uint8_t* x_lds = x_of(stage);
-    if (ends && (p.K & 15)) {  // bytes past K inside the last 16 of each row
-      const int K = here_s(p.K), left = K & 15, in = (K & (kFp8Block - 1)) >> 4;
-      for (int row = threadIdx.x; row < T::kRows; row += T::kThreads) {
-        uint8_t* of = row < T::BN ? w_lds + row * kFp8Block : x_lds + (row - T::BN) * kFp8Block;
-        i32x4* v = reinterpret_cast<i32x4*>(of + 16 * (in ^ (row >> 1 & 7)));
-        *v = mask_tail(*v, left);
-      }
+    const int after = stage + 1 == S ? 0 : stage + 1;
+    if (kDeep) {
+      asm volatile("s_barrier" ::: "memory");  // each wave's reads of the last stage were waited for by its products
+      if (!kPlain && (ends ? padded : now.left - kFp8Block) <= kFp8Block && (p.K & 15)) patch(after);
+    } else {
       lds_barrier();
-    }
-    auto frag = [&](const uint8_t* base, int row, int half) __attribute__((always_inline)) {  // lanes (r, g): row r, bytes 64 half + 32 g .. + 31
-      const uint8_t* of = base + (row + r) * kFp8Block;
-      const int c = 4 * half + 2 * g;
-      return join(*reinterpret_cast<const i32x4*>(of + 16 * (c ^ (r >> 1 & 7))),
-                  *reinterpret_cast<const i32x4*>(of + 16 * ((c + 1) ^ (r >> 1 & 7))));
-    };
-    i32x8 bx[FM][2];
-    float s[FM];
+      if (!kPlain && ends && (p.K & 15)) patch(stage);
 #pragma unroll
-    for (int j = 0; j < FM; ++j) {
-      const int row = (wm * FM + j) * 32;
-      bx[j][0] = frag(x_lds, row, 0);
-      bx[j][1] = frag(x_lds, row, 1);
-      s[j] = *reinterpret_cast<const float*>(scales_of(stage) + (row + r) / T::kScales * 256 + (row + r) % T::kScales * 4);
+      for (int j = 0; j < FM; ++j) read_x(stage, j);
+      read_w(stage, 0, 0);
     }
-    // One fragment and one product ahead: the next columns' fragments are read
-    // and the next product runs while the last one's is scaled and added.
-    auto promote = [&](const f32x16& d, int i, int j, int half) __attribute__((always_inline)) {
-#pragma unroll
-      for (int e = half; e < half + 8; ++e) acc[i][j][e] = fmaf(d[e], s[j], acc[i][j][e]);
-    };
     // The loads go between the products: issued all at once they fill the queue, and every wave waits behind it.
     auto load_between = [&](int product) __attribute__((always_inline)) {
       if (S == 2) {  // weights beside the first column fragment, tokens behind the second barrier
@@ -423,40 +451,39 @@ __global__ __launch_bounds__(64 * WN * WM, 2) void tile_kernel(Linear p) {
         }
       }
     };
-    i32x8 a[2][2];
-    f32x16 d[2];
-    a[0][0] = frag(w_lds, wn * FN * 32, 0);
-    a[0][1] = frag(w_lds, wn * FN * 32, 1);
 #pragma unroll
     for (int i = 0; i < FN; ++i) {
-      if (S == 2 && i == 1) lds_barrier();  // every wave holds its tokens' fragments
-      if (i + 1 < FN) {
-        a[(i + 1) & 1][0] = frag(w_lds, (wn * FN + i + 1) * 32, 0);
-        a[(i + 1) & 1][1] = frag(w_lds, (wn * FN + i + 1) * 32, 1);
-      }
+      if (!kDeep && i == 1) lds_barrier();  // every wave holds its tokens' fragments
+      if (i + 1 < FN) read_w(stage, i + 1, (i + 1) & 1);
+      else if (kDeep) read_w(after, 0, 0);
 #pragma unroll
       for (int j = 0; j < FM; ++j) {
         const int at = i * FM + j;
+        const int from = at > 0 ? at - 1 : kLast;  // the product to scale and add while this one runs
         f32x16 zero = {};
         d[at & 1] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(a[i & 1][0], bx[j][0], zero, 0, 0, 0, 0, 0, 0);
         __builtin_amdgcn_sched_barrier(0);
         if (at == 0) {  // the scales are needed from here on; the next block's weight scale starts on its way
 #pragma unroll
-          for (int k = 0; k < FM; ++k) s[k] *= sw;
+          for (int k = 0; k < FM; ++k) s[k] = sx[k] * sw;
           sw = *(const_float*)(now.ws + (ends ? 0 : p.ws_block));
         }
         load_between(at);
-        if (at > 0) promote(d[(at - 1) & 1], (at - 1) / FM, (at - 1) % FM, 0);
+        if (at > 0 || kDeep) promote(d[from & 1], at > 0 ? s[from % FM] : s_last, from / FM, from % FM, 0);
         __builtin_amdgcn_sched_barrier(0);
         d[at & 1] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(a[i & 1][1], bx[j][1], d[at & 1], 0, 0, 0, 0, 0, 0);
         __builtin_amdgcn_sched_barrier(0);
-        if (at > 0) promote(d[(at - 1) & 1], (at - 1) / FM, (at - 1) % FM, 8);
+        if (kDeep && i + 1 == FN) read_x(after, j);
+        if (at > 0 || kDeep) promote(d[from & 1], at > 0 ? s[from % FM] : s_last, from / FM, from % FM, 8);
         __builtin_amdgcn_sched_barrier(0);
       }
     }
-    promote(d[(FN * FM - 1) & 1], FN - 1, FM - 1, 0);
-    promote(d[(FN * FM - 1) & 1], FN - 1, FM - 1, 8);
-    if (ends) {
+    s_last = s[FM - 1];
+    if (!kDeep || (!kPlain && ends)) {
+      promote(d[kLast & 1], s_last, FN - 1, FM - 1, 0);
+      promote(d[kLast & 1], s_last, FN - 1, FM - 1, 8);
+    }
+    if (!kPlain && ends) {
       // Registers 4 q .. 4 q + 3 hold columns 8 q + 4 g .. + 3 of token r.  The
       // halves of the wave trade theirs, so that a lane has 8 consecutive columns;
       // then 16 tokens of 64 columns at a time go through LDS and out as rows of
@@ -469,7 +496,7 @@ __global__ __launch_bounds__(64 * WN * WM, 2) void tile_kernel(Linear p) {
       const bool wide = here_s(p.wide_out) && (beside % 8 == 0 || beside >= T::BN);
       const int l = here(lane), r = l & 31, g = l >> 5;
       lds_barrier();  // nobody reads this step's weights any more, and no load goes there before the next barrier
-      uint8_t* mine = w_lds + wave * T::kOut;
+      uint8_t* mine = w_of(stage) + wave * T::kOut;
       OUT* tile = static_cast<OUT*>(p.out) + static_cast<int64_t>(m0) * stride + n0;
       const auto rsrc = rsrc_of(tile, (static_cast<uint32_t>(rows - 1) * stride + (beside < T::BN ? beside : T::BN)) * 2u);
 #pragma unroll
@@ -519,19 +546,27 @@ __global__ __launch_bounds__(64 * WN * WM, 2) void tile_kernel(Linear p) {
           for (int e = 0; e < 16; ++e) acc[i][j][e] = acc[i + 1][j][e] = 0.f;
         }
       stored = wide;
+      if (kDeep) {
+#pragma unroll
+        for (int e = 0; e < 16; ++e) d[kLast & 1][e] = 0.f;
+      }
     }
     step(now);
     step(ahead);
     step(ahead_x);
-    if (min(now.left, min(ahead.left, S == 2 ? ahead_x.left : 1)) <= 0) {
+    stage = after;
+    if (!kPlain) {
       turn(now);
-      if (now.t >= last) break;
       turn(ahead);
       turn(ahead_x);
-      if (ends) sw = *(const_float*)now.ws;
+      if (ends && now.t < last) sw = *(const_float*)now.ws;
     }
-    stage = stage + 1 == S ? 0 : stage + 1;
-  }
+  };
+  do {
+    const int plain = (min(now.left - kFp8Block, min(ahead.left, S == 2 ? ahead_x.left : ahead.left)) - 1) / kFp8Block;
+    for (int i = 0; i < plain; ++i) one_step(std::true_type{});
+    one_step(std::false_type{});
+  } while (now.t < last);
   wait_loads<0>();  // no load may land in LDS that is somebody else's by then
 }
 
