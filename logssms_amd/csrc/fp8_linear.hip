@@ -582,11 +582,6 @@ int launch_linear(Linear p, hipStream_t s) {
     hipLaunchKernelGGL((few_rows_kernel<OUT, MT, NT, W, S>), dim3(static_cast<unsigned>(grid)), dim3(64 * W), 0, s, p);
     return GDN_LAUNCH_CHECK("gdn_fp8_linear launch");
   };
-  if (p.M <= 64) {
-    if (p.M <= 16) return few(GDN_INT(1), GDN_INT(1), GDN_INT(8), GDN_INT(2));
-    if (p.M <= 32) return few(GDN_INT(2), GDN_INT(2), GDN_INT(8), GDN_INT(2));
-    return few(GDN_INT(4), GDN_INT(2), GDN_INT(4), GDN_INT(3));
-  }
   auto go = [&](auto WNc, auto WMc, auto FNc, auto FMc, auto Sc) -> int {
     constexpr int WN = decltype(WNc)::value, WM = decltype(WMc)::value, FN = decltype(FNc)::value,
                   FM = decltype(FMc)::value, S = decltype(Sc)::value;
@@ -600,8 +595,35 @@ int launch_linear(Linear p, hipStream_t s) {
     hipLaunchKernelGGL((tile_kernel<OUT, WN, WM, FN, FM, S>), dim3(grid), dim3(T::kThreads), 0, s, p);
     return GDN_LAUNCH_CHECK("gdn_fp8_linear launch");
   };
-  const int64_t big = static_cast<int64_t>((p.M + 255) / 256) * ((p.N + 255) / 256);
-  if (big >= 256) return go(GDN_INT(2), GDN_INT(4), GDN_INT(4), GDN_INT(2), GDN_INT(2));
+  // Of the tiles, the smallest of which one round covers the output: at most one
+  // for each of the 256 CUs.  Smaller ones repeat a round's start and end (2048
+  // columns, K = 4096: 512 tokens in 16.1 us with 64 x 32 tiles, 12.1 with 64 x
+  // 64, and 17.8 with 64 x 128), larger ones leave CUs idle.  us by tokens x
+  // columns of the tile, the chosen one first:
+  //   1 x 12288 x 2048       16 x 64: 7.0    32 x 64: 7.2     16 x 32: 8.7
+  //   32 x 2048 x 4096       16 x 16: 5.9    16 x 32: 6.1     32 x 32: 7.3
+  //   128 x 2048 x 4096      32 x 32: 7.3    32 x 64: 7.4     64 x 64: 9.5
+  //   64 x 12288 x 2048      64 x 64: 9.8    64 x 128: 11.5   32 x 64: 11.5
+  //   256 x 12288 x 2048     128 x 128: 14.6 two a CU: 16.4   64 x 128: 19.6
+  const auto tiles = [&](int m, int n) {
+    return static_cast<int64_t>((p.M + m - 1) / m) * ((p.N + n - 1) / n);
+  };
+  constexpr int kCus = 256;
+  if (tiles(16, 16) <= kCus) return few(GDN_INT(1), GDN_INT(1), GDN_INT(8), GDN_INT(2));
+  if (tiles(16, 32) <= kCus) return few(GDN_INT(1), GDN_INT(2), GDN_INT(8), GDN_INT(2));
+  if (p.M <= 16) return few(GDN_INT(1), GDN_INT(4), GDN_INT(8), GDN_INT(1));  // however many: the weights stream past
+  if (tiles(32, 32) <= kCus) return few(GDN_INT(2), GDN_INT(2), GDN_INT(8), GDN_INT(2));
+  if (p.M <= 32 || tiles(32, 64) <= kCus) return few(GDN_INT(2), GDN_INT(4), GDN_INT(8), GDN_INT(1));
+  if (tiles(64, 64) <= kCus) return few(GDN_INT(4), GDN_INT(4), GDN_INT(8), GDN_INT(1));
+  if (p.M <= 64 || tiles(64, 128) <= kCus) return go(GDN_INT(2), GDN_INT(2), GDN_INT(2), GDN_INT(1), GDN_INT(4));
+  if (tiles(128, 128) <= kCus) return go(GDN_INT(2), GDN_INT(4), GDN_INT(2), GDN_INT(1), GDN_INT(4));
+  // Several rounds: tiles of 256 x 256, or of 128 x 128 two to a CU.  A round of
+  // the first costs 3, a round of 512 of the second 2, half a one 1 (us a step
+  // of K: 1.65, 1.1, 0.6).  1536 x 12288 x 2048: 288 large tiles 63 us, 1152
+  // small ones 50; 4096 x 12288 x 2048: 768 large ones 109, 3072 small ones 124.
+  const int64_t large = 3 * ((tiles(256, 256) + kCus - 1) / kCus), small = tiles(128, 128), rest = small % (2 * kCus);
+  if (large < 2 * (small / (2 * kCus)) + (rest > kCus ? 2 : rest > 0))
+    return go(GDN_INT(2), GDN_INT(4), GDN_INT(4), GDN_INT(2), GDN_INT(2));
   return go(GDN_INT(2), GDN_INT(2), GDN_INT(2), GDN_INT(2), GDN_INT(2));
 #undef GDN_INT
 }
