@@ -7,7 +7,7 @@ from .linear_attention_logstate import (
     LogStateLinearAttnMetadata,
 )
 from .linear_attention_mixed import MixedLinearCopyPlan, prepare_mixed_linear_metadata
-from .norm import RMSNormGated
+from .norm import RMSNorm, RMSNormGated
 
 __all__ = ["GatedDeltaConfig", "GatedDeltaLogStateBackend", "GatedDeltaNet", "LogStateLinearAttnCaptureData",
-           "LogStateLinearAttnMetadata", "MixedLinearCopyPlan", "RMSNormGated", "prepare_mixed_linear_metadata"]
+           "LogStateLinearAttnMetadata", "MixedLinearCopyPlan", "RMSNorm", "RMSNormGated", "prepare_mixed_linear_metadata"]

@@ -5,8 +5,10 @@ The layer is the boundary either side of the GDN path: the merged input
 projections whose column slices feed the conv and the gates as strided views
 (no copies), the backend call, and the gated RMS norm plus output projection.
 With one GPU the column- and row-parallel linears are plain GEMMs
-(``torch.nn.functional.linear``, i.e. hipBLASLt); the tensor-parallel head
-split and the row-parallel all-reduce are not part of this build."""
+(``torch.nn.functional.linear``, i.e. hipBLASLt), or, where a projection's
+weight is an ``Fp8Tensor``, the block-scaled 8-bit product (``fp8_linear``); the
+tensor-parallel head split and the row-parallel all-reduce are not part of this
+build."""
 
 from __future__ import annotations
 
@@ -15,6 +17,7 @@ from dataclasses import dataclass
 import torch
 import torch.nn.functional as F
 
+from ..kernel.fp8 import Fp8Tensor, fp8_linear, quantize_fp8, quantize_fp8_weight
 from .norm import RMSNormGated
 
 
@@ -43,7 +46,13 @@ class GatedDeltaNet:
     hidden]``, ``in_proj_ba_weight [2 HV, hidden]``, ``conv1d_weight
     [conv_dim, 1, W]``, ``dt_bias [HV]`` (ones), ``A_log [HV]`` (fp32 zeros),
     ``norm.weight [head_v_dim]`` (fp32 ones), ``out_proj_weight [hidden,
-    value_dim]``; the projections are left uninitialised, as there."""
+    value_dim]``; the projections are left uninitialised, as there.
+
+    ``in_proj_qkvz_weight`` and ``out_proj_weight`` may be ``Fp8Tensor``s of the
+    same shapes (a block-scaled checkpoint's values and scales, or
+    ``quantize_weights``); these projections then run in 8 bits.  The gates'
+    ``in_proj_ba_weight``, 2 HV rows that set each head's decay, stays in the
+    model dtype."""
 
     def __init__(
         self,
@@ -81,15 +90,30 @@ class GatedDeltaNet:
     def config(self) -> GatedDeltaConfig:
         return self._config
 
-    def forward(self, x: torch.Tensor) -> torch.Tensor:
-        mixed_qkv, z, beta, gate = self.proj(x)
+    def quantize_weights(self) -> None:
+        """The two large projections' weights in block-scaled 8 bits from here on."""
+        for name in ("in_proj_qkvz_weight", "out_proj_weight"):
+            weight = getattr(self, name)
+            if not isinstance(weight, Fp8Tensor):
+                setattr(self, name, quantize_fp8_weight(weight))
+
+    def forward(self, x: torch.Tensor, x_fp8: Fp8Tensor | None = None) -> torch.Tensor:
+        """``x_fp8``: ``x`` in 8 bits, where the norm in front of the layer has
+        written it (``RMSNorm.forward_fp8``); quantised here when None."""
+        mixed_qkv, z, beta, gate = self.proj(x, x_fp8)
         core_output = self.attend(mixed_qkv, beta, gate)
         return self.output(core_output, z)
 
-    def proj(self, x: torch.Tensor) -> tuple[torch.Tensor, ...]:
+    def proj(self, x: torch.Tensor, x_fp8: Fp8Tensor | None = None) -> tuple[torch.Tensor, ...]:
         """``:99-105``: column slices of the two projections, as views."""
         config = self._config
-        mixed_qkv, z = F.linear(x, self.in_proj_qkvz_weight).split([config.conv_dim, config.value_dim], dim=-1)
+        weight = self.in_proj_qkvz_weight
+        if isinstance(weight, Fp8Tensor):
+            qkvz = fp8_linear(quantize_fp8(x) if x_fp8 is None else x_fp8, weight, x.dtype)
+        else:
+            assert x_fp8 is None, "8-bit inputs need 8-bit projection weights"
+            qkvz = F.linear(x, weight)
+        mixed_qkv, z = qkvz.split([config.conv_dim, config.value_dim], dim=-1)
         beta, gate = F.linear(x, self.in_proj_ba_weight).chunk(2, dim=-1)
         return mixed_qkv, z, beta, gate
 
@@ -113,6 +137,9 @@ class GatedDeltaNet:
         """``:133-139``: gated RMS norm per v-head, then the output projection."""
         config = self._config
         shape = (core_output.shape[0], config.num_v_heads, config.head_v_dim)
+        if isinstance(self.out_proj_weight, Fp8Tensor):
+            return fp8_linear(self.norm.forward_fp8(core_output.reshape(shape), z.view(shape)), self.out_proj_weight,
+                              core_output.dtype)
         output = self.norm.forward(core_output.reshape(shape), z.view(shape)).reshape(core_output.shape[0], -1)
         return F.linear(output, self.out_proj_weight)
 
