@@ -36,7 +36,7 @@ __device__ __forceinline__ float block_scale(uint32_t amax_bits) {
 }
 
 // Eight values times 1 / s as e4m3 (round to nearest even; |y| / s <= 448 but
-// for the rounding of 1 / s, which cannot reach the next code's border).
+// for the last bit of 1 / s, which cannot reach the next code's border).
 __device__ __forceinline__ uint2 pack8_fp8(const float (&y)[8], float inv) {
   int lo = 0, hi = 0;
   lo = __builtin_amdgcn_cvt_pk_fp8_f32(y[0] * inv, y[1] * inv, lo, false);
@@ -66,7 +66,7 @@ __device__ __forceinline__ void store_fp8(const Fp8Rows& q, int64_t r, int64_t v
   m = block_amax(m);
   const float s = block_scale(m);
   const int64_t padded = (cols + 15) & ~int64_t{15};
-  if (8 * vec < padded) *reinterpret_cast<uint2*>(q.values + r * q.row_stride + 8 * vec) = pack8_fp8(y, 1.0f / s);
+  if (8 * vec < padded) *reinterpret_cast<uint2*>(q.values + r * q.row_stride + 8 * vec) = pack8_fp8(y, __builtin_amdgcn_rcpf(s));
   if ((vec & 15) == 0 && 8 * vec < cols)
     q.scales[r * q.scale_row_stride + (vec >> 4) * q.scale_block_stride] = s;
 }
