@@ -233,15 +233,17 @@ template <int WN, int WM, int FN, int FM, int S>
 struct Tile {
   static constexpr int kWaves = WN * WM, kThreads = 64 * kWaves;
   static constexpr int BN = 32 * FN * WN, BM = 32 * FM * WM, kRows = BN + BM;
-  static constexpr int kW = BN * kFp8Block, kX = BM * kFp8Block, kS = 256 * kWaves;  // bytes of a step's operands and scales
+  // 8 rows a load, as many loads for each wave; where they come to more than the rows, the rest is out of range
+  static constexpr int JN = (BN / 8 + kWaves - 1) / kWaves, JM = (BM / 8 + kWaves - 1) / kWaves;
+  // bytes of a step's operands and scales: 32 tokens' scales for a wave, in 256 bytes of its own
+  static constexpr int kW = JN * kWaves * 1024, kX = JM * kWaves * 1024, kS = 256 * kWaves;
   static constexpr int kLds = S * (kW + kX + kS);
-  static constexpr int JN = BN / 8 / kWaves, JM = BM / 8 / kWaves, kScales = BM / kWaves;  // loads and scales per wave
   static constexpr int kStores = 2 * FN * FM;
   static constexpr int kOut = 2048;  // per wave: 16 tokens of 64 columns on their way out, in place of a step's weights
   // loads that are newer than those that have to be there when a step begins
   static constexpr int kAhead = S == 2 ? JM + 1 : (S - 3) * (JN + JM + 1);
-  static_assert(kOut * kWaves <= kW && kLds <= 160 * 1024 && kAhead + kStores < 64 && S != 3, "fits");
-  static_assert(JN * 8 * kWaves == BN && JM * 8 * kWaves == BM && kScales <= 64, "whole loads per wave");
+  static_assert(kOut * kWaves <= kW && kLds <= 160 * 1024 && kAhead + kStores < 64, "fits");
+  static_assert(BM <= 32 * kWaves, "the scales' loads cover the tokens");
   static_assert(kFp8Block % (32 * FN) == 0 && FN % 2 == 0, "one row of weight scales per wave");
 };
 
@@ -311,9 +313,9 @@ __global__ __launch_bounds__(64 * WN * WM, 2) void tile_kernel(Linear p) {
   for (int j = 0; j < T::JM; ++j)
     x_at[j] = static_cast<uint32_t>(((wave * T::JM + j) * 8 + (lane >> 3)) * p.x_stride) +
               16 * (chunk ^ (4 * ((wave * T::JM + j) & 1)));
-  // each wave brings kScales of the tokens' scales into 256 bytes of its own (no branch: a branch here lets the
-  // compiler move the scaling behind it, for which there are no registers)
-  const uint32_t xs_at = lane < T::kScales ? static_cast<uint32_t>((wave * T::kScales + lane) * p.xs_row * 4) : 0xffffff00u;
+  // each wave brings 32 of the tokens' scales (no branch: a branch here lets the compiler move the scaling behind
+  // it, for which there are no registers)
+  const uint32_t xs_at = lane < 32 ? static_cast<uint32_t>((wave * 32 + lane) * p.xs_row * 4) : 0xffffff00u;
   auto load_rows = [&](const uint8_t* src, uint32_t span, int left, uint32_t at, int group, uint8_t* dst) __attribute__((always_inline)) {
     const int width = min(kFp8Block, left);
     const bool past = 16 * (chunk ^ (4 * (group & 1))) >= width;
@@ -385,7 +387,7 @@ __global__ __launch_bounds__(64 * WN * WM, 2) void tile_kernel(Linear p) {
     const int row = (wm * FM + j) * 32;
     bx[j][0] = frag(x_of(stage), row, 0);
     bx[j][1] = frag(x_of(stage), row, 1);
-    sx[j] = *reinterpret_cast<const float*>(scales_of(stage) + (row + r) / T::kScales * 256 + (row + r) % T::kScales * 4);
+    sx[j] = *reinterpret_cast<const float*>(scales_of(stage) + row * 8 + r * 4);
   };
   auto read_w = [&](int stage, int i, int to) __attribute__((always_inline)) {
     a[to][0] = frag(w_of(stage), (wn * FN + i) * 32, 0);
