@@ -239,7 +239,8 @@ struct Tile {
   static constexpr int kW = JN * kWaves * 1024, kX = JM * kWaves * 1024, kS = 256 * kWaves;
   static constexpr int kLds = S * (kW + kX + kS);
   static constexpr int kStores = 2 * FN * FM;
-  static constexpr int kOut = 2048;  // per wave: 16 tokens of 64 columns on their way out, in place of a step's weights
+  // tokens (of 64 columns) of a wave that go out at a time, in place of a step's weights
+  static constexpr int kPass = kW / kWaves >= 4096 ? 32 : 16, kOut = kPass * 128;
   // loads that are newer than those that have to be there when a step begins
   static constexpr int kAhead = S == 2 ? JM + 1 : (S - 3) * (JN + JM + 1);
   static_assert(kOut * kWaves <= kW && kLds <= 160 * 1024 && kAhead + kStores < 64, "fits");
@@ -316,20 +317,23 @@ __global__ __launch_bounds__(64 * WN * WM, 2) void tile_kernel(Linear p) {
   // each wave brings 32 of the tokens' scales (no branch: a branch here lets the compiler move the scaling behind
   // it, for which there are no registers)
   const uint32_t xs_at = lane < 32 ? static_cast<uint32_t>((wave * 32 + lane) * p.xs_row * 4) : 0xffffff00u;
-  auto load_rows = [&](const uint8_t* src, uint32_t span, int left, uint32_t at, int group, uint8_t* dst) __attribute__((always_inline)) {
-    const int width = min(kFp8Block, left);
-    const bool past = 16 * (chunk ^ (4 * (group & 1))) >= width;
+  // whole: the step has 128 columns of K
+  auto load_rows = [&](const uint8_t* src, uint32_t span, int left, bool whole, uint32_t at, int group, uint8_t* dst)
+                       __attribute__((always_inline)) {
+    const int width = whole ? kFp8Block : min(kFp8Block, left);
+    const bool past = !whole && 16 * (chunk ^ (4 * (group & 1))) >= width;
     dma16(src, span + width, past ? 0xffffff00u : at, dst + group * 1024);
   };
   auto w_of = [&](int stage) __attribute__((always_inline)) { return lds + stage * T::kW; };
   auto x_of = [&](int stage) __attribute__((always_inline)) { return lds + S * T::kW + stage * T::kX; };
   auto scales_of = [&](int stage) __attribute__((always_inline)) { return lds + S * (T::kW + T::kX) + stage * T::kS; };
-  auto load_w = [&](const Walk& c, int j, int stage) __attribute__((always_inline)) {
-    load_rows(c.w, c.w_span, c.left, w_at[j], wave * T::JN + j, w_of(stage));
+  auto load_w = [&](const Walk& c, bool whole, int j, int stage) __attribute__((always_inline)) {
+    load_rows(c.w, c.w_span, c.left, whole, w_at[j], wave * T::JN + j, w_of(stage));
   };
-  auto load_x = [&](const Walk& c, int j, int stage) __attribute__((always_inline)) {  // the last one brings the tokens' scales
+  // the last one brings the tokens' scales
+  auto load_x = [&](const Walk& c, bool whole, int j, int stage) __attribute__((always_inline)) {
     if (j < T::JM)
-      load_rows(c.x, c.x_span, c.left, x_at[j], wave * T::JM + j, x_of(stage));
+      load_rows(c.x, c.x_span, c.left, whole, x_at[j], wave * T::JM + j, x_of(stage));
     else
       dma4(c.xs, c.xs_span, xs_at, scales_of(stage) + wave * 256);
   };
@@ -361,19 +365,19 @@ __global__ __launch_bounds__(64 * WN * WM, 2) void tile_kernel(Linear p) {
 #pragma unroll
   for (int i = 0; i < S - 1; ++i) {
 #pragma unroll
-    for (int j = 0; j < T::JN; ++j) load_w(ahead, j, i);
+    for (int j = 0; j < T::JN; ++j) load_w(ahead, false, j, i);
 #pragma unroll
-    for (int j = 0; j <= T::JM; ++j) load_x(ahead, j, i);
+    for (int j = 0; j <= T::JM; ++j) load_x(ahead, false, j, i);
     next(ahead);
     next(ahead_x);
   }
   if (S == 2) {
 #pragma unroll
-    for (int j = 0; j <= T::JM; ++j) load_x(ahead_x, j, 1);
+    for (int j = 0; j <= T::JM; ++j) load_x(ahead_x, false, j, 1);
     next(ahead_x);
   }
   float sw = *(const_float*)now.ws;
-  i32x8 bx[FM][2], a[2][2];
+  i32x8 bx[FM][2], a[2][2], bx_next[FM][2], a_next[2];  // _next: the next step's first ones
   f32x16 d[2];
   float s[FM], sx[FM], s_last = 0.f;  // s_last: of the product whose scaling is left
   auto frag = [&](const uint8_t* base, int row, int half) __attribute__((always_inline)) {
@@ -383,19 +387,19 @@ __global__ __launch_bounds__(64 * WN * WM, 2) void tile_kernel(Linear p) {
     return join(*reinterpret_cast<const i32x4*>(of + 16 * (c ^ (r >> 1 & 7))),
                 *reinterpret_cast<const i32x4*>(of + 16 * ((c + 1) ^ (r >> 1 & 7))));
   };
-  auto read_x = [&](int stage, int j) __attribute__((always_inline)) {
+  auto read_x = [&](int stage, int j, i32x8 (&to)[FM][2]) __attribute__((always_inline)) {
     const int row = (wm * FM + j) * 32;
-    bx[j][0] = frag(x_of(stage), row, 0);
-    bx[j][1] = frag(x_of(stage), row, 1);
+    to[j][0] = frag(x_of(stage), row, 0);
+    to[j][1] = frag(x_of(stage), row, 1);
     sx[j] = *reinterpret_cast<const float*>(scales_of(stage) + row * 8 + r * 4);
   };
-  auto read_w = [&](int stage, int i, int to) __attribute__((always_inline)) {
-    a[to][0] = frag(w_of(stage), (wn * FN + i) * 32, 0);
-    a[to][1] = frag(w_of(stage), (wn * FN + i) * 32, 1);
+  auto read_w = [&](int stage, int i, i32x8 (&to)[2]) __attribute__((always_inline)) {
+    to[0] = frag(w_of(stage), (wn * FN + i) * 32, 0);
+    to[1] = frag(w_of(stage), (wn * FN + i) * 32, 1);
   };
   auto patch = [&](int stage) __attribute__((always_inline)) {  // bytes past K inside the last 16 of each row
     const int K = here_s(p.K), left = K & 15, in = (K & (kFp8Block - 1)) >> 4;
-    for (int row = threadIdx.x; row < T::kRows; row += T::kThreads) {
+    for (int row = here(threadIdx.x); row < T::kRows; row += T::kThreads) {
       uint8_t* of = row < T::BN ? w_of(stage) + row * kFp8Block : x_of(stage) + (row - T::BN) * kFp8Block;
       i32x4* v = reinterpret_cast<i32x4*>(of + 16 * (in ^ (row >> 1 & 7)));
       *v = mask_tail(*v, left);
@@ -412,8 +416,8 @@ __global__ __launch_bounds__(64 * WN * WM, 2) void tile_kernel(Linear p) {
     lds_barrier();
     if (padded <= kFp8Block && (p.K & 15)) patch(0);
 #pragma unroll
-    for (int j = 0; j < FM; ++j) read_x(0, j);
-    read_w(0, 0, 0);
+    for (int j = 0; j < FM; ++j) read_x(0, j, bx);
+    read_w(0, 0, a[0]);
 #pragma unroll
     for (int e = 0; e < 16; ++e) d[kLast & 1][e] = 0.f;
   }
@@ -433,31 +437,30 @@ __global__ __launch_bounds__(64 * WN * WM, 2) void tile_kernel(Linear p) {
       lds_barrier();
       if (!kPlain && ends && (p.K & 15)) patch(stage);
 #pragma unroll
-      for (int j = 0; j < FM; ++j) read_x(stage, j);
-      read_w(stage, 0, 0);
+      for (int j = 0; j < FM; ++j) read_x(stage, j, bx);
+      read_w(stage, 0, a[0]);
     }
     // The loads go between the products: issued all at once they fill the queue, and every wave waits behind it.
     auto load_between = [&](int product) __attribute__((always_inline)) {
       if (S == 2) {  // weights beside the first column fragment, tokens behind the second barrier
         constexpr int kLater = (FN - 1) * FM;
         if (product < FM) {
-          for (int k = product * T::JN / FM; k < (product + 1) * T::JN / FM; ++k) load_w(ahead, k, into);
+          for (int k = product * T::JN / FM; k < (product + 1) * T::JN / FM; ++k) load_w(ahead, kPlain, k, into);
         } else {
           for (int k = (product - FM) * (T::JM + 1) / kLater; k < (product - FM + 1) * (T::JM + 1) / kLater; ++k)
-            load_x(ahead_x, k, stage);
+            load_x(ahead_x, kPlain, k, stage);
         }
       } else {
         constexpr int kAll = T::JN + T::JM + 1;
         for (int k = product * kAll / (FN * FM); k < (product + 1) * kAll / (FN * FM); ++k) {
-          if (k < T::JN) load_w(ahead, k, into); else load_x(ahead, k - T::JN, into);
+          if (k < T::JN) load_w(ahead, kPlain, k, into); else load_x(ahead, kPlain, k - T::JN, into);
         }
       }
     };
 #pragma unroll
     for (int i = 0; i < FN; ++i) {
       if (!kDeep && i == 1) lds_barrier();  // every wave holds its tokens' fragments
-      if (i + 1 < FN) read_w(stage, i + 1, (i + 1) & 1);
-      else if (kDeep) read_w(after, 0, 0);
+      if (i + 1 < FN) read_w(stage, i + 1, a[(i + 1) & 1]);
 #pragma unroll
       for (int j = 0; j < FM; ++j) {
         const int at = i * FM + j;
@@ -475,12 +478,24 @@ __global__ __launch_bounds__(64 * WN * WM, 2) void tile_kernel(Linear p) {
         __builtin_amdgcn_sched_barrier(0);
         d[at & 1] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(a[i & 1][1], bx[j][1], d[at & 1], 0, 0, 0, 0, 0, 0);
         __builtin_amdgcn_sched_barrier(0);
-        if (kDeep && i + 1 == FN) read_x(after, j);
+        if (kDeep && at == 0) {
+          read_w(after, 0, a_next);
+#pragma unroll
+          for (int k = 0; k < FM; ++k) read_x(after, k, bx_next);
+        }
         if (at > 0 || kDeep) promote(d[from & 1], at > 0 ? s[from % FM] : s_last, from / FM, from % FM, 8);
         __builtin_amdgcn_sched_barrier(0);
       }
     }
     s_last = s[FM - 1];
+    if (kDeep) {
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        a[0][h] = a_next[h];
+#pragma unroll
+        for (int k = 0; k < FM; ++k) bx[k][h] = bx_next[k][h];
+      }
+    }
     if (!kDeep || (!kPlain && ends)) {
       promote(d[kLast & 1], s_last, FN - 1, FM - 1, 0);
       promote(d[kLast & 1], s_last, FN - 1, FM - 1, 8);
@@ -488,7 +503,7 @@ __global__ __launch_bounds__(64 * WN * WM, 2) void tile_kernel(Linear p) {
     if (!kPlain && ends) {
       // Registers 4 q .. 4 q + 3 hold columns 8 q + 4 g .. + 3 of token r.  The
       // halves of the wave trade theirs, so that a lane has 8 consecutive columns;
-      // then 16 tokens of 64 columns at a time go through LDS and out as rows of
+      // then 32 (16) tokens of 64 columns at a time go through LDS and out as rows of
       // 128 bytes (stored as they lie, in pieces of 32 bytes, the last product of
       // 16384 x 12288 x 2048 took 437 us, without any stores 361).
       int m0, n0;
@@ -522,18 +537,18 @@ __global__ __launch_bounds__(64 * WN * WM, 2) void tile_kernel(Linear p) {
                              static_cast<int>(hi[1])};  // columns 8 (q + g) .. + 7
           }
 #pragma unroll
-          for (int half = 0; half < 2; ++half) {
-            if (r / 16 == half) {
+          for (int pass = 0; pass < 32 / T::kPass; ++pass) {
+            if (T::kPass == 32 || r / T::kPass == pass) {
 #pragma unroll
               for (int q = 0; q < 8; q += 2)
-                *reinterpret_cast<i32x4*>(mine + r % 16 * 128 + 16 * ((q + g) ^ (r >> 1 & 7))) = v[q / 2];
+                *reinterpret_cast<i32x4*>(mine + r % T::kPass * 128 + 16 * ((q + g) ^ (r >> 1 & 7))) = v[q / 2];
             }
             wave_fence();
 #pragma unroll
-            for (int k = 0; k < 2; ++k) {  // lane l: 8 columns of row 8 k + l / 8
+            for (int k = 0; k < T::kPass / 8; ++k) {  // lane l: 8 columns of row 8 k + l / 8
               const int row = 8 * k + (l >> 3), c = l & 7;
               const i32x4 out = *reinterpret_cast<const i32x4*>(mine + row * 128 + 16 * (c ^ (row >> 1 & 7)));
-              const int m = (wm * FM + j) * 32 + 16 * half + row, n = (wn * FN + i) * 32 + 8 * c;
+              const int m = (wm * FM + j) * 32 + T::kPass * pass + row, n = (wn * FN + i) * 32 + 8 * c;
               if (wide) {  // always kStores stores: rows and columns that are not there fall out of range
                 const bool there = m < rows && n < beside;
                 __builtin_amdgcn_raw_buffer_store_b128(

@@ -205,3 +205,63 @@ def test_norms_and_products_in_one_graph(m):
             assert ((got - want).abs() <= 2.0 ** -8 * want.abs() + 2.0 ** -12 * want.square().mean().sqrt() * 8).all()
         assert ((p.dequantize().double().cpu() - gated).abs()
                 <= 2.0 ** -4 * 1.01 * gated.abs() + 2.0 ** -10 * 0.02).all()
+
+
+# tokens, columns: a size for each form and tile of the kernel, none of them a multiple of the tile
+FORMS = [(5, 270), (9, 5003), (16, 33001), (45, 2050), (100, 1500), (30, 9001), (120, 4001), (64, 20001), (130, 6001),
+         (450, 8003), (700, 6002), (1530, 2050), (4090, 4093)]
+
+
+@pytest.mark.parametrize("k", [7, 128, 255, 384, 1041])
+@pytest.mark.parametrize("size", FORMS, ids=str)
+def test_every_form_with_its_tails(size, k):
+    """Each form of the kernel with one block of K and several, whole and not;
+    the output lies in a larger buffer whose other values stay."""
+    from logssms_amd.kernel import fp8_linear
+    m, n = size
+    print(f"fp8_linear form {size} {k}", flush=True)
+    g = gen(m + k)
+    x, w = operands(m, n, k, g, 0.5)
+    dx, dw = to_dev(x), to_dev(w)
+    rows = torch.unique(torch.cat([torch.arange(min(m, 40)), torch.randint(0, m, (100,), generator=g),
+                                   torch.arange(max(0, m - 40), m)]))
+    cols = torch.unique(torch.cat([torch.arange(40), torch.randint(0, n, (100,), generator=g), torch.arange(n - 40, n)]))
+    got = fp8_linear(dx, dw)
+    check(got, x, w, torch.bfloat16, rows, cols)
+    a, b = ref.dequantize(*x).to(DEV), ref.dequantize(*w).to(DEV)
+    # every element: by the oracle's bound at most 7 * 2^-12 of the sum of the
+    # products' sizes is lost, and 2^-15 of it in the fp32 sums of these K; both,
+    # with the rounding of them, are below 2^-9; half a step of the output
+    size_of, want = a.abs() @ b.abs().t(), a @ b.t()
+    for pad in (3, 8):
+        out = torch.full((m + 2, (n + 2 * pad + 7) // 8 * 8), 7.0, dtype=torch.bfloat16, device=DEV)
+        view = out[1:m + 1, pad:pad + n]
+        assert fp8_linear(dx, dw, out=view) is view
+        assert torch.equal(view, got)
+        assert ((view.double() - want).abs() <= 2.0 ** -9 * size_of + 2.0 ** -8 * want.abs() + 2.0 ** -134).all()
+        view.fill_(7.0)
+        assert (out == 7.0).all()
+
+
+@pytest.mark.parametrize("size", FORMS, ids=str)
+def test_every_form_keeps_rows_and_columns_apart(size):
+    """NaN codes and infinite scales reach their own row or column only, and a
+    row's bits do not depend on its place among the others."""
+    from logssms_amd.kernel import Fp8Tensor, fp8_linear
+    m, n = size
+    k = 300
+    print(f"fp8_linear apart {size}", flush=True)
+    x, w = operands(m, n, k, gen(m))
+    dx, dw = to_dev(x), to_dev(w)
+    clean = fp8_linear(dx, dw)
+    perm = torch.randperm(m, generator=gen(1)).to(DEV)
+    codes = dx.values.view(torch.uint8).as_strided((m, 304), (304, 1))[perm].view(FP8)[:, :k]
+    assert torch.equal(fp8_linear(Fp8Tensor(codes, dx.scales[perm]), dw), clean[perm])
+    row, col = m // 2, n - 1 - n // 3
+    dx.values.view(torch.uint8)[row, k - 1] = 0x7F
+    dx.scales[m - 1, 1] = float("inf")
+    dw.values.view(torch.uint8)[col, 0] = 0xFF
+    got = fp8_linear(dx, dw)
+    assert got[row].isnan().all() and got[:, col].isnan().all() and not got[m - 1].isfinite().any()
+    got[row], got[m - 1], got[:, col] = clean[row], clean[m - 1], clean[:, col]
+    assert torch.equal(got, clean)
