@@ -552,7 +552,7 @@ __global__ __launch_bounds__(64 * WN * WM, 2) void tile_kernel(Linear p) {
               if (wide) {  // always kStores stores: rows and columns that are not there fall out of range
                 const bool there = m < rows && n < beside;
                 __builtin_amdgcn_raw_buffer_store_b128(
-                    out, rsrc, there ? (static_cast<uint32_t>(m) * stride + n) * 2u : 0xffffff00u, 0, 0);
+                    out, rsrc, there ? (static_cast<uint32_t>(m) * stride + n) * 2u : 0xffffff00u, 0, 2);
               } else if (m < rows) {
                 store_any(reinterpret_cast<uint16_t*>(tile) + static_cast<int64_t>(m) * stride + n, out, beside - n);
               }
