@@ -71,23 +71,19 @@ __device__ __forceinline__ void store_row(const NormRows& p, int64_t r, int64_t 
   }
 }
 
-// L lanes of one wave per row, N vectors of 8 elements per lane.
-template <class T, bool VEC, int L, int N>
+// L lanes of one wave per row, a vector of 8 elements per lane.
+template <class T, bool VEC, int L>
 __global__ __launch_bounds__(kThreads) void norm_wave_kernel(NormRows p) {
   const int lane = threadIdx.x % L;
   const int64_t r = static_cast<int64_t>(blockIdx.x) * (kThreads / L) + threadIdx.x / L;
   if (r >= p.rows) return;  // whole lane groups
-  float h[N][8];
+  float h[8];
   float ss = 0.f;
+  load_sum<T, VEC>(p, r, 8 * lane, h);
 #pragma unroll
-  for (int v = 0; v < N; ++v) load_sum<T, VEC>(p, r, 8 * (v * L + lane), h[v]);
-#pragma unroll
-  for (int v = 0; v < N; ++v)
-#pragma unroll
-    for (int e = 0; e < 8; ++e) ss = fmaf(h[v][e], h[v][e], ss);
+  for (int e = 0; e < 8; ++e) ss = fmaf(h[e], h[e], ss);
   const float rn = rsqrtf(head_sum<L>(ss) / static_cast<float>(p.cols) + p.eps);
-#pragma unroll
-  for (int v = 0; v < N; ++v) store_row<T, VEC>(p, r, v * L + lane, h[v], rn);
+  store_row<T, VEC>(p, r, lane, h, rn);
 }
 
 // One block of B threads per row; N vectors per thread are held, wider rows
@@ -232,31 +228,42 @@ __global__ __launch_bounds__(kThreads) void gated_any_kernel(GatedRows p) {
 // A launch holds fewer than 2^32 threads.
 bool grid_fits(int64_t blocks, int64_t threads) { return blocks <= 0xffffffffll / threads; }
 
+// Lanes that take a row of the norm: one vector of 8 elements each, as far as
+// they go (37 rows of 4096 in 3.7 us, 5.3 with four vectors a lane; 16384 of
+// 2048 in 48 us, 55 with a wave a row).
+int row_lanes(int64_t cols) {
+  const int64_t vecs = (cols + 7) / 8;
+  if (vecs <= 16) return 16;
+  for (int lanes = 64; lanes < 1024; lanes *= 2)
+    if (vecs <= lanes) return lanes;
+  return 1024;
+}
+
 bool known_dtype(int d) { return d == GDN_F32 || d == GDN_BF16 || d == GDN_F16; }
 
 template <class T, bool VEC>
 int launch_norm(const NormRows& p, hipStream_t s) {
-  auto wave = [&](auto Lc, auto Nc) {
-    constexpr int L = decltype(Lc)::value, N = decltype(Nc)::value;
+  auto wave = [&](auto Lc) {
+    constexpr int L = decltype(Lc)::value;
     const int64_t blocks = (p.rows + kThreads / L - 1) / (kThreads / L);
-    hipLaunchKernelGGL((norm_wave_kernel<T, VEC, L, N>), dim3(static_cast<unsigned>(blocks)), dim3(kThreads), 0, s, p);
+    hipLaunchKernelGGL((norm_wave_kernel<T, VEC, L>), dim3(static_cast<unsigned>(blocks)), dim3(kThreads), 0, s, p);
   };
   auto block = [&](auto Bc, auto Nc) {
     constexpr int B = decltype(Bc)::value, N = decltype(Nc)::value;
     hipLaunchKernelGGL((norm_block_kernel<T, VEC, B, N>), dim3(static_cast<unsigned>(p.rows)), dim3(B), 0, s, p);
   };
 #define GDN_INT(v) std::integral_constant<int, v>{}
-  // one vector a lane, as many lanes as the row has: 37 rows of 4096 in 3.7 us (5.3 with four vectors a lane),
-  // 16384 of 2048 in 48 (55 with a wave a row)
-  const int64_t vecs = (p.cols + 7) / 8;
-  if (vecs <= 16) wave(GDN_INT(16), GDN_INT(1));
-  else if (vecs <= 64) wave(GDN_INT(64), GDN_INT(1));
-  else if (vecs <= 128) block(GDN_INT(128), GDN_INT(1));
-  else if (vecs <= 256) block(GDN_INT(256), GDN_INT(1));
-  else if (vecs <= 512) block(GDN_INT(512), GDN_INT(1));
-  else if (vecs <= 1024) block(GDN_INT(1024), GDN_INT(1));
-  else if (vecs <= 2048) block(GDN_INT(1024), GDN_INT(2));
-  else block(GDN_INT(1024), GDN_INT(0));
+  switch (row_lanes(p.cols)) {
+    case 16: wave(GDN_INT(16)); break;
+    case 64: wave(GDN_INT(64)); break;
+    case 128: block(GDN_INT(128), GDN_INT(1)); break;
+    case 256: block(GDN_INT(256), GDN_INT(1)); break;
+    case 512: block(GDN_INT(512), GDN_INT(1)); break;
+    default:
+      if (p.cols <= 8 * 1024) block(GDN_INT(1024), GDN_INT(1));
+      else if (p.cols <= 16 * 1024) block(GDN_INT(1024), GDN_INT(2));
+      else block(GDN_INT(1024), GDN_INT(0));
+  }
   return GDN_LAUNCH_CHECK("gdn_rms_norm launch");
 }
 
@@ -303,6 +310,7 @@ int launch_gated(const GatedRows& p, hipStream_t s) {
       return GDN_LAUNCH_CHECK("gdn_rms_norm_gated_fp8 launch");
     }
   }
+  GDN_REQUIRE(grid_fits(p.tokens, kThreads), "gdn_rms_norm_gated_fp8: too many tokens");
   hipLaunchKernelGGL((gated_any_kernel<T>), dim3(static_cast<unsigned>(p.tokens)), dim3(kThreads),
                      static_cast<size_t>(p.heads) * sizeof(float), s, p);
   return GDN_LAUNCH_CHECK("gdn_rms_norm_gated_fp8 launch");
@@ -330,7 +338,7 @@ extern "C" int gdn_rms_norm(const void* x, int dtype, int64_t rows, int64_t cols
   GDN_REQUIRE(rows >= 0 && cols > 0, "gdn_rms_norm: bad shape (rows %lld, cols %lld)", static_cast<long long>(rows),
               static_cast<long long>(cols));
   GDN_REQUIRE(known_dtype(dtype) && known_dtype(weight_dtype), "gdn_rms_norm: unknown dtype");
-  GDN_REQUIRE(cols <= 0x7fffffff && grid_fits(rows, cols <= 8192 ? kThreads : 1024),
+  GDN_REQUIRE(cols <= 0x7fffffff && rows <= 0xffffffffll - kThreads && grid_fits(rows + kThreads / 16, row_lanes(cols)),
               "gdn_rms_norm: too many rows or columns");
   if (rows == 0) return GDN_OK;
   GDN_REQUIRE(x && weight, "gdn_rms_norm: null input");
@@ -391,8 +399,7 @@ extern "C" int gdn_rms_norm_gated_fp8(const void* x, int dtype, int64_t tokens, 
               "gdn_rms_norm_gated_fp8: bad shape (tokens %lld, heads %lld, dim %lld)", static_cast<long long>(tokens),
               static_cast<long long>(heads), static_cast<long long>(dim));
   GDN_REQUIRE(known_dtype(dtype) && known_dtype(weight_dtype), "gdn_rms_norm_gated_fp8: unknown dtype");
-  GDN_REQUIRE(tokens <= 0x7fffffff && grid_fits((tokens + 15) * ((heads * dim + kFp8Block + 511) / kFp8Block), 16) &&
-                  grid_fits(tokens, kThreads),
+  GDN_REQUIRE(tokens <= 0x7fffffff && grid_fits((tokens + 15) * ((heads * dim + kFp8Block + 511) / kFp8Block), 16),
               "gdn_rms_norm_gated_fp8: too many tokens");
   if (heads > 16384) {  // the norms of a token's heads are kept in 64 KiB of LDS
     set_error("gdn_rms_norm_gated_fp8: more than 16384 heads");

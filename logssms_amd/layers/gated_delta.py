@@ -109,6 +109,8 @@ class GatedDeltaNet:
         config = self._config
         weight = self.in_proj_qkvz_weight
         if isinstance(weight, Fp8Tensor):
+            assert x.ndim == 2, "8-bit projections take [tokens, hidden]"
+            assert x_fp8 is None or x_fp8.values.shape == x.shape, "x_fp8 must be x in 8 bits"
             qkvz = fp8_linear(quantize_fp8(x) if x_fp8 is None else x_fp8, weight, x.dtype)
         else:
             assert x_fp8 is None, "8-bit inputs need 8-bit projection weights"

@@ -203,3 +203,29 @@ def test_entry_points_check_before_they_launch():
         assert b"gdn_fp8_linear:" in lib.gdn_last_error()
     for kw in (dict(xst=1 << 24), dict(wst=1 << 24), dict(xsr=1 << 22)):
         assert linear(**kw) == 2, kw
+
+
+def test_norm_counts_the_threads_of_a_row():
+    """A launch holds fewer than 2^32 threads; a row of up to 128 values takes
+    16 of them, one of more than 4096 all 1024 of a block."""
+    lib = _built()
+    d = 0x10000
+    for rows, cols in ((1 << 22, 4104), (1 << 22, 8192), (1 << 23, 4096), (1 << 25, 1000), (1 << 28, 64), (1 << 62, 8)):
+        rc = lib.gdn_rms_norm(d, 1, rows, cols, cols, None, cols, d, 0, 0.0, 1e-6, None, cols, d, cols, None, 0, None, 0,
+                              0, None)
+        assert rc == 1 and b"too many rows" in lib.gdn_last_error(), (rows, cols)
+
+
+def test_layer_refuses_8_bit_rows_of_another_input():
+    from logssms_amd.layers import GatedDeltaNet
+    _built()
+    net = GatedDeltaNet(64, 2, 4, 32, 32, 4, 1e-6, 0, device="cpu", dtype=torch.bfloat16)
+    net.in_proj_qkvz_weight.zero_()
+    net.out_proj_weight.zero_()
+    net.quantize_weights()
+    x = torch.zeros(5, 64, dtype=torch.bfloat16)
+    for given in (_pair(4, 64), _pair(5, 48), _pair(1, 64)):
+        with pytest.raises(AssertionError, match="x in 8 bits"):
+            net.proj(x, given)
+    with pytest.raises(AssertionError, match="tokens"):
+        net.proj(x.view(5, 1, 64))
