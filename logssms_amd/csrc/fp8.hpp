@@ -66,7 +66,8 @@ __device__ __forceinline__ void store_fp8(const Fp8Rows& q, int64_t r, int64_t v
   m = block_amax(m);
   const float s = block_scale(m);
   const int64_t padded = (cols + 15) & ~int64_t{15};
-  if (8 * vec < padded) *reinterpret_cast<uint2*>(q.values + r * q.row_stride + 8 * vec) = pack8_fp8(y, __builtin_amdgcn_rcpf(s));
+  if (8 * vec < padded)
+    *reinterpret_cast<uint2*>(q.values + r * q.row_stride + 8 * vec) = pack8_fp8(y, __builtin_amdgcn_rcpf(s));
   if ((vec & 15) == 0 && 8 * vec < cols)
     q.scales[r * q.scale_row_stride + (vec >> 4) * q.scale_block_stride] = s;
 }

@@ -42,7 +42,7 @@ struct Linear {
 __device__ __forceinline__ __amdgpu_buffer_rsrc_t rsrc_of(const void* from, uint32_t bytes) {
   return __builtin_amdgcn_make_buffer_rsrc(const_cast<void*>(from), 0, bytes, 0x00020000);
 }
-// Direct-to-LDS loads of 16 or 4 bytes per active lane: lane l lands at lds + 16 l (4 l), zeros where off is past bytes.
+// Direct-to-LDS loads of 16 or 4 bytes a lane: lane l lands at lds + 16 l (4 l), zeros where off is past bytes.
 __device__ __forceinline__ void dma16(const void* src, uint32_t bytes, uint32_t off, void* lds) {
   __builtin_amdgcn_raw_ptr_buffer_load_lds(rsrc_of(src, bytes), (lds_void*)lds, 16, off, 0, 0, 0);
 }
@@ -58,7 +58,9 @@ __device__ __forceinline__ int here_s(int v) {  // the same for a value that all
   asm volatile("" : "+s"(v));
   return v;
 }
-__device__ __forceinline__ i32x8 join(i32x4 a, i32x4 b) { return __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7); }
+__device__ __forceinline__ i32x8 join(i32x4 a, i32x4 b) {
+  return __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7);
+}
 
 // Up to 8 columns of an output row at any even address.
 __device__ __forceinline__ void store_any(uint16_t* to, i32x4 v, int columns) {
@@ -80,7 +82,10 @@ __device__ __forceinline__ i32x4 mask_tail(i32x4 v, int left) {
   return v;
 }
 
-template <int N> __device__ __forceinline__ void wait_loads() { asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory"); }
+template <int N>
+__device__ __forceinline__ void wait_loads() {
+  asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory");
+}
 // LDS traffic between the lanes of one wave: in order in hardware, so only the compiler has to be told.
 __device__ __forceinline__ void wave_fence() { asm volatile("" ::: "memory"); }
 __device__ __forceinline__ void lds_barrier() { asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory"); }
@@ -125,18 +130,22 @@ __global__ __launch_bounds__(64 * W, 2) void few_rows_kernel(Linear p) {
   const int chunk = (lane & 7) ^ (lane >> 4);
   uint32_t w_at[2 * NT], x_at[2 * MT];
 #pragma unroll
-  for (int j = 0; j < 2 * NT; ++j) w_at[j] = static_cast<uint32_t>((8 * j + (lane >> 3)) * p.w_stride) + 16 * (chunk ^ (4 * (j & 1)));
+  for (int j = 0; j < 2 * NT; ++j)
+    w_at[j] = static_cast<uint32_t>((8 * j + (lane >> 3)) * p.w_stride) + 16 * (chunk ^ (4 * (j & 1)));
 #pragma unroll
-  for (int j = 0; j < 2 * MT; ++j) x_at[j] = static_cast<uint32_t>((8 * j + (lane >> 3)) * p.x_stride) + 16 * (chunk ^ (4 * (j & 1)));
+  for (int j = 0; j < 2 * MT; ++j)
+    x_at[j] = static_cast<uint32_t>((8 * j + (lane >> 3)) * p.x_stride) + 16 * (chunk ^ (4 * (j & 1)));
   const uint32_t xs_at = lane < 16 * MT ? static_cast<uint32_t>(lane * p.xs_row * 4) : 0xffffff00u;
-  auto load = [&](int b, int stage) __attribute__((always_inline)) {  // past the last block: counted, but nothing in range
+  // past the last block: counted, but nothing in range
+  auto load = [&](int b, int stage) __attribute__((always_inline)) {
     const int width = b < blocks ? min(kFp8Block, padded - b * kFp8Block) : 0;
     const uint32_t w_bytes = width ? static_cast<uint32_t>((rows_n - 1) * p.w_stride + width) : 0u;
     const uint32_t x_bytes = width ? static_cast<uint32_t>((rows_m - 1) * p.x_stride + width) : 0u;
     uint8_t* to = mine + stage * F::kStage;
     const bool past[2] = {16 * chunk >= width, 16 * (chunk ^ 4) >= width};
 #pragma unroll
-    for (int j = 0; j < 2 * NT; ++j) dma16(w + b * kFp8Block, w_bytes, past[j & 1] ? 0xffffff00u : w_at[j], to + j * 1024);
+    for (int j = 0; j < 2 * NT; ++j)
+      dma16(w + b * kFp8Block, w_bytes, past[j & 1] ? 0xffffff00u : w_at[j], to + j * 1024);
 #pragma unroll
     for (int j = 0; j < 2 * MT; ++j)
       dma16(x + b * kFp8Block, x_bytes, past[j & 1] ? 0xffffff00u : x_at[j], to + (2 * NT + j) * 1024);
@@ -222,13 +231,21 @@ __global__ __launch_bounds__(64 * W, 2) void few_rows_kernel(Linear p) {
 
 // ------------------------------------------------------------------ tiles
 // A block of WN x WM waves owns a tile of BN = 32 FN WN columns and BM = 32 FM
-// WM tokens at a time.  Both operands of a block of K go straight to LDS, one
-// step ahead of the products, rows of 128 bytes with the 16-byte chunk c of
-// row r at c ^ (r / 2 % 8): a fragment read takes the same chunk of 16
-// consecutive rows at a time, two rows of which fill the 64 banks, so this
-// spreads them over all of the banks (c ^ (r % 8) cost 4 conflict cycles on
-// each 4).  The direct loads land in lane order, so the lanes' source chunks
-// are permuted instead.
+// WM tokens at a time.  Both operands of a block of K go straight to LDS, ahead
+// of the products, rows of 128 bytes with the 16-byte chunk c of row r at
+// c ^ (r / 2 % 8): a fragment read takes the same chunk of 16 consecutive rows
+// at a time, two rows of which fill the 64 banks, so this spreads them over all
+// of the banks (c ^ (r % 8) cost 4 conflict cycles on each 4).  The direct loads
+// land in lane order, so the lanes' source chunks are permuted instead.
+//
+// What bounds it: 16384 x 12288 x 2048 takes 395 us (2.1 PFLOP/s), 8192^3 460
+// (2.4).  The matrix instructions with the scaling between them, out of
+// registers, reach 4.8 PFLOP/s; under this load the card lowers its clock to
+// 1.8 to 2.0 GHz.  Of the first product's 406 us at the time, the output took
+// 46, the scaling 50 and the second barrier 15 (each left out, by turns); loads
+// that touch the lines of later steps first made it slower.  Where a CU has one
+// tile (256 x 12288 x 2048: 13.5 us, 16 steps) a step takes 0.49 us, 0.24 of
+// them matrix instructions: the rest is the wait for 32 KB from the L2.
 template <int WN, int WM, int FN, int FM, int S>
 struct Tile {
   static constexpr int kWaves = WN * WM, kThreads = 64 * kWaves;
@@ -503,9 +520,11 @@ __global__ __launch_bounds__(64 * WN * WM, 2) void tile_kernel(Linear p) {
     if (!kPlain && ends) {
       // Registers 4 q .. 4 q + 3 hold columns 8 q + 4 g .. + 3 of token r.  The
       // halves of the wave trade theirs, so that a lane has 8 consecutive columns;
-      // then 32 (16) tokens of 64 columns at a time go through LDS and out as rows of
-      // 128 bytes (stored as they lie, in pieces of 32 bytes, the last product of
-      // 16384 x 12288 x 2048 took 437 us, without any stores 361).
+      // then kPass tokens of 64 columns at a time go through LDS and out as rows of
+      // 128 bytes (as they lie, in pieces of 32 bytes, the stores took 76 us of
+      // 16384 x 12288 x 2048; these take 46).  They are not kept in the L2, which
+      // the end of the kernel would write back (512 x 12288 x 2048: 19.4 us, 20.4
+      // through it).
       int m0, n0;
       corner(now.t, m0, n0);
       const int below = here_s(p.M) - m0, beside = here_s(p.N) - n0, stride = here_s(p.out_stride);
@@ -613,15 +632,16 @@ int launch_linear(Linear p, hipStream_t s) {
     return GDN_LAUNCH_CHECK("gdn_fp8_linear launch");
   };
   // Of the tiles, the smallest of which one round covers the output: at most one
-  // for each of the 256 CUs.  Smaller ones repeat a round's start and end (2048
-  // columns, K = 4096: 512 tokens in 16.1 us with 64 x 32 tiles, 12.1 with 64 x
-  // 64, and 17.8 with 64 x 128), larger ones leave CUs idle.  us by tokens x
-  // columns of the tile, the chosen one first:
-  //   1 x 12288 x 2048       16 x 64: 7.0    32 x 64: 7.2     16 x 32: 8.7
-  //   32 x 2048 x 4096       16 x 16: 5.9    16 x 32: 6.1     32 x 32: 7.3
-  //   128 x 2048 x 4096      32 x 32: 7.3    32 x 64: 7.4     64 x 64: 9.5
-  //   64 x 12288 x 2048      64 x 64: 9.8    64 x 128: 11.5   32 x 64: 11.5
-  //   256 x 12288 x 2048     128 x 128: 14.6 two a CU: 16.4   64 x 128: 19.6
+  // for each of the 256 CUs.  Smaller ones repeat a round's start and end, larger
+  // ones leave CUs idle.  us by tokens x columns of the tile, the chosen first:
+  //   1 x 12288 x 2048       16 x 64: 7.2    32 x 64: 7.3     16 x 32: 8.6
+  //   32 x 2048 x 4096       16 x 16: 5.3    16 x 32: 5.6     32 x 32: 6.3
+  //   128 x 2048 x 4096      32 x 32: 6.8    32 x 64: 8.0     64 x 64: 10.4
+  //   512 x 2048 x 4096      64 x 64: 11.6   32 x 64: 15.7    64 x 128: 16.5
+  //   64 x 12288 x 2048      64 x 64: 9.2    64 x 128: 10.7   32 x 64: 11.0
+  //   128 x 12288 x 2048     64 x 128: 11.0  64 x 64: 14.4
+  //   1024 x 2048 x 4096     64 x 128: 17.7  128 x 128: 20.7
+  //   256 x 12288 x 2048     128 x 128: 13.5 two a CU: 15.0   64 x 128: 18.8
   const auto tiles = [&](int m, int n) {
     return static_cast<int64_t>((p.M + m - 1) / m) * ((p.N + n - 1) / n);
   };
@@ -636,8 +656,9 @@ int launch_linear(Linear p, hipStream_t s) {
   if (tiles(128, 128) <= kCus) return go(GDN_INT(2), GDN_INT(4), GDN_INT(2), GDN_INT(1), GDN_INT(4));
   // Several rounds: tiles of 256 x 256, or of 128 x 128 two to a CU.  A round of
   // the first costs 3, a round of 512 of the second 2, half a one 1 (us a step
-  // of K: 1.65, 1.1, 0.6).  1536 x 12288 x 2048: 288 large tiles 63 us, 1152
-  // small ones 50; 4096 x 12288 x 2048: 768 large ones 109, 3072 small ones 124.
+  // of K, a tile's start and end among them: 1.75, 1.05, 0.7).  1536 x 12288 x
+  // 2048: 288 large tiles 58 us, 1152 small ones 46; 4096 x 12288 x 2048: 768
+  // large ones 103, 3072 small ones 114.
   const int64_t large = 3 * ((tiles(256, 256) + kCus - 1) / kCus), small = tiles(128, 128), rest = small % (2 * kCus);
   if (large < 2 * (small / (2 * kCus)) + (rest > kCus ? 2 : rest > 0))
     return go(GDN_INT(2), GDN_INT(4), GDN_INT(4), GDN_INT(2), GDN_INT(2));
@@ -679,7 +700,8 @@ extern "C" int gdn_fp8_linear(const void* x, int64_t x_row_stride, const float* 
   }
   Linear p{static_cast<const uint8_t*>(x), static_cast<const uint8_t*>(weight), x_scales, weight_scales, out,
            static_cast<int>(x_row_stride), static_cast<int>(weight_row_stride), static_cast<int>(out_row_stride),
-           static_cast<int>(xs_row_stride), xs_block_stride, ws_row_stride, ws_block_stride, static_cast<int>(M), static_cast<int>(N), static_cast<int>(K), 0, 0, 0};
+           static_cast<int>(xs_row_stride), xs_block_stride, ws_row_stride, ws_block_stride, static_cast<int>(M),
+           static_cast<int>(N), static_cast<int>(K), 0, 0, 0};
   p.wide_out = aligned16(out) && (M == 1 || out_row_stride % 8 == 0);
   hipStream_t s = static_cast<hipStream_t>(stream);
   return out_dtype == GDN_BF16 ? launch_linear<bf16>(p, s) : launch_linear<f16>(p, s);

@@ -373,7 +373,8 @@ extern "C" int gdn_quantize_fp8(const void* x, int dtype, int64_t rows, int64_t 
   GDN_REQUIRE(rows >= 0 && cols > 0, "gdn_quantize_fp8: bad shape (rows %lld, cols %lld)",
               static_cast<long long>(rows), static_cast<long long>(cols));
   GDN_REQUIRE(known_dtype(dtype), "gdn_quantize_fp8: unknown dtype");
-  GDN_REQUIRE(cols <= 0x7fffffff && rows <= 0x7fffffff && grid_fits((rows + 15) * ((cols + kFp8Block - 1) / kFp8Block), 16),
+  GDN_REQUIRE(cols <= 0x7fffffff && rows <= 0x7fffffff &&
+                  grid_fits((rows + 15) * ((cols + kFp8Block - 1) / kFp8Block), 16),
               "gdn_quantize_fp8: too many rows");
   if (rows == 0) return GDN_OK;
   GDN_REQUIRE(x, "gdn_quantize_fp8: null input");
