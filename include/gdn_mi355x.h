@@ -731,7 +731,9 @@ int gdn_rms_norm_gated_fp8(const void* x, int dtype, int64_t tokens, int64_t hea
  *   out [M, N] bf16 or f16, unit column stride.
  * Accumulated in fp32, rounded once.  The 8-bit matrix instructions drop, of each
  * eight consecutive products, what lies 2^-13 below the largest of the eight.
- * Row strides up to 2^23 (GDN_ERR_UNSUPPORTED beyond).
+ * A token's scale times a weight block's is taken in fp32 and has to be finite there.
+ * Row strides up to 2^23 bytes of x and weight, 2^22 elements of out, 2^21 of
+ * x_scales, and sizes below 2^31 - 4096 (GDN_ERR_UNSUPPORTED beyond).
  */
 int gdn_fp8_linear(const void* x, int64_t x_row_stride, const float* x_scales, int64_t xs_row_stride,
                    int64_t xs_block_stride, const void* weight, int64_t weight_row_stride, const float* weight_scales,

@@ -689,11 +689,13 @@ extern "C" int gdn_fp8_linear(const void* x, int64_t x_row_stride, const float* 
   GDN_REQUIRE(rows_ok(x, M, x_row_stride, K) && rows_ok(weight, N, weight_row_stride, K),
               "gdn_fp8_linear: the rows of x and weight must start at multiples of 16 bytes and not overlap");
   GDN_REQUIRE(out_row_stride >= N && (reinterpret_cast<uintptr_t>(out) & 1) == 0, "gdn_fp8_linear: bad output rows");
+  GDN_REQUIRE(((reinterpret_cast<uintptr_t>(x_scales) | reinterpret_cast<uintptr_t>(weight_scales)) & 3) == 0,
+              "gdn_fp8_linear: misaligned scales");
   GDN_REQUIRE(xs_row_stride >= 0 && xs_block_stride >= 0 && ws_row_stride >= 0 && ws_block_stride >= 0,
               "gdn_fp8_linear: negative scale strides");
   // offsets inside a tile of up to 256 rows are 32-bit
-  constexpr int64_t kMostStride = int64_t{1} << 23;
-  if (M > 0x7fffff00 || N > 0x7fffff00 || K > 0x7fffff00 || x_row_stride > kMostStride ||
+  constexpr int64_t kMostStride = int64_t{1} << 23, kMost = 0x7ffff000;  // rounded up to a tile: still an int
+  if (M > kMost || N > kMost || K > kMost || x_row_stride > kMostStride ||
       weight_row_stride > kMostStride || out_row_stride > kMostStride / 2 || xs_row_stride > kMostStride / 4) {
     set_error("gdn_fp8_linear: sizes or row strides beyond 2^23 are not covered");
     return GDN_ERR_UNSUPPORTED;

@@ -229,3 +229,18 @@ def test_layer_refuses_8_bit_rows_of_another_input():
             net.proj(x, given)
     with pytest.raises(AssertionError, match="tokens"):
         net.proj(x.view(5, 1, 64))
+
+
+def test_product_refuses_what_its_offsets_cannot_reach():
+    lib = _built()
+    d = 0x10000
+
+    def linear(M=4, N=64, xs=d, ws=d, ost=64):
+        return lib.gdn_fp8_linear(d, 128, xs, 1, 4, d, 128, ws, 1, 1, M, N, 128, d, 1, ost, None)
+
+    most = (1 << 31) - 4096
+    for kw in (dict(M=most + 1), dict(N=most + 1, ost=most + 1), dict(M=1, N=1 << 40, ost=1 << 40),
+               dict(ost=(1 << 22) + 1)):
+        assert linear(**kw) == 2, kw
+    for kw in (dict(xs=d + 2), dict(ws=d + 1)):
+        assert linear(**kw) == 1 and b"misaligned scales" in lib.gdn_last_error(), kw

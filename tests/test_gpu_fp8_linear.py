@@ -265,3 +265,33 @@ def test_every_form_keeps_rows_and_columns_apart(size):
     assert got[row].isnan().all() and got[:, col].isnan().all() and not got[m - 1].isfinite().any()
     got[row], got[m - 1], got[:, col] = clean[row], clean[m - 1], clean[:, col]
     assert torch.equal(got, clean)
+
+
+@pytest.mark.parametrize("size", [(66000, 40000, 48), (3, 270000, 16400), (270000, 3, 16400), (70000, 500, 65000)], ids=str)
+def test_offsets_beyond_32_bits(size):
+    """Weights, tokens and outputs of more than 2^32 bytes, checked at their ends."""
+    from logssms_amd.kernel import Fp8Tensor, fp8_linear
+    m, n, k = size
+    print(f"fp8_linear far {size}", flush=True)
+    g = torch.Generator(device=DEV).manual_seed(m + n)
+    kb = -(-k // 128)
+
+    def made(count, scale_rows):
+        wide = (k + 15) // 16 * 16
+        codes = torch.randint(0, 256, (count, wide), generator=g, device=DEV, dtype=torch.uint8)
+        codes &= 0xBF  # below 2: no NaN codes, and sums far from overflow
+        return Fp8Tensor(codes.view(FP8)[:, :k], 0.5 + torch.rand(kb, scale_rows, generator=g, device=DEV).t())
+
+    x, w = made(m, m), made(n, -(-n // 128))
+    got = fp8_linear(x, w)
+    rows = torch.unique(torch.cat([torch.arange(min(m, 20)), torch.arange(max(0, m - 40), m)])).to(DEV)
+    cols = torch.unique(torch.cat([torch.arange(min(n, 20)), torch.arange(max(0, n - 40), n)])).to(DEV)
+    # the sampled rows of the weights carry their blocks' scales as rows of their own
+    a = (x.values.view(torch.uint8)[rows].view(FP8).cpu(), x.scales[rows].cpu())
+    b = w.values.view(torch.uint8)[cols].view(FP8).cpu(), w.scales[cols // 128].cpu()
+    va, vb = ref.dequantize(*a), ref.dequantize(*b)
+    want, size_of = va @ vb.t(), va.abs() @ vb.abs().t()
+    # the oracle's bound: 7 * 2^-12 of the products' sizes, and K / 8 + K / 128 + 2
+    # additions of 2^-23 of them; half a step of bf16
+    err = (got[rows][:, cols].cpu().double() - want).abs()
+    assert (err <= (2.0 ** -8 * want.abs() + (2.0 ** -9 + (k / 8 + k / 128 + 2) * 2.0 ** -23) * 1.01 * size_of)).all()

@@ -226,3 +226,25 @@ def test_rows_graph_replay_on_a_side_stream():
         torch.cuda.synchronize()
         for a, b in zip(graphed, eager):
             assert torch.equal(a.contiguous().view(torch.uint8), b.contiguous().view(torch.uint8))
+
+
+def test_rows_beyond_32_bits():
+    """Rows whose offsets pass 2^32 bytes: the last ones are what they are alone."""
+    from logssms_amd.kernel import add_rms_norm_fp8, quantize_fp8, rms_norm_gated_fp8
+    rows, cols = 300000, 8192
+    print("far rows", flush=True)
+    g = torch.Generator(device=DEV).manual_seed(9)
+    x = torch.empty(rows, cols, dtype=torch.bfloat16, device=DEV).normal_(generator=g)
+    res = torch.empty_like(x).normal_(generator=g)
+    weight = 1 + 0.1 * torch.randn(cols, generator=g, device=DEV)
+    last = slice(rows - 5, rows)
+    q, y, total = add_rms_norm_fp8(x, res, weight, 1e-6, keep=True)
+    q1, y1, total1 = add_rms_norm_fp8(x[last], res[last], weight, 1e-6, keep=True)
+    assert torch.equal(y[last], y1) and torch.equal(total[last], total1) and torch.equal(q.scales[last], q1.scales)
+    assert torch.equal(q.values[last].view(torch.uint8), q1.values.view(torch.uint8))
+    heads, heads_res, w128 = x.view(rows, 64, 128), res.view(rows, 64, 128), weight[:128].contiguous()
+    for far, alone in ((quantize_fp8(x), quantize_fp8(x[last])),
+                       (rms_norm_gated_fp8(heads, heads_res, w128, 1e-6),
+                        rms_norm_gated_fp8(heads[last], heads_res[last], w128, 1e-6))):
+        assert torch.equal(far.scales[last], alone.scales)
+        assert torch.equal(far.values[last].view(torch.uint8), alone.values.view(torch.uint8))
