@@ -37,8 +37,7 @@ __device__ __forceinline__ void load_weight(const NormRows& p, int64_t c, float 
   } else if (VEC) {
     load8<float, VEC>(static_cast<const float*>(p.weight), c, p.cols, w);
   } else {
-#pragma unroll
-    for (int e = 0; e < 8; ++e) w[e] = c + e < p.cols ? load_any(p.weight, c + e, p.weight_dtype) : 0.f;
+    load8_any(p.weight, p.weight_dtype, c, p.cols, w);
   }
 }
 
@@ -187,37 +186,49 @@ __global__ __launch_bounds__(kThreads) void gated_vec_kernel(GatedRows p, uint32
   store_fp8(p.q, r, vec, p.heads * p.dim, y);
 }
 
-// Any head width, dtype of the weight and alignment: a block per token, the
-// heads' norms first (a wave per head), then the row's blocks of 128.
-template <class T>
-__global__ __launch_bounds__(kThreads) void gated_any_kernel(GatedRows p) {
+// Any head width, dtype of the weight and alignment: a block of B threads per
+// token, the heads' norms first (L lanes a head), then the row in vectors of 8,
+// most of which lie within a head.  The second reading of x comes from the
+// caches.  16384 tokens of 5 heads of 96: 13 us (36 element by element).
+template <class T, int B, int L>
+__global__ __launch_bounds__(B) void gated_any_kernel(GatedRows p) {
   extern __shared__ float rn[];  // [heads]
   const int64_t r = blockIdx.x;
   const T* x = static_cast<const T*>(p.x) + r * p.x_token_stride;
   const T* gate = static_cast<const T*>(p.gate) + r * p.gate_token_stride;
-  const int lane = threadIdx.x & 63;
-  for (int64_t head = threadIdx.x >> 6; head < p.heads; head += kThreads / 64) {
+  const uint32_t heads = static_cast<uint32_t>(p.heads), dim = static_cast<uint32_t>(p.dim), cols = heads * dim;
+  for (uint32_t head = threadIdx.x / L; head < heads; head += B / L) {  // whole groups of L lanes
     float ss = 0.f;
-    for (int64_t c = lane; c < p.dim; c += 64) {
-      const float v = to_f32(x[head * p.x_head_stride + c]);
-      ss = fmaf(v, v, ss);
+    for (uint32_t c = 8 * (threadIdx.x % L); c < dim; c += 8 * L) {
+      float v[8];
+      load8<T, false>(x + head * p.x_head_stride, c, dim, v);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) ss = fmaf(v[e], v[e], ss);
     }
-    ss = head_sum<64>(ss);
-    if (lane == 0) rn[head] = rsqrtf(ss / static_cast<float>(p.dim) + p.eps);
+    ss = head_sum<L>(ss);
+    if (threadIdx.x % L == 0) rn[head] = rsqrtf(ss / static_cast<float>(p.dim) + p.eps);
   }
   __syncthreads();
-  const int64_t cols = p.heads * p.dim;
-  const int64_t vecs = (cols + kFp8Block - 1) / kFp8Block * (kFp8Block / 8);
-  for (int64_t vec = threadIdx.x; vec < vecs; vec += kThreads) {  // whole 16-lane groups
+  const uint32_t vecs = (cols + kFp8Block - 1) / kFp8Block * (kFp8Block / 8);
+  for (uint32_t vec = threadIdx.x; vec < vecs; vec += B) {  // whole 16-lane groups
+    uint32_t head = 8 * vec / dim, c = 8 * vec - head * dim;
     float y[8];
+    if (head < heads && c + 8 <= dim) {
+      float z[8], w[8];
+      load8<T, false>(x + head * p.x_head_stride, c, dim, y);
+      load8<T, false>(gate + head * p.gate_head_stride, c, dim, z);
+      load8_any(p.weight, p.weight_dtype, c, dim, w);
 #pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      const int64_t i = 8 * vec + e;
-      y[e] = 0.f;
-      if (i < cols) {
-        const int64_t head = i / p.dim, c = i - head * p.dim;
-        y[e] = (to_f32(x[head * p.x_head_stride + c]) * rn[head]) * load_any(p.weight, c, p.weight_dtype) *
-               fast_silu(to_f32(gate[head * p.gate_head_stride + c]));
+      for (int e = 0; e < 8; ++e) y[e] = (y[e] * rn[head]) * w[e] * fast_silu(z[e]);
+    } else {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        y[e] = 0.f;
+        if (head < heads) {
+          y[e] = (to_f32(x[head * p.x_head_stride + c]) * rn[head]) * load_any(p.weight, c, p.weight_dtype) *
+                 fast_silu(to_f32(gate[head * p.gate_head_stride + c]));
+          if (++c == dim) c = 0, ++head;
+        }
       }
     }
     store_fp8(p.q, r, vec, cols, y);
@@ -310,9 +321,18 @@ int launch_gated(const GatedRows& p, hipStream_t s) {
       return GDN_LAUNCH_CHECK("gdn_rms_norm_gated_fp8 launch");
     }
   }
+  // rows of up to 128 vectors take one wave, heads of up to 16 vectors 16 lanes
   GDN_REQUIRE(grid_fits(p.tokens, kThreads), "gdn_rms_norm_gated_fp8: too many tokens");
-  hipLaunchKernelGGL((gated_any_kernel<T>), dim3(static_cast<unsigned>(p.tokens)), dim3(kThreads),
-                     static_cast<size_t>(p.heads) * sizeof(float), s, p);
+  auto any = [&](auto Bc, auto Lc) {
+    constexpr int B = decltype(Bc)::value, L = decltype(Lc)::value;
+    hipLaunchKernelGGL((gated_any_kernel<T, B, L>), dim3(static_cast<unsigned>(p.tokens)), dim3(B),
+                       static_cast<size_t>(p.heads) * sizeof(float), s, p);
+  };
+  if (cols <= 1024) {
+    if (p.dim <= 128) any(GDN_INT(64), GDN_INT(16)); else any(GDN_INT(64), GDN_INT(64));
+  } else {
+    if (p.dim <= 128) any(GDN_INT(256), GDN_INT(16)); else any(GDN_INT(256), GDN_INT(64));
+  }
   return GDN_LAUNCH_CHECK("gdn_rms_norm_gated_fp8 launch");
 }
 #undef GDN_INT
