@@ -247,6 +247,10 @@ PyObject* conv_recurrent(PyObject*, PyObject* const* args, Py_ssize_t n) {
 constexpr int64_t kFp8Block = 128;
 int64_t blocks_of(int64_t n) { return (n + kFp8Block - 1) / kFp8Block; }
 int64_t padded16(int64_t n) { return (n + 15) / 16 * 16; }
+// The stride of rows of 8-bit values that this package makes: whole cache lines
+// where that adds at most a fifth (2900 x 1111 x 1000: 11.8 us with rows of 1008
+// bytes, 10.7 with rows of 1024).
+int64_t fp8_stride(int64_t cols) { return cols > 512 ? (cols + 127) / 128 * 128 : padded16(cols); }
 
 void require_device(const at::Tensor& t) {
   if (t.is_cuda()) return;
@@ -288,7 +292,7 @@ struct Fp8Out {
 };
 Fp8Out fp8_out(int64_t rows, int64_t cols, const at::Tensor& like) {
   const int64_t shape[] = {rows, blocks_of(cols)}, strides[] = {1, std::max<int64_t>(rows, 1)};
-  Fp8Out out{fresh({rows, padded16(cols)}, at::kFloat8_e4m3fn, like),
+  Fp8Out out{fresh({rows, fp8_stride(cols)}, at::kFloat8_e4m3fn, like),
              like.is_cuda() ? at::Tensor(at::detail::empty_strided_cuda(shape, strides, at::kFloat, like.device()))
                             : at::empty_strided(shape, strides, like.options().dtype(at::kFloat))};
   if (out.values.size(1) != cols) out.values = out.values.narrow(1, 0, cols);
