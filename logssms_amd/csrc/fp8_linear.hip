@@ -640,7 +640,10 @@ int launch_linear(Linear p, hipStream_t s) {
   //   1 x 12288 x 2048       16 x 64: 7.2    32 x 64: 7.3     16 x 32: 8.6
   //   32 x 2048 x 4096       16 x 16: 5.3    16 x 32: 5.6     32 x 32: 6.3
   //   128 x 2048 x 4096      32 x 32: 6.8    32 x 64: 8.0     64 x 64: 10.4
-  //   512 x 2048 x 4096      64 x 64: 11.6   32 x 64: 15.7    64 x 128: 16.5
+  //   384 x 2048 x 4096      48 x 64: 9.7    64 x 64: 10.9    32 x 64: 14.4
+  //   512 x 2048 x 4096      64 x 64: 11.1   32 x 64: 15.1    64 x 128: 16.9
+  //   539 x 2048 x 4096      64 x 80: 12.2   64 x 64: 18.2    64 x 128: 16.9
+  //   64 x 18000 x 2048      64 x 128: 11.5  64 x 80: 12.0
   //   64 x 12288 x 2048      64 x 64: 9.2    64 x 128: 10.7   32 x 64: 11.0
   //   128 x 12288 x 2048     64 x 128: 11.0  64 x 64: 14.4
   //   1024 x 2048 x 4096     64 x 128: 17.7  128 x 128: 20.7
@@ -654,7 +657,9 @@ int launch_linear(Linear p, hipStream_t s) {
   if (p.M <= 16) return few(GDN_INT(1), GDN_INT(4), GDN_INT(8), GDN_INT(1));  // however many: the weights stream past
   if (tiles(32, 32) <= kCus) return few(GDN_INT(2), GDN_INT(2), GDN_INT(8), GDN_INT(2));
   if (p.M <= 32 || tiles(32, 64) <= kCus) return few(GDN_INT(2), GDN_INT(4), GDN_INT(8), GDN_INT(1));
+  if (tiles(48, 64) <= kCus) return few(GDN_INT(3), GDN_INT(4), GDN_INT(8), GDN_INT(1));
   if (tiles(64, 64) <= kCus) return few(GDN_INT(4), GDN_INT(4), GDN_INT(8), GDN_INT(1));
+  if (p.M > 64 && tiles(64, 80) <= kCus) return few(GDN_INT(4), GDN_INT(5), GDN_INT(8), GDN_INT(1));
   if (p.M <= 64 || tiles(64, 128) <= kCus) return go(GDN_INT(2), GDN_INT(2), GDN_INT(2), GDN_INT(1), GDN_INT(4));
   if (tiles(128, 128) <= kCus) return go(GDN_INT(2), GDN_INT(4), GDN_INT(2), GDN_INT(1), GDN_INT(4));
   // Several rounds: tiles of 256 x 256, or of 128 x 128 two to a CU.  A round of

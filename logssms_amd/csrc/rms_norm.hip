@@ -245,7 +245,7 @@ bool grid_fits(int64_t blocks, int64_t threads) { return blocks <= 0xffffffffll 
 int row_lanes(int64_t cols) {
   const int64_t vecs = (cols + 7) / 8;
   if (vecs <= 16) return 16;
-  for (int lanes = 64; lanes < 1024; lanes *= 2)
+  for (int lanes : {64, 128, 256, 384, 512, 768})
     if (vecs <= lanes) return lanes;
   return 1024;
 }
@@ -269,7 +269,9 @@ int launch_norm(const NormRows& p, hipStream_t s) {
     case 64: wave(GDN_INT(64)); break;
     case 128: block(GDN_INT(128), GDN_INT(1)); break;
     case 256: block(GDN_INT(256), GDN_INT(1)); break;
+    case 384: block(GDN_INT(384), GDN_INT(1)); break;
     case 512: block(GDN_INT(512), GDN_INT(1)); break;
+    case 768: block(GDN_INT(768), GDN_INT(1)); break;
     default:
       if (p.cols <= 8 * 1024) block(GDN_INT(1024), GDN_INT(1));
       else if (p.cols <= 16 * 1024) block(GDN_INT(1024), GDN_INT(2));
