@@ -207,10 +207,11 @@ def test_entry_points_check_before_they_launch():
 
 def test_norm_counts_the_threads_of_a_row():
     """A launch holds fewer than 2^32 threads; a row of up to 128 values takes
-    16 of them, one of more than 4096 all 1024 of a block."""
+    16 of them, one of up to 6144 768, a wider one all 1024 of a block."""
     lib = _built()
     d = 0x10000
-    for rows, cols in ((1 << 22, 4104), (1 << 22, 8192), (1 << 23, 4096), (1 << 25, 1000), (1 << 28, 64), (1 << 62, 8)):
+    for rows, cols in ((1 << 22, 6152), (1 << 22, 8192), (6 << 20, 4104), (1 << 23, 4096), (1 << 25, 1000), (1 << 28, 64),
+                       (1 << 62, 8)):
         rc = lib.gdn_rms_norm(d, 1, rows, cols, cols, None, cols, d, 0, 0.0, 1e-6, None, cols, d, cols, None, 0, None, 0,
                               0, None)
         assert rc == 1 and b"too many rows" in lib.gdn_last_error(), (rows, cols)
