@@ -225,7 +225,8 @@ def test_every_form_with_its_tails(size, k):
     dx, dw = to_dev(x), to_dev(w)
     rows = torch.unique(torch.cat([torch.arange(min(m, 40)), torch.randint(0, m, (100,), generator=g),
                                    torch.arange(max(0, m - 40), m)]))
-    cols = torch.unique(torch.cat([torch.arange(40), torch.randint(0, n, (100,), generator=g), torch.arange(n - 40, n)]))
+    cols = torch.unique(torch.cat([torch.arange(min(n, 40)), torch.randint(0, n, (100,), generator=g),
+                                   torch.arange(max(0, n - 40), n)]))
     got = fp8_linear(dx, dw)
     check(got, x, w, torch.bfloat16, rows, cols)
     a, b = ref.dequantize(*x).to(DEV), ref.dequantize(*w).to(DEV)
@@ -267,7 +268,8 @@ def test_every_form_keeps_rows_and_columns_apart(size):
     assert torch.equal(got, clean)
 
 
-@pytest.mark.parametrize("size", [(66000, 40000, 48), (3, 270000, 16400), (270000, 3, 16400), (70000, 500, 65000)], ids=str)
+@pytest.mark.parametrize("size", [(66000, 40000, 48), (3, 270000, 16400), (270000, 3, 16400), (70000, 500, 65000)],
+                         ids=str)
 def test_offsets_beyond_32_bits(size):
     """Weights, tokens and outputs of more than 2^32 bytes, checked at their ends."""
     from logssms_amd.kernel import Fp8Tensor, fp8_linear
@@ -295,3 +297,14 @@ def test_offsets_beyond_32_bits(size):
     # additions of 2^-23 of them; half a step of bf16
     err = (got[rows][:, cols].cpu().double() - want).abs()
     assert (err <= (2.0 ** -8 * want.abs() + (2.0 ** -9 + (k / 8 + k / 128 + 2) * 2.0 ** -23) * 1.01 * size_of)).all()
+
+
+@pytest.mark.parametrize("k", [30, 128, 1041, 2600])
+@pytest.mark.parametrize("size", [(140, 5003), (190, 5001), (131, 5900), (200, 8001), (16000, 40), (9000, 20),
+                                  (5000, 130)], ids=str)
+def test_forms_between_and_narrow_outputs(size, k):
+    """48 x 64, 64 x 64 and 64 x 80 outputs a block, 64 x 128 of more than 64
+    rows, and outputs that are narrower than a tile."""
+    test_every_form_with_its_tails(size, k)
+    if k == 1041:
+        test_every_form_keeps_rows_and_columns_apart(size)

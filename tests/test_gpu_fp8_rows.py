@@ -248,3 +248,44 @@ def test_rows_beyond_32_bits():
                         rms_norm_gated_fp8(heads[last], heads_res[last], w128, 1e-6))):
         assert torch.equal(far.scales[last], alone.scales)
         assert torch.equal(far.values[last].view(torch.uint8), alone.values.view(torch.uint8))
+
+
+@pytest.mark.parametrize("dtype", DTYPES, ids=str)
+@pytest.mark.parametrize("shape", [(5, 2157), (4, 2600), (3, 4801), (3, 6136), (2, 9001), (7, 333), (40, 12)], ids=str)
+def test_rows_at_odd_addresses(shape, dtype):
+    """Rows, residual and its destination at odd addresses and strides, in place;
+    what lies beside the destination stays."""
+    from logssms_amd.kernel import add_rms_norm, add_rms_norm_fp8, quantize_fp8
+    rows, cols = shape
+    print(f"odd rows {shape} {dtype}", flush=True)
+    g = gen(rows + 7 * cols)
+    wide = randn(3, rows + 1, cols + 5, g=g, dtype=dtype).to(DEV)
+    x, res = wide[0][1:, 3:3 + cols], wide[1][1:, 1:1 + cols]
+    w = randn(cols + 1, g=g).to(DEV)[1:]
+    h, y = ref.rms_norm(x.cpu(), w.cpu(), EPS, residual=res.cpu(), weight_offset=1.0)
+    around = wide[1].clone()
+    got, total = add_rms_norm(x, res, w, EPS, weight_offset=1.0)
+    assert_rounded(got, y, dtype)
+    assert_rounded(total, h, dtype)
+    assert_quantised(quantize_fp8(x), x.double().cpu())
+    q, y8, place = add_rms_norm_fp8(x, res, w, EPS, weight_offset=1.0, keep=True, residual_out=res)
+    assert_quantised(q, y)
+    assert torch.equal(y8, got) and place is res and torch.equal(res, total)
+    wide[1][1:, 1:1 + cols] = around[1:, 1:1 + cols]
+    assert torch.equal(wide[1], around)
+
+
+@pytest.mark.parametrize("case", [(3, 5, 96), (2, 3, 200), (3, 40, 96), (2, 10, 200), (2, 9, 130), (5, 4, 7),
+                                  (1, 16384, 2)], ids=str)
+def test_gated_heads_of_any_width(case):
+    """One wave and four to a token, 16 and 64 lanes to a head, heads at odd addresses."""
+    test_gated_norm_in_8_bits(case, torch.bfloat16)
+    from logssms_amd.kernel import rms_norm_gated_fp8
+    tokens, heads, dim = case
+    g = gen(tokens + heads + dim)
+    wide = randn(2, tokens, heads, dim + 3, g=g, dtype=torch.float16)
+    x, z = wide[0][..., 1:1 + dim], wide[1][..., 2:2 + dim]
+    w = randn(dim, g=g, std=0.5).half()
+    on = wide.to(DEV)
+    got = rms_norm_gated_fp8(on[0][..., 1:1 + dim], on[1][..., 2:2 + dim], w.to(DEV), EPS)
+    assert_quantised(got, ref.rms_norm_gated(x, z, w, EPS))
