@@ -665,8 +665,8 @@ int launch_linear(Linear p, hipStream_t s) {
   // Several rounds: tiles of 256 x 256, or of 128 x 128 two to a CU.  A round of
   // the first costs 3, a round of 512 of the second 2, half a one 1 (us a step
   // of K, a tile's start and end among them: 1.75, 1.05, 0.7).  1536 x 12288 x
-  // 2048: 288 large tiles 58 us, 1152 small ones 46; 4096 x 12288 x 2048: 768
-  // large ones 103, 3072 small ones 114.
+  // 2048: large tiles 58 us, small ones 46; 4096 x 12288 x 2048: large ones 103,
+  // small ones 114.
   const int64_t large = 3 * ((tiles(256, 256) + kCus - 1) / kCus), small = tiles(128, 128), rest = small % (2 * kCus);
   if (large < 2 * (small / (2 * kCus)) + (rest > kCus ? 2 : rest > 0))
     return go(GDN_INT(2), GDN_INT(4), GDN_INT(4), GDN_INT(2), GDN_INT(2));
