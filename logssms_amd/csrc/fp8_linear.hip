@@ -258,6 +258,7 @@ struct Tile {
   // bytes of a step's operands and scales: 32 tokens' scales for a wave, in 256 bytes of its own
   static constexpr int kW = JN * kWaves * 1024, kX = JM * kWaves * 1024, kS = 256 * kWaves;
   static constexpr int kLds = S * (kW + kX + kS);
+  static constexpr int kPerCu = 160 * 1024 / kLds, kPerSimd = kPerCu * kWaves / 4;  // blocks, waves
   static constexpr int kStores = 2 * FN * FM;
   // tokens (of 64 columns) of a wave that go out at a time, in place of a step's weights
   static constexpr int kPass = kW / kWaves >= 4096 ? 32 : 16, kOut = kPass * 128;
@@ -269,7 +270,7 @@ struct Tile {
 };
 
 template <class OUT, int WN, int WM, int FN, int FM, int S>
-__global__ __launch_bounds__(64 * WN * WM, 2) void tile_kernel(Linear p) {
+__global__ __launch_bounds__(64 * WN * WM, (Tile<WN, WM, FN, FM, S>::kPerSimd)) void tile_kernel(Linear p) {
   using T = Tile<WN, WM, FN, FM, S>;
   __shared__ __align__(16) uint8_t lds[T::kLds];
   const int lane = threadIdx.x & 63;
@@ -629,8 +630,7 @@ int launch_linear(Linear p, hipStream_t s) {
     p.tiles_n = (p.N + T::BN - 1) / T::BN;
     const int64_t tiles = static_cast<int64_t>(p.tiles_m) * p.tiles_n;
     GDN_REQUIRE(tiles <= 0x7fffffff / 8, "gdn_fp8_linear: too many tiles");
-    constexpr int kPerCu = (160 * 1024) / T::kLds;
-    const int grid = static_cast<int>(tiles < 256 * kPerCu ? (tiles + 7) / 8 * 8 : 256 * kPerCu);
+    const int grid = static_cast<int>(tiles < 256 * T::kPerCu ? (tiles + 7) / 8 * 8 : 256 * T::kPerCu);
     hipLaunchKernelGGL((tile_kernel<OUT, WN, WM, FN, FM, S>), dim3(grid), dim3(T::kThreads), 0, s, p);
     return GDN_LAUNCH_CHECK("gdn_fp8_linear launch");
   };
