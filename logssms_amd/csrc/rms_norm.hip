@@ -241,8 +241,7 @@ bool grid_fits(int64_t blocks, int64_t threads) { return blocks <= 0xffffffffll 
 
 // Lanes that take a row of the norm: one vector of 8 elements each, as far as
 // they go (37 rows of 4096 in 3.7 us, 5.3 with four vectors a lane; 100000 of
-// 256 in 18 us, 23 with a wave a row; 16384 of
-// 2048 in 48 us, 55 with a wave a row).
+// 256 in 18 us, 23 with a wave a row).
 int row_lanes(int64_t cols) {
   const int64_t vecs = (cols + 7) / 8;
   for (int lanes : {16, 32, 64, 128, 256, 384, 512, 768})
