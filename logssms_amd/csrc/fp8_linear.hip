@@ -586,9 +586,10 @@ __global__ __launch_bounds__(64 * WN * WM, (Tile<WN, WM, FN, FM, S>::kPerSimd)) 
           for (int e = 0; e < 16; ++e) acc[i][j][e] = acc[i + 1][j][e] = 0.f;
         }
       stored = wide;
-      if (kDeep) {
+      if (kDeep) {  // nothing is left to scale: the next tile's first step adds 0 * 0 (an old scale may be infinite)
 #pragma unroll
         for (int e = 0; e < 16; ++e) d[kLast & 1][e] = 0.f;
+        s_last = 0.f;
       }
     }
     step(now);

@@ -1,0 +1,41 @@
+"""The block-scaled product where a block of the kernel walks over several
+output tiles, and what one tile may leave for the next: scales that are not
+finite, tails of K, narrow stores.  Bounds as in ``test_gpu_fp8_linear``."""
+
+import pytest
+import torch
+
+from tests.gpu_util import DEV, gen
+from tests.test_gpu_fp8_linear import operands, test_every_form_keeps_rows_and_columns_apart as keeps_apart
+from tests.test_gpu_fp8_linear import test_every_form_with_its_tails as form_with_its_tails
+from tests.test_gpu_fp8_linear import to_dev
+
+pytestmark = pytest.mark.gpu
+
+# tokens, columns: more tiles than blocks for 64 x 128 outputs a block (four
+# stages; two and three tiles a block), 128 x 128 two to a CU and 256 x 256
+WALKS = [(40, 40001), (64, 70000), (4097, 4099), (4090, 8003)]
+# one tile a block, or a form without tiles
+SINGLE = [(9, 5003), (60, 2050), (64, 20001), (130, 6001), (700, 6002)]
+
+
+@pytest.mark.parametrize("value", [float("inf"), float("nan")], ids=str)
+@pytest.mark.parametrize("size", WALKS + SINGLE, ids=str)
+def test_a_weight_scale_that_is_not_finite_stays_in_its_block(size, value):
+    """In the last block of K of an early column block: its 128 columns change, nothing else."""
+    from logssms_amd.kernel import fp8_linear
+    m, n = size
+    print(f"fp8_linear weight scale {size} {value}", flush=True)
+    x, w = operands(m, n, 300, gen(m + n))
+    dx, dw = to_dev(x), to_dev(w)
+    clean = fp8_linear(dx, dw)
+    assert clean.isfinite().all()
+    for block in (0, 5):
+        keep = dw.scales[block, -1].clone()
+        dw.scales[block, -1] = value
+        got = fp8_linear(dx, dw)
+        dw.scales[block, -1] = keep
+        part = slice(128 * block, 128 * block + 128)
+        assert not got[:, part].isfinite().any()
+        got[:, part] = clean[:, part]
+        assert torch.equal(got, clean)
