@@ -684,9 +684,10 @@ int gdn_rms_norm_gated(const void* x, int dtype, int64_t rows, int64_t cols, con
  * path in block-scaled 8 bits, and the norms that feed them.
  *
  * A quantised row holds OCP e4m3 values and one fp32 scale for each 128 of
- * them (the last block may be shorter): it stands for value * scale, and
+ * them (the last block may be shorter): it stands for value * scale, with
  * scale = max|block| / 448 (2^-126 for a block of zeros; NaN or infinite, and
- * the block NaN as a whole, where it holds a NaN or an infinity).
+ * the block NaN as a whole, where it holds a NaN or an infinity) and value =
+ * e4m3(y / scale), both divisions rounded to fp32.
  *   values [rows, cols] at a row stride (bytes) that is a multiple of 16, 16-byte
  *     aligned; the bytes from cols up to the next multiple of 16 belong to the row
  *     (written as zeros here, read and ignored by gdn_fp8_linear).
