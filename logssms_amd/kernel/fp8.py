@@ -64,7 +64,8 @@ def quantize_fp8_weight(weight: torch.Tensor) -> Fp8Tensor:
     w = torch.zeros(nb * BLOCK, kb * BLOCK, dtype=torch.float32, device=weight.device)
     w[:n, :k] = weight
     w = w.view(nb, BLOCK, kb, BLOCK)
-    scales = (w.abs().amax((1, 3)) / _TOP).clamp_min(_LEAST_SCALE)
+    # by a tensor: on a GPU, torch divides by a number as a product with its reciprocal
+    scales = (w.abs().amax((1, 3)) / w.new_tensor(_TOP)).clamp_min(_LEAST_SCALE)
     w = (w / scales[:, None, :, None]).to(FP8).view(nb * BLOCK, kb * BLOCK)
     # rows at multiples of 16 bytes, zeros behind them
     return Fp8Tensor(w.view(torch.uint8)[:n, :_stride(k)].contiguous().view(FP8)[:, :k], scales)

@@ -90,3 +90,16 @@ def test_codes_of_the_gated_norm(dim):
     want = [divided((y * near).reshape(50, -1)) for near in (1.0, 1 + 2.0 ** -23, 1 - 2.0 ** -24)]
     codes = got.values.cpu().contiguous().view(torch.uint8)
     assert any(torch.equal(got.scales.cpu(), s) and torch.equal(codes, c) for c, s in want)
+
+
+def test_weights_are_quantised_alike_on_every_device():
+    from logssms_amd.kernel import quantize_fp8_weight
+    w = randn(1000, 1111, g=gen(2)) * torch.exp(randn(1000, 1, g=gen(3)))
+    here, there = quantize_fp8_weight(w), quantize_fp8_weight(w.to(DEV))
+    assert torch.equal(there.scales.cpu(), here.scales)
+    assert torch.equal(there.values.cpu().contiguous().view(torch.uint8), here.values.contiguous().view(torch.uint8))
+    # rows of weights and of tokens lie at the same strides
+    from logssms_amd.kernel import quantize_fp8
+    for cols in (1, 15, 16, 17, 500, 512, 513, 528, 529, 640, 641, 1000, 1024, 1025, 4096):
+        x = torch.ones(2, cols)
+        assert quantize_fp8(x.to(DEV)).values.stride() == quantize_fp8_weight(x).values.stride(), cols
