@@ -55,9 +55,10 @@ def quantize_fp8(x: torch.Tensor) -> Fp8Tensor:
     return Fp8Tensor(*_lib.host().quantize_fp8(x))
 
 
+@torch.no_grad()
 def quantize_fp8_weight(weight: torch.Tensor) -> Fp8Tensor:
     """A projection's weights [N, K] with a scale for each 128 x 128 block.
-    Once per load: elementary torch operations, on any device."""
+    Once per load: elementary torch operations, on any device, without a gradient."""
     assert weight.ndim == 2 and weight.numel() > 0, "weight must be [N, K]"
     n, k = weight.shape
     nb, kb = -(-n // BLOCK), -(-k // BLOCK)

@@ -245,3 +245,13 @@ def test_product_refuses_what_its_offsets_cannot_reach():
         assert linear(**kw) == 2, kw
     for kw in (dict(xs=d + 2), dict(ws=d + 1)):
         assert linear(**kw) == 1 and b"misaligned scales" in lib.gdn_last_error(), kw
+
+
+def test_weights_are_quantised_without_a_gradient():
+    """A parameter's values and scales are data: they keep no graph of the weight alive."""
+    from logssms_amd.kernel.fp8 import quantize_fp8_weight
+    w = torch.nn.Parameter(torch.randn(130, 200, generator=_gen(4)))
+    q = quantize_fp8_weight(w)
+    assert not q.values.requires_grad and not q.scales.requires_grad and q.scales.grad_fn is None
+    want = quantize_fp8_weight(w.detach())
+    assert torch.equal(q.scales, want.scales) and torch.equal(q.dequantize(), want.dequantize())
