@@ -732,9 +732,13 @@ int gdn_rms_norm_gated_fp8(const void* x, int dtype, int64_t tokens, int64_t hea
  *   out [M, N] bf16 or f16, unit column stride.
  * Accumulated in fp32, rounded once.  The 8-bit matrix instructions drop, of each
  * eight consecutive products, what lies 2^-13 below the largest of the eight.
- * A token's scale times a weight block's is taken in fp32 and has to be finite there.
- * Row strides up to 2^23 bytes of x and weight, 2^22 elements of out, 2^21 of
- * x_scales, and sizes below 2^31 - 4096 (GDN_ERR_UNSUPPORTED beyond).
+ * A token's scale times a weight block's is taken in fp32: it has to be finite
+ * there, and below 2^-126 keeps what a subnormal does.
+ * Covered (GDN_ERR_UNSUPPORTED beyond): sizes up to 2^31 - 4096; between rows,
+ * strides up to 2^23 bytes of x and weight (so K up to 2^23 unless M and N are
+ * 1), 2^22 elements of out (so N up to 2^22 unless M is 1) and 2^21 of x_scales.
+ * More tiles than a launch has room for (N from 2^29 on for a few tokens) are
+ * GDN_ERR_INVALID.
  */
 int gdn_fp8_linear(const void* x, int64_t x_row_stride, const float* x_scales, int64_t xs_row_stride,
                    int64_t xs_block_stride, const void* weight, int64_t weight_row_stride, const float* weight_scales,

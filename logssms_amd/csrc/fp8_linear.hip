@@ -688,16 +688,16 @@ extern "C" int gdn_fp8_linear(const void* x, int64_t x_row_stride, const float* 
   GDN_REQUIRE(out_dtype == GDN_BF16 || out_dtype == GDN_F16, "gdn_fp8_linear: the output is bf16 or f16");
   if (M == 0) return GDN_OK;
   GDN_REQUIRE(x && x_scales && weight && weight_scales && out, "gdn_fp8_linear: null input");
-  // the stride of a single row means nothing
-  const int64_t padded = (K + 15) & ~int64_t{15};
-  if (M == 1) x_row_stride = padded, xs_row_stride = 0, out_row_stride = N;
-  if (N == 1) weight_row_stride = padded;
+  // the stride of a single row means nothing: any that keeps the rows behind it out of range
+  if (M == 1) x_row_stride = kFp8Block, xs_row_stride = 0, out_row_stride = 0;
+  if (N == 1) weight_row_stride = kFp8Block;
   const auto rows_ok = [](const void* ptr, int64_t rows, int64_t stride, int64_t cols) {
     return aligned16(ptr) && (rows == 1 || (stride % 16 == 0 && stride >= cols));
   };
   GDN_REQUIRE(rows_ok(x, M, x_row_stride, K) && rows_ok(weight, N, weight_row_stride, K),
               "gdn_fp8_linear: the rows of x and weight must start at multiples of 16 bytes and not overlap");
-  GDN_REQUIRE(out_row_stride >= N && (reinterpret_cast<uintptr_t>(out) & 1) == 0, "gdn_fp8_linear: bad output rows");
+  GDN_REQUIRE((M == 1 || out_row_stride >= N) && (reinterpret_cast<uintptr_t>(out) & 1) == 0,
+              "gdn_fp8_linear: bad output rows");
   GDN_REQUIRE(((reinterpret_cast<uintptr_t>(x_scales) | reinterpret_cast<uintptr_t>(weight_scales)) & 3) == 0,
               "gdn_fp8_linear: misaligned scales");
   GDN_REQUIRE(xs_row_stride >= 0 && xs_block_stride >= 0 && ws_row_stride >= 0 && ws_block_stride >= 0,
@@ -706,7 +706,8 @@ extern "C" int gdn_fp8_linear(const void* x, int64_t x_row_stride, const float* 
   constexpr int64_t kMostStride = int64_t{1} << 23, kMost = 0x7ffff000;  // rounded up to a tile: still an int
   if (M > kMost || N > kMost || K > kMost || x_row_stride > kMostStride ||
       weight_row_stride > kMostStride || out_row_stride > kMostStride / 2 || xs_row_stride > kMostStride / 4) {
-    set_error("gdn_fp8_linear: sizes or row strides beyond 2^23 are not covered");
+    set_error("gdn_fp8_linear: sizes from 2^31 - 4095 on, and strides between rows beyond 2^23 bytes of x and weight, "
+              "2^22 elements of out and 2^21 of x's scales, are not covered");
     return GDN_ERR_UNSUPPORTED;
   }
   Linear p{static_cast<const uint8_t*>(x), static_cast<const uint8_t*>(weight), x_scales, weight_scales, out,

@@ -255,3 +255,19 @@ def test_weights_are_quantised_without_a_gradient():
     assert not q.values.requires_grad and not q.scales.requires_grad and q.scales.grad_fn is None
     want = quantize_fp8_weight(w.detach())
     assert torch.equal(q.scales, want.scales) and torch.equal(q.dequantize(), want.dequantize())
+
+
+def test_limits_of_strides_are_not_those_of_a_single_row():
+    """Where there is more than one row, they are refused with the limits' own words."""
+    lib = _built()
+    d = 0x10000
+
+    def linear(M, N, K, xst, wst, ost):
+        return lib.gdn_fp8_linear(d, xst, d, 1, 4, d, wst, d, 1, 1, M, N, K, d, 1, ost, None)
+
+    far = 1 << 24
+    for kw in (dict(M=2, N=2, K=128, xst=128, wst=128, ost=(1 << 22) + 1),
+               dict(M=2, N=2, K=128, xst=far, wst=128, ost=2), dict(M=2, N=2, K=128, xst=128, wst=far, ost=2),
+               dict(M=1, N=2, K=far, xst=far, wst=far, ost=2)):
+        assert linear(**kw) == 2, kw
+        assert b"strides between rows" in lib.gdn_last_error()

@@ -39,3 +39,26 @@ def test_a_weight_scale_that_is_not_finite_stays_in_its_block(size, value):
         assert not got[:, part].isfinite().any()
         got[:, part] = clean[:, part]
         assert torch.equal(got, clean)
+
+
+def test_a_single_row_has_no_stride_to_limit():
+    """One token by more than 2^22 columns, and one token by one column over more
+    than 2^23 of K: the stride of a single row means nothing.  Sums of small whole
+    numbers, exact in any order; above 256 they are rounded to bf16 once."""
+    from logssms_amd.kernel import Fp8Tensor, fp8_linear
+    fp8 = torch.float8_e4m3fn
+    g = torch.Generator(device=DEV).manual_seed(1)
+
+    def whole(rows, k):
+        v = torch.randint(-2, 3, (rows, -(-k // 16) * 16), generator=g, device=DEV, dtype=torch.int8)
+        return v.bfloat16().to(fp8)[:, :k]
+
+    for n, k in (((1 << 22) + 1, 128), ((1 << 22) + 24, 40), (1, (1 << 23) + 16), (1, (1 << 23) + 1001)):
+        print(f"fp8_linear single row 1 x {n} x {k}", flush=True)
+        x, w = whole(1, k), whole(n, k)
+        blocks = -(-k // 128)
+        got = fp8_linear(Fp8Tensor(x, torch.ones(1, blocks, device=DEV)),
+                         Fp8Tensor(w, torch.ones(-(-n // 128), blocks, device=DEV)))
+        # the hardware drops nothing: products of a group are at most 4 and at least 1 apart from zero
+        want = (w.float() * x.float()).sum(1) if k < 1000 else (w.double() * x.double()).sum(1).float()
+        assert torch.equal(got, want.bfloat16()[None])
