@@ -696,8 +696,9 @@ int gdn_rms_norm_gated(const void* x, int dtype, int64_t rows, int64_t cols, con
 
 /*
  * h = x + residual (x alone without one); y = h * rsqrt(mean(h^2) + eps) *
- * (weight + weight_offset) per row, in fp32.  Writes any of: residual_out = h
- * and out = y in `dtype`, values / scales = the quantised y.
+ * (weight + weight_offset) per row, in fp32.  Writes out = y in `dtype`, values /
+ * scales = the quantised y, or both; beside them, with a residual and where it is
+ * not NULL, residual_out = h in `dtype`.
  *   x, residual, out, residual_out: [rows, cols], unit column stride, row strides
  *     in elements; residual_out may be the residual itself (or x), whole rows in place.
  *   weight [cols] of `weight_dtype`.

@@ -121,7 +121,7 @@ __global__ __launch_bounds__(B) void norm_block_kernel(NormRows p) {
 #pragma unroll
     for (int v = 0; v < N; ++v) store_row<T, VEC>(p, r, v * B + t, h[v], rn);
   } else {
-    // residual_out may be the residual itself: an element is read and written by the same thread
+    // residual_out may be the residual or x itself: an element is read and written by the same thread
     for (int64_t v = t; v < vecs; v += B) {  // whole 16-lane groups
       load_sum<T, VEC>(p, r, 8 * v, h[0]);
       store_row<T, VEC>(p, r, v, h[0], rn);

@@ -53,7 +53,7 @@ def add_rms_norm(x: torch.Tensor, residual: torch.Tensor, weight: torch.Tensor, 
                  ) -> tuple[torch.Tensor, torch.Tensor]:
     """``rms_norm(x + residual)`` and the sum itself, the next residual, rounded
     to the dtype of ``x`` (the norm takes the unrounded sum).  ``residual_out``
-    may be ``residual``, which is then updated in place; it is allocated when None."""
+    may be ``residual`` or ``x``, which is then updated in place; it is allocated when None."""
     _, _, y, total = _lib.host().rms_norm(x, residual, weight, eps, weight_offset, residual_out, False, True)
     return y, total
 

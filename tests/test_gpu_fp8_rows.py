@@ -289,3 +289,26 @@ def test_gated_heads_of_any_width(case):
     on = wide.to(DEV)
     got = rms_norm_gated_fp8(on[0][..., 1:1 + dim], on[1][..., 2:2 + dim], w.to(DEV), EPS)
     assert_quantised(got, ref.rms_norm_gated(x, z, w, EPS))
+
+
+@pytest.mark.parametrize("dtype", DTYPES, ids=str)
+@pytest.mark.parametrize("cols", [7, 200, 2056, 9001, 17000, 20001])
+def test_the_sum_may_take_the_place_of_x(cols, dtype):
+    """``residual_out`` is ``x``: every form of the norm, aligned and not, rows inside a larger buffer."""
+    from logssms_amd.kernel import add_rms_norm, add_rms_norm_fp8
+    g = gen(cols)
+    w = randn(cols, g=g).to(DEV)
+    for start in (0, 3):
+        wide = randn(6, cols + 8, g=g, dtype=dtype).to(DEV)
+        x, res = wide[1:, start:start + cols], randn(5, cols, g=g, dtype=dtype).to(DEV)
+        kept, before = x.clone(), wide.clone()
+        q1, y1, total = add_rms_norm_fp8(kept, res, w, EPS, keep=True)
+        assert torch.equal(total, (kept.float() + res.float()).to(dtype))
+        y, place = add_rms_norm(x, res, w, EPS, residual_out=x)
+        assert place is x and torch.equal(x, total) and torch.equal(y, y1)
+        x.copy_(kept)
+        q, y, place = add_rms_norm_fp8(x, res, w, EPS, keep=True, residual_out=x)
+        assert place is x and torch.equal(x, total) and torch.equal(y, y1)
+        assert torch.equal(q.scales, q1.scales) and torch.equal(q.dequantize(), q1.dequantize())
+        x.copy_(kept)
+        assert torch.equal(wide, before)
