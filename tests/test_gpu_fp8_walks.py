@@ -62,3 +62,16 @@ def test_a_single_row_has_no_stride_to_limit():
         # the hardware drops nothing: products of a group are at most 4 and at least 1 apart from zero
         want = (w.float() * x.float()).sum(1) if k < 1000 else (w.double() * x.double()).sum(1).float()
         assert torch.equal(got, want.bfloat16()[None])
+
+
+@pytest.mark.parametrize("k", [7, 128, 255, 1041])
+@pytest.mark.parametrize("size", WALKS, ids=str)
+def test_several_tiles_a_block_with_their_tails(size, k):
+    """The turn to the next tile, the end of K in its first step, the scaling that
+    a step leaves to the next, wide and narrow stores behind one another."""
+    form_with_its_tails(size, k)
+
+
+@pytest.mark.parametrize("size", WALKS, ids=str)
+def test_several_tiles_a_block_keep_rows_and_columns_apart(size):
+    keeps_apart(size)
