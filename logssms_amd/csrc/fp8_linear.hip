@@ -253,10 +253,11 @@ template <int WN, int WM, int FN, int FM, int S>
 struct Tile {
   static constexpr int kWaves = WN * WM, kThreads = 64 * kWaves;
   static constexpr int BN = 32 * FN * WN, BM = 32 * FM * WM, kRows = BN + BM;
-  // 8 rows a load, as many loads for each wave; where they come to more than the rows, the rest is out of range
-  static constexpr int JN = (BN / 8 + kWaves - 1) / kWaves, JM = (BM / 8 + kWaves - 1) / kWaves;
+  // 8 rows a load, as many loads for each wave
+  static constexpr int JN = BN / 8 / kWaves, JM = BM / 8 / kWaves;
+  static_assert(JN * 8 * kWaves == BN && JM * 8 * kWaves == BM, "whole loads for each wave");
   // bytes of a step's operands and scales: 32 tokens' scales for a wave, in 256 bytes of its own
-  static constexpr int kW = JN * kWaves * 1024, kX = JM * kWaves * 1024, kS = 256 * kWaves;
+  static constexpr int kW = BN * kFp8Block, kX = BM * kFp8Block, kS = 256 * kWaves;
   static constexpr int kLds = S * (kW + kX + kS);
   static constexpr int kPerCu = 160 * 1024 / kLds, kPerSimd = kPerCu * kWaves / 4;  // blocks, waves
   static constexpr int kStores = 2 * FN * FM;

@@ -248,8 +248,9 @@ constexpr int64_t kFp8Block = 128;
 int64_t blocks_of(int64_t n) { return (n + kFp8Block - 1) / kFp8Block; }
 int64_t padded16(int64_t n) { return (n + 15) / 16 * 16; }
 // The stride of rows of 8-bit values that this package makes: whole cache lines
-// where that adds at most a fifth (2900 x 1111 x 1000: 11.8 us with rows of 1008
-// bytes, 10.7 with rows of 1024).
+// from 513 values on, where that adds at most a quarter (2900 x 1111 x 1000: 11.8
+// us with rows of 1008 bytes, 10.7 with rows of 1024).  kernel/fp8.py lays out
+// weights by the same rule.
 int64_t fp8_stride(int64_t cols) { return cols > 512 ? (cols + 127) / 128 * 128 : padded16(cols); }
 
 void require_device(const at::Tensor& t) {
