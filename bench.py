@@ -459,11 +459,13 @@ def norm_gpu(dev, T=16384, seed=6):
     return step, 3 * T * HV * D * 2
 
 
-def layer_gpu(dev, hidden=2048, seed=7):
+def layer_gpu(dev, hidden=2048, seed=7, fp8=False):
     """The whole GatedDeltaNet layer (Qwen3-Next shape, hidden 2048) on the
     config 2 batch: merged projections (hipBLASLt GEMMs) whose column slices
     feed the backend prefill as strided views, the gated RMS norm and the
-    output projection.  Returns (step, parts): parts times the three stages."""
+    output projection.  Returns (step, parts): parts times the three stages.
+    ``fp8``: the two large projections in block-scaled 8 bits, the layer's own
+    quantisation of its input among them."""
     from logssms_amd.cache import LinearStatePool
     from logssms_amd.core import Batch, Context, Request, set_global_ctx
     from logssms_amd.layers import GatedDeltaNet
@@ -474,6 +476,8 @@ def layer_gpu(dev, hidden=2048, seed=7):
     net.conv1d_weight.normal_(0.0, 0.02, generator=g)
     net.A_log.uniform_(-1.0, 0.0, generator=g)
     net.dt_bias.zero_()
+    if fp8:
+        net.quantize_weights()
     lengths = [4096] * 4
     pool = LinearStatePool(8, 1, CONV_DIM, W, HV, D, D, dev, torch.bfloat16)
     table = torch.arange(8, device=dev, dtype=torch.int32)[:4, None].expand(4, 4096).contiguous()
@@ -909,14 +913,16 @@ def main():
                                              "gate a column slice of a 2x wider projection output",
                                    "ms": ms, "bytes": nb, "GB/s": nb / (ms * 1e-3) / 1e9,
                                    "frac_hbm": nb / (ms * 1e-3) / PEAK_HBM, "traffic": _traffic("norm_vec_kernel_cfg2")}
-    if args.only in ("all", "layer"):
-        step, parts = layer_gpu(dev)
+    # the layer with 8-bit projections beside it only where the layer is asked for
+    for fp8 in {"all": [False], "layer": [False, True]}.get(args.only, []):
+        step, parts = layer_gpu(dev, fp8=fp8)
         ms = _time(step, max(args.steps // 2, 5), args.warmup)
         stages = {k: _time(fn, max(args.steps // 2, 5), args.warmup) for k, fn in parts().items()}
         T = 4 * 4096
-        extra["gated_delta_layer"] = {
+        extra["gated_delta_layer_fp8" if fp8 else "gated_delta_layer"] = {
             "config": "GatedDeltaNet layer, hidden 2048, config 2 batch (4 x 4096): in_proj_qkvz/in_proj_ba GEMMs, "
-                      "GDN prefill on their strided column slices, gated RMS norm, out_proj GEMM",
+                      "GDN prefill on their strided column slices, gated RMS norm, out_proj GEMM"
+                      + (", in_proj_qkvz and out_proj in block-scaled 8 bits" if fp8 else ""),
             "ms": ms, "tokens/s": T / (ms * 1e-3), "stage_ms": stages}
         del step, parts
         torch.cuda.empty_cache()

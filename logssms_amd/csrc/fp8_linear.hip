@@ -242,13 +242,19 @@ __global__ __launch_bounds__(64 * W, 2) void few_rows_kernel(Linear p) {
 // land in lane order, so the lanes' source chunks are permuted instead.
 //
 // What bounds it: 16384 x 12288 x 2048 takes 395 us (2.1 PFLOP/s), 8192^3 460
-// (2.4).  The matrix instructions with the scaling between them, out of
-// registers, reach 4.8 PFLOP/s; under this load the card lowers its clock to
-// 1.8 to 2.0 GHz.  Of the first product's 406 us at the time, the output took
-// 46, the scaling 50 and the second barrier 15 (each left out, by turns); loads
-// that touch the lines of later steps first made it slower.  Where a CU has one
-// tile (256 x 12288 x 2048: 13.5 us, 16 steps) a step takes 0.49 us, 0.24 of
-// them matrix instructions: the rest is the wait for 32 KB from the L2.
+// (2.4): the matrix cores are busy for 53 and 62 % of the cycles, and the load
+// lowers the clock to 1.8 and 1.7 GHz.  The matrix instructions with the scaling
+// between them, out of registers, reach 4.8 PFLOP/s.  Of the first
+// product's 406 us at the time, the output took 46, the scaling 50 and the second
+// barrier 15 (each left out, by turns); loads that touch the lines of later steps
+// first made it slower.  The compiled step waits where it need not: for all
+// eighteen LDS reads before its first matrix instruction; for the stores of the
+// last tile in the first plain step; and for every load in the steps that reload
+// one of the three registers that the 256 x 256 tile spills.  Where a CU has one
+// tile (256 x 12288 x 2048: 13.5 us, 16 steps) a step takes 0.49 us, 0.24 of them
+// matrix instructions.  The four-stage step waits in its middle for all nine reads
+// of the next step's operands, because the scalar load of the weight scale is in
+// flight among them, and scalar loads can only be waited for together.
 template <int WN, int WM, int FN, int FM, int S>
 struct Tile {
   static constexpr int kWaves = WN * WM, kThreads = 64 * kWaves;
@@ -446,7 +452,8 @@ __global__ __launch_bounds__(64 * WN * WM, (Tile<WN, WM, FN, FM, S>::kPerSimd)) 
   // One step.  Plain: not a tile's last one nor the one before, and no place turns to another tile behind it.
   auto one_step = [&](auto plainc) __attribute__((always_inline)) {
     constexpr bool kPlain = decltype(plainc)::value;
-    // all but the newer loads, and what the last tile stored behind them, have landed
+    // all but the newer loads have landed; a step that is not plain leaves the last tile's stores, which are newer
+    // still, in flight too (a plain one, the next step where K has more than a few blocks, waits for most of them)
     if (!kPlain && stored) wait_loads<T::kAhead + T::kStores>(); else wait_loads<T::kAhead>();
     stored = false;
     const bool ends = !kPlain && now.left <= kFp8Block;

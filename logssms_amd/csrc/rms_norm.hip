@@ -159,9 +159,9 @@ struct GatedRows {
 // Heads of 8 G channels, G a power of two: G lanes hold a head, 16 a block of
 // 128 of the flattened row, and both are aligned groups of one wave.  A thread
 // block takes the same columns of 16 rows (8, 4 of wider heads), as the
-// quantisation does.  16384 tokens of 32 heads of 128: 72 us, 4.7 TB/s (with an
-// IEEE division in the gate and a block along the row 84: vector instructions),
-// before the codes' own division.
+// quantisation does.  16384 tokens of 32 heads of 128: 74 us, 4.6 TB/s (72
+// without the codes' own division; then 84 with an IEEE division in the gate and a
+// block along the row: vector instructions).
 template <class T, int G>
 __global__ __launch_bounds__(kThreads) void gated_vec_kernel(GatedRows p, uint32_t spans_per_row) {
   constexpr int kSpan = G > 16 ? G : 16;  // lanes that must stay together
