@@ -75,3 +75,29 @@ def test_several_tiles_a_block_with_their_tails(size, k):
 @pytest.mark.parametrize("size", WALKS, ids=str)
 def test_several_tiles_a_block_keep_rows_and_columns_apart(size):
     keeps_apart(size)
+
+
+@pytest.mark.parametrize("k", [7, 300, 1041])
+@pytest.mark.parametrize("m", [1, 300, 9000, 20000, 70000])
+def test_a_single_column(m, k):
+    """One row of weights, in the forms for few tokens and in each tile that so many tokens take."""
+    form_with_its_tails((m, 1), k)
+
+
+def test_strides_of_single_rows_are_not_read():
+    """Operands, scales and output of one row at strides that no row could have."""
+    from logssms_amd.kernel import Fp8Tensor, fp8_linear
+    for m, n in ((1, 200), (40, 1), (1, 1)):
+        print(f"fp8_linear strides of single rows {m} x {n}", flush=True)
+        x, w = operands(m, n, 272, gen(m + n))
+        dx, dw = to_dev(x), to_dev(w)
+        want = fp8_linear(dx, dw)
+
+        def odd(t, stride):
+            return t.as_strided(t.shape, (stride, t.stride(1))) if t.shape[0] == 1 else t
+
+        for stride in (0, 3, 1 << 40):
+            out = torch.empty(m, n, dtype=torch.bfloat16, device=DEV)
+            got = fp8_linear(Fp8Tensor(odd(dx.values, stride), odd(dx.scales, stride)),
+                             Fp8Tensor(odd(dw.values, stride), odd(dw.scales, stride)), out=odd(out, stride))
+            assert torch.equal(got, want) and torch.equal(out, want)
