@@ -43,8 +43,9 @@ __device__ __forceinline__ float block_scale(uint32_t amax_bits) {
 // start within an ulp and every y around a code's border, the code is the
 // division's, but for the significand of ones.  That one, scales whose residuals
 // could be subnormal, and those that are not finite take the division itself.
-// (The gated norm of 16384 x 32 x 128 takes 79 us with it, 75 without; the other
-// row kernels, further from the vector units' rate, within 2 %.)
+// (It costs the gated norm of 16384 x 32 x 128 2 to 5 %, 72 to 74 us and 75 to 79
+// with other strides of the gate; the other row kernels, further from the vector
+// units' rate, up to 2 %.)
 __device__ __forceinline__ uint2 pack8_fp8(const float (&y)[8], float s) {
   float q[8];
   if (s >= 0x1p-80f && s < 0x1p+120f && (~__float_as_uint(s) & 0x7fffffu)) {
