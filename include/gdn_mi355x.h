@@ -747,6 +747,74 @@ int gdn_fp8_linear(const void* x, int64_t x_row_stride, const float* x_scales, i
                    int out_dtype, int64_t out_row_stride, void* stream);
 
 /*
+ * Rotary positions and a paged cache (no counterpart here of the reference's
+ * attention side).
+ *
+ * Pair i of a head's first `rotated` channels, (x[i], x[i + rotated / 2]) or,
+ * interleaved, (x[2i], x[2i + 1]), is turned by 2 pi turns[i] position and
+ * multiplied by scale; the channels behind them are copied.
+ *   q [tokens, q_heads, dim] and k [tokens, k_heads, dim] (NULL with no heads),
+ *     unit channel stride, of `dtype` (f32, bf16, f16); q_out, k_out like them,
+ *     or the operand itself, whole, in place.
+ *   positions [tokens]; turns [rotated / 2] in 64 bits on the device.
+ * GDN_ERR_UNSUPPORTED from 2^24 channels a token on and for dim above 4096.
+ */
+int gdn_apply_rotary(const void* q, int64_t q_token_stride, int64_t q_head_stride, int64_t q_heads, const void* k,
+                     int64_t k_token_stride, int64_t k_head_stride, int64_t k_heads, int dtype, int64_t tokens,
+                     int64_t dim, const void* positions, int positions_dtype, const double* turns, int64_t rotated,
+                     int interleaved, float scale, void* q_out, int64_t q_out_token_stride, int64_t q_out_head_stride,
+                     void* k_out, int64_t k_out_token_stride, int64_t k_out_head_stride, void* stream);
+
+/*
+ * k_cache[slot / page_size, slot % page_size] = k turned as above, v_cache[...] = v,
+ * for slot = slots[token]; nothing is written for a slot below 0 or from pages *
+ * page_size on.  The slots of one call differ.  q (q_heads 0: none) is turned to q_out.
+ *   k, v [tokens, kv_heads, dim]; caches [pages, page_size, kv_heads, dim] with
+ *   unit channel stride.  rotated 0 (positions and turns unused): k and q as they are.
+ */
+int gdn_append_paged_kv(const void* k, int64_t k_token_stride, int64_t k_head_stride, const void* v,
+                        int64_t v_token_stride, int64_t v_head_stride, int64_t kv_heads, int dtype, int64_t tokens,
+                        int64_t dim, const void* slots, int slots_dtype, void* k_cache, int64_t k_page_stride,
+                        int64_t k_cache_token_stride, int64_t k_cache_head_stride, void* v_cache,
+                        int64_t v_page_stride, int64_t v_cache_token_stride, int64_t v_cache_head_stride,
+                        int64_t pages, int64_t page_size, const void* positions, int positions_dtype,
+                        const double* turns, int64_t rotated, int interleaved, float scale, const void* q,
+                        int64_t q_token_stride, int64_t q_head_stride, int64_t q_heads, void* q_out,
+                        int64_t q_out_token_stride, int64_t q_out_head_stride, void* stream);
+
+/*
+ * Causal attention over a paged cache, the positions that groups of requests share
+ * attended once for each group:
+ *   out[t, h] = sum_p softmax_p(scale q[t, h] . k[p, h / (heads / kv_heads)]) v[p, ...]
+ * Request r owns the tokens cu_seqlens[r] .. cu_seqlens[r + 1] - 1 (token r without
+ * cu_seqlens), the last of its seq_lens[r] positions: the last of them sees them
+ * all, each one before it one less.  Position p of it lies in page
+ * page_table[r, p / page_size]; an entry outside of the cache stands for zero keys
+ * and values; positions past the table are not there.  A token that sees nothing
+ * gives zeros (lse -infinity); tokens that no request owns are left as they were.
+ *   Group g holds the requests group_offsets[g] .. group_offsets[g + 1] - 1 (all of
+ *   them without offsets); their first shared_lens[g] positions have to lie in
+ *   the same pages: they are read through the first request's row.
+ *   q, out [tokens, heads, dim] bf16 or f16, caches [pages, page_size, kv_heads,
+ *   dim] alike, unit channel stride, rows at multiples of 16 bytes (out: 8);
+ *   page_size a multiple of 16; lse fp32 [tokens, heads] (natural logarithm) or NULL.
+ * dim 64, 128 or 256 (GDN_ERR_UNSUPPORTED beyond).  Sums and statistics are fp32;
+ * the softmax's weights are rounded to the io type in front of the product with v.
+ * workspace: gdn_paged_attention_workspace_bytes, varlen 1 with cu_seqlens.
+ */
+int64_t gdn_paged_attention_workspace_bytes(int64_t tokens, int64_t requests, int64_t groups, int64_t heads,
+                                            int64_t kv_heads, int64_t dim, int varlen);
+int gdn_paged_attention(const void* q, int64_t q_token_stride, int64_t q_head_stride, int dtype, int64_t tokens,
+                        int64_t heads, int64_t dim, const void* k_cache, int64_t k_page_stride, int64_t k_token_stride,
+                        int64_t k_head_stride, const void* v_cache, int64_t v_page_stride, int64_t v_token_stride,
+                        int64_t v_head_stride, int64_t kv_heads, int64_t pages, int64_t page_size,
+                        const void* page_table, int table_dtype, int64_t table_row_stride, int64_t table_width,
+                        const void* seq_lens, int lens_dtype, int64_t requests, const void* shared_lens,
+                        int shared_dtype, const void* group_offsets, int offsets_dtype, int64_t groups,
+                        const void* cu_seqlens, int cu_dtype, float scale, void* out, int64_t out_token_stride,
+                        int64_t out_head_stride, float* lse, void* workspace, int64_t workspace_bytes, void* stream);
+
+/*
  * No counterpart in the reference.  For callers that cannot allocate device
  * memory (code under HIP graph capture, serving loops or harnesses that
  * forbid hipMalloc): the fused prefill of gdn_prefill_qk + gdn_prefill_fused

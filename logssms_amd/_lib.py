@@ -54,6 +54,13 @@ SIGNATURES = {
     "gdn_quantize_fp8": [P, I32, I64, I64, I64, P, I64, P, I64, I64, P],
     "gdn_rms_norm_gated_fp8": [P, I32, I64, I64, I64, I64, I64, P, I64, I64, P, I32, F32, P, I64, P, I64, I64, P],
     "gdn_fp8_linear": [P, I64, P, I64, I64, P, I64, P, I64, I64, I64, I64, I64, P, I32, I64, P],
+    "gdn_apply_rotary": [P, I64, I64, I64, P, I64, I64, I64, I32, I64, I64, P, I32, P, I64, I32, F32, P, I64, I64, P,
+                         I64, I64, P],
+    "gdn_append_paged_kv": [P, I64, I64, P, I64, I64, I64, I32, I64, I64, P, I32, P, I64, I64, I64, P, I64, I64, I64,
+                            I64, I64, P, I32, P, I64, I32, F32, P, I64, I64, I64, P, I64, I64, P],
+    "gdn_paged_attention_workspace_bytes": [I64, I64, I64, I64, I64, I64, I32],
+    "gdn_paged_attention": [P, I64, I64, I32, I64, I64, I64, P, I64, I64, I64, P, I64, I64, I64, I64, I64, I64, P,
+                            I32, I64, I64, P, I32, I64, P, I32, P, I32, I64, P, I32, F32, P, I64, I64, P, P, I64, P],
     "gdn_conv_snapshots": [P, I64, I32, P, I32, I64, I64, I64, I32, P, I64, I64, I64, P, I32, P, I32, P, I32, I64,
                            P],
     "gdn_chunk_gated_delta_rule": [P, P, P, I32, P, P, P, I32, I64, I64, I64, I64, I64, I64, P, I32, I64, I64, I64,

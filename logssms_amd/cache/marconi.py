@@ -146,6 +146,15 @@ class HybridBlockPool:
         return self.storage.as_strided((starts, self.layout.layers_per_group, *inner_shape),
                                        (block_stride, lane_stride, *inner), storage_offset=offset)
 
+    def kv_cache(self, lane: int) -> tuple[torch.Tensor, torch.Tensor]:
+        """Keys and values of full-attention layer ``lane``, ``[blocks, block size, kv
+        heads, head dim]`` each: a block that holds tokens has their keys, then
+        their values.  The caches that ``append_paged_kv`` writes and
+        ``paged_attention`` reads, a block being a page."""
+        layout = self.layout
+        blocks = self.storage[lane].view(self.num_blocks, 2, layout.block_size, layout.kv_heads, layout.head_dim)
+        return blocks[:, 0], blocks[:, 1]
+
     @property
     def device(self):
         return self._device

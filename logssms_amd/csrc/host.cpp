@@ -5,7 +5,9 @@
 //   * conv_recurrent, the checks and the call of one decode or verify step
 //     with tensors in hand;
 //   * rms_norm, quantize_fp8, rms_norm_gated_fp8 and fp8_linear, the same for
-//     the 8-bit projections.
+//     the 8-bit projections;
+//   * apply_rotary, append_paged_kv and paged_attention, the same for the
+//     full-attention layers.
 // A decode step of one sequence is an 8 us kernel behind what the host does
 // to launch it: 15.8 us in Python and ctypes, 5.8 us through this module.
 #include <Python.h>
@@ -51,7 +53,11 @@ namespace {
   X(gdn_rms_norm)                         \
   X(gdn_quantize_fp8)                     \
   X(gdn_rms_norm_gated_fp8)               \
-  X(gdn_fp8_linear)
+  X(gdn_fp8_linear)                       \
+  X(gdn_apply_rotary)                     \
+  X(gdn_append_paged_kv)                  \
+  X(gdn_paged_attention_workspace_bytes)  \
+  X(gdn_paged_attention)
 namespace lib {
 #define GDN_POINTER(name) decltype(&::name) name = nullptr;
 GDN_TYPED(GDN_POINTER)
@@ -493,6 +499,225 @@ PyObject* fp8_linear(PyObject*, PyObject* const* args, Py_ssize_t n) {
   END_HANDLE_TH_ERRORS
 }
 
+// ---------------------------------------------------------------- full attention
+int64_t span(const at::Tensor& t, int64_t d) { return t.size(d) > 1 ? t.stride(d) * (t.size(d) - 1) : 0; }
+// Rows [tokens, heads, dim] of unit channel stride, none on top of another.
+bool apart(const at::Tensor& t) {
+  if (t.numel() == 0) return true;
+  const int64_t dim = t.size(2);
+  if (dim > 1 && t.stride(2) != 1) return false;
+  auto nested = [&](int64_t inner, int64_t outer) {
+    return (t.size(inner) == 1 || t.stride(inner) >= dim) &&
+           (t.size(outer) == 1 || t.stride(outer) >= span(t, inner) + dim);
+  };
+  return nested(1, 0) || nested(0, 1);
+}
+// A stride that is walked: 0 along an axis of one, whatever the view says.
+int64_t step(const at::Tensor& t, int64_t d) { return t.size(d) > 1 ? t.stride(d) : 0; }
+at::Tensor unit_channels(const at::Tensor& t) { return t.size(2) == 1 || t.stride(2) == 1 ? t : t.contiguous(); }
+// One index for each of n, side by side.
+at::Tensor indices(const at::Tensor& t, int64_t n, const at::Tensor& like, const char* what) {
+  require(t.dim() == 1 && t.size(0) == n, what);
+  require(t.device() == like.device(), "all operands on one device");
+  index_code(t);
+  return t.is_contiguous() ? t : t.contiguous();
+}
+
+struct Turns {
+  at::Tensor positions, turns;
+  int64_t rotated = 0;
+  const void* positions_at() const { return positions.defined() ? positions.data_ptr() : nullptr; }
+  const double* turns_at() const { return turns.defined() ? turns.data_ptr<double>() : nullptr; }
+  int code() const { return positions.defined() ? index_code(positions) : GDN_I32; }
+};
+Turns turns_of(PyObject* positions, PyObject* turns, const at::Tensor& x) {
+  Turns t;
+  const at::Tensor& given = tensor(turns);
+  require(given.dim() == 1 && given.scalar_type() == at::kDouble, "frequencies must be float64 [rotated / 2]");
+  require(given.device() == x.device(), "all operands on one device");
+  t.turns = given.contiguous();
+  t.rotated = 2 * given.size(0);
+  require(t.rotated <= x.size(2), "more rotated channels than the head has");
+  t.positions = indices(tensor(positions), x.size(0), x, "positions must be [tokens]");
+  return t;
+}
+
+// The result of rotating x: given (like x, its rows apart) or fresh.
+at::Tensor rotated_out(PyObject* given, const at::Tensor& x) {
+  if (given == Py_None) return fresh(x.sizes(), x.scalar_type(), x);
+  const at::Tensor& out = tensor(given);
+  require(out.sizes() == x.sizes() && out.scalar_type() == x.scalar_type() && out.device() == x.device(),
+          "an output must be like its input");
+  require(apart(out), "an output needs rows of unit stride that do not overlap");
+  return out;
+}
+
+// apply_rotary(q, k or None, positions, turns, interleaved, scale, q_out or None, k_out or None) -> (q_out, k_out)
+PyObject* apply_rotary(PyObject*, PyObject* const* args, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  try {
+    require(n == 8, "apply_rotary: 8 arguments expected");
+    const at::Tensor& given = tensor(args[0]);
+    require(given.dim() == 3 && given.size(2) > 0, "q must be [tokens, heads, dim]");
+    const int code = dtype_code(given);
+    at::Tensor k, k_out;
+    if (args[1] != Py_None) {
+      const at::Tensor& given_k = tensor(args[1]);
+      require(given_k.dim() == 3 && given_k.size(0) == given.size(0) && given_k.size(2) == given.size(2) &&
+                  given_k.scalar_type() == given.scalar_type() && given_k.device() == given.device(),
+              "k must be [tokens, heads, dim] like q");
+      k = unit_channels(given_k);
+    } else {
+      require(args[7] == Py_None, "k_out without k");
+    }
+    const at::Tensor q = unit_channels(given);
+    const Turns t = turns_of(args[2], args[3], q);
+    const bool interleaved = truth(args[4]);
+    const float scale = real(args[5]);
+    const at::Tensor q_out = rotated_out(args[6], q);
+    if (k.defined()) k_out = rotated_out(args[7], k);
+    require_device(q);
+    const bool both = k.defined();
+    launch("gdn_apply_rotary", lib::gdn_apply_rotary, q, q.data_ptr(), step(q, 0), step(q, 1), q.size(1),
+           both ? k.data_ptr() : nullptr, both ? step(k, 0) : 0, both ? step(k, 1) : 0, both ? k.size(1) : 0, code,
+           q.size(0), q.size(2), t.positions_at(), t.code(), t.turns_at(), t.rotated, interleaved ? 1 : 0, scale,
+           q_out.data_ptr(), step(q_out, 0), step(q_out, 1), both ? k_out.data_ptr() : nullptr,
+           both ? step(k_out, 0) : 0, both ? step(k_out, 1) : 0);
+    return tuple_of(q_out, k_out);
+  } catch (const Failed&) {
+    return nullptr;
+  }
+  END_HANDLE_TH_ERRORS
+}
+
+void check_cache(const at::Tensor& cache, const at::Tensor& like, int64_t heads, int64_t dim) {
+  require(cache.dim() == 4 && cache.size(2) == heads && cache.size(3) == dim && cache.size(1) > 0,
+          "a cache must be [pages, page size, kv heads, dim]");
+  require(cache.scalar_type() == like.scalar_type() && cache.device() == like.device(),
+          "caches must have the dtype and the device of what goes with them");
+  require(dim == 1 || cache.stride(3) == 1, "a cache needs unit channel stride");
+}
+
+// append_paged_kv(k, v, k_cache, v_cache, slots, positions or None, turns or None, interleaved, scale, q or None,
+//   q_out or None) -> q_out or None
+PyObject* append_paged_kv(PyObject*, PyObject* const* args, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  try {
+    require(n == 11, "append_paged_kv: 11 arguments expected");
+    const at::Tensor &given_k = tensor(args[0]), &given_v = tensor(args[1]), &k_cache = tensor(args[2]),
+                     &v_cache = tensor(args[3]);
+    require(given_k.dim() == 3 && given_k.size(1) > 0 && given_k.size(2) > 0, "k must be [tokens, kv heads, dim]");
+    require(given_v.sizes() == given_k.sizes() && given_v.scalar_type() == given_k.scalar_type() &&
+                given_v.device() == given_k.device(),
+            "v must be like k");
+    const int code = dtype_code(given_k);
+    const at::Tensor k = unit_channels(given_k), v = unit_channels(given_v);
+    const int64_t tokens = k.size(0), heads = k.size(1), dim = k.size(2);
+    check_cache(k_cache, k, heads, dim);
+    check_cache(v_cache, k, heads, dim);
+    require(v_cache.size(0) == k_cache.size(0) && v_cache.size(1) == k_cache.size(1), "caches of one size");
+    const at::Tensor slots = indices(tensor(args[4]), tokens, k, "slots must be [tokens]");
+    Turns t;
+    require((args[5] == Py_None) == (args[6] == Py_None), "positions go with a rotation");
+    if (args[6] != Py_None) t = turns_of(args[5], args[6], k);
+    const bool interleaved = truth(args[7]);
+    const float scale = real(args[8]);
+    at::Tensor q, q_out;
+    if (args[9] != Py_None) {
+      const at::Tensor& given_q = tensor(args[9]);
+      require(given_q.dim() == 3 && given_q.size(0) == tokens && given_q.size(2) == dim &&
+                  given_q.scalar_type() == k.scalar_type() && given_q.device() == k.device(),
+              "q must be [tokens, heads, dim] like k");
+      q = unit_channels(given_q);
+      q_out = rotated_out(args[10], q);
+    } else {
+      require(args[10] == Py_None, "q_out without q");
+    }
+    require_device(k);
+    const bool with_q = q.defined();
+    launch("gdn_append_paged_kv", lib::gdn_append_paged_kv, k, k.data_ptr(), step(k, 0), step(k, 1), v.data_ptr(),
+           step(v, 0), step(v, 1), heads, code, tokens, dim, slots.data_ptr(), index_code(slots), k_cache.data_ptr(),
+           step(k_cache, 0), step(k_cache, 1), step(k_cache, 2), v_cache.data_ptr(), step(v_cache, 0),
+           step(v_cache, 1), step(v_cache, 2), k_cache.size(0), k_cache.size(1), t.positions_at(), t.code(),
+           t.turns_at(), t.rotated, interleaved ? 1 : 0, scale, with_q ? q.data_ptr() : nullptr,
+           with_q ? step(q, 0) : 0, with_q ? step(q, 1) : 0, with_q ? q.size(1) : 0,
+           with_q ? q_out.data_ptr() : nullptr, with_q ? step(q_out, 0) : 0, with_q ? step(q_out, 1) : 0);
+    return wrap(q_out);
+  } catch (const Failed&) {
+    return nullptr;
+  }
+  END_HANDLE_TH_ERRORS
+}
+
+// paged_attention(q, k_cache, v_cache, page_table, seq_lens, shared_lens or None, group_offsets or None,
+//   cu_seqlens or None, scale, out or None, lse) -> (out, lse or None)
+PyObject* paged_attention(PyObject*, PyObject* const* args, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  try {
+    require(n == 11, "paged_attention: 11 arguments expected");
+    const at::Tensor &given = tensor(args[0]), &k_cache = tensor(args[1]), &v_cache = tensor(args[2]),
+                     &given_table = tensor(args[3]);
+    require(given.dim() == 3 && given.size(1) > 0 && given.size(2) > 0, "q must be [tokens, heads, dim]");
+    const int code = dtype_code(given);
+    const int64_t tokens = given.size(0), heads = given.size(1), dim = given.size(2);
+    require(code != GDN_F32, "q must be bfloat16 or float16");
+    require(k_cache.dim() == 4 && k_cache.size(2) > 0 && heads % k_cache.size(2) == 0,
+            "the query heads must be a multiple of the key heads");
+    check_cache(k_cache, given, k_cache.size(2), dim);
+    check_cache(v_cache, given, k_cache.size(2), dim);
+    require(v_cache.size(0) == k_cache.size(0) && v_cache.size(1) == k_cache.size(1), "caches of one size");
+    // rows at multiples of 16 bytes; a copy where they are not
+    const bool wide = given.stride(2) == 1 && step(given, 0) % 8 == 0 && step(given, 1) % 8 == 0 &&
+                      reinterpret_cast<uintptr_t>(given.data_ptr()) % 16 == 0;
+    const at::Tensor q = wide ? given : given.is_contiguous() ? given.clone() : given.contiguous();
+    require(given_table.dim() == 2, "page_table must be [requests, pages]");
+    require(given_table.device() == q.device(), "all operands on one device");
+    const int table_code = index_code(given_table);
+    const at::Tensor table = given_table.size(1) <= 1 || given_table.stride(1) == 1 ? given_table : given_table.contiguous();
+    const int64_t requests = table.size(0);
+    const at::Tensor lens = indices(tensor(args[4]), requests, q, "seq_lens must be [requests]");
+    at::Tensor shared, offsets, cu;
+    if (args[5] != Py_None) {
+      const at::Tensor& t = tensor(args[5]);
+      require(t.dim() == 1 && t.size(0) > 0, "shared_lens must be [groups]");
+      shared = indices(t, t.size(0), q, "shared_lens must be [groups]");
+    }
+    const int64_t groups = shared.defined() ? shared.size(0) : 0;
+    if (args[6] != Py_None) {
+      require(shared.defined(), "group_offsets without shared_lens");
+      offsets = indices(tensor(args[6]), groups + 1, q, "group_offsets must be [groups + 1]");
+    }
+    require(groups <= 1 || offsets.defined(), "several groups need their offsets");
+    if (args[7] != Py_None)
+      cu = indices(tensor(args[7]), requests + 1, q, "cu_seqlens must be [requests + 1]");
+    else
+      require(tokens == requests, "one token for each request without cu_seqlens");
+    const float scale = real(args[8]);
+    at::Tensor out = args[9] == Py_None ? fresh(q.sizes(), q.scalar_type(), q) : tensor(args[9]), lse;
+    require(out.sizes() == q.sizes() && out.scalar_type() == q.scalar_type() && out.device() == q.device(),
+            "out must be like q");
+    require(apart(out), "out needs rows of unit stride that do not overlap");
+    require_device(q);
+    if (truth(args[10])) lse = fresh({tokens, heads}, at::kFloat, q);
+    if (!bound(lib::gdn_paged_attention_workspace_bytes != nullptr)) throw Failed();
+    const int64_t bytes = lib::gdn_paged_attention_workspace_bytes(tokens, requests, groups, heads, k_cache.size(2), dim,
+                                                                   cu.defined() ? 1 : 0);
+    const at::Tensor workspace = fresh({bytes}, at::kByte, q);
+    auto at_of = [](const at::Tensor& t) -> void* { return t.defined() ? t.data_ptr() : nullptr; };
+    auto code_of = [](const at::Tensor& t) { return t.defined() ? index_code(t) : GDN_I32; };
+    launch("gdn_paged_attention", lib::gdn_paged_attention, q, q.data_ptr(), step(q, 0), step(q, 1), code, tokens,
+           heads, dim, k_cache.data_ptr(), step(k_cache, 0), step(k_cache, 1), step(k_cache, 2), v_cache.data_ptr(),
+           step(v_cache, 0), step(v_cache, 1), step(v_cache, 2), k_cache.size(2), k_cache.size(0), k_cache.size(1),
+           table.data_ptr(), table_code, table.stride(0), table.size(1), lens.data_ptr(), index_code(lens), requests,
+           at_of(shared), code_of(shared), at_of(offsets), code_of(offsets), groups, at_of(cu), code_of(cu), scale,
+           out.data_ptr(), step(out, 0), step(out, 1), static_cast<float*>(at_of(lse)), workspace.data_ptr(), bytes);
+    return tuple_of(out, lse);
+  } catch (const Failed&) {
+    return nullptr;
+  }
+  END_HANDLE_TH_ERRORS
+}
+
 #define GDN_METHOD(name) {#name, reinterpret_cast<PyCFunction>(&Entry<&lib::name>::call), METH_FASTCALL, nullptr},
 PyMethodDef kMethods[] = {
     {"bind", &bind, METH_O, nullptr},
@@ -501,6 +726,9 @@ PyMethodDef kMethods[] = {
     {"quantize_fp8", &quantize_fp8, METH_O, nullptr},
     {"rms_norm_gated_fp8", reinterpret_cast<PyCFunction>(&rms_norm_gated_fp8), METH_FASTCALL, nullptr},
     {"fp8_linear", reinterpret_cast<PyCFunction>(&fp8_linear), METH_FASTCALL, nullptr},
+    {"apply_rotary", reinterpret_cast<PyCFunction>(&apply_rotary), METH_FASTCALL, nullptr},
+    {"append_paged_kv", reinterpret_cast<PyCFunction>(&append_paged_kv), METH_FASTCALL, nullptr},
+    {"paged_attention", reinterpret_cast<PyCFunction>(&paged_attention), METH_FASTCALL, nullptr},
     GDN_TYPED(GDN_METHOD)
     {nullptr, nullptr, 0, nullptr}};
 PyModuleDef kModule = {PyModuleDef_HEAD_INIT, "_host", nullptr, -1, kMethods, nullptr, nullptr, nullptr, nullptr};

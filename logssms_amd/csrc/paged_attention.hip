@@ -1,0 +1,964 @@
+// Attention over a paged cache for a batch whose requests share prefixes.
+//
+//   o[t, h] = sum_p softmax_p(scale q[t, h] . k[p]) v[p],  p visible to t
+//
+// over the positions p of the request that token t belongs to.  The positions
+// that a group of requests shares are attended once for the group: all of its
+// queries are the rows of one product with the shared keys.  The positions behind
+// them are attended request by request.  Each piece of that work leaves, per row,
+// the running maximum m and sum l of its scores and the unnormalised sum of the
+// values; a last kernel joins the pieces of a row.
+//
+// A row is one (token, query head): the rows of a key head are the `per` query
+// heads that read it, token after token.  Work is cut into items: (segment, key
+// head, range of keys, tile of rows), where a segment is a group's shared
+// positions or a request's own.  Every block counts the items from the lengths on
+// the device (schedule), so that a captured call follows them at each replay.
+//
+// All products are transposed: S^T = K Q^T and O^T = V^T P^T on 32x32x16 matrix
+// instructions.  A lane then holds scores, maximum, sum and output of one row (and
+// another lane the other half of its keys), so that a row's statistics take one
+// exchange between two lanes, and the accumulators of S^T are the right operand
+// of the second product as they stand, with the keys of each 16 in the order
+// 0-3, 8-11 | 4-7, 12-15, in which V is read as well.
+#include <algorithm>
+
+#include "common.hpp"
+
+namespace gdn {
+namespace {
+
+typedef float f32x16 __attribute__((ext_vector_type(16)));
+typedef short s16x4 __attribute__((ext_vector_type(4)));
+typedef short s16x8 __attribute__((ext_vector_type(8)));
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
+typedef __attribute__((address_space(3))) void lds_void;
+
+constexpr int kFew = 32;        // rows of a segment up to which its waves split the keys instead of the rows
+constexpr int kThreads = 256;   // of every kernel here
+constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
+constexpr float kLater = 8.0f;  // a maximum may lag by 2^8 before the sums are rescaled
+
+struct Cache {
+  const void* at;
+  int64_t page, token, head;  // strides, elements
+};
+
+struct Attend {
+  const void* q;
+  int64_t q_token, q_head;
+  Cache k, v;
+  const void* table;  // [requests, width] pages
+  int64_t table_row;
+  const void *lens, *shared, *groups, *cu;  // shared NULL: nothing shared; groups NULL: one; cu NULL: a token each
+  int table_is64, lens_is64, shared_is64, groups_is64, cu_is64;
+  int tokens, requests, num_groups, heads, kv_heads, per;
+  int pages, capacity;  // of the cache; positions of a row of the table
+  Div32 page;
+  float factor;  // scale log2 e
+  void* out;
+  int64_t out_token, out_head;
+  float* lse;  // [tokens, heads] or NULL
+  // workspace: per kind (0: few rows, 1: many) the items' sums [items, rows, dim], statistics (m, l) [items, rows];
+  // the first item and the number of key ranges of each segment
+  float* sums[2];
+  float2* stats[2];
+  int items_max[2], target[2], min_units[2];
+  int2* places;
+};
+
+// ------------------------------------------------------------------ segments
+struct Segment {
+  int token, tokens;  // first query token, their number
+  int lo, hi;         // positions
+  int request;        // whose row of the table is read
+};
+
+__device__ __forceinline__ int uniform(int v) { return __builtin_amdgcn_readfirstlane(v); }
+__device__ __forceinline__ int clampi(int64_t v, int lo, int hi) {
+  return static_cast<int>(v < lo ? lo : v > hi ? hi : v);
+}
+__device__ __forceinline__ int token_of(const Attend& p, int request) {
+  return p.cu ? clampi(load_index(p.cu, request, p.cu_is64), 0, p.tokens) : request;
+}
+__device__ __forceinline__ int group_start(const Attend& p, int g) {
+  return p.groups ? clampi(load_index(p.groups, g, p.groups_is64), 0, p.requests) : g == 0 ? 0 : p.requests;
+}
+__device__ __forceinline__ int shared_of(const Attend& p, int g) {
+  return clampi(load_index(p.shared, g, p.shared_is64), 0, p.capacity);
+}
+// The group of a request: the last that starts at or before it, or -1 where its end does not reach it.
+__device__ __forceinline__ int group_of(const Attend& p, int request) {
+  if (!p.shared) return -1;
+  int lo = 0, hi = p.num_groups - 1;
+  while (lo < hi) {
+    const int mid = (lo + hi + 1) >> 1;
+    if (group_start(p, mid) <= request) lo = mid; else hi = mid - 1;
+  }
+  return group_start(p, lo) <= request && request < group_start(p, lo + 1) ? lo : -1;
+}
+__device__ __forceinline__ int shared_before(const Attend& p, int request) {
+  const int g = group_of(p, request);
+  return g < 0 ? 0 : shared_of(p, g);
+}
+__device__ __forceinline__ int segments_of(const Attend& p) { return p.requests + (p.shared ? p.num_groups : 0); }
+
+__device__ __forceinline__ Segment segment(const Attend& p, int s) {
+  Segment seg;
+  const int shared = p.shared ? p.num_groups : 0;
+  if (s < shared) {
+    const int r0 = group_start(p, s), r1 = max(r0, group_start(p, s + 1));
+    seg.token = token_of(p, r0);
+    seg.tokens = max(0, token_of(p, r1) - seg.token);
+    seg.lo = 0;
+    seg.hi = shared_of(p, s);
+    seg.request = min(r0, p.requests - 1);
+  } else {
+    const int r = s - shared;
+    seg.token = token_of(p, r);
+    seg.tokens = max(0, token_of(p, r + 1) - seg.token);
+    seg.lo = shared_before(p, r);
+    seg.hi = clampi(load_index(p.lens, r, p.lens_is64), 0, p.capacity);
+    seg.request = r;
+  }
+  return seg;
+}
+
+// Cut of a segment: tiles of `rows` rows and units of `unit` positions from a multiple of 16 on.
+struct Cut {
+  int tiles, units;
+};
+template <bool MANY, int ROWS, int UNIT>
+__device__ __forceinline__ Cut cut_of(const Attend& p, const Segment& seg) {
+  const int rows = seg.tokens * p.per, from = seg.lo & ~15;
+  if (rows == 0 || (rows > kFew) != MANY || seg.hi <= seg.lo) return {0, 0};
+  return {(rows + ROWS - 1) / ROWS, (seg.hi - from + UNIT - 1) / UNIT};
+}
+
+// ------------------------------------------------------------------ schedule
+struct Plan {
+  int base[kThreads + 2];  // items before each thread's segments, and all of them
+  int64_t units[kThreads / 64];
+  int count[kThreads / 64];
+};
+
+// Counts the items of the launch: thread i answers for `each` consecutive
+// segments.  A range of keys is as long as it has to be for `target` items.
+// Block 0 notes for the joining kernel where each segment's items lie.
+template <bool MANY, int ROWS, int UNIT>
+__device__ int schedule(const Attend& p, Plan& plan, int& each, int& range) {
+  const int n = segments_of(p), lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  each = (n + kThreads - 1) / kThreads;
+  const int from = threadIdx.x * each, to = min(n, from + each);
+  int64_t units = 0;
+  Cut first{0, 0};
+  for (int s = from; s < to; ++s) {
+    const Cut c = cut_of<MANY, ROWS, UNIT>(p, segment(p, s));
+    if (s == from) first = c;
+    units += static_cast<int64_t>(c.tiles) * c.units;
+  }
+#pragma unroll
+  for (int off = 32; off > 0; off >>= 1) units += __shfl_xor(units, off, 64);
+  if (lane == 0) plan.units[wave] = units;
+  __syncthreads();
+  units = 0;
+#pragma unroll
+  for (int w = 0; w < kThreads / 64; ++w) units += plan.units[w];
+  const int64_t wanted = (units * p.kv_heads + p.target[MANY] - 1) / p.target[MANY];
+  range = static_cast<int>(wanted < p.min_units[MANY] ? p.min_units[MANY] : wanted);
+  int items = 0;
+  for (int s = from; s < to; ++s) {
+    const Cut c = s == from ? first : cut_of<MANY, ROWS, UNIT>(p, segment(p, s));
+    items += c.tiles * p.kv_heads * ((c.units + range - 1) / range);
+  }
+  int sum = items;
+#pragma unroll
+  for (int off = 1; off < 64; off <<= 1) {
+    const int below = __shfl_up(sum, off, 64);
+    if (lane >= off) sum += below;
+  }
+  if (lane == 63) plan.count[wave] = sum;
+  __syncthreads();
+  int before = sum - items, total = 0;
+#pragma unroll
+  for (int w = 0; w < kThreads / 64; ++w) {
+    if (w < wave) before += plan.count[w];
+    total += plan.count[w];
+  }
+  plan.base[threadIdx.x] = before;
+  if (threadIdx.x == 0) plan.base[kThreads] = total;
+  if (blockIdx.x == 0)
+    for (int s = from; s < to; ++s) {
+      const Segment seg = segment(p, s);
+      const Cut c = cut_of<MANY, ROWS, UNIT>(p, seg);
+      const int ranges = (c.units + range - 1) / range;
+      if ((seg.tokens * p.per > kFew) == MANY) p.places[s] = make_int2(before, ranges);
+      before += c.tiles * p.kv_heads * ranges;
+    }
+  __syncthreads();
+  return min(total, p.items_max[MANY]);
+}
+
+typedef float2 Stats[4][32];  // maximum and sum of four waves' rows
+// One LDS array holds it all in a kernel with direct loads: beside a second one, the
+// compiler waits for every load in flight in front of each read.
+static_assert(sizeof(Plan) % 8 == 0, "what lies behind it is aligned");
+
+struct Item {
+  Segment seg;
+  int head, tile;  // key head, tile of rows
+  int from, to;    // positions, from a multiple of 16
+  int ranges;      // of the segment
+  bool own;        // of a request, not of a group
+};
+
+template <bool MANY, int ROWS, int UNIT>
+__device__ Item item_of(const Attend& p, const Plan& plan, int each, int range, int item) {
+  int lo = 0, hi = kThreads - 1;  // the last thread whose base is at most item
+  while (lo < hi) {
+    const int mid = (lo + hi + 1) >> 1;
+    if (plan.base[mid] <= item) lo = mid; else hi = mid - 1;
+  }
+  int at = item - plan.base[lo];
+  const int last = min(segments_of(p), (lo + 1) * each) - 1;
+  for (int s = lo * each;; ++s) {
+    const Segment seg = segment(p, s);
+    const Cut c = cut_of<MANY, ROWS, UNIT>(p, seg);
+    const int ranges = (c.units + range - 1) / range, items = c.tiles * p.kv_heads * ranges;
+    if (at < items || s >= last) {
+      // the same in all lanes: kept in scalar registers
+      Item it;
+      it.seg = {uniform(seg.token), uniform(seg.tokens), uniform(seg.lo), uniform(seg.hi), uniform(seg.request)};
+      it.ranges = uniform(ranges);
+      it.own = uniform(s) >= segments_of(p) - p.requests;
+      const int tiles = max(1, c.tiles), across = at / tiles, head = across / max(1, ranges);
+      it.tile = uniform(at - across * tiles);
+      it.head = uniform(head);
+      it.from = uniform((seg.lo & ~15) + (across - head * max(1, ranges)) * range * UNIT);
+      it.to = min(it.seg.hi, it.from + uniform(range) * UNIT);
+      return it;
+    }
+    at -= items;
+  }
+}
+
+// ------------------------------------------------------------------ matrix instructions and loads
+template <class T> struct Op;
+template <> struct Op<bf16> {
+  using frag = bf16x8;
+  static constexpr uint32_t kExponent = 0x7f80;
+  static __device__ __forceinline__ f32x16 mma(frag a, frag b, f32x16 c) {
+    return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0);
+  }
+};
+template <> struct Op<f16> {
+  using frag = f16x8;
+  static constexpr uint32_t kExponent = 0x7c00;
+  static __device__ __forceinline__ f32x16 mma(frag a, frag b, f32x16 c) {
+    return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0);
+  }
+};
+
+__device__ __forceinline__ int page_at(const Attend& p, int request, int index) {
+  typedef const __attribute__((address_space(4))) int32_t const_int;  // scalar loads
+  const int64_t at = static_cast<int64_t>(request) * p.table_row + index;
+  return *(const_int*)(static_cast<const int32_t*>(p.table) + (p.table_is64 ? 2 * at : at));
+}
+
+template <int N> __device__ __forceinline__ void wait_loads() { asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory"); }
+__device__ __forceinline__ void reads_done() { asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory"); }
+__device__ __forceinline__ void lds_barrier() { asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory"); }
+
+// Rows of a head in LDS: [positions][dim], pieces of 16 bytes.  Those of K lie
+// at piece ^ (row % 16), those of V at piece ^ 4 (row % 4) (rows of 128 bytes, two
+// of which fill the 64 banks: half as many), so that the lanes of one read touch
+// different banks: K is read by 16 rows at the same piece, V by 4 rows at 4.
+template <int D> struct Tile {
+  static constexpr int kPieces = D / 8, kRow = 2 * D;
+  static constexpr int kPerLoad = 1024 / kRow;  // rows that a wave's load of 16 bytes a lane brings
+  static __device__ __forceinline__ int swizzle_k(int row) { return D == 64 ? (row >> 1) & 7 : row & 15; }
+  static __device__ __forceinline__ int swizzle_v(int row) { return D == 64 ? 4 * (row >> 1 & 1) : 4 * (row & 3); }
+};
+
+// Direct loads of 16 positions of one head to LDS; zeros for those past `valid`.
+template <int D, bool V>
+__device__ __forceinline__ void load16(const Cache& c, int page, int in_page, int head, int valid, char* lds, int lane) {
+  using L = Tile<D>;
+  const char* base = static_cast<const char*>(c.at) + 2 * (page * c.page + in_page * c.token + head * c.head);
+  const uint32_t stride = static_cast<uint32_t>(2 * c.token);
+  const uint32_t bytes = valid > 0 ? (valid - 1) * stride + L::kRow : 0;
+  const __amdgpu_buffer_rsrc_t rsrc =
+      __builtin_amdgcn_make_buffer_rsrc(const_cast<char*>(base), 0, bytes, 0x00020000);
+  const int row = lane / L::kPieces, piece = lane % L::kPieces;
+#pragma unroll
+  for (int i = 0; i < 16 / L::kPerLoad; ++i) {
+    const int r = i * L::kPerLoad + row;
+    const int from = piece ^ (V ? L::swizzle_v(r) : L::swizzle_k(r));
+    __builtin_amdgcn_raw_ptr_buffer_load_lds(rsrc, (lds_void*)(lds + i * 1024), 16, r * stride + 16 * from, 0, 0, 0);
+  }
+}
+
+// 16 positions from `at` (a multiple of 16) of a request's row of the table, of
+// which those before `end` are there.  A page outside of the cache reads as zeros.
+template <int D, bool V>
+__device__ __forceinline__ void load_positions(const Attend& p, int request, int at, int end, int head, char* lds,
+                                               int lane) {
+  int valid = end - at < 16 ? end - at : 16, page = 0, in = 0;
+  if (valid > 0) {
+    const uint32_t index = p.page.div(at);
+    in = at - index * p.page.d;
+    page = page_at(p, request, index);
+    if (page < 0 || page >= p.pages) valid = 0, page = 0;
+  }
+  load16<D, V>(V ? p.v : p.k, page, in, head, valid, lds, lane);
+}
+
+// Left operand of S^T: lane l holds row l % 32 of K, channels 16 step + 8 (l / 32) .. + 7.
+template <class T, int D>
+__device__ __forceinline__ typename Op<T>::frag k_frag(const char* lds, int row, int step, int lane) {
+  const int r = row + (lane & 31), piece = (2 * step + (lane >> 5)) ^ Tile<D>::swizzle_k(lane & 31);
+  return *reinterpret_cast<const typename Op<T>::frag*>(lds + r * Tile<D>::kRow + 16 * piece);
+}
+// Left operand of O^T: lane l holds channel 32 tile + l % 32, keys row + 4 (l / 32) .. + 3 and 8 behind these.
+template <class T, int D>
+__device__ __forceinline__ typename Op<T>::frag v_frag(const char* lds, int row, int tile, int lane) {
+  typedef __attribute__((address_space(3))) s16x4 lds_s16x4;
+  // the 16 lanes of a read bring 4 rows of 16 channels, lane i of them row i / 4, and receive channel i each
+  const int r = row + 4 * (lane >> 5) + ((lane & 15) >> 2);
+  const int piece = (4 * tile + 2 * (lane >> 4 & 1) + ((lane & 3) >> 1)) ^ Tile<D>::swizzle_v(4 * (lane >> 5) + ((lane & 15) >> 2));
+  const char* at = lds + r * Tile<D>::kRow + 16 * piece + 8 * (lane & 1);
+  const s16x4 a = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(at));
+  const s16x4 b = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(at + 8 * Tile<D>::kRow));
+  return __builtin_bit_cast(typename Op<T>::frag, __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7));
+}
+
+__device__ __forceinline__ float other_half(float v) { return __shfl_xor(v, 32, 64); }
+
+// One wave's rows: 32 of them, a lane and its partner 32 lanes on share one.
+template <class T, int D>
+struct Rows {
+  using Frag = typename Op<T>::frag;
+  Frag q[D / 16];
+  f32x16 o[D / 32];
+  float m, l;    // maximum of the scaled scores (base 2), and this lane's part of the sum
+  int limit;     // positions before it are visible to the row
+  int least, most;  // of the wave's rows
+
+  __device__ __forceinline__ void clear() {
+#pragma unroll
+    for (int i = 0; i < D / 32; ++i)
+#pragma unroll
+      for (int e = 0; e < 16; ++e) o[i][e] = 0.f;
+    m = -INFINITY, l = 0.f;
+  }
+
+  // Row `row` of the segment: its token and head, its queries, the positions visible to it.
+  __device__ __forceinline__ void load(const Attend& p, const Item& it, int row, int lane) {
+    const bool there = row < it.seg.tokens * p.per;
+    const int in = there ? row / p.per : 0, token = it.seg.token + in;
+    const int head = it.head * p.per + (there ? row - in * p.per : 0);
+    const T* from = static_cast<const T*>(p.q) + token * p.q_token + head * p.q_head + 8 * (lane >> 5);
+#pragma unroll
+    for (int i = 0; i < D / 16; ++i) {
+      const uint4 raw = there ? *reinterpret_cast<const uint4*>(from + 16 * i) : make_uint4(0, 0, 0, 0);
+      q[i] = __builtin_bit_cast(Frag, raw);
+    }
+    limit = 0;
+    if (there) {
+      int r = it.seg.request;
+      if (!it.own) r = p.cu ? static_cast<int>(find_sequence(p.cu, p.cu_is64, p.requests, token)) : token;
+      const int64_t end = load_index(p.lens, r, p.lens_is64) - (token_of(p, r + 1) - 1 - token);
+      limit = clampi(end, 0, it.seg.hi);
+    }
+    int a = there ? limit : INT32_MAX, b = limit;
+#pragma unroll
+    for (int off = 16; off > 0; off >>= 1) a = min(a, __shfl_xor(a, off, 64)), b = max(b, __shfl_xor(b, off, 64));
+    least = uniform(a), most = uniform(b);
+  }
+
+  // 32 KEYS positions from `at` on, whose keys and values lie in LDS.
+  template <int TILES>
+  __device__ __forceinline__ void scores(const char* k, int lane, f32x16 (&s)[TILES]) const {
+#pragma unroll
+    for (int t = 0; t < TILES; ++t) {
+#pragma unroll
+      for (int e = 0; e < 16; ++e) s[t][e] = 0.f;
+#pragma unroll
+      for (int i = 0; i < D / 16; ++i) s[t] = Op<T>::mma(k_frag<T, D>(k, 32 * t, i, lane), q[i], s[t]);
+    }
+  }
+  // Whether some row of the wave does not see all of the 32 TILES positions from `at` on (uniform).
+  template <int TILES>
+  __device__ __forceinline__ bool partly(const Segment& seg, int at) const {
+    return at < seg.lo || at + 32 * TILES > least;
+  }
+  // The softmax's step: s becomes the weights, in the io type as the right operand.
+  template <int TILES>
+  __device__ __forceinline__ void weights(const Attend& p, const Segment& seg, int at, int lane, f32x16 (&s)[TILES],
+                                          Frag (&w)[2 * TILES]) {
+    if (partly<TILES>(seg, at)) {
+#pragma unroll
+      for (int t = 0; t < TILES; ++t)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) {
+          const int pos = at + 32 * t + 8 * (e >> 2) + 4 * (lane >> 5) + (e & 3);
+          if (pos < seg.lo || pos >= limit) s[t][e] = -INFINITY;
+        }
+    }
+    float top = s[0][0];
+#pragma unroll
+    for (int t = 0; t < TILES; ++t)
+#pragma unroll
+      for (int e = 0; e < 16; ++e) top = fmaxf(top, s[t][e]);
+    top = fmaxf(top, other_half(top)) * p.factor;
+    // rescaled only where the maximum has grown by more than 2^8: fp32 sums have room for that
+    const bool grown = top > m + kLater;
+    if (__any(grown)) {
+      const float alpha = grown ? fast_exp2(m - top) : 1.0f;
+      m = grown ? top : m;
+      l *= alpha;
+#pragma unroll
+      for (int i = 0; i < D / 32; ++i)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) o[i][e] *= alpha;
+    }
+    const float less = m == -INFINITY ? 0.f : m;
+    float sum = 0.f;
+#pragma unroll
+    for (int t = 0; t < TILES; ++t) {
+#pragma unroll
+      for (int e = 0; e < 16; ++e) {
+        s[t][e] = fast_exp2(fmaf(s[t][e], p.factor, -less));
+        sum += s[t][e];
+      }
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const uint4 packed =
+            make_uint4(out_pack2<T>(s[t][8 * h], s[t][8 * h + 1]), out_pack2<T>(s[t][8 * h + 2], s[t][8 * h + 3]),
+                       out_pack2<T>(s[t][8 * h + 4], s[t][8 * h + 5]), out_pack2<T>(s[t][8 * h + 6], s[t][8 * h + 7]));
+        w[2 * t + h] = __builtin_bit_cast(Frag, packed);
+      }
+    }
+    l += sum;
+  }
+  template <int TILES>
+  __device__ __forceinline__ void values(const char* v, int lane, const Frag (&w)[2 * TILES]) {
+#pragma unroll
+    for (int d = 0; d < D / 32; ++d)
+#pragma unroll
+      for (int i = 0; i < 2 * TILES; ++i) o[d] = Op<T>::mma(v_frag<T, D>(v, 16 * i, d, lane), w[i], o[d]);
+  }
+};
+
+// A weight of zero does not silence a value that is not finite.  Where rows of an
+// item do not see all of a tile's positions, such values are taken out of it, and
+// for each channel the first position of a positive and of a negative one is kept
+// (of both for a NaN): they go to the rows that see it when the item is done.
+template <int D> struct NotFinite {
+  int found, pad[3];
+  int first[2][D];
+  __device__ __forceinline__ void clear() {  // by the whole block
+    if (threadIdx.x == 0) found = 0;
+    for (int i = threadIdx.x; i < 2 * D; i += kThreads) first[i / D][i % D] = INT32_MAX;
+  }
+  __device__ __forceinline__ float added(int channel, int limit) const {
+    return (first[0][channel] < limit ? INFINITY : 0.f) - (first[1][channel] < limit ? INFINITY : 0.f);
+  }
+};
+
+// Of the 16 positions from `at` on whose values this wave has brought to LDS.
+template <class T, int D>
+__device__ __forceinline__ void take_out(char* v, int at, int lo, NotFinite<D>& bad, int lane) {
+  using L = Tile<D>;
+  constexpr uint32_t kBits = Op<T>::kExponent, kMask = kBits * 0x10001u, kStep = (0x8000u - kBits) * 0x10001u;
+  uint32_t found = 0;  // the top bit of a half: its exponent had no room for one more
+#pragma unroll
+  for (int i = 0; i < 16 / L::kPerLoad; ++i) {
+    const uint4 raw = *reinterpret_cast<const uint4*>(v + i * 1024 + lane * 16);
+    found |= ((raw.x & kMask) + kStep) | ((raw.y & kMask) + kStep) | ((raw.z & kMask) + kStep) | ((raw.w & kMask) + kStep);
+  }
+  if (!__any((found & 0x80008000u) != 0)) return;
+#pragma unroll 1
+  for (int i = 0; i < 16 / L::kPerLoad; ++i) {
+    const int row = i * L::kPerLoad + lane / L::kPieces, piece = (lane % L::kPieces) ^ L::swizzle_v(row);
+    uint16_t* values = reinterpret_cast<uint16_t*>(v + i * 1024 + lane * 16);
+#pragma unroll 1
+    for (int e = 0; e < 8; ++e) {
+      const uint32_t bits = values[e];
+      if ((bits & kBits) != kBits) continue;
+      values[e] = 0;
+      if (at + row < lo) continue;
+      const bool nan = (bits & 0x7fff) != kBits, negative = bits >> 15;
+      if (nan || !negative) atomicMin(&bad.first[0][8 * piece + e], at + row);
+      if (nan || negative) atomicMin(&bad.first[1][8 * piece + e], at + row);
+      bad.found = 1;
+    }
+  }
+}
+
+// Whether an item holds all that its rows see: nothing has to be joined.
+__device__ __forceinline__ bool whole(const Item& it) { return it.own && it.ranges == 1 && it.seg.lo == 0; }
+
+// Four channels of a finished row.
+template <class T>
+__device__ __forceinline__ void put4(const Attend& p, int token, int head, int channel, const float (&y)[4]) {
+  T* to = static_cast<T*>(p.out) + token * p.out_token + head * p.out_head + channel;
+  *reinterpret_cast<uint2*>(to) = make_uint2(out_pack2<T>(y[0], y[1]), out_pack2<T>(y[2], y[3]));
+}
+// The factor of a piece with maximum m and sum l under the joint maximum; 0 where the
+// piece saw nothing (a NaN stays one).
+__device__ __forceinline__ float weight_of(float m, float l, float top) { return l == 0.f ? 0.f : fast_exp2(m - top); }
+__device__ __forceinline__ float lse_of(float m, float l) { return l > 0.f || l != l ? (m + log2f(l)) * kLn2 : -INFINITY; }
+
+// ------------------------------------------------------------------ many rows
+// Four waves of 32 rows each; the block's keys and values come through two LDS
+// buffers, one loaded while the other is read.
+template <int D> struct Many {
+  static constexpr int kRows = 128, kTiles = D == 256 ? 1 : 2, kKeys = 32 * kTiles;
+  static constexpr int kHalf = kKeys * 2 * D, kBuffer = 2 * kHalf;
+  static constexpr int kLds = 2 * kBuffer;
+};
+
+template <class T, int D>
+__global__ __launch_bounds__(kThreads, D == 256 ? 1 : 2) void many_rows_kernel(Attend p) {
+  using M = Many<D>;
+  __shared__ __align__(16) char lds[M::kLds + sizeof(NotFinite<D>) + sizeof(Plan) + 16];
+  NotFinite<D>& bad = *reinterpret_cast<NotFinite<D>*>(lds + M::kLds);
+  Plan& plan = *reinterpret_cast<Plan*>(lds + M::kLds + sizeof(bad));
+  int* least = reinterpret_cast<int*>(lds + M::kLds + sizeof(bad) + sizeof(Plan));  // of each wave's rows
+  const int lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6);
+  int each, range;
+  const int total = schedule<true, M::kRows, M::kKeys>(p, plan, each, range);
+  // blocks with the same index modulo 8 share an XCD and its L2: neighbours in the order of items, which share keys
+  const int xcd = blockIdx.x & 7, last = static_cast<int>(static_cast<int64_t>(total) * (xcd + 1) / 8);
+  for (int item = static_cast<int>(static_cast<int64_t>(total) * xcd / 8) + (blockIdx.x >> 3); item < last;
+       item += gridDim.x >> 3) {
+    const Item it = item_of<true, M::kRows, M::kKeys>(p, plan, each, range, item);
+    Rows<T, D> rows;
+    const int row = it.tile * M::kRows + 32 * wave + (lane & 31);
+    rows.load(p, it, row, lane);
+    rows.clear();
+    // nothing behind the last position that a row of the tile sees
+    const int last_token = min(it.seg.tokens - 1, (it.tile * M::kRows + M::kRows - 1) / p.per);
+    int to = it.to;
+    if (it.own) {
+      const int64_t end = load_index(p.lens, it.seg.request, p.lens_is64) - (it.seg.tokens - 1 - last_token);
+      to = clampi(end, 0, to);
+    }
+    to = uniform(to);
+    const int end = it.seg.hi, steps = to > it.from ? (to - it.from + M::kKeys - 1) / M::kKeys : 0;
+    auto load = [&](int step) __attribute__((always_inline)) {
+      char* buffer = lds + (step & 1) * M::kBuffer;
+      const int at = it.from + step * M::kKeys;
+      if constexpr (M::kTiles == 2) {  // a wave brings 16 positions
+        load_positions<D, false>(p, it.seg.request, at + 16 * wave, end, it.head, buffer + wave * 32 * D, lane);
+        load_positions<D, true>(p, it.seg.request, at + 16 * wave, end, it.head, buffer + M::kHalf + wave * 32 * D, lane);
+      } else if (wave < 2) {
+        load_positions<D, false>(p, it.seg.request, at + 16 * wave, end, it.head, buffer + wave * 32 * D, lane);
+      } else {
+        load_positions<D, true>(p, it.seg.request, at + 16 * (wave - 2), end, it.head,
+                                buffer + M::kHalf + (wave - 2) * 32 * D, lane);
+      }
+    };
+    lds_barrier();  // the last item's buffers are free
+    bad.clear();
+    if (lane == 0) least[wave] = rows.least;
+    if (steps > 0) load(0);
+    lds_barrier();
+    const int all_see = uniform(min(min(least[0], least[1]), min(least[2], least[3])));
+    for (int step = 0; step < steps; ++step) {
+      wait_loads<0>();
+      if (it.from + step * M::kKeys < it.seg.lo || it.from + (step + 1) * M::kKeys > all_see) {
+        const int sub = M::kTiles == 2 ? wave : wave - 2;
+        if (sub >= 0)
+          take_out<T, D>(lds + (step & 1) * M::kBuffer + M::kHalf + sub * 32 * D, it.from + step * M::kKeys + 16 * sub,
+                         it.seg.lo, bad, lane);
+      }
+      lds_barrier();
+      if (step + 1 < steps) load(step + 1);
+      const char* buffer = lds + (step & 1) * M::kBuffer;
+      const int at = it.from + step * M::kKeys;
+      if (at < rows.most) {
+        f32x16 s[M::kTiles];
+        typename Op<T>::frag w[2 * M::kTiles];
+        rows.template scores<M::kTiles>(buffer, lane, s);
+        rows.template weights<M::kTiles>(p, it.seg, at, lane, s, w);
+        rows.template values<M::kTiles>(buffer + M::kHalf, lane, w);
+      }
+    }
+    const float l = rows.l + other_half(rows.l);
+    if (uniform(bad.found)) {
+#pragma unroll
+      for (int d = 0; d < D / 32; ++d)
+#pragma unroll
+        for (int e = 0; e < 16; ++e)
+          rows.o[d][e] += bad.added(32 * d + 8 * (e >> 2) + 4 * (lane >> 5) + (e & 3), rows.limit);
+    }
+    const bool there = row < it.seg.tokens * p.per;
+    if (there && whole(it)) {
+      const int in = row / p.per, token = it.seg.token + in, head = it.head * p.per + row - in * p.per;
+      const float inverse = l > 0.f || l != l ? 1.0f / l : 0.f;
+#pragma unroll
+      for (int d = 0; d < D / 32; ++d)
+#pragma unroll
+        for (int e = 0; e < 16; e += 4) {
+          const float y[4] = {rows.o[d][e] * inverse, rows.o[d][e + 1] * inverse, rows.o[d][e + 2] * inverse,
+                              rows.o[d][e + 3] * inverse};
+          put4<T>(p, token, head, 32 * d + 2 * e + 4 * (lane >> 5), y);
+        }
+      if (p.lse && lane < 32) p.lse[static_cast<int64_t>(token) * p.heads + head] = lse_of(rows.m, l);
+    } else if (there) {
+      const int64_t at = static_cast<int64_t>(item) * M::kRows + 32 * wave + (lane & 31);
+      float* sums = p.sums[1] + at * D + 4 * (lane >> 5);
+#pragma unroll
+      for (int d = 0; d < D / 32; ++d)
+#pragma unroll
+        for (int e = 0; e < 16; e += 4)
+          *reinterpret_cast<float4*>(sums + 32 * d + 2 * e) =
+              make_float4(rows.o[d][e], rows.o[d][e + 1], rows.o[d][e + 2], rows.o[d][e + 3]);
+      if (lane < 32) p.stats[1][at] = make_float2(rows.m, l);
+    }
+  }
+}
+
+// ------------------------------------------------------------------ few rows
+// A segment of at most 32 rows: what bounds it is how fast its keys come in.  The
+// four waves take the steps of 32 positions by turns, each with LDS of its own for
+// one step's keys and one step's values and no barrier among them; the next keys
+// are loaded when these have become scores, the next values when these have been
+// summed.  The waves join their sums through LDS.
+template <int D> struct Few {
+  static constexpr int kHalf = 32 * 2 * D, kWave = 2 * kHalf, kLds = 4 * kWave;
+  static constexpr int kLoads = kHalf / 1024;
+  static constexpr int kUnit = 128;
+  static constexpr int kBlocks = 160 * 1024 / (kLds + 4096) < 2 ? 1 : 2;
+  static_assert(kWave == 32 * D * 4, "a wave's sums take the place of its keys and values");
+};
+
+template <class T, int D>
+__global__ __launch_bounds__(kThreads, Few<D>::kBlocks) void few_rows_kernel(Attend p) {
+  using F = Few<D>;
+  __shared__ __align__(16) char lds[F::kLds + sizeof(NotFinite<D>) + sizeof(Plan) + sizeof(Stats) + 128];
+  NotFinite<D>& bad = *reinterpret_cast<NotFinite<D>*>(lds + F::kLds);
+  Plan& plan = *reinterpret_cast<Plan*>(lds + F::kLds + sizeof(bad));
+  Stats& stats = *reinterpret_cast<Stats*>(lds + F::kLds + sizeof(bad) + sizeof(Plan));
+  int* limits = reinterpret_cast<int*>(lds + F::kLds + sizeof(bad) + sizeof(Plan) + sizeof(Stats));
+  const int lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6);
+  int each, range;
+  const int total = schedule<false, kFew, F::kUnit>(p, plan, each, range);
+  char* mine = lds + wave * F::kWave;
+  for (int item = blockIdx.x; item < total; item += gridDim.x) {
+    const Item it = item_of<false, kFew, F::kUnit>(p, plan, each, range, item);
+    Rows<T, D> rows;
+    rows.load(p, it, lane & 31, lane);
+    rows.clear();
+    wait_loads<0>();
+    const int end = it.seg.hi, to = min(it.to, rows.most);
+    const int steps = to > it.from ? (to - it.from + 31) / 32 : 0;
+    auto load_k = [&](int step) __attribute__((always_inline)) {
+      const int at = it.from + 32 * step;
+      load_positions<D, false>(p, it.seg.request, at, step < steps ? end : 0, it.head, mine, lane);
+      load_positions<D, false>(p, it.seg.request, at + 16, step < steps ? end : 0, it.head, mine + 32 * D, lane);
+    };
+    auto load_v = [&](int step) __attribute__((always_inline)) {
+      const int at = it.from + 32 * step;
+      load_positions<D, true>(p, it.seg.request, at, step < steps ? end : 0, it.head, mine + F::kHalf, lane);
+      load_positions<D, true>(p, it.seg.request, at + 16, step < steps ? end : 0, it.head, mine + F::kHalf + 32 * D, lane);
+    };
+    lds_barrier();  // the last item's sums have been read
+    load_k(wave);
+    load_v(wave);
+    bad.clear();
+    if (wave == 0 && lane < 32) limits[lane] = rows.limit;
+    lds_barrier();
+    for (int step = wave; step < steps; step += 4) {
+      f32x16 s[1];
+      typename Op<T>::frag w[2];
+      wait_loads<F::kLoads>();  // the keys; the values may be on their way
+      rows.template scores<1>(mine, lane, s);
+      reads_done();
+      load_k(step + 4);
+      rows.template weights<1>(p, it.seg, it.from + 32 * step, lane, s, w);
+      wait_loads<F::kLoads>();
+      if (rows.template partly<1>(it.seg, it.from + 32 * step)) {
+        take_out<T, D>(mine + F::kHalf, it.from + 32 * step, it.seg.lo, bad, lane);
+        take_out<T, D>(mine + F::kHalf + 32 * D, it.from + 32 * step + 16, it.seg.lo, bad, lane);
+      }
+      rows.template values<1>(mine + F::kHalf, lane, w);
+      reads_done();
+      load_v(step + 4);
+    }
+    wait_loads<0>();  // those past the end too, before the sums take their place
+    float l = rows.l + other_half(rows.l);
+    if (lane < 32) stats[wave][lane] = make_float2(rows.m, l);
+    lds_barrier();
+    float m = -INFINITY;
+#pragma unroll
+    for (int w = 0; w < 4; ++w) m = fmaxf(m, stats[w][lane & 31].x);
+    const float mine_to = weight_of(rows.m, l, m);
+    // [D / 4][32 rows][4 channels]: lanes side by side
+#pragma unroll
+    for (int d = 0; d < D / 32; ++d)
+#pragma unroll
+      for (int e = 0; e < 16; e += 4) {
+        const int quad = 8 * d + 2 * (e >> 2) + (lane >> 5);
+        *reinterpret_cast<float4*>(mine + (quad * 32 + (lane & 31)) * 16) =
+            make_float4(rows.o[d][e] * mine_to, rows.o[d][e + 1] * mine_to, rows.o[d][e + 2] * mine_to,
+                        rows.o[d][e + 3] * mine_to);
+      }
+    lds_barrier();
+    const int count = it.seg.tokens * p.per;
+    for (int i = threadIdx.x; i < count * (D / 4); i += kThreads) {
+      const int r = i / (D / 4), quad = i % (D / 4);
+      float y[4] = {0.f, 0.f, 0.f, 0.f};
+      float top = -INFINITY, sum = 0.f;
+#pragma unroll
+      for (int w = 0; w < 4; ++w) {
+        const float4 part = *reinterpret_cast<const float4*>(lds + w * F::kWave + (quad * 32 + r) * 16);
+        y[0] += part.x, y[1] += part.y, y[2] += part.z, y[3] += part.w;
+        top = fmaxf(top, stats[w][r].x);
+      }
+#pragma unroll
+      for (int w = 0; w < 4; ++w) sum += stats[w][r].y * weight_of(stats[w][r].x, stats[w][r].y, top);
+      if (bad.found) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) y[e] += bad.added(4 * quad + e, limits[r]);
+      }
+      if (whole(it)) {
+        const int in = r / p.per, token = it.seg.token + in, head = it.head * p.per + r - in * p.per;
+        const float inverse = sum > 0.f || sum != sum ? 1.0f / sum : 0.f;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) y[e] *= inverse;
+        put4<T>(p, token, head, 4 * quad, y);
+        if (p.lse && quad == 0) p.lse[static_cast<int64_t>(token) * p.heads + head] = lse_of(top, sum);
+      } else {
+        const int64_t at = static_cast<int64_t>(item) * kFew + r;
+        *reinterpret_cast<float4*>(p.sums[0] + at * D + 4 * quad) = make_float4(y[0], y[1], y[2], y[3]);
+        if (quad == 0) p.stats[0][at] = make_float2(top, sum);
+      }
+    }
+  }
+}
+
+// ------------------------------------------------------------------ join
+// WAVES waves a row: the pieces of the row's shared and own segments by turns.
+template <class T, int D, int WAVES>
+__global__ __launch_bounds__(kThreads) void join_kernel(Attend p) {
+  constexpr int kRowsABlock = kThreads / (64 * WAVES), kLane = D / 64;  // channels a lane
+  __shared__ float sums[4][D];
+  __shared__ float2 stats[4];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int64_t at = static_cast<int64_t>(blockIdx.x) * kRowsABlock + (WAVES == 1 ? wave : 0);
+  const int64_t rows = static_cast<int64_t>(p.tokens) * p.heads;
+  const bool there = at < rows;
+  const int token = there ? static_cast<int>(at / p.heads) : 0, head = there ? static_cast<int>(at % p.heads) : 0;
+  const int request = p.cu ? static_cast<int>(find_sequence(p.cu, p.cu_is64, p.requests, token)) : token;
+  const int group = group_of(p, request), shared = p.shared ? p.num_groups : 0;
+  float m = -INFINITY, l = 0.f, y[kLane];
+#pragma unroll
+  for (int e = 0; e < kLane; ++e) y[e] = 0.f;
+  // tokens behind the last request (or before the first) are nobody's: left as they were
+  bool done = !there || token < token_of(p, request) || token >= token_of(p, request + 1);
+#pragma unroll
+  for (int which = 0; which < 2; ++which) {
+    const int s = which ? shared + request : group;
+    if (s < 0 || done) continue;
+    const Segment seg = segment(p, s);
+    const int row = (token - seg.token) * p.per + head % p.per;
+    if (row < 0 || row >= seg.tokens * p.per || seg.hi <= seg.lo) continue;
+    const int many = seg.tokens * p.per > kFew, tile_rows = many ? Many<D>::kRows : kFew;
+    const int tiles = (seg.tokens * p.per + tile_rows - 1) / tile_rows;
+    const int2 place = p.places[s];
+    if (which && place.y == 1 && seg.lo == 0) {  // the item wrote the row itself
+      done = true;
+      continue;
+    }
+    const int first = place.x + head / p.per * place.y * tiles + row / tile_rows;
+    for (int i = WAVES == 1 ? 0 : wave; i < place.y; i += WAVES) {
+      const int item = first + i * tiles;
+      if (item >= p.items_max[many]) break;
+      const int64_t from = static_cast<int64_t>(item) * tile_rows + row % tile_rows;
+      const float2 st = p.stats[many][from];
+      const float* part = p.sums[many] + from * D + lane * kLane;
+      float x[kLane];
+#pragma unroll
+      for (int e = 0; e < kLane; ++e) x[e] = part[e];
+      const float top = fmaxf(m, st.x), a = weight_of(m, l, top), b = weight_of(st.x, st.y, top);
+      l = l * a + st.y * b;
+#pragma unroll
+      for (int e = 0; e < kLane; ++e) y[e] = y[e] * a + x[e] * b;
+      m = top;
+    }
+  }
+  if constexpr (WAVES > 1) {
+#pragma unroll
+    for (int e = 0; e < kLane; ++e) sums[wave][lane * kLane + e] = y[e];
+    if (lane == 0) stats[wave] = make_float2(m, l);
+    __syncthreads();
+    if (wave > 0) return;
+    m = -INFINITY, l = 0.f;
+#pragma unroll
+    for (int w = 0; w < WAVES; ++w) m = fmaxf(m, stats[w].x);
+#pragma unroll
+    for (int e = 0; e < kLane; ++e) y[e] = 0.f;
+#pragma unroll
+    for (int w = 0; w < WAVES; ++w) {
+      const float b = weight_of(stats[w].x, stats[w].y, m);
+      l += stats[w].y * b;
+#pragma unroll
+      for (int e = 0; e < kLane; ++e) y[e] += sums[w][lane * kLane + e] * b;
+    }
+  }
+  if (done) return;
+  const float inverse = l > 0.f || l != l ? 1.0f / l : 0.f;
+  T* to = static_cast<T*>(p.out) + token * p.out_token + head * p.out_head + lane * kLane;
+#pragma unroll
+  for (int e = 0; e < kLane; ++e) to[e] = from_f32<T>(y[e] * inverse);
+  if (p.lse && lane == 0) p.lse[at] = lse_of(m, l);
+}
+
+// ------------------------------------------------------------------ host
+constexpr int kCus = 256;
+inline int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
+inline int64_t aligned(int64_t n) { return (n + 255) / 256 * 256; }
+
+struct Sizes {
+  bool few, many;  // whether segments of that kind can be there
+  int64_t items[2], target[2];
+  int64_t sums[2], stats[2], places, bytes;  // offsets
+};
+
+// Bounds from what the host knows.  Each of a kind's items is one of `target` (a
+// range of keys is at least all units over it) or the last range of a tile.
+Sizes sizes_of(int64_t tokens, int64_t requests, int64_t groups, int64_t heads, int64_t kv_heads, int64_t dim,
+               bool varlen) {
+  Sizes z{};
+  const int64_t per = heads / kv_heads, rows = tokens * per, sets = groups > 0 ? 2 : 1;
+  z.few = per <= kFew;
+  z.many = rows > kFew && (varlen || per > kFew || groups > 0);
+  z.target[0] = 2 * kCus * (dim == 256 ? 1 : 2);
+  z.target[1] = 2 * kCus;
+  const int64_t few_tiles = requests + groups, many_tiles = sets * (rows / 128 + std::min(requests + groups, rows / kFew + 1));
+  z.items[0] = z.few ? z.target[0] + few_tiles * kv_heads : 0;
+  z.items[1] = z.many ? z.target[1] + many_tiles * kv_heads : 0;
+  int64_t at = 0;
+  auto take = [&](int64_t bytes) {
+    const int64_t from = at;
+    at += aligned(bytes);
+    return from;
+  };
+  for (int kind = 0; kind < 2; ++kind) {
+    const int64_t n = z.items[kind] * (kind ? 128 : kFew);
+    z.sums[kind] = take(n * dim * 4);
+    z.stats[kind] = take(n * 8);
+  }
+  z.places = take((requests + groups) * 8);
+  z.bytes = at;
+  return z;
+}
+
+template <class T, int D>
+int launch_attend(const Attend& p, const Sizes& z, hipStream_t stream) {
+  if (z.many) many_rows_kernel<T, D><<<2 * kCus, kThreads, 0, stream>>>(p);
+  if (z.few)
+    few_rows_kernel<T, D><<<static_cast<uint32_t>(std::min(z.items[0], z.target[0])), kThreads, 0, stream>>>(p);
+  const int64_t rows = static_cast<int64_t>(p.tokens) * p.heads;
+  if (rows <= 16 * kCus)
+    join_kernel<T, D, 4><<<static_cast<uint32_t>(rows), kThreads, 0, stream>>>(p);
+  else
+    join_kernel<T, D, 1><<<static_cast<uint32_t>(ceil_div(rows, 4)), kThreads, 0, stream>>>(p);
+  return GDN_LAUNCH_CHECK("paged attention");
+}
+
+}  // namespace
+}  // namespace gdn
+
+using namespace gdn;
+
+extern "C" int64_t gdn_paged_attention_workspace_bytes(int64_t tokens, int64_t requests, int64_t groups, int64_t heads,
+                                                       int64_t kv_heads, int64_t dim, int varlen) {
+  if (tokens <= 0 || requests <= 0 || groups < 0 || kv_heads <= 0 || heads < kv_heads || dim <= 0) return 0;
+  return sizes_of(tokens, requests, groups, heads, kv_heads, dim, varlen != 0).bytes;
+}
+
+extern "C" int gdn_paged_attention(const void* q, int64_t q_token_stride, int64_t q_head_stride, int dtype,
+                                   int64_t tokens, int64_t heads, int64_t dim, const void* k_cache,
+                                   int64_t k_page_stride, int64_t k_token_stride, int64_t k_head_stride,
+                                   const void* v_cache, int64_t v_page_stride, int64_t v_token_stride,
+                                   int64_t v_head_stride, int64_t kv_heads, int64_t pages, int64_t page_size,
+                                   const void* page_table, int table_dtype, int64_t table_row_stride,
+                                   int64_t table_width, const void* seq_lens, int lens_dtype, int64_t requests,
+                                   const void* shared_lens, int shared_dtype, const void* group_offsets,
+                                   int offsets_dtype, int64_t groups, const void* cu_seqlens, int cu_dtype, float scale,
+                                   void* out, int64_t out_token_stride, int64_t out_head_stride, float* lse,
+                                   void* workspace, int64_t workspace_bytes, void* stream) {
+  GDN_REQUIRE(dtype == GDN_BF16 || dtype == GDN_F16, "dtype must be bf16 or f16");
+  GDN_REQUIRE(tokens >= 0 && requests >= 0 && heads > 0 && kv_heads > 0 && heads % kv_heads == 0 && pages >= 0 &&
+                  table_width >= 0 && groups >= 0,
+              "bad shape");
+  GDN_REQUIRE(page_size > 0 && page_size % 16 == 0, "pages of a multiple of 16 tokens");
+  GDN_REQUIRE(scale > 0.f && scale <= 3.4e38f, "scale must be positive and finite");
+  GDN_REQUIRE(cu_seqlens || tokens == requests, "one token for each request without cu_seqlens");
+  GDN_REQUIRE(groups == 0 || shared_lens, "groups without shared lengths");
+  GDN_REQUIRE(groups <= 1 || group_offsets, "several groups need their offsets");
+  if (dim != 64 && dim != 128 && dim != 256) {
+    set_error("head dims 64, 128 and 256");
+    return GDN_ERR_UNSUPPORTED;
+  }
+  if (tokens * heads >= (int64_t{1} << 31) || requests + groups >= (int64_t{1} << 24) ||
+      table_width * page_size > (int64_t{1} << 30) || pages >= (int64_t{1} << 31)) {
+    set_error("up to 2^31 rows, 2^24 requests, 2^30 positions and 2^31 pages");
+    return GDN_ERR_UNSUPPORTED;
+  }
+  if (tokens == 0 || requests == 0) return GDN_OK;
+  GDN_REQUIRE(q && out && (pages == 0 || (k_cache && v_cache)) && seq_lens && (table_width == 0 || page_table),
+              "null operand");
+  const int codes[] = {table_dtype, lens_dtype, shared_dtype, offsets_dtype, cu_dtype};
+  for (int code : codes) GDN_REQUIRE(code == GDN_I32 || code == GDN_I64, "indices must be int32 or int64");
+  const int64_t strides[] = {q_token_stride, q_head_stride, k_page_stride, k_token_stride,
+                             k_head_stride,  v_page_stride, v_token_stride, v_head_stride};
+  for (int64_t n : strides) GDN_REQUIRE(n % 8 == 0, "rows must start at multiples of 16 bytes");
+  GDN_REQUIRE(aligned16(q) && aligned16(k_cache) && aligned16(v_cache), "rows must start at multiples of 16 bytes");
+  GDN_REQUIRE(out_token_stride % 4 == 0 && out_head_stride % 4 == 0 && reinterpret_cast<uintptr_t>(out) % 8 == 0,
+              "rows of out must start at multiples of 8 bytes");
+  // 16 positions are addressed by 32-bit byte offsets
+  GDN_REQUIRE(k_token_stride >= 0 && v_token_stride >= 0 && k_token_stride < (1 << 24) && v_token_stride < (1 << 24),
+              "tokens of a page up to 2^24 elements apart");
+  const Sizes z = sizes_of(tokens, requests, groups, heads, kv_heads, dim, cu_seqlens != nullptr);
+  GDN_REQUIRE(workspace && workspace_bytes >= z.bytes && reinterpret_cast<uintptr_t>(workspace) % 16 == 0,
+              "a workspace of %lld bytes is needed", static_cast<long long>(z.bytes));
+
+  Attend p{};
+  p.q = q, p.q_token = q_token_stride, p.q_head = q_head_stride;
+  p.k = {k_cache, k_page_stride, k_token_stride, k_head_stride};
+  p.v = {v_cache, v_page_stride, v_token_stride, v_head_stride};
+  p.table = page_table, p.table_row = table_row_stride, p.table_is64 = table_dtype == GDN_I64;
+  p.lens = seq_lens, p.lens_is64 = lens_dtype == GDN_I64;
+  if (groups > 0) p.shared = shared_lens, p.shared_is64 = shared_dtype == GDN_I64;
+  p.groups = group_offsets, p.groups_is64 = offsets_dtype == GDN_I64;
+  p.cu = cu_seqlens, p.cu_is64 = cu_dtype == GDN_I64;
+  p.tokens = static_cast<int>(tokens), p.requests = static_cast<int>(requests), p.num_groups = static_cast<int>(groups);
+  p.heads = static_cast<int>(heads), p.kv_heads = static_cast<int>(kv_heads), p.per = static_cast<int>(heads / kv_heads);
+  p.pages = static_cast<int>(pages), p.capacity = static_cast<int>(table_width * page_size);
+  p.page = make_div32(page_size);
+  p.factor = scale * kLog2e;
+  p.out = out, p.out_token = out_token_stride, p.out_head = out_head_stride;
+  p.lse = lse;
+  char* ws = static_cast<char*>(workspace);
+  for (int kind = 0; kind < 2; ++kind) {
+    p.sums[kind] = reinterpret_cast<float*>(ws + z.sums[kind]);
+    p.stats[kind] = reinterpret_cast<float2*>(ws + z.stats[kind]);
+    p.items_max[kind] = static_cast<int>(z.items[kind]);
+    p.target[kind] = static_cast<int>(z.target[kind]);
+    p.min_units[kind] = 1;
+  }
+  p.places = reinterpret_cast<int2*>(ws + z.places);
+  auto go = [&](auto type) {
+    using T = decltype(type);
+    const hipStream_t on = static_cast<hipStream_t>(stream);
+    return dim == 64 ? launch_attend<T, 64>(p, z, on) : dim == 128 ? launch_attend<T, 128>(p, z, on)
+                                                                   : launch_attend<T, 256>(p, z, on);
+  };
+  return dtype == GDN_BF16 ? go(bf16{}) : go(f16{});
+}

@@ -1,0 +1,265 @@
+// Rotary positions, and the append of keys and values to a paged cache with the
+// rotation on the way.
+//
+// Pair i of a head's first R channels, (x[i], x[i + R/2]) in the half layout or
+// (x[2i], x[2i + 1]) interleaved, is turned by the angle 2 pi turns[i] position
+// and multiplied by `scale`; the channels behind them pass through.  Angles are
+// products in 64 bits of which only the fraction of a revolution is kept, so that
+// a position of any size costs no precision and there is no table to outgrow.
+//
+// Bound by memory: 16 bytes a lane, each value read and written once.  A block
+// takes a few tokens; its cosines and sines are computed once into LDS and serve
+// all heads.
+#include <algorithm>
+
+#include "common.hpp"
+
+namespace gdn {
+namespace {
+
+constexpr int kThreads = 256;
+constexpr int kAngles = 2048;  // cosines and sines of a block in LDS
+
+// Rows of one operand: [tokens, heads, dim], unit channel stride.
+struct Rows {
+  const void* src;
+  void* dst;
+  int64_t src_token, src_head, dst_token, dst_head;  // elements
+  int64_t dst_page;                                  // of a cache: dst_token inside a page
+};
+
+struct Turn {
+  Rows rows[3];  // q, k, v
+  int first[4];  // heads before each of them
+  const void* positions;
+  const double* turns;
+  const void* slots;  // NULL: every dst is [tokens, heads, dim]
+  int positions_is64, slots_is64;
+  int tokens, per_block, dim, rotated, interleaved;
+  Div32 page;
+  int64_t capacity;  // slots of the cache
+  float scale;
+  int copy_rest;  // bit s: operand s has channels behind the rotated ones to copy
+};
+
+template <class T> struct Vec16 {
+  static constexpr int n = 16 / sizeof(T);
+  static __device__ __forceinline__ void get(uint4 raw, float (&x)[n]) { unpack8<T>(raw, x); }
+  static __device__ __forceinline__ uint4 put(const float (&x)[n]) { return pack8_io<T>(x); }
+};
+template <> struct Vec16<float> {
+  static constexpr int n = 4;
+  static __device__ __forceinline__ void get(uint4 raw, float (&x)[4]) {
+    x[0] = __uint_as_float(raw.x), x[1] = __uint_as_float(raw.y);
+    x[2] = __uint_as_float(raw.z), x[3] = __uint_as_float(raw.w);
+  }
+  static __device__ __forceinline__ uint4 put(const float (&x)[4]) {
+    return make_uint4(__float_as_uint(x[0]), __float_as_uint(x[1]), __float_as_uint(x[2]), __float_as_uint(x[3]));
+  }
+};
+
+// The pair (a, b) turned; `cs` holds scale cos and scale sin.
+__device__ __forceinline__ void turn_pair(float2 cs, float& a, float& b) {
+  const float x = a;
+  a = x * cs.x - b * cs.y;
+  b = b * cs.x + x * cs.y;
+}
+
+// WIDE: rows in pieces of 16 bytes; a unit of work is a pair of pieces (half
+// layout), a piece of pairs (interleaved), or a piece to copy.  Otherwise a unit
+// is one pair, or one value to copy.
+template <class T, bool WIDE>
+__global__ __launch_bounds__(kThreads) void rotary_kernel(Turn p) {
+  constexpr int V = WIDE ? Vec16<T>::n : 1;
+  __shared__ float2 angle[kAngles];
+  __shared__ int64_t place[kThreads][2];  // page and offset inside it of a token's slot; page -1: none
+  const int64_t t0 = static_cast<int64_t>(blockIdx.x) * p.per_block;
+  const int count = static_cast<int>(min<int64_t>(p.per_block, p.tokens - t0));
+  const int half = p.rotated / 2;
+  for (int i = threadIdx.x; i < count * half; i += kThreads) {
+    const int t = i / half, pair = i - t * half;
+    const double position = static_cast<double>(load_index(p.positions, t0 + t, p.positions_is64));
+    double turns = position * p.turns[pair];
+    turns -= rint(turns);
+    float s, c;
+    sincospif(2.0f * static_cast<float>(turns), &s, &c);
+    angle[i] = make_float2(c * p.scale, s * p.scale);
+  }
+  if (p.slots)
+    for (int t = threadIdx.x; t < count; t += kThreads) {
+      const int64_t slot = load_index(p.slots, t0 + t, p.slots_is64);
+      const bool in = slot >= 0 && slot < p.capacity;
+      place[t][0] = in ? static_cast<int64_t>(p.page.div(static_cast<uint32_t>(slot))) : int64_t{-1};
+      place[t][1] = in ? static_cast<int64_t>(p.page.mod(static_cast<uint32_t>(slot))) : int64_t{0};
+    }
+  __syncthreads();
+
+  const int turned = WIDE && p.interleaved ? p.rotated / V : WIDE ? half / V : half;  // units of the rotated part
+  const int units = turned + (p.dim - p.rotated) / V, plain = p.dim / V;
+  // heads of q and k have `units` units, those of v `plain`
+  const int of_qk = p.first[2] * units, of_token = of_qk + (p.first[3] - p.first[2]) * plain;
+  for (int item = threadIdx.x; item < count * of_token; item += kThreads) {
+    const int t = item / of_token, in = item - t * of_token;
+    int head, unit;
+    bool turns;
+    if (in < of_qk) {
+      head = in / units, unit = in - head * units;
+      turns = unit < turned;
+    } else {
+      head = p.first[2] + (in - of_qk) / plain, unit = (in - of_qk) % plain;
+      turns = false;
+    }
+    const int which = head < p.first[1] ? 0 : head < p.first[2] ? 1 : 2;
+    const Rows& r = p.rows[which];
+    head -= p.first[which];
+    if (!turns && !(p.copy_rest >> which & 1)) continue;
+    const T* src = static_cast<const T*>(r.src) + (t0 + t) * r.src_token + head * r.src_head;
+    T* dst = static_cast<T*>(r.dst) + head * r.dst_head;
+    if (p.slots && which > 0) {
+      if (place[t][0] < 0) continue;
+      dst += place[t][0] * r.dst_page + place[t][1] * r.dst_token;
+    } else {
+      dst += (t0 + t) * r.dst_token;
+    }
+    const float2* of = angle + t * half;
+    if constexpr (WIDE) {
+      const int at = turns ? unit * V : which < 2 ? p.rotated + (unit - turned) * V : unit * V;
+      uint4 a = *reinterpret_cast<const uint4*>(src + at);
+      if (turns) {
+        float x[V];
+        Vec16<T>::get(a, x);
+        if (p.interleaved) {
+#pragma unroll
+          for (int e = 0; e < V; e += 2) turn_pair(of[(at + e) / 2], x[e], x[e + 1]);
+        } else {
+          float y[V];
+          Vec16<T>::get(*reinterpret_cast<const uint4*>(src + at + half), y);
+#pragma unroll
+          for (int e = 0; e < V; ++e) turn_pair(of[at + e], x[e], y[e]);
+          *reinterpret_cast<uint4*>(dst + at + half) = Vec16<T>::put(y);
+        }
+        a = Vec16<T>::put(x);
+      }
+      *reinterpret_cast<uint4*>(dst + at) = a;
+    } else if (turns) {
+      const int i = p.interleaved ? 2 * unit : unit, j = p.interleaved ? i + 1 : i + half;
+      float x = to_f32(src[i]), y = to_f32(src[j]);
+      turn_pair(of[unit], x, y);
+      dst[i] = from_f32<T>(x), dst[j] = from_f32<T>(y);
+    } else {
+      const int at = which < 2 ? p.rotated + unit - turned : unit;
+      dst[at] = src[at];
+    }
+  }
+}
+
+int launch_turn(Turn& p, int dtype, hipStream_t stream) {
+  const int size = dtype == GDN_F32 ? 4 : 2, vec = 16 / size;
+  const int streams = p.first[3] > p.first[2] ? 3 : 2;
+  bool wide = p.dim % vec == 0 && p.rotated % (p.interleaved ? vec : 2 * vec) == 0;
+  for (int s = 0; s < streams; ++s) {
+    const Rows& r = p.rows[s];
+    if (p.first[s + 1] == p.first[s]) continue;
+    wide = wide && aligned16(r.src) && aligned16(r.dst) &&
+           ((r.src_token | r.src_head | r.dst_token | r.dst_head | r.dst_page) & (vec - 1)) == 0;
+    if (s == 2 || (r.src != r.dst && p.dim > p.rotated)) p.copy_rest |= 1 << s;
+  }
+  // a block's tokens: two passes of its threads over them, as far as LDS holds their angles
+  const int64_t heads = p.first[3];
+  const int64_t pieces = std::max<int64_t>(1, heads * p.dim / (wide ? vec : 1));
+  int64_t per = std::max<int64_t>(1, 2 * kThreads / pieces);
+  if (p.rotated) per = std::min<int64_t>(per, std::max(1, 2 * kAngles / p.rotated));
+  p.per_block = static_cast<int>(std::min<int64_t>(per, kThreads));
+  const int64_t blocks = (p.tokens + p.per_block - 1) / p.per_block;
+  auto go = [&](auto kernel) { kernel<<<static_cast<uint32_t>(blocks), kThreads, 0, stream>>>(p); };
+  switch (dtype) {
+    case GDN_F32: wide ? go(rotary_kernel<float, true>) : go(rotary_kernel<float, false>); break;
+    case GDN_BF16: wide ? go(rotary_kernel<bf16, true>) : go(rotary_kernel<bf16, false>); break;
+    default: wide ? go(rotary_kernel<f16, true>) : go(rotary_kernel<f16, false>); break;
+  }
+  return GDN_LAUNCH_CHECK("rotary");
+}
+
+// Sizes shared by both entry points; GDN_OK, or the error.
+int set_turn(Turn& p, int dtype, int64_t tokens, int64_t heads, int64_t dim, const void* positions, int positions_dtype,
+             const double* turns, int64_t rotated, int interleaved, float scale) {
+  GDN_REQUIRE(dtype == GDN_F32 || dtype == GDN_BF16 || dtype == GDN_F16, "dtype must be f32, bf16 or f16");
+  GDN_REQUIRE(tokens >= 0 && tokens < (int64_t{1} << 31) && heads >= 0 && dim > 0, "bad shape");
+  GDN_REQUIRE(rotated >= 0 && rotated % 2 == 0 && rotated <= dim, "the rotated channels must be an even part of the head");
+  GDN_REQUIRE(tokens == 0 || rotated == 0 || (positions && turns), "null positions or frequencies");
+  GDN_REQUIRE(positions_dtype == GDN_I32 || positions_dtype == GDN_I64, "positions must be int32 or int64");
+  if (heads * dim >= (int64_t{1} << 24) || dim > 2 * kAngles) {
+    set_error("heads x dim up to 2^24, dim up to %d", 2 * kAngles);
+    return GDN_ERR_UNSUPPORTED;
+  }
+  p.positions = positions;
+  p.positions_is64 = positions_dtype == GDN_I64;
+  p.turns = turns;
+  p.tokens = static_cast<int>(tokens);
+  p.dim = static_cast<int>(dim);
+  p.rotated = static_cast<int>(rotated);
+  p.interleaved = interleaved != 0;
+  p.scale = scale;
+  return GDN_OK;
+}
+
+}  // namespace
+}  // namespace gdn
+
+using namespace gdn;
+
+extern "C" int gdn_apply_rotary(const void* q, int64_t q_token_stride, int64_t q_head_stride, int64_t q_heads,
+                                const void* k, int64_t k_token_stride, int64_t k_head_stride, int64_t k_heads, int dtype,
+                                int64_t tokens, int64_t dim, const void* positions, int positions_dtype,
+                                const double* turns, int64_t rotated, int interleaved, float scale, void* q_out,
+                                int64_t q_out_token_stride, int64_t q_out_head_stride, void* k_out,
+                                int64_t k_out_token_stride, int64_t k_out_head_stride, void* stream) {
+  Turn p{};
+  GDN_REQUIRE(q_heads >= 0 && k_heads >= 0, "bad shape");
+  if (const int rc = set_turn(p, dtype, tokens, q_heads + k_heads, dim, positions, positions_dtype, turns, rotated,
+                              interleaved, scale))
+    return rc;
+  if (tokens == 0 || q_heads + k_heads == 0) return GDN_OK;
+  GDN_REQUIRE((q_heads == 0 || (q && q_out)) && (k_heads == 0 || (k && k_out)), "null rows");
+  p.rows[0] = {q, q_out, q_token_stride, q_head_stride, q_out_token_stride, q_out_head_stride, 0};
+  p.rows[1] = {k, k_out, k_token_stride, k_head_stride, k_out_token_stride, k_out_head_stride, 0};
+  p.first[1] = static_cast<int>(q_heads);
+  p.first[2] = p.first[3] = static_cast<int>(q_heads + k_heads);
+  return launch_turn(p, dtype, static_cast<hipStream_t>(stream));
+}
+
+extern "C" int gdn_append_paged_kv(const void* k, int64_t k_token_stride, int64_t k_head_stride, const void* v,
+                                   int64_t v_token_stride, int64_t v_head_stride, int64_t kv_heads, int dtype,
+                                   int64_t tokens, int64_t dim, const void* slots, int slots_dtype, void* k_cache,
+                                   int64_t k_page_stride, int64_t k_cache_token_stride, int64_t k_cache_head_stride,
+                                   void* v_cache, int64_t v_page_stride, int64_t v_cache_token_stride,
+                                   int64_t v_cache_head_stride, int64_t pages, int64_t page_size, const void* positions,
+                                   int positions_dtype, const double* turns, int64_t rotated, int interleaved,
+                                   float scale, const void* q, int64_t q_token_stride, int64_t q_head_stride,
+                                   int64_t q_heads, void* q_out, int64_t q_out_token_stride, int64_t q_out_head_stride,
+                                   void* stream) {
+  Turn p{};
+  GDN_REQUIRE(q_heads >= 0 && kv_heads > 0, "bad shape");
+  if (const int rc = set_turn(p, dtype, tokens, q_heads + 2 * kv_heads, dim, positions, positions_dtype, turns, rotated,
+                              interleaved, scale))
+    return rc;
+  GDN_REQUIRE(pages >= 0 && page_size > 0, "bad cache shape");
+  GDN_REQUIRE(slots_dtype == GDN_I32 || slots_dtype == GDN_I64, "slots must be int32 or int64");
+  if (page_size >= (int64_t{1} << 31) || pages * page_size >= (int64_t{1} << 31)) {
+    set_error("a cache of up to 2^31 tokens");
+    return GDN_ERR_UNSUPPORTED;
+  }
+  if (tokens == 0) return GDN_OK;
+  GDN_REQUIRE(k && v && slots && (pages == 0 || (k_cache && v_cache)) && (q_heads == 0 || (q && q_out)), "null operand");
+  p.rows[0] = {q, q_out, q_token_stride, q_head_stride, q_out_token_stride, q_out_head_stride, 0};
+  p.rows[1] = {k, k_cache, k_token_stride, k_head_stride, k_cache_token_stride, k_cache_head_stride, k_page_stride};
+  p.rows[2] = {v, v_cache, v_token_stride, v_head_stride, v_cache_token_stride, v_cache_head_stride, v_page_stride};
+  p.first[1] = static_cast<int>(q_heads);
+  p.first[2] = static_cast<int>(q_heads + kv_heads);
+  p.first[3] = static_cast<int>(q_heads + 2 * kv_heads);
+  p.slots = slots;
+  p.slots_is64 = slots_dtype == GDN_I64;
+  p.page = make_div32(page_size);
+  p.capacity = pages * page_size;
+  return launch_turn(p, dtype, static_cast<hipStream_t>(stream));
+}
