@@ -260,11 +260,22 @@ template <> struct Op<f16> {
   }
 };
 
-__device__ __forceinline__ int page_at(const Attend& p, int request, int index) {
-  typedef const __attribute__((address_space(4))) int32_t const_int;  // scalar loads
-  const int64_t at = static_cast<int64_t>(request) * p.table_row + index;
-  return *(const_int*)(static_cast<const int32_t*>(p.table) + (p.table_is64 ? 2 * at : at));
-}
+// Where 64 subtiles of 16 positions lie, one in each lane, looked up together so
+// that the steps' loads wait for no table.
+struct Pages {
+  int id, in;  // page (-1: none), first position inside it
+  // lane l: the positions from `at` on (a multiple of 16) of a request's row of the table
+  __device__ __forceinline__ void find(const Attend& p, int request, int at, int end) {
+    id = -1, in = 0;
+    if (at < end) {
+      const uint32_t index = p.page.div(at);
+      in = at - static_cast<int>(index * p.page.d);
+      const int64_t entry = static_cast<int64_t>(request) * p.table_row + index;
+      id = static_cast<int>(load_index(p.table, entry, p.table_is64));
+      if (id < 0 || id >= p.pages) id = -1;
+    }
+  }
+};
 
 template <int N> __device__ __forceinline__ void wait_loads() { asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory"); }
 __device__ __forceinline__ void reads_done() { asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory"); }
@@ -299,18 +310,13 @@ __device__ __forceinline__ void load16(const Cache& c, int page, int in_page, in
   }
 }
 
-// 16 positions from `at` (a multiple of 16) of a request's row of the table, of
-// which those before `end` are there.  A page outside of the cache reads as zeros.
+// The subtile of lane `which` of `pages`, at `at`, of which the positions before
+// `end` are there.  A page outside of the cache reads as zeros.
 template <int D, bool V>
-__device__ __forceinline__ void load_positions(const Attend& p, int request, int at, int end, int head, char* lds,
-                                               int lane) {
-  int valid = end - at < 16 ? end - at : 16, page = 0, in = 0;
-  if (valid > 0) {
-    const uint32_t index = p.page.div(at);
-    in = at - index * p.page.d;
-    page = page_at(p, request, index);
-    if (page < 0 || page >= p.pages) valid = 0, page = 0;
-  }
+__device__ __forceinline__ void load_positions(const Attend& p, const Pages& pages, int which, int at, int end, int head,
+                                               char* lds, int lane) {
+  const int page = __builtin_amdgcn_readlane(pages.id, which), in = __builtin_amdgcn_readlane(pages.in, which);
+  const int there = page < 0 ? 0 : end - at, valid = there < 16 ? there : 16;
   load16<D, V>(V ? p.v : p.k, page, in, head, valid, lds, lane);
 }
 
@@ -393,36 +399,42 @@ struct Rows {
   __device__ __forceinline__ bool partly(const Segment& seg, int at) const {
     return at < seg.lo || at + 32 * TILES > least;
   }
-  // The softmax's step: s becomes the weights, in the io type as the right operand.
   template <int TILES>
-  __device__ __forceinline__ void weights(const Attend& p, const Segment& seg, int at, int lane, f32x16 (&s)[TILES],
-                                          Frag (&w)[2 * TILES]) {
-    if (partly<TILES>(seg, at)) {
+  __device__ __forceinline__ void mask(const Segment& seg, int at, int lane, f32x16 (&s)[TILES]) const {
+    if (!partly<TILES>(seg, at)) return;
 #pragma unroll
-      for (int t = 0; t < TILES; ++t)
+    for (int t = 0; t < TILES; ++t)
 #pragma unroll
-        for (int e = 0; e < 16; ++e) {
-          const int pos = at + 32 * t + 8 * (e >> 2) + 4 * (lane >> 5) + (e & 3);
-          if (pos < seg.lo || pos >= limit) s[t][e] = -INFINITY;
-        }
-    }
+      for (int e = 0; e < 16; ++e) {
+        const int pos = at + 32 * t + 8 * (e >> 2) + 4 * (lane >> 5) + (e & 3);
+        if (pos < seg.lo || pos >= limit) s[t][e] = -INFINITY;
+      }
+  }
+  // The row's largest score of the tile (base 2).
+  template <int TILES>
+  __device__ __forceinline__ float largest(const Attend& p, const f32x16 (&s)[TILES]) const {
     float top = s[0][0];
 #pragma unroll
     for (int t = 0; t < TILES; ++t)
 #pragma unroll
       for (int e = 0; e < 16; ++e) top = fmaxf(top, s[t][e]);
-    top = fmaxf(top, other_half(top)) * p.factor;
-    // rescaled only where the maximum has grown by more than 2^8: fp32 sums have room for that
+    return fmaxf(top, other_half(top)) * p.factor;
+  }
+  // The maximum raised to `top`, where that is more than 2^8 above it: fp32 sums have room for less.
+  __device__ __forceinline__ void raise(float top) {
     const bool grown = top > m + kLater;
-    if (__any(grown)) {
-      const float alpha = grown ? fast_exp2(m - top) : 1.0f;
-      m = grown ? top : m;
-      l *= alpha;
+    if (!__any(grown)) return;
+    const float alpha = grown ? fast_exp2(m - top) : 1.0f;
+    m = grown ? top : m;
+    l *= alpha;
 #pragma unroll
-      for (int i = 0; i < D / 32; ++i)
+    for (int i = 0; i < D / 32; ++i)
 #pragma unroll
-        for (int e = 0; e < 16; ++e) o[i][e] *= alpha;
-    }
+      for (int e = 0; e < 16; ++e) o[i][e] *= alpha;
+  }
+  // Scores to weights, in the io type as the right operand.
+  template <int TILES>
+  __device__ __forceinline__ void weights(const Attend& p, f32x16 (&s)[TILES], Frag (&w)[2 * TILES]) {
     const float less = m == -INFINITY ? 0.f : m;
     float sum = 0.f;
 #pragma unroll
@@ -512,12 +524,14 @@ __device__ __forceinline__ float weight_of(float m, float l, float top) { return
 __device__ __forceinline__ float lse_of(float m, float l) { return l > 0.f || l != l ? (m + log2f(l)) * kLn2 : -INFINITY; }
 
 // ------------------------------------------------------------------ many rows
-// Four waves of 32 rows each; the block's keys and values come through two LDS
-// buffers, one loaded while the other is read.
+// Four waves of 32 rows each.  Keys and values come through a ring of LDS tiles,
+// loaded three steps ahead.  A step computes the scores of the next tile while it
+// turns those of this one into weights (matrix and vector instructions beside each
+// other), then adds this tile's values while it finds the next tile's maximum.
 template <int D> struct Many {
-  static constexpr int kRows = 128, kTiles = D == 256 ? 1 : 2, kKeys = 32 * kTiles;
-  static constexpr int kHalf = kKeys * 2 * D, kBuffer = 2 * kHalf;
-  static constexpr int kLds = 2 * kBuffer;
+  static constexpr int kRows = 128, kTiles = D == 64 ? 2 : 1, kKeys = 32 * kTiles;
+  static constexpr int kHalf = kKeys * 2 * D, kTile = 2 * kHalf, kRing = 4, kLds = kRing * kTile;
+  static constexpr int kLoads = kTile / 1024 / 4;  // of a wave and step
 };
 
 template <class T, int D>
@@ -548,45 +562,57 @@ __global__ __launch_bounds__(kThreads, D == 256 ? 1 : 2) void many_rows_kernel(A
     }
     to = uniform(to);
     const int end = it.seg.hi, steps = to > it.from ? (to - it.from + M::kKeys - 1) / M::kKeys : 0;
+    // a wave brings 16 positions of a step: their keys and values, or in steps of 32 one of both
+    const bool brings_k = M::kTiles == 2 || wave < 2, brings_v = M::kTiles == 2 || wave >= 2;
+    const int sub = M::kTiles == 2 ? wave : wave & 1;
+    Pages pages;
     auto load = [&](int step) __attribute__((always_inline)) {
-      char* buffer = lds + (step & 1) * M::kBuffer;
-      const int at = it.from + step * M::kKeys;
-      if constexpr (M::kTiles == 2) {  // a wave brings 16 positions
-        load_positions<D, false>(p, it.seg.request, at + 16 * wave, end, it.head, buffer + wave * 32 * D, lane);
-        load_positions<D, true>(p, it.seg.request, at + 16 * wave, end, it.head, buffer + M::kHalf + wave * 32 * D, lane);
-      } else if (wave < 2) {
-        load_positions<D, false>(p, it.seg.request, at + 16 * wave, end, it.head, buffer + wave * 32 * D, lane);
-      } else {
-        load_positions<D, true>(p, it.seg.request, at + 16 * (wave - 2), end, it.head,
-                                buffer + M::kHalf + (wave - 2) * 32 * D, lane);
-      }
+      if ((step & 63) == 0) pages.find(p, it.seg.request, it.from + (step + lane) * M::kKeys + 16 * sub, end);
+      char* tile = lds + (step % M::kRing) * M::kTile + sub * 32 * D;
+      const int at = it.from + step * M::kKeys + 16 * sub, until = step < steps ? end : 0;
+      if (brings_k) load_positions<D, false>(p, pages, step & 63, at, until, it.head, tile, lane);
+      if (brings_v) load_positions<D, true>(p, pages, step & 63, at, until, it.head, tile + M::kHalf, lane);
     };
-    lds_barrier();  // the last item's buffers are free
+    lds_barrier();  // the last item's ring is free
     bad.clear();
     if (lane == 0) least[wave] = rows.least;
-    if (steps > 0) load(0);
+#pragma unroll
+    for (int step = 0; step < M::kRing - 1; ++step) load(step);
     lds_barrier();
     const int all_see = uniform(min(min(least[0], least[1]), min(least[2], least[3])));
-    for (int step = 0; step < steps; ++step) {
-      wait_loads<0>();
-      if (it.from + step * M::kKeys < it.seg.lo || it.from + (step + 1) * M::kKeys > all_see) {
-        const int sub = M::kTiles == 2 ? wave : wave - 2;
-        if (sub >= 0)
-          take_out<T, D>(lds + (step & 1) * M::kBuffer + M::kHalf + sub * 32 * D, it.from + step * M::kKeys + 16 * sub,
-                         it.seg.lo, bad, lane);
-      }
-      lds_barrier();
-      if (step + 1 < steps) load(step + 1);
-      const char* buffer = lds + (step & 1) * M::kBuffer;
+    // this wave's part of the step's tile is there
+    auto arrived = [&](int step) __attribute__((always_inline)) {
       const int at = it.from + step * M::kKeys;
-      if (at < rows.most) {
-        f32x16 s[M::kTiles];
-        typename Op<T>::frag w[2 * M::kTiles];
-        rows.template scores<M::kTiles>(buffer, lane, s);
-        rows.template weights<M::kTiles>(p, it.seg, at, lane, s, w);
-        rows.template values<M::kTiles>(buffer + M::kHalf, lane, w);
-      }
+      if (brings_v && step < steps && (at < it.seg.lo || at + M::kKeys > all_see))
+        take_out<T, D>(lds + (step % M::kRing) * M::kTile + M::kHalf + sub * 32 * D, at + 16 * sub, it.seg.lo, bad, lane);
+    };
+    using Scores = f32x16[M::kTiles];
+    Scores s[2];
+    typename Op<T>::frag w[2 * M::kTiles];
+    wait_loads<2 * M::kLoads>();
+    arrived(0);
+    lds_barrier();
+    rows.template scores<M::kTiles>(lds, lane, s[0]);
+    rows.template mask<M::kTiles>(it.seg, it.from, lane, s[0]);
+    // a tile behind the last is all zeros, and its scores may not raise anything
+    if (steps > 0) rows.raise(rows.template largest<M::kTiles>(p, s[0]));
+    auto advance = [&](int step, Scores& now, Scores& next) __attribute__((always_inline)) {
+      wait_loads<M::kLoads>();
+      arrived(step + 1);
+      lds_barrier();  // the next tile is there, the one before this free
+      load(step + 3);
+      rows.template scores<M::kTiles>(lds + ((step + 1) % M::kRing) * M::kTile, lane, next);
+      rows.template weights<M::kTiles>(p, now, w);
+      rows.template mask<M::kTiles>(it.seg, it.from + (step + 1) * M::kKeys, lane, next);
+      rows.template values<M::kTiles>(lds + (step % M::kRing) * M::kTile + M::kHalf, lane, w);
+      if (step + 1 < steps) rows.raise(rows.template largest<M::kTiles>(p, next));
+    };
+    for (int step = 0; step < steps; step += 2) {
+      advance(step, s[0], s[1]);
+      if (step + 1 == steps) break;
+      advance(step + 1, s[1], s[0]);
     }
+    wait_loads<0>();  // those past the end too, before the ring is used again
     const float l = rows.l + other_half(rows.l);
     if (uniform(bad.found)) {
 #pragma unroll
@@ -650,23 +676,25 @@ __global__ __launch_bounds__(kThreads, Few<D>::kBlocks) void few_rows_kernel(Att
   char* mine = lds + wave * F::kWave;
   for (int item = blockIdx.x; item < total; item += gridDim.x) {
     const Item it = item_of<false, kFew, F::kUnit>(p, plan, each, range, item);
+    const int end = it.seg.hi, steps = (it.to - it.from + 31) / 32;
+    Pages pages;
+    // this wave's steps are wave, wave + 4, ...: 32 of them to a lookup
+    auto load_k = [&](int step) __attribute__((always_inline)) {
+      if ((step >> 2 & 31) == 0)
+        pages.find(p, it.seg.request, it.from + 32 * (step + 4 * (lane >> 1)) + 16 * (lane & 1), end);
+      const int at = it.from + 32 * step, which = 2 * (step >> 2 & 31), until = step < steps ? end : 0;
+      load_positions<D, false>(p, pages, which, at, until, it.head, mine, lane);
+      load_positions<D, false>(p, pages, which + 1, at + 16, until, it.head, mine + 32 * D, lane);
+    };
+    auto load_v = [&](int step) __attribute__((always_inline)) {
+      const int at = it.from + 32 * step, which = 2 * (step >> 2 & 31), until = step < steps ? end : 0;
+      load_positions<D, true>(p, pages, which, at, until, it.head, mine + F::kHalf, lane);
+      load_positions<D, true>(p, pages, which + 1, at + 16, until, it.head, mine + F::kHalf + 32 * D, lane);
+    };
+    lds_barrier();  // the last item's sums have been read
     Rows<T, D> rows;
     rows.load(p, it, lane & 31, lane);
     rows.clear();
-    wait_loads<0>();
-    const int end = it.seg.hi, to = min(it.to, rows.most);
-    const int steps = to > it.from ? (to - it.from + 31) / 32 : 0;
-    auto load_k = [&](int step) __attribute__((always_inline)) {
-      const int at = it.from + 32 * step;
-      load_positions<D, false>(p, it.seg.request, at, step < steps ? end : 0, it.head, mine, lane);
-      load_positions<D, false>(p, it.seg.request, at + 16, step < steps ? end : 0, it.head, mine + 32 * D, lane);
-    };
-    auto load_v = [&](int step) __attribute__((always_inline)) {
-      const int at = it.from + 32 * step;
-      load_positions<D, true>(p, it.seg.request, at, step < steps ? end : 0, it.head, mine + F::kHalf, lane);
-      load_positions<D, true>(p, it.seg.request, at + 16, step < steps ? end : 0, it.head, mine + F::kHalf + 32 * D, lane);
-    };
-    lds_barrier();  // the last item's sums have been read
     load_k(wave);
     load_v(wave);
     bad.clear();
@@ -678,12 +706,15 @@ __global__ __launch_bounds__(kThreads, Few<D>::kBlocks) void few_rows_kernel(Att
       wait_loads<F::kLoads>();  // the keys; the values may be on their way
       rows.template scores<1>(mine, lane, s);
       reads_done();
+      const int at = it.from + 32 * step;
       load_k(step + 4);
-      rows.template weights<1>(p, it.seg, it.from + 32 * step, lane, s, w);
+      rows.template mask<1>(it.seg, at, lane, s);
+      rows.raise(rows.template largest<1>(p, s));
+      rows.template weights<1>(p, s, w);
       wait_loads<F::kLoads>();
-      if (rows.template partly<1>(it.seg, it.from + 32 * step)) {
-        take_out<T, D>(mine + F::kHalf, it.from + 32 * step, it.seg.lo, bad, lane);
-        take_out<T, D>(mine + F::kHalf + 32 * D, it.from + 32 * step + 16, it.seg.lo, bad, lane);
+      if (rows.template partly<1>(it.seg, at)) {
+        take_out<T, D>(mine + F::kHalf, at, it.seg.lo, bad, lane);
+        take_out<T, D>(mine + F::kHalf + 32 * D, at + 16, it.seg.lo, bad, lane);
       }
       rows.template values<1>(mine + F::kHalf, lane, w);
       reads_done();
