@@ -339,6 +339,9 @@ __device__ __forceinline__ typename Op<T>::frag v_frag(const char* lds, int row,
   return __builtin_bit_cast(typename Op<T>::frag, __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7));
 }
 
+// Instructions stay on their side of it.
+__device__ __forceinline__ void in_order() { __builtin_amdgcn_sched_barrier(0); }
+
 __device__ __forceinline__ float other_half(float v) { return __shfl_xor(v, 32, 64); }
 
 // One wave's rows: 32 of them, a lane and its partner 32 lanes on share one.
@@ -383,15 +386,26 @@ struct Rows {
     least = uniform(a), most = uniform(b);
   }
 
-  // 32 KEYS positions from `at` on, whose keys and values lie in LDS.
-  template <int TILES>
-  __device__ __forceinline__ void scores(const char* k, int lane, f32x16 (&s)[TILES]) const {
+  // Scores of 32 TILES positions whose keys lie in LDS.  Fragments are read AHEAD of their
+  // instructions; beside(i) goes behind the i-th matrix instruction.
+  template <int TILES, class Beside>
+  __device__ __forceinline__ void scores(const char* k, int lane, f32x16 (&s)[TILES], Beside beside) const {
+    constexpr int kMmas = D / 16 * TILES, kAhead = 4;
+    Frag f[kAhead];
+    auto read = [&](int i) __attribute__((always_inline)) { return k_frag<T, D>(k, i / (D / 16) * 32, i % (D / 16), lane); };
 #pragma unroll
-    for (int t = 0; t < TILES; ++t) {
+    for (int i = 0; i < kAhead; ++i) f[i] = read(i);
+#pragma unroll
+    for (int t = 0; t < TILES; ++t)
 #pragma unroll
       for (int e = 0; e < 16; ++e) s[t][e] = 0.f;
+    in_order();
 #pragma unroll
-      for (int i = 0; i < D / 16; ++i) s[t] = Op<T>::mma(k_frag<T, D>(k, 32 * t, i, lane), q[i], s[t]);
+    for (int i = 0; i < kMmas; ++i) {
+      s[i / (D / 16)] = Op<T>::mma(f[i % kAhead], q[i % (D / 16)], s[i / (D / 16)]);
+      if (i + kAhead < kMmas) f[i % kAhead] = read(i + kAhead);
+      beside(i);
+      in_order();
     }
   }
   // Whether some row of the wave does not see all of the 32 TILES positions from `at` on (uniform).
@@ -410,14 +424,8 @@ struct Rows {
         if (pos < seg.lo || pos >= limit) s[t][e] = -INFINITY;
       }
   }
-  // The row's largest score of the tile (base 2).
-  template <int TILES>
-  __device__ __forceinline__ float largest(const Attend& p, const f32x16 (&s)[TILES]) const {
-    float top = s[0][0];
-#pragma unroll
-    for (int t = 0; t < TILES; ++t)
-#pragma unroll
-      for (int e = 0; e < 16; ++e) top = fmaxf(top, s[t][e]);
+  // The row's largest score (base 2) from the largest of the lane's own.
+  __device__ __forceinline__ float of_row(const Attend& p, float top) const {
     return fmaxf(top, other_half(top)) * p.factor;
   }
   // The maximum raised to `top`, where that is more than 2^8 above it: fp32 sums have room for less.
@@ -432,34 +440,41 @@ struct Rows {
 #pragma unroll
       for (int e = 0; e < 16; ++e) o[i][e] *= alpha;
   }
-  // Scores to weights, in the io type as the right operand.
+  // Elements first .. last - 1 of the scores to weights, in the io type as the right operand.
   template <int TILES>
-  __device__ __forceinline__ void weights(const Attend& p, f32x16 (&s)[TILES], Frag (&w)[2 * TILES]) {
-    const float less = m == -INFINITY ? 0.f : m;
-    float sum = 0.f;
+  __device__ __forceinline__ void weights(const Attend& p, int first, int last, float less, f32x16 (&s)[TILES],
+                                          uint4 (&w)[2 * TILES]) {
 #pragma unroll
-    for (int t = 0; t < TILES; ++t) {
-#pragma unroll
-      for (int e = 0; e < 16; ++e) {
-        s[t][e] = fast_exp2(fmaf(s[t][e], p.factor, -less));
-        sum += s[t][e];
-      }
-#pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        const uint4 packed =
-            make_uint4(out_pack2<T>(s[t][8 * h], s[t][8 * h + 1]), out_pack2<T>(s[t][8 * h + 2], s[t][8 * h + 3]),
-                       out_pack2<T>(s[t][8 * h + 4], s[t][8 * h + 5]), out_pack2<T>(s[t][8 * h + 6], s[t][8 * h + 7]));
-        w[2 * t + h] = __builtin_bit_cast(Frag, packed);
+    for (int i = first; i < last; ++i) {
+      float& x = reinterpret_cast<float*>(&s[i / 16])[i % 16];
+      x = fast_exp2(fmaf(x, p.factor, -less));
+      l += x;
+      if (i & 1) {
+        const uint32_t pair = out_pack2<T>(reinterpret_cast<float*>(&s[i / 16])[i % 16 - 1], x);
+        reinterpret_cast<uint32_t*>(&w[i / 8])[i % 8 / 2] = pair;
       }
     }
-    l += sum;
   }
-  template <int TILES>
-  __device__ __forceinline__ void values(const char* v, int lane, const Frag (&w)[2 * TILES]) {
+  __device__ __forceinline__ float subtracted() const { return m == -INFINITY ? 0.f : m; }
+  // O^T += V^T P^T of 32 TILES positions.
+  template <int TILES, class Beside>
+  __device__ __forceinline__ void values(const char* v, int lane, const uint4 (&w)[2 * TILES], Beside beside) {
+    constexpr int kMmas = D / 32 * 2 * TILES, kAhead = 4;
+    Frag f[kAhead];
+    auto read = [&](int i) __attribute__((always_inline)) {
+      return v_frag<T, D>(v, 16 * (i % (2 * TILES)), i / (2 * TILES), lane);
+    };
 #pragma unroll
-    for (int d = 0; d < D / 32; ++d)
+    for (int i = 0; i < kAhead; ++i) f[i] = read(i);
+    in_order();
 #pragma unroll
-      for (int i = 0; i < 2 * TILES; ++i) o[d] = Op<T>::mma(v_frag<T, D>(v, 16 * i, d, lane), w[i], o[d]);
+    for (int i = 0; i < kMmas; ++i) {
+      f32x16& sum = o[i / (2 * TILES)];
+      sum = Op<T>::mma(f[i % kAhead], __builtin_bit_cast(Frag, w[i % (2 * TILES)]), sum);
+      if (i + kAhead < kMmas) f[i % kAhead] = read(i + kAhead);
+      beside(i);
+      in_order();
+    }
   }
 };
 
@@ -588,24 +603,41 @@ __global__ __launch_bounds__(kThreads, D == 256 ? 1 : 2) void many_rows_kernel(A
     };
     using Scores = f32x16[M::kTiles];
     Scores s[2];
-    typename Op<T>::frag w[2 * M::kTiles];
+    uint4 w[2 * M::kTiles];
+    constexpr int kScores = 16 * M::kTiles, kMmas = D / 16 * M::kTiles, kBeside = kScores / kMmas;
+    auto nothing = [](int) __attribute__((always_inline)) {};
     wait_loads<2 * M::kLoads>();
     arrived(0);
     lds_barrier();
-    rows.template scores<M::kTiles>(lds, lane, s[0]);
+    rows.template scores<M::kTiles>(lds, lane, s[0], nothing);
     rows.template mask<M::kTiles>(it.seg, it.from, lane, s[0]);
+    float top = -INFINITY;
+    auto larger = [&](Scores& of, int i) __attribute__((always_inline)) {
+      top = fmaxf(top, of[i / 16][i % 16]);
+    };
+#pragma unroll
+    for (int i = 0; i < kScores; ++i) larger(s[0], i);
     // a tile behind the last is all zeros, and its scores may not raise anything
-    if (steps > 0) rows.raise(rows.template largest<M::kTiles>(p, s[0]));
+    if (steps > 0) rows.raise(rows.of_row(p, top));
     auto advance = [&](int step, Scores& now, Scores& next) __attribute__((always_inline)) {
       wait_loads<M::kLoads>();
       arrived(step + 1);
       lds_barrier();  // the next tile is there, the one before this free
       load(step + 3);
-      rows.template scores<M::kTiles>(lds + ((step + 1) % M::kRing) * M::kTile, lane, next);
-      rows.template weights<M::kTiles>(p, now, w);
+      const float less = rows.subtracted();
+      rows.template scores<M::kTiles>(lds + ((step + 1) % M::kRing) * M::kTile, lane, next, [&](int i) __attribute__((always_inline)) {
+        rows.template weights<M::kTiles>(p, i * kBeside, (i + 1) * kBeside, less, now, w);
+      });
       rows.template mask<M::kTiles>(it.seg, it.from + (step + 1) * M::kKeys, lane, next);
-      rows.template values<M::kTiles>(lds + (step % M::kRing) * M::kTile + M::kHalf, lane, w);
-      if (step + 1 < steps) rows.raise(rows.template largest<M::kTiles>(p, next));
+      top = -INFINITY;
+      // behind the first quarter: the scores' last matrix instruction is done by then
+      rows.template values<M::kTiles>(lds + (step % M::kRing) * M::kTile + M::kHalf, lane, w, [&](int i) __attribute__((always_inline)) {
+        constexpr int kFrom = kMmas / 4, kEach = (kScores + kMmas - kFrom - 1) / (kMmas - kFrom);
+#pragma unroll
+        for (int e = 0; e < kEach; ++e)
+          if (i >= kFrom && (i - kFrom) * kEach + e < kScores) larger(next, (i - kFrom) * kEach + e);
+      });
+      if (step + 1 < steps) rows.raise(rows.of_row(p, top));
     };
     for (int step = 0; step < steps; step += 2) {
       advance(step, s[0], s[1]);
@@ -702,21 +734,24 @@ __global__ __launch_bounds__(kThreads, Few<D>::kBlocks) void few_rows_kernel(Att
     lds_barrier();
     for (int step = wave; step < steps; step += 4) {
       f32x16 s[1];
-      typename Op<T>::frag w[2];
+      uint4 w[2];
       wait_loads<F::kLoads>();  // the keys; the values may be on their way
-      rows.template scores<1>(mine, lane, s);
+      rows.template scores<1>(mine, lane, s, [](int) {});
       reads_done();
       const int at = it.from + 32 * step;
       load_k(step + 4);
       rows.template mask<1>(it.seg, at, lane, s);
-      rows.raise(rows.template largest<1>(p, s));
-      rows.template weights<1>(p, s, w);
+      float top = s[0][0];
+#pragma unroll
+      for (int e = 1; e < 16; ++e) top = fmaxf(top, s[0][e]);
+      rows.raise(rows.of_row(p, top));
+      rows.template weights<1>(p, 0, 16, rows.subtracted(), s, w);
       wait_loads<F::kLoads>();
       if (rows.template partly<1>(it.seg, at)) {
         take_out<T, D>(mine + F::kHalf, at, it.seg.lo, bad, lane);
         take_out<T, D>(mine + F::kHalf + 32 * D, at + 16, it.seg.lo, bad, lane);
       }
-      rows.template values<1>(mine + F::kHalf, lane, w);
+      rows.template values<1>(mine + F::kHalf, lane, w, [](int) {});
       reads_done();
       load_v(step + 4);
     }
