@@ -29,6 +29,7 @@ namespace gdn {
 namespace {
 
 typedef float f32x16 __attribute__((ext_vector_type(16)));
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 typedef short s16x4 __attribute__((ext_vector_type(4)));
 typedef short s16x8 __attribute__((ext_vector_type(8)));
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
@@ -292,50 +293,83 @@ template <int D> struct Tile {
   static __device__ __forceinline__ int swizzle_v(int row) { return D == 64 ? 4 * (row >> 1 & 1) : 4 * (row & 3); }
 };
 
-// Direct loads of 16 positions of one head to LDS; zeros for those past `valid`.
-template <int D, bool V>
-__device__ __forceinline__ void load16(const Cache& c, int page, int in_page, int head, int valid, char* lds, int lane) {
-  using L = Tile<D>;
-  const char* base = static_cast<const char*>(c.at) + 2 * (page * c.page + in_page * c.token + head * c.head);
-  const uint32_t stride = static_cast<uint32_t>(2 * c.token);
-  const uint32_t bytes = valid > 0 ? (valid - 1) * stride + L::kRow : 0;
-  const __amdgpu_buffer_rsrc_t rsrc =
-      __builtin_amdgcn_make_buffer_rsrc(const_cast<char*>(base), 0, bytes, 0x00020000);
-  const int row = lane / L::kPieces, piece = lane % L::kPieces;
+// A direct-to-LDS load of 16 bytes a lane: lane l lands at lds + 16 l, zeros where off is past bytes.
+__device__ __forceinline__ __amdgpu_buffer_rsrc_t rsrc_of(const void* from, uint32_t bytes) {
+  return __builtin_amdgcn_make_buffer_rsrc(const_cast<void*>(from), 0, bytes, 0x00020000);
+}
+__device__ __forceinline__ void dma16(const void* src, uint32_t bytes, uint32_t off, void* lds) {
+  __builtin_amdgcn_raw_ptr_buffer_load_lds(rsrc_of(src, bytes), (lds_void*)lds, 16, off, 0, 0, 0);
+}
+// Direct loads of one head's keys or values to LDS, 16 positions at a time: lane l of
+// the i-th load of 16 bytes a lane lands 16 l behind lds + 1024 i.
+template <int D>
+struct Feed {
+  static constexpr int kLoads = 16 / Tile<D>::kPerLoad;
+  const char* head;      // the head's first channel in the first page
+  int64_t page, token;   // strides, bytes
+  uint32_t from[kLoads];  // the lane's piece of each load, bytes behind the first position's
+  const char* at;        // what aim() has found: the first position, the bytes that may be read
+  uint32_t bytes;
+
+  __device__ __forceinline__ void start(const Cache& c, int of, bool values, int lane) {
+    using L = Tile<D>;
+    head = static_cast<const char*>(c.at) + 2 * of * c.head;
+    page = 2 * c.page, token = 2 * c.token;
+    const int row = lane / L::kPieces, piece = lane % L::kPieces;
 #pragma unroll
-  for (int i = 0; i < 16 / L::kPerLoad; ++i) {
-    const int r = i * L::kPerLoad + row;
-    const int from = piece ^ (V ? L::swizzle_v(r) : L::swizzle_k(r));
-    __builtin_amdgcn_raw_ptr_buffer_load_lds(rsrc, (lds_void*)(lds + i * 1024), 16, r * stride + 16 * from, 0, 0, 0);
+    for (int i = 0; i < kLoads; ++i) {
+      const int r = i * L::kPerLoad + row;
+      from[i] = r * static_cast<uint32_t>(token) + 16 * (piece ^ (values ? L::swizzle_v(r) : L::swizzle_k(r)));
+    }
   }
-}
+  // The subtile in lane `which` of `pages`, of which `there` positions (or more than 16)
+  // may be read: zeros behind them, and for a page outside of the cache.
+  __device__ __forceinline__ void aim(const Pages& pages, int which, int there) {
+    const int id = __builtin_amdgcn_readlane(pages.id, which), in = __builtin_amdgcn_readlane(pages.in, which);
+    const int valid = id < 0 ? 0 : there < 16 ? there : 16;
+    at = head + id * page + in * token;
+    bytes = valid > 0 ? (valid - 1) * static_cast<uint32_t>(token) + Tile<D>::kRow : 0;
+  }
+  __device__ __forceinline__ void load(int i, char* lds) const {
+    dma16(at, bytes, from[i], lds + 1024 * i);
+  }
+  __device__ __forceinline__ void load_all(char* lds) const {
+#pragma unroll
+    for (int i = 0; i < kLoads; ++i) load(i, lds);
+  }
+};
 
-// The subtile of lane `which` of `pages`, at `at`, of which the positions before
-// `end` are there.  A page outside of the cache reads as zeros.
-template <int D, bool V>
-__device__ __forceinline__ void load_positions(const Attend& p, const Pages& pages, int which, int at, int end, int head,
-                                               char* lds, int lane) {
-  const int page = __builtin_amdgcn_readlane(pages.id, which), in = __builtin_amdgcn_readlane(pages.in, which);
-  const int there = page < 0 ? 0 : end - at, valid = there < 16 ? there : 16;
-  load16<D, V>(V ? p.v : p.k, page, in, head, valid, lds, lane);
+// Fragments of a tile of keys or values `off` bytes into LDS (a multiple of 1024, and
+// this lane's share of it): what differs from one fragment to the next is some bits
+// of the offset, and a constant.
+//
+// Left operand of S^T, channels 16 step .. + 15 of 32 keys from `row` on: lane l holds
+// row l % 32, channels 8 (l / 32) .. + 7 of these.
+template <int D> __device__ __forceinline__ int lane_k(int lane) {
+  return (lane & 31) * Tile<D>::kRow + 16 * ((lane >> 5) ^ Tile<D>::swizzle_k(lane & 31));
 }
-
-// Left operand of S^T: lane l holds row l % 32 of K, channels 16 step + 8 (l / 32) .. + 7.
 template <class T, int D>
-__device__ __forceinline__ typename Op<T>::frag k_frag(const char* lds, int row, int step, int lane) {
-  const int r = row + (lane & 31), piece = (2 * step + (lane >> 5)) ^ Tile<D>::swizzle_k(lane & 31);
-  return *reinterpret_cast<const typename Op<T>::frag*>(lds + r * Tile<D>::kRow + 16 * piece);
+__device__ __forceinline__ typename Op<T>::frag k_frag(const char* lds, int off, int row, int step) {
+  return *reinterpret_cast<const typename Op<T>::frag*>(lds + (off ^ 32 * (step & 7)) + 256 * (step >> 3) +
+                                                        row * Tile<D>::kRow);
 }
-// Left operand of O^T: lane l holds channel 32 tile + l % 32, keys row + 4 (l / 32) .. + 3 and 8 behind these.
+// Left operand of O^T, channels 32 tile .. + 31 of 16 keys from `row` on: lane l holds
+// channel l % 32 of these, keys 4 (l / 32) .. + 3 and 8 behind these.  The 16 lanes of a
+// read bring 4 rows of 16 channels, lane i of them row i / 4, and receive channel i each.
+template <int D> __device__ __forceinline__ int lane_v(int lane) {
+  const int row = 4 * (lane >> 5) + ((lane & 15) >> 2), piece = 2 * (lane >> 4 & 1) + ((lane & 3) >> 1);
+  return row * Tile<D>::kRow + 16 * (piece ^ Tile<D>::swizzle_v(row)) + 8 * (lane & 1);
+}
+typedef __attribute__((address_space(3))) s16x4 lds_s16x4;
+// `restrict` tells the compiler that what is read here is none of the direct loads in
+// flight; it would wait for all of them.  (Other reads it tells apart by their types.)
+__device__ __forceinline__ s16x4 read_across(lds_s16x4* __restrict__ at) {
+  return __builtin_amdgcn_ds_read_tr16_b64_v4i16(at);
+}
 template <class T, int D>
-__device__ __forceinline__ typename Op<T>::frag v_frag(const char* lds, int row, int tile, int lane) {
-  typedef __attribute__((address_space(3))) s16x4 lds_s16x4;
-  // the 16 lanes of a read bring 4 rows of 16 channels, lane i of them row i / 4, and receive channel i each
-  const int r = row + 4 * (lane >> 5) + ((lane & 15) >> 2);
-  const int piece = (4 * tile + 2 * (lane >> 4 & 1) + ((lane & 3) >> 1)) ^ Tile<D>::swizzle_v(4 * (lane >> 5) + ((lane & 15) >> 2));
-  const char* at = lds + r * Tile<D>::kRow + 16 * piece + 8 * (lane & 1);
-  const s16x4 a = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(at));
-  const s16x4 b = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(at + 8 * Tile<D>::kRow));
+__device__ __forceinline__ typename Op<T>::frag v_frag(const char* lds, int off, int row, int tile) {
+  const char* at = lds + (off ^ 64 * (tile & 3)) + 256 * (tile >> 2) + row * Tile<D>::kRow;
+  const s16x4 a = read_across((lds_s16x4*)(at)), b = read_across((lds_s16x4*)(at + 8 * Tile<D>::kRow));
   return __builtin_bit_cast(typename Op<T>::frag, __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7));
 }
 
@@ -348,6 +382,7 @@ __device__ __forceinline__ float other_half(float v) { return __shfl_xor(v, 32, 
 template <class T, int D>
 struct Rows {
   using Frag = typename Op<T>::frag;
+  static constexpr int kAhead = 4;  // fragments that are read before their matrix instructions
   Frag q[D / 16];
   f32x16 o[D / 32];
   float m, l;    // maximum of the scaled scores (base 2), and this lane's part of the sum
@@ -386,15 +421,21 @@ struct Rows {
     least = uniform(a), most = uniform(b);
   }
 
-  // Scores of 32 TILES positions whose keys lie in LDS.  Fragments are read AHEAD of their
-  // instructions; beside(i) goes behind the i-th matrix instruction.
+  // The i-th fragment of 32 TILES positions.
+  template <int TILES>
+  static __device__ __forceinline__ Frag key(const char* lds, int off, int i) {
+    return k_frag<T, D>(lds, off, i / (D / 16) * 32, i % (D / 16));
+  }
+  template <int TILES>
+  static __device__ __forceinline__ Frag value(const char* lds, int off, int i) {
+    return v_frag<T, D>(lds, off, 16 * (i % (2 * TILES)), i / (2 * TILES));
+  }
+  // Scores of 32 TILES positions; the first kAhead fragments are in f.  beside(i) goes
+  // behind the i-th matrix instruction.
   template <int TILES, class Beside>
-  __device__ __forceinline__ void scores(const char* k, int lane, f32x16 (&s)[TILES], Beside beside) const {
-    constexpr int kMmas = D / 16 * TILES, kAhead = 4;
-    Frag f[kAhead];
-    auto read = [&](int i) __attribute__((always_inline)) { return k_frag<T, D>(k, i / (D / 16) * 32, i % (D / 16), lane); };
-#pragma unroll
-    for (int i = 0; i < kAhead; ++i) f[i] = read(i);
+  __device__ __forceinline__ void scores(const char* lds, int off, Frag (&f)[kAhead], f32x16 (&s)[TILES],
+                                         Beside beside) const {
+    constexpr int kMmas = D / 16 * TILES;
 #pragma unroll
     for (int t = 0; t < TILES; ++t)
 #pragma unroll
@@ -403,7 +444,7 @@ struct Rows {
 #pragma unroll
     for (int i = 0; i < kMmas; ++i) {
       s[i / (D / 16)] = Op<T>::mma(f[i % kAhead], q[i % (D / 16)], s[i / (D / 16)]);
-      if (i + kAhead < kMmas) f[i % kAhead] = read(i + kAhead);
+      if (i + kAhead < kMmas) f[i % kAhead] = key<TILES>(lds, off, i + kAhead);
       beside(i);
       in_order();
     }
@@ -456,22 +497,17 @@ struct Rows {
     }
   }
   __device__ __forceinline__ float subtracted() const { return m == -INFINITY ? 0.f : m; }
-  // O^T += V^T P^T of 32 TILES positions.
+  // O^T += V^T P^T of 32 TILES positions, as above.
   template <int TILES, class Beside>
-  __device__ __forceinline__ void values(const char* v, int lane, const uint4 (&w)[2 * TILES], Beside beside) {
-    constexpr int kMmas = D / 32 * 2 * TILES, kAhead = 4;
-    Frag f[kAhead];
-    auto read = [&](int i) __attribute__((always_inline)) {
-      return v_frag<T, D>(v, 16 * (i % (2 * TILES)), i / (2 * TILES), lane);
-    };
-#pragma unroll
-    for (int i = 0; i < kAhead; ++i) f[i] = read(i);
+  __device__ __forceinline__ void values(const char* lds, int off, Frag (&f)[kAhead], const uint4 (&w)[2 * TILES],
+                                         Beside beside) {
+    constexpr int kMmas = D / 32 * 2 * TILES;
     in_order();
 #pragma unroll
     for (int i = 0; i < kMmas; ++i) {
       f32x16& sum = o[i / (2 * TILES)];
       sum = Op<T>::mma(f[i % kAhead], __builtin_bit_cast(Frag, w[i % (2 * TILES)]), sum);
-      if (i + kAhead < kMmas) f[i % kAhead] = read(i + kAhead);
+      if (i + kAhead < kMmas) f[i % kAhead] = value<TILES>(lds, off, i + kAhead);
       beside(i);
       in_order();
     }
@@ -502,8 +538,8 @@ __device__ __forceinline__ void take_out(char* v, int at, int lo, NotFinite<D>& 
   uint32_t found = 0;  // the top bit of a half: its exponent had no room for one more
 #pragma unroll
   for (int i = 0; i < 16 / L::kPerLoad; ++i) {
-    const uint4 raw = *reinterpret_cast<const uint4*>(v + i * 1024 + lane * 16);
-    found |= ((raw.x & kMask) + kStep) | ((raw.y & kMask) + kStep) | ((raw.z & kMask) + kStep) | ((raw.w & kMask) + kStep);
+    const u32x4 raw = *reinterpret_cast<const u32x4*>(v + i * 1024 + lane * 16);
+    found |= ((raw[0] & kMask) + kStep) | ((raw[1] & kMask) + kStep) | ((raw[2] & kMask) + kStep) | ((raw[3] & kMask) + kStep);
   }
   if (!__any((found & 0x80008000u) != 0)) return;
 #pragma unroll 1
@@ -539,20 +575,24 @@ __device__ __forceinline__ float weight_of(float m, float l, float top) { return
 __device__ __forceinline__ float lse_of(float m, float l) { return l > 0.f || l != l ? (m + log2f(l)) * kLn2 : -INFINITY; }
 
 // ------------------------------------------------------------------ many rows
-// Four waves of 32 rows each.  Keys and values come through a ring of LDS tiles,
-// loaded three steps ahead.  A step computes the scores of the next tile while it
-// turns those of this one into weights (matrix and vector instructions beside each
-// other), then adds this tile's values while it finds the next tile's maximum.
+// Four waves of 32 rows each.  Step j computes the scores of tile j + 1 while it turns
+// those of tile j into weights, then adds the values of tile j while it finds the
+// next maximum and issues the loads of the keys of tile j + 4 and the values of tile
+// j + 2; so keys lie in a ring of four tiles, values in one of three, and a load has
+// a step and a half to arrive.  The first fragments of each product are read during
+// the last matrix instructions of the one before it.
 template <int D> struct Many {
   static constexpr int kRows = 128, kTiles = D == 64 ? 2 : 1, kKeys = 32 * kTiles;
-  static constexpr int kHalf = kKeys * 2 * D, kTile = 2 * kHalf, kRing = 4, kLds = kRing * kTile;
-  static constexpr int kLoads = kTile / 1024 / 4;  // of a wave and step
+  static constexpr int kTile = kKeys * 2 * D, kKeyRing = 4, kValueRing = 3, kLds = (kKeyRing + kValueRing) * kTile;
+  static constexpr int kLoads = 2 * kTile / 1024 / 4;  // of a wave and step
 };
 
 template <class T, int D>
 __global__ __launch_bounds__(kThreads, D == 256 ? 1 : 2) void many_rows_kernel(Attend p) {
   using M = Many<D>;
-  __shared__ __align__(16) char lds[M::kLds + sizeof(NotFinite<D>) + sizeof(Plan) + 16];
+  using R = Rows<T, D>;
+  constexpr int kTiles = M::kTiles, kScores = 16 * kTiles, kMmas = D / 16 * kTiles, kAhead = R::kAhead;
+  __shared__ __align__(1024) char lds[M::kLds + sizeof(NotFinite<D>) + sizeof(Plan) + 16];
   NotFinite<D>& bad = *reinterpret_cast<NotFinite<D>*>(lds + M::kLds);
   Plan& plan = *reinterpret_cast<Plan*>(lds + M::kLds + sizeof(bad));
   int* least = reinterpret_cast<int*>(lds + M::kLds + sizeof(bad) + sizeof(Plan));  // of each wave's rows
@@ -564,7 +604,7 @@ __global__ __launch_bounds__(kThreads, D == 256 ? 1 : 2) void many_rows_kernel(A
   for (int item = static_cast<int>(static_cast<int64_t>(total) * xcd / 8) + (blockIdx.x >> 3); item < last;
        item += gridDim.x >> 3) {
     const Item it = item_of<true, M::kRows, M::kKeys>(p, plan, each, range, item);
-    Rows<T, D> rows;
+    R rows;
     const int row = it.tile * M::kRows + 32 * wave + (lane & 31);
     rows.load(p, it, row, lane);
     rows.clear();
@@ -577,74 +617,100 @@ __global__ __launch_bounds__(kThreads, D == 256 ? 1 : 2) void many_rows_kernel(A
     }
     to = uniform(to);
     const int end = it.seg.hi, steps = to > it.from ? (to - it.from + M::kKeys - 1) / M::kKeys : 0;
-    // a wave brings 16 positions of a step: their keys and values, or in steps of 32 one of both
-    const bool brings_k = M::kTiles == 2 || wave < 2, brings_v = M::kTiles == 2 || wave >= 2;
-    const int sub = M::kTiles == 2 ? wave : wave & 1;
-    Pages pages;
-    auto load = [&](int step) __attribute__((always_inline)) {
-      if ((step & 63) == 0) pages.find(p, it.seg.request, it.from + (step + lane) * M::kKeys + 16 * sub, end);
-      char* tile = lds + (step % M::kRing) * M::kTile + sub * 32 * D;
-      const int at = it.from + step * M::kKeys + 16 * sub, until = step < steps ? end : 0;
-      if (brings_k) load_positions<D, false>(p, pages, step & 63, at, until, it.head, tile, lane);
-      if (brings_v) load_positions<D, true>(p, pages, step & 63, at, until, it.head, tile + M::kHalf, lane);
+    // A wave brings 16 positions of a step: of the keys or of the values, or (steps of 64) of both.  A
+    // feed's loads of steps past the end are issued as well, with nothing in range, so that every step counts alike.
+    constexpr bool kBoth = kTiles == 2;
+    const bool of_values = !kBoth && wave >= 2;
+    const int sub = kBoth ? wave : wave & 1;
+    Feed<D> feed[kBoth ? 2 : 1];
+    Pages pages[kBoth ? 2 : 1];
+    feed[0].start(of_values ? p.v : p.k, it.head, of_values, lane);
+    if constexpr (kBoth) feed[1].start(p.v, it.head, true, lane);
+    auto aim = [&](int which, int tile) __attribute__((always_inline)) {
+      if ((tile & 63) == 0) pages[which].find(p, it.seg.request, it.from + (tile + lane) * M::kKeys + 16 * sub, end);
+      feed[which].aim(pages[which], tile & 63, tile < steps ? end - (it.from + tile * M::kKeys + 16 * sub) : 0);
     };
-    lds_barrier();  // the last item's ring is free
+    char* const share = lds + sub * 32 * D;
+    auto key_at = [](int tile) __attribute__((always_inline)) { return tile % M::kKeyRing * M::kTile; };
+    auto value_at = [](int slot) __attribute__((always_inline)) { return (M::kKeyRing + slot) * M::kTile; };
+    lds_barrier();  // the last item's rings are free
     bad.clear();
     if (lane == 0) least[wave] = rows.least;
 #pragma unroll
-    for (int step = 0; step < M::kRing - 1; ++step) load(step);
-    lds_barrier();
-    const int all_see = uniform(min(min(least[0], least[1]), min(least[2], least[3])));
-    // this wave's part of the step's tile is there
-    auto arrived = [&](int step) __attribute__((always_inline)) {
-      const int at = it.from + step * M::kKeys;
-      if (brings_v && step < steps && (at < it.seg.lo || at + M::kKeys > all_see))
-        take_out<T, D>(lds + (step % M::kRing) * M::kTile + M::kHalf + sub * 32 * D, at + 16 * sub, it.seg.lo, bad, lane);
-    };
-    using Scores = f32x16[M::kTiles];
-    Scores s[2];
-    uint4 w[2 * M::kTiles];
-    constexpr int kScores = 16 * M::kTiles, kMmas = D / 16 * M::kTiles, kBeside = kScores / kMmas;
-    auto nothing = [](int) __attribute__((always_inline)) {};
+    for (int tile = 0; tile < M::kKeyRing; ++tile) {  // keys of tiles 0 to 3, beside the last two values of 0 and 1
+      if (!of_values) {
+        aim(0, tile);
+        feed[0].load_all(share + key_at(tile));
+      }
+      if (tile >= 2 && (kBoth || of_values)) {
+        aim(kBoth ? 1 : 0, tile - 2);
+        feed[kBoth ? 1 : 0].load_all(share + value_at(tile - 2));
+      }
+    }
     wait_loads<2 * M::kLoads>();
-    arrived(0);
-    lds_barrier();
-    rows.template scores<M::kTiles>(lds, lane, s[0], nothing);
-    rows.template mask<M::kTiles>(it.seg, it.from, lane, s[0]);
+    lds_barrier();  // the keys of tiles 0 and 1 are there
+    const int all_see = uniform(min(min(least[0], least[1]), min(least[2], least[3])));
+    using Scores = f32x16[kTiles];
+    Scores s[2];
+    uint4 w[2 * kTiles];
+    typename R::Frag keys[kAhead], values[kAhead];
+    const int of_k = lane_k<D>(lane), of_v = lane_v<D>(lane);
+#pragma unroll
+    for (int i = 0; i < kAhead; ++i) keys[i] = R::template key<kTiles>(lds, of_k, i);
+    rows.template scores<kTiles>(lds, of_k, keys, s[0], [](int) __attribute__((always_inline)) {});
+#pragma unroll
+    for (int i = 0; i < kAhead; ++i) keys[i] = R::template key<kTiles>(lds, key_at(1) + of_k, i);
+    rows.template mask<kTiles>(it.seg, it.from, lane, s[0]);
     float top = -INFINITY;
-    auto larger = [&](Scores& of, int i) __attribute__((always_inline)) {
-      top = fmaxf(top, of[i / 16][i % 16]);
-    };
+    auto larger = [&](const Scores& of, int i) __attribute__((always_inline)) { top = fmaxf(top, of[i / 16][i % 16]); };
 #pragma unroll
     for (int i = 0; i < kScores; ++i) larger(s[0], i);
     // a tile behind the last is all zeros, and its scores may not raise anything
     if (steps > 0) rows.raise(rows.of_row(p, top));
+    int slot = 0;  // of the step's values
     auto advance = [&](int step, Scores& now, Scores& next) __attribute__((always_inline)) {
-      wait_loads<M::kLoads>();
-      arrived(step + 1);
-      lds_barrier();  // the next tile is there, the one before this free
-      load(step + 3);
+      wait_loads<M::kLoads>();  // the keys of step + 2 and the values of step
+      const int at = it.from + step * M::kKeys;
+      if ((kBoth || of_values) && (at < it.seg.lo || at + M::kKeys > all_see))
+        take_out<T, D>(share + value_at(slot), at + 16 * sub, it.seg.lo, bad, lane);
+      lds_barrier();
       const float less = rows.subtracted();
-      rows.template scores<M::kTiles>(lds + ((step + 1) % M::kRing) * M::kTile, lane, next, [&](int i) __attribute__((always_inline)) {
-        rows.template weights<M::kTiles>(p, i * kBeside, (i + 1) * kBeside, less, now, w);
+      const int v_at = value_at(slot) + of_v;
+      rows.template scores<kTiles>(lds, key_at(step + 1) + of_k, keys, next, [&](int i) __attribute__((always_inline)) {
+        rows.template weights<kTiles>(p, i * kScores / kMmas, (i + 1) * kScores / kMmas, less, now, w);
+        if (i >= kMmas - kAhead) values[i - (kMmas - kAhead)] = R::template value<kTiles>(lds, v_at, i - (kMmas - kAhead));
       });
-      rows.template mask<M::kTiles>(it.seg, it.from + (step + 1) * M::kKeys, lane, next);
+      rows.template mask<kTiles>(it.seg, at + M::kKeys, lane, next);
+      // the loads of a later tile, in the shares that the tiles before these have left
+      const int later = slot == 0 ? 2 : slot - 1;
+      char* to0 = share + (of_values ? value_at(later) : key_at(step));
+      char* to1 = share + value_at(later);
+      aim(0, of_values ? step + 2 : step + 4);
+      if constexpr (kBoth) aim(1, step + 2);
+      const int k_next = key_at(step + 2) + of_k;
       top = -INFINITY;
-      // behind the first quarter: the scores' last matrix instruction is done by then
-      rows.template values<M::kTiles>(lds + (step % M::kRing) * M::kTile + M::kHalf, lane, w, [&](int i) __attribute__((always_inline)) {
+      rows.template values<kTiles>(lds, v_at, values, w, [&](int i) __attribute__((always_inline)) {
+        // behind the first quarter: the scores' last matrix instruction is done by then
         constexpr int kFrom = kMmas / 4, kEach = (kScores + kMmas - kFrom - 1) / (kMmas - kFrom);
+        constexpr int kIssue = M::kLoads;
+        if (i < kIssue) {
+          if (!kBoth || i < kIssue / 2) feed[0].load(i, to0);
+          else feed[kBoth ? 1 : 0].load(i - kIssue / 2, to1);
+        }
 #pragma unroll
         for (int e = 0; e < kEach; ++e)
           if (i >= kFrom && (i - kFrom) * kEach + e < kScores) larger(next, (i - kFrom) * kEach + e);
+        if (i >= kMmas - kAhead) keys[i - (kMmas - kAhead)] = R::template key<kTiles>(lds, k_next, i - (kMmas - kAhead));
       });
       if (step + 1 < steps) rows.raise(rows.of_row(p, top));
+      slot = slot == 2 ? 0 : slot + 1;
     };
     for (int step = 0; step < steps; step += 2) {
       advance(step, s[0], s[1]);
       if (step + 1 == steps) break;
       advance(step + 1, s[1], s[0]);
     }
-    wait_loads<0>();  // those past the end too, before the ring is used again
+    wait_loads<0>();  // those past the end too, before the rings are used again
     const float l = rows.l + other_half(rows.l);
     if (uniform(bad.found)) {
 #pragma unroll
@@ -697,7 +763,7 @@ template <int D> struct Few {
 template <class T, int D>
 __global__ __launch_bounds__(kThreads, Few<D>::kBlocks) void few_rows_kernel(Attend p) {
   using F = Few<D>;
-  __shared__ __align__(16) char lds[F::kLds + sizeof(NotFinite<D>) + sizeof(Plan) + sizeof(Stats) + 128];
+  __shared__ __align__(1024) char lds[F::kLds + sizeof(NotFinite<D>) + sizeof(Plan) + sizeof(Stats) + 128];
   NotFinite<D>& bad = *reinterpret_cast<NotFinite<D>*>(lds + F::kLds);
   Plan& plan = *reinterpret_cast<Plan*>(lds + F::kLds + sizeof(bad));
   Stats& stats = *reinterpret_cast<Stats*>(lds + F::kLds + sizeof(bad) + sizeof(Plan));
@@ -706,22 +772,30 @@ __global__ __launch_bounds__(kThreads, Few<D>::kBlocks) void few_rows_kernel(Att
   int each, range;
   const int total = schedule<false, kFew, F::kUnit>(p, plan, each, range);
   char* mine = lds + wave * F::kWave;
+  const int of_k = lane_k<D>(lane), of_v = lane_v<D>(lane);
   for (int item = blockIdx.x; item < total; item += gridDim.x) {
     const Item it = item_of<false, kFew, F::kUnit>(p, plan, each, range, item);
     const int end = it.seg.hi, steps = (it.to - it.from + 31) / 32;
     Pages pages;
+    Feed<D> k_feed, v_feed;
+    k_feed.start(p.k, it.head, false, lane);
+    v_feed.start(p.v, it.head, true, lane);
     // this wave's steps are wave, wave + 4, ...: 32 of them to a lookup
     auto load_k = [&](int step) __attribute__((always_inline)) {
       if ((step >> 2 & 31) == 0)
         pages.find(p, it.seg.request, it.from + 32 * (step + 4 * (lane >> 1)) + 16 * (lane & 1), end);
-      const int at = it.from + 32 * step, which = 2 * (step >> 2 & 31), until = step < steps ? end : 0;
-      load_positions<D, false>(p, pages, which, at, until, it.head, mine, lane);
-      load_positions<D, false>(p, pages, which + 1, at + 16, until, it.head, mine + 32 * D, lane);
+      const int there = step < steps ? end - (it.from + 32 * step) : 0, which = 2 * (step >> 2 & 31);
+      k_feed.aim(pages, which, there);
+      k_feed.load_all(mine);
+      k_feed.aim(pages, which + 1, there - 16);
+      k_feed.load_all(mine + 32 * D);
     };
     auto load_v = [&](int step) __attribute__((always_inline)) {
-      const int at = it.from + 32 * step, which = 2 * (step >> 2 & 31), until = step < steps ? end : 0;
-      load_positions<D, true>(p, pages, which, at, until, it.head, mine + F::kHalf, lane);
-      load_positions<D, true>(p, pages, which + 1, at + 16, until, it.head, mine + F::kHalf + 32 * D, lane);
+      const int there = step < steps ? end - (it.from + 32 * step) : 0, which = 2 * (step >> 2 & 31);
+      v_feed.aim(pages, which, there);
+      v_feed.load_all(mine + F::kHalf);
+      v_feed.aim(pages, which + 1, there - 16);
+      v_feed.load_all(mine + F::kHalf + 32 * D);
     };
     lds_barrier();  // the last item's sums have been read
     Rows<T, D> rows;
@@ -736,7 +810,10 @@ __global__ __launch_bounds__(kThreads, Few<D>::kBlocks) void few_rows_kernel(Att
       f32x16 s[1];
       uint4 w[2];
       wait_loads<F::kLoads>();  // the keys; the values may be on their way
-      rows.template scores<1>(mine, lane, s, [](int) {});
+      typename Rows<T, D>::Frag f[Rows<T, D>::kAhead];
+#pragma unroll
+      for (int i = 0; i < Rows<T, D>::kAhead; ++i) f[i] = Rows<T, D>::template key<1>(mine, of_k, i);
+      rows.template scores<1>(mine, of_k, f, s, [](int) {});
       reads_done();
       const int at = it.from + 32 * step;
       load_k(step + 4);
@@ -751,7 +828,9 @@ __global__ __launch_bounds__(kThreads, Few<D>::kBlocks) void few_rows_kernel(Att
         take_out<T, D>(mine + F::kHalf, at, it.seg.lo, bad, lane);
         take_out<T, D>(mine + F::kHalf + 32 * D, at + 16, it.seg.lo, bad, lane);
       }
-      rows.template values<1>(mine + F::kHalf, lane, w, [](int) {});
+#pragma unroll
+      for (int i = 0; i < Rows<T, D>::kAhead; ++i) f[i] = Rows<T, D>::template value<1>(mine + F::kHalf, of_v, i);
+      rows.template values<1>(mine + F::kHalf, of_v, f, w, [](int) {});
       reads_done();
       load_v(step + 4);
     }
