@@ -74,6 +74,7 @@ struct Segment {
   int token, tokens;  // first query token, their number
   int lo, hi;         // positions
   int request;        // whose row of the table is read
+  int length;         // of the request, as given (a group's: unused)
 };
 
 __device__ __forceinline__ int uniform(int v) { return __builtin_amdgcn_readfirstlane(v); }
@@ -115,12 +116,14 @@ __device__ __forceinline__ Segment segment(const Attend& p, int s) {
     seg.lo = 0;
     seg.hi = shared_of(p, s);
     seg.request = min(r0, p.requests - 1);
+    seg.length = 0;
   } else {
     const int r = s - shared;
     seg.token = token_of(p, r);
     seg.tokens = max(0, token_of(p, r + 1) - seg.token);
     seg.lo = shared_before(p, r);
-    seg.hi = clampi(load_index(p.lens, r, p.lens_is64), 0, p.capacity);
+    seg.length = static_cast<int>(load_index(p.lens, r, p.lens_is64));
+    seg.hi = clampi(seg.length, 0, p.capacity);
     seg.request = r;
   }
   return seg;
@@ -139,26 +142,33 @@ __device__ __forceinline__ Cut cut_of(const Attend& p, const Segment& seg) {
 
 // ------------------------------------------------------------------ schedule
 struct Plan {
-  int base[kThreads + 2];  // items before each thread's segments, and all of them
+  int base[kThreads];  // items before each thread's segments
+  Segment segments[kThreads];  // each thread's first one: all, of up to kThreads
   int64_t units[kThreads / 64];
   int count[kThreads / 64];
+  int each, range;     // segments of a thread; units of a range of keys
 };
+// One LDS array holds it all in a kernel with direct loads: beside a second one, the
+// compiler waits for every load in flight in front of each read.
+static_assert(sizeof(Plan) % 8 == 0, "what lies behind it is aligned");
 
 // Counts the items of the launch: thread i answers for `each` consecutive
 // segments.  A range of keys is as long as it has to be for `target` items.
 // Block 0 notes for the joining kernel where each segment's items lie.
 template <bool MANY, int ROWS, int UNIT>
-__device__ int schedule(const Attend& p, Plan& plan, int& each, int& range) {
+__device__ int schedule(const Attend& p, Plan& plan) {
   const int n = segments_of(p), lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  each = (n + kThreads - 1) / kThreads;
+  const int each = (n + kThreads - 1) / kThreads;
   const int from = threadIdx.x * each, to = min(n, from + each);
   int64_t units = 0;
-  Cut first{0, 0};
+  Segment first{};
   for (int s = from; s < to; ++s) {
-    const Cut c = cut_of<MANY, ROWS, UNIT>(p, segment(p, s));
-    if (s == from) first = c;
+    const Segment seg = segment(p, s);
+    const Cut c = cut_of<MANY, ROWS, UNIT>(p, seg);
+    if (s == from) first = seg;
     units += static_cast<int64_t>(c.tiles) * c.units;
   }
+  plan.segments[threadIdx.x] = first;
 #pragma unroll
   for (int off = 32; off > 0; off >>= 1) units += __shfl_xor(units, off, 64);
   if (lane == 0) plan.units[wave] = units;
@@ -167,10 +177,10 @@ __device__ int schedule(const Attend& p, Plan& plan, int& each, int& range) {
 #pragma unroll
   for (int w = 0; w < kThreads / 64; ++w) units += plan.units[w];
   const int64_t wanted = (units * p.kv_heads + p.target[MANY] - 1) / p.target[MANY];
-  range = static_cast<int>(wanted < p.min_units[MANY] ? p.min_units[MANY] : wanted);
+  const int range = static_cast<int>(wanted < p.min_units[MANY] ? p.min_units[MANY] : wanted);
   int items = 0;
   for (int s = from; s < to; ++s) {
-    const Cut c = s == from ? first : cut_of<MANY, ROWS, UNIT>(p, segment(p, s));
+    const Cut c = cut_of<MANY, ROWS, UNIT>(p, s == from ? first : segment(p, s));
     items += c.tiles * p.kv_heads * ((c.units + range - 1) / range);
   }
   int sum = items;
@@ -188,10 +198,10 @@ __device__ int schedule(const Attend& p, Plan& plan, int& each, int& range) {
     total += plan.count[w];
   }
   plan.base[threadIdx.x] = before;
-  if (threadIdx.x == 0) plan.base[kThreads] = total;
+  if (threadIdx.x == 0) plan.each = each, plan.range = range;
   if (blockIdx.x == 0)
     for (int s = from; s < to; ++s) {
-      const Segment seg = segment(p, s);
+      const Segment seg = s == from ? first : segment(p, s);
       const Cut c = cut_of<MANY, ROWS, UNIT>(p, seg);
       const int ranges = (c.units + range - 1) / range;
       if ((seg.tokens * p.per > kFew) == MANY) p.places[s] = make_int2(before, ranges);
@@ -201,11 +211,6 @@ __device__ int schedule(const Attend& p, Plan& plan, int& each, int& range) {
   return min(total, p.items_max[MANY]);
 }
 
-typedef float2 Stats[4][32];  // maximum and sum of four waves' rows
-// One LDS array holds it all in a kernel with direct loads: beside a second one, the
-// compiler waits for every load in flight in front of each read.
-static_assert(sizeof(Plan) % 8 == 0, "what lies behind it is aligned");
-
 struct Item {
   Segment seg;
   int head, tile;  // key head, tile of rows
@@ -214,30 +219,32 @@ struct Item {
   bool own;        // of a request, not of a group
 };
 
+// Called by whole waves: what it finds is the same in all lanes, and kept in scalar registers.
 template <bool MANY, int ROWS, int UNIT>
-__device__ Item item_of(const Attend& p, const Plan& plan, int each, int range, int item) {
-  int lo = 0, hi = kThreads - 1;  // the last thread whose base is at most item
-  while (lo < hi) {
-    const int mid = (lo + hi + 1) >> 1;
-    if (plan.base[mid] <= item) lo = mid; else hi = mid - 1;
-  }
-  int at = item - plan.base[lo];
-  const int last = min(segments_of(p), (lo + 1) * each) - 1;
-  for (int s = lo * each;; ++s) {
-    const Segment seg = segment(p, s);
+__device__ Item item_of(const Attend& p, const Plan& plan, int item) {
+  static_assert(kThreads == 256, "four bases a lane");
+  const int lane = threadIdx.x & 63, each = uniform(plan.each), range = uniform(plan.range);
+  int thread = -1;  // the last whose base is at most `item`
+#pragma unroll
+  for (int i = 0; i < 4; ++i) thread += __popcll(__ballot(plan.base[4 * lane + i] <= item));
+  thread = uniform(thread);
+  int at = item - uniform(plan.base[thread]);
+  const int last = min(segments_of(p), (thread + 1) * each) - 1;
+  for (int s = thread * each;; ++s) {
+    const Segment seg = s == thread * each ? plan.segments[thread] : segment(p, s);
     const Cut c = cut_of<MANY, ROWS, UNIT>(p, seg);
-    const int ranges = (c.units + range - 1) / range, items = c.tiles * p.kv_heads * ranges;
+    const int ranges = uniform((c.units + range - 1) / range), tiles = uniform(c.tiles), items = tiles * p.kv_heads * ranges;
     if (at < items || s >= last) {
-      // the same in all lanes: kept in scalar registers
       Item it;
-      it.seg = {uniform(seg.token), uniform(seg.tokens), uniform(seg.lo), uniform(seg.hi), uniform(seg.request)};
-      it.ranges = uniform(ranges);
-      it.own = uniform(s) >= segments_of(p) - p.requests;
-      const int tiles = max(1, c.tiles), across = at / tiles, head = across / max(1, ranges);
-      it.tile = uniform(at - across * tiles);
-      it.head = uniform(head);
-      it.from = uniform((seg.lo & ~15) + (across - head * max(1, ranges)) * range * UNIT);
-      it.to = min(it.seg.hi, it.from + uniform(range) * UNIT);
+      it.seg = {uniform(seg.token), uniform(seg.tokens), uniform(seg.lo),
+                uniform(seg.hi),    uniform(seg.request), uniform(seg.length)};
+      it.ranges = ranges;
+      it.own = s >= segments_of(p) - p.requests;
+      const int across = uniform(at / max(1, tiles));
+      it.tile = at - across * max(1, tiles);
+      it.head = uniform(across / max(1, ranges));
+      it.from = (it.seg.lo & ~15) + (across - it.head * max(1, ranges)) * range * UNIT;
+      it.to = min(it.seg.hi, it.from + range * UNIT);
       return it;
     }
     at -= items;
@@ -373,10 +380,75 @@ __device__ __forceinline__ typename Op<T>::frag v_frag(const char* lds, int off,
   return __builtin_bit_cast(typename Op<T>::frag, __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7));
 }
 
+// v, computed where it stands: not moved down to where it is used.
+template <class V> __device__ __forceinline__ V here(V v) {
+  asm volatile("" : "+v"(v));
+  return v;
+}
 // Instructions stay on their side of it.
 __device__ __forceinline__ void in_order() { __builtin_amdgcn_sched_barrier(0); }
 
 __device__ __forceinline__ float other_half(float v) { return __shfl_xor(v, 32, 64); }
+
+// A weight of zero does not silence a value that is not finite.  Where rows of an
+// item do not see all of a tile's positions, such values are taken out of it, and
+// for each channel the first position of a positive and of a negative one is kept
+// (of both for a NaN): they go to the rows that see it when the item is done.
+template <int D> struct NotFinite {
+  int found, pad[3];
+  int first[2][D];
+  __device__ __forceinline__ void clear(int thread, int threads) {
+    if (thread == 0) found = 0;
+    for (int i = thread; i < 2 * D; i += threads) first[i / D][i % D] = INT32_MAX;
+  }
+  __device__ __forceinline__ float added(int channel, int limit) const {
+    return (first[0][channel] < limit ? INFINITY : 0.f) - (first[1][channel] < limit ? INFINITY : 0.f);
+  }
+};
+
+// Of the 16 positions from `at` on whose values this wave has brought to LDS.
+template <class T, int D>
+__device__ __forceinline__ void take_out(char* v, int at, int lo, NotFinite<D>& bad, int lane) {
+  using L = Tile<D>;
+  constexpr uint32_t kBits = Op<T>::kExponent, kMask = kBits * 0x10001u, kStep = (0x8000u - kBits) * 0x10001u;
+  uint32_t found = 0;  // the top bit of a half: its exponent had no room for one more
+#pragma unroll
+  for (int i = 0; i < 16 / L::kPerLoad; ++i) {
+    const u32x4 raw = *reinterpret_cast<const u32x4*>(v + i * 1024 + lane * 16);
+    found |= ((raw[0] & kMask) + kStep) | ((raw[1] & kMask) + kStep) | ((raw[2] & kMask) + kStep) | ((raw[3] & kMask) + kStep);
+  }
+  if (!__any((found & 0x80008000u) != 0)) return;
+#pragma unroll 1
+  for (int i = 0; i < 16 / L::kPerLoad; ++i) {
+    const int row = i * L::kPerLoad + lane / L::kPieces, piece = (lane % L::kPieces) ^ L::swizzle_v(row);
+    uint16_t* values = reinterpret_cast<uint16_t*>(v + i * 1024 + lane * 16);
+#pragma unroll 1
+    for (int e = 0; e < 8; ++e) {
+      const uint32_t bits = values[e];
+      if ((bits & kBits) != kBits) continue;
+      values[e] = 0;
+      if (at + row < lo) continue;
+      const bool nan = (bits & 0x7fff) != kBits, negative = bits >> 15;
+      if (nan || !negative) atomicMin(&bad.first[0][8 * piece + e], at + row);
+      if (nan || negative) atomicMin(&bad.first[1][8 * piece + e], at + row);
+      bad.found = 1;
+    }
+  }
+}
+
+// Whether an item holds all that its rows see: nothing has to be joined.
+__device__ __forceinline__ bool whole(const Item& it) { return it.own && it.ranges == 1 && it.seg.lo == 0; }
+
+// Four channels of a finished row.
+template <class T>
+__device__ __forceinline__ void put4(const Attend& p, int token, int head, int channel, const float (&y)[4]) {
+  T* to = static_cast<T*>(p.out) + token * p.out_token + head * p.out_head + channel;
+  *reinterpret_cast<uint2*>(to) = make_uint2(out_pack2<T>(y[0], y[1]), out_pack2<T>(y[2], y[3]));
+}
+// The factor of a piece with maximum m and sum l under the joint maximum; 0 where the
+// piece saw nothing (a NaN stays one).
+__device__ __forceinline__ float weight_of(float m, float l, float top) { return l == 0.f ? 0.f : fast_exp2(m - top); }
+__device__ __forceinline__ float lse_of(float m, float l) { return l > 0.f || l != l ? (m + log2f(l)) * kLn2 : -INFINITY; }
 
 // One wave's rows: 32 of them, a lane and its partner 32 lanes on share one.
 template <class T, int D>
@@ -410,10 +482,13 @@ struct Rows {
     }
     limit = 0;
     if (there) {
-      int r = it.seg.request;
-      if (!it.own) r = p.cu ? static_cast<int>(find_sequence(p.cu, p.cu_is64, p.requests, token)) : token;
-      const int64_t end = load_index(p.lens, r, p.lens_is64) - (token_of(p, r + 1) - 1 - token);
-      limit = clampi(end, 0, it.seg.hi);
+      int length = it.seg.length, behind = it.seg.tokens - 1 - in;  // tokens of the request behind this one
+      if (!it.own) {
+        const int r = p.cu ? static_cast<int>(find_sequence(p.cu, p.cu_is64, p.requests, token)) : token;
+        length = static_cast<int>(load_index(p.lens, r, p.lens_is64));
+        behind = token_of(p, r + 1) - 1 - token;
+      }
+      limit = clampi(static_cast<int64_t>(length) - behind, 0, it.seg.hi);
     }
     int a = there ? limit : INT32_MAX, b = limit;
 #pragma unroll
@@ -492,9 +567,10 @@ struct Rows {
       l += x;
       if (i & 1) {
         const uint32_t pair = out_pack2<T>(reinterpret_cast<float*>(&s[i / 16])[i % 16 - 1], x);
-        reinterpret_cast<uint32_t*>(&w[i / 8])[i % 8 / 2] = pair;
+        reinterpret_cast<uint32_t*>(&w[i / 8])[i % 8 / 2] = here(pair);
       }
     }
+    l = here(l);
   }
   __device__ __forceinline__ float subtracted() const { return m == -INFINITY ? 0.f : m; }
   // O^T += V^T P^T of 32 TILES positions, as above.
@@ -512,67 +588,38 @@ struct Rows {
       in_order();
     }
   }
-};
-
-// A weight of zero does not silence a value that is not finite.  Where rows of an
-// item do not see all of a tile's positions, such values are taken out of it, and
-// for each channel the first position of a positive and of a negative one is kept
-// (of both for a NaN): they go to the rows that see it when the item is done.
-template <int D> struct NotFinite {
-  int found, pad[3];
-  int first[2][D];
-  __device__ __forceinline__ void clear() {  // by the whole block
-    if (threadIdx.x == 0) found = 0;
-    for (int i = threadIdx.x; i < 2 * D; i += kThreads) first[i / D][i % D] = INT32_MAX;
-  }
-  __device__ __forceinline__ float added(int channel, int limit) const {
-    return (first[0][channel] < limit ? INFINITY : 0.f) - (first[1][channel] < limit ? INFINITY : 0.f);
-  }
-};
-
-// Of the 16 positions from `at` on whose values this wave has brought to LDS.
-template <class T, int D>
-__device__ __forceinline__ void take_out(char* v, int at, int lo, NotFinite<D>& bad, int lane) {
-  using L = Tile<D>;
-  constexpr uint32_t kBits = Op<T>::kExponent, kMask = kBits * 0x10001u, kStep = (0x8000u - kBits) * 0x10001u;
-  uint32_t found = 0;  // the top bit of a half: its exponent had no room for one more
+  __device__ __forceinline__ void add_not_finite(const NotFinite<D>& bad, int lane) {
 #pragma unroll
-  for (int i = 0; i < 16 / L::kPerLoad; ++i) {
-    const u32x4 raw = *reinterpret_cast<const u32x4*>(v + i * 1024 + lane * 16);
-    found |= ((raw[0] & kMask) + kStep) | ((raw[1] & kMask) + kStep) | ((raw[2] & kMask) + kStep) | ((raw[3] & kMask) + kStep);
+    for (int d = 0; d < D / 32; ++d)
+#pragma unroll
+      for (int e = 0; e < 16; ++e) o[d][e] += bad.added(32 * d + 8 * (e >> 2) + 4 * (lane >> 5) + (e & 3), limit);
   }
-  if (!__any((found & 0x80008000u) != 0)) return;
-#pragma unroll 1
-  for (int i = 0; i < 16 / L::kPerLoad; ++i) {
-    const int row = i * L::kPerLoad + lane / L::kPieces, piece = (lane % L::kPieces) ^ L::swizzle_v(row);
-    uint16_t* values = reinterpret_cast<uint16_t*>(v + i * 1024 + lane * 16);
-#pragma unroll 1
-    for (int e = 0; e < 8; ++e) {
-      const uint32_t bits = values[e];
-      if ((bits & kBits) != kBits) continue;
-      values[e] = 0;
-      if (at + row < lo) continue;
-      const bool nan = (bits & 0x7fff) != kBits, negative = bits >> 15;
-      if (nan || !negative) atomicMin(&bad.first[0][8 * piece + e], at + row);
-      if (nan || negative) atomicMin(&bad.first[1][8 * piece + e], at + row);
-      bad.found = 1;
+  // Row `row` of the segment out: finished, or as a piece to be joined, row `to` of its kind's sums.
+  __device__ __forceinline__ void put(const Attend& p, const Item& it, int row, int kind, int64_t to, int lane) {
+    const float sum = l + other_half(l);
+    if (row >= it.seg.tokens * p.per) return;
+    if (whole(it)) {
+      const int in = row / p.per, token = it.seg.token + in, head = it.head * p.per + row - in * p.per;
+      const float inverse = sum > 0.f || sum != sum ? 1.0f / sum : 0.f;
+#pragma unroll
+      for (int d = 0; d < D / 32; ++d)
+#pragma unroll
+        for (int e = 0; e < 16; e += 4) {
+          const float y[4] = {o[d][e] * inverse, o[d][e + 1] * inverse, o[d][e + 2] * inverse, o[d][e + 3] * inverse};
+          put4<T>(p, token, head, 32 * d + 2 * e + 4 * (lane >> 5), y);
+        }
+      if (p.lse && lane < 32) p.lse[static_cast<int64_t>(token) * p.heads + head] = lse_of(m, sum);
+    } else {
+      float* sums = p.sums[kind] + to * D + 4 * (lane >> 5);
+#pragma unroll
+      for (int d = 0; d < D / 32; ++d)
+#pragma unroll
+        for (int e = 0; e < 16; e += 4)
+          *reinterpret_cast<float4*>(sums + 32 * d + 2 * e) = make_float4(o[d][e], o[d][e + 1], o[d][e + 2], o[d][e + 3]);
+      if (lane < 32) p.stats[kind][to] = make_float2(m, sum);
     }
   }
-}
-
-// Whether an item holds all that its rows see: nothing has to be joined.
-__device__ __forceinline__ bool whole(const Item& it) { return it.own && it.ranges == 1 && it.seg.lo == 0; }
-
-// Four channels of a finished row.
-template <class T>
-__device__ __forceinline__ void put4(const Attend& p, int token, int head, int channel, const float (&y)[4]) {
-  T* to = static_cast<T*>(p.out) + token * p.out_token + head * p.out_head + channel;
-  *reinterpret_cast<uint2*>(to) = make_uint2(out_pack2<T>(y[0], y[1]), out_pack2<T>(y[2], y[3]));
-}
-// The factor of a piece with maximum m and sum l under the joint maximum; 0 where the
-// piece saw nothing (a NaN stays one).
-__device__ __forceinline__ float weight_of(float m, float l, float top) { return l == 0.f ? 0.f : fast_exp2(m - top); }
-__device__ __forceinline__ float lse_of(float m, float l) { return l > 0.f || l != l ? (m + log2f(l)) * kLn2 : -INFINITY; }
+};
 
 // ------------------------------------------------------------------ many rows
 // Four waves of 32 rows each.  Step j computes the scores of tile j + 1 while it turns
@@ -597,13 +644,12 @@ __global__ __launch_bounds__(kThreads, D == 256 ? 1 : 2) void many_rows_kernel(A
   Plan& plan = *reinterpret_cast<Plan*>(lds + M::kLds + sizeof(bad));
   int* least = reinterpret_cast<int*>(lds + M::kLds + sizeof(bad) + sizeof(Plan));  // of each wave's rows
   const int lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6);
-  int each, range;
-  const int total = schedule<true, M::kRows, M::kKeys>(p, plan, each, range);
+  const int total = schedule<true, M::kRows, M::kKeys>(p, plan);
   // blocks with the same index modulo 8 share an XCD and its L2: neighbours in the order of items, which share keys
   const int xcd = blockIdx.x & 7, last = static_cast<int>(static_cast<int64_t>(total) * (xcd + 1) / 8);
   for (int item = static_cast<int>(static_cast<int64_t>(total) * xcd / 8) + (blockIdx.x >> 3); item < last;
        item += gridDim.x >> 3) {
-    const Item it = item_of<true, M::kRows, M::kKeys>(p, plan, each, range, item);
+    const Item it = item_of<true, M::kRows, M::kKeys>(p, plan, item);
     R rows;
     const int row = it.tile * M::kRows + 32 * wave + (lane & 31);
     rows.load(p, it, row, lane);
@@ -611,11 +657,7 @@ __global__ __launch_bounds__(kThreads, D == 256 ? 1 : 2) void many_rows_kernel(A
     // nothing behind the last position that a row of the tile sees
     const int last_token = min(it.seg.tokens - 1, (it.tile * M::kRows + M::kRows - 1) / p.per);
     int to = it.to;
-    if (it.own) {
-      const int64_t end = load_index(p.lens, it.seg.request, p.lens_is64) - (it.seg.tokens - 1 - last_token);
-      to = clampi(end, 0, to);
-    }
-    to = uniform(to);
+    if (it.own) to = uniform(clampi(static_cast<int64_t>(it.seg.length) - (it.seg.tokens - 1 - last_token), 0, to));
     const int end = it.seg.hi, steps = to > it.from ? (to - it.from + M::kKeys - 1) / M::kKeys : 0;
     // A wave brings 16 positions of a step: of the keys or of the values, or (steps of 64) of both.  A
     // feed's loads of steps past the end are issued as well, with nothing in range, so that every step counts alike.
@@ -634,7 +676,7 @@ __global__ __launch_bounds__(kThreads, D == 256 ? 1 : 2) void many_rows_kernel(A
     auto key_at = [](int tile) __attribute__((always_inline)) { return tile % M::kKeyRing * M::kTile; };
     auto value_at = [](int slot) __attribute__((always_inline)) { return (M::kKeyRing + slot) * M::kTile; };
     lds_barrier();  // the last item's rings are free
-    bad.clear();
+    bad.clear(threadIdx.x, kThreads);
     if (lane == 0) least[wave] = rows.least;
 #pragma unroll
     for (int tile = 0; tile < M::kKeyRing; ++tile) {  // keys of tiles 0 to 3, beside the last two values of 0 and 1
@@ -711,112 +753,77 @@ __global__ __launch_bounds__(kThreads, D == 256 ? 1 : 2) void many_rows_kernel(A
       advance(step + 1, s[1], s[0]);
     }
     wait_loads<0>();  // those past the end too, before the rings are used again
-    const float l = rows.l + other_half(rows.l);
-    if (uniform(bad.found)) {
-#pragma unroll
-      for (int d = 0; d < D / 32; ++d)
-#pragma unroll
-        for (int e = 0; e < 16; ++e)
-          rows.o[d][e] += bad.added(32 * d + 8 * (e >> 2) + 4 * (lane >> 5) + (e & 3), rows.limit);
-    }
-    const bool there = row < it.seg.tokens * p.per;
-    if (there && whole(it)) {
-      const int in = row / p.per, token = it.seg.token + in, head = it.head * p.per + row - in * p.per;
-      const float inverse = l > 0.f || l != l ? 1.0f / l : 0.f;
-#pragma unroll
-      for (int d = 0; d < D / 32; ++d)
-#pragma unroll
-        for (int e = 0; e < 16; e += 4) {
-          const float y[4] = {rows.o[d][e] * inverse, rows.o[d][e + 1] * inverse, rows.o[d][e + 2] * inverse,
-                              rows.o[d][e + 3] * inverse};
-          put4<T>(p, token, head, 32 * d + 2 * e + 4 * (lane >> 5), y);
-        }
-      if (p.lse && lane < 32) p.lse[static_cast<int64_t>(token) * p.heads + head] = lse_of(rows.m, l);
-    } else if (there) {
-      const int64_t at = static_cast<int64_t>(item) * M::kRows + 32 * wave + (lane & 31);
-      float* sums = p.sums[1] + at * D + 4 * (lane >> 5);
-#pragma unroll
-      for (int d = 0; d < D / 32; ++d)
-#pragma unroll
-        for (int e = 0; e < 16; e += 4)
-          *reinterpret_cast<float4*>(sums + 32 * d + 2 * e) =
-              make_float4(rows.o[d][e], rows.o[d][e + 1], rows.o[d][e + 2], rows.o[d][e + 3]);
-      if (lane < 32) p.stats[1][at] = make_float2(rows.m, l);
-    }
+    if (uniform(bad.found)) rows.add_not_finite(bad, lane);
+    rows.put(p, it, row, 1, static_cast<int64_t>(item) * M::kRows + 32 * wave + (lane & 31), lane);
   }
 }
 
 // ------------------------------------------------------------------ few rows
-// A segment of at most 32 rows: what bounds it is how fast its keys come in.  The
-// four waves take the steps of 32 positions by turns, each with LDS of its own for
-// one step's keys and one step's values and no barrier among them; the next keys
-// are loaded when these have become scores, the next values when these have been
-// summed.  The waves join their sums through LDS.
+// A segment of at most 32 rows: what bounds it is how fast its keys come in.  Each
+// wave takes items of its own, in LDS of its own for 32 positions' keys and values;
+// the next keys are loaded when these have become scores, the next values when
+// these have been summed.  There is no barrier among the waves.
 template <int D> struct Few {
-  static constexpr int kHalf = 32 * 2 * D, kWave = 2 * kHalf, kLds = 4 * kWave;
-  static constexpr int kLoads = kHalf / 1024;
-  static constexpr int kUnit = 128;
-  static constexpr int kBlocks = 160 * 1024 / (kLds + 4096) < 2 ? 1 : 2;
-  static_assert(kWave == 32 * D * 4, "a wave's sums take the place of its keys and values");
+  static constexpr int kHalf = 32 * 2 * D, kWave = 2 * kHalf, kLoads = kHalf / 1024;
+  static constexpr int kLds = 4 * (kWave + static_cast<int>(sizeof(NotFinite<D>))) + static_cast<int>(sizeof(Plan));
+  static constexpr int kBlocks = D == 256 ? 1 : D == 128 ? 2 : 3;  // of a CU
+  static_assert(kBlocks * kLds <= 160 * 1024, "fits");
 };
 
 template <class T, int D>
 __global__ __launch_bounds__(kThreads, Few<D>::kBlocks) void few_rows_kernel(Attend p) {
   using F = Few<D>;
-  __shared__ __align__(1024) char lds[F::kLds + sizeof(NotFinite<D>) + sizeof(Plan) + sizeof(Stats) + 128];
-  NotFinite<D>& bad = *reinterpret_cast<NotFinite<D>*>(lds + F::kLds);
-  Plan& plan = *reinterpret_cast<Plan*>(lds + F::kLds + sizeof(bad));
-  Stats& stats = *reinterpret_cast<Stats*>(lds + F::kLds + sizeof(bad) + sizeof(Plan));
-  int* limits = reinterpret_cast<int*>(lds + F::kLds + sizeof(bad) + sizeof(Plan) + sizeof(Stats));
+  using R = Rows<T, D>;
+  __shared__ __align__(1024) char lds[F::kLds];
   const int lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6);
-  int each, range;
-  const int total = schedule<false, kFew, F::kUnit>(p, plan, each, range);
-  char* mine = lds + wave * F::kWave;
+  char* const keys = lds + wave * F::kWave;
+  char* const values = keys + F::kHalf;
+  NotFinite<D>& bad = reinterpret_cast<NotFinite<D>*>(lds + 4 * F::kWave)[wave];
+  Plan& plan = *reinterpret_cast<Plan*>(lds + 4 * (F::kWave + sizeof(bad)));
+  const int total = schedule<false, kFew, 32>(p, plan);
   const int of_k = lane_k<D>(lane), of_v = lane_v<D>(lane);
-  for (int item = blockIdx.x; item < total; item += gridDim.x) {
-    const Item it = item_of<false, kFew, F::kUnit>(p, plan, each, range, item);
+  // neighbours in the order of items share keys or a table: side by side in a block
+  for (int item = blockIdx.x * 4 + wave; item < total; item += gridDim.x * 4) {
+    const Item it = item_of<false, kFew, 32>(p, plan, item);
     const int end = it.seg.hi, steps = (it.to - it.from + 31) / 32;
     Pages pages;
+    pages.find(p, it.seg.request, it.from + 16 * lane, end);
+    R rows;
+    rows.load(p, it, lane & 31, lane);
+    rows.clear();
     Feed<D> k_feed, v_feed;
     k_feed.start(p.k, it.head, false, lane);
     v_feed.start(p.v, it.head, true, lane);
-    // this wave's steps are wave, wave + 4, ...: 32 of them to a lookup
+    // 32 steps to a lookup; a step's keys are loaded before its values
     auto load_k = [&](int step) __attribute__((always_inline)) {
-      if ((step >> 2 & 31) == 0)
-        pages.find(p, it.seg.request, it.from + 32 * (step + 4 * (lane >> 1)) + 16 * (lane & 1), end);
-      const int there = step < steps ? end - (it.from + 32 * step) : 0, which = 2 * (step >> 2 & 31);
+      if ((step & 31) == 0 && step > 0) pages.find(p, it.seg.request, it.from + 32 * step + 16 * lane, end);
+      const int there = step < steps ? end - (it.from + 32 * step) : 0, which = 2 * (step & 31);
       k_feed.aim(pages, which, there);
-      k_feed.load_all(mine);
+      k_feed.load_all(keys);
       k_feed.aim(pages, which + 1, there - 16);
-      k_feed.load_all(mine + 32 * D);
+      k_feed.load_all(keys + 32 * D);
     };
     auto load_v = [&](int step) __attribute__((always_inline)) {
-      const int there = step < steps ? end - (it.from + 32 * step) : 0, which = 2 * (step >> 2 & 31);
+      const int there = step < steps ? end - (it.from + 32 * step) : 0, which = 2 * (step & 31);
       v_feed.aim(pages, which, there);
-      v_feed.load_all(mine + F::kHalf);
+      v_feed.load_all(values);
       v_feed.aim(pages, which + 1, there - 16);
-      v_feed.load_all(mine + F::kHalf + 32 * D);
+      v_feed.load_all(values + 32 * D);
     };
-    lds_barrier();  // the last item's sums have been read
-    Rows<T, D> rows;
-    rows.load(p, it, lane & 31, lane);
-    rows.clear();
-    load_k(wave);
-    load_v(wave);
-    bad.clear();
-    if (wave == 0 && lane < 32) limits[lane] = rows.limit;
-    lds_barrier();
-    for (int step = wave; step < steps; step += 4) {
+    load_k(0);
+    load_v(0);
+    bool searched = false;
+    for (int step = 0; step < steps; ++step) {
       f32x16 s[1];
       uint4 w[2];
-      wait_loads<F::kLoads>();  // the keys; the values may be on their way
-      typename Rows<T, D>::Frag f[Rows<T, D>::kAhead];
-#pragma unroll
-      for (int i = 0; i < Rows<T, D>::kAhead; ++i) f[i] = Rows<T, D>::template key<1>(mine, of_k, i);
-      rows.template scores<1>(mine, of_k, f, s, [](int) {});
-      reads_done();
+      typename R::Frag f[R::kAhead];
       const int at = it.from + 32 * step;
-      load_k(step + 4);
+      wait_loads<F::kLoads>();  // the keys; the values may be on their way
+#pragma unroll
+      for (int i = 0; i < R::kAhead; ++i) f[i] = R::template key<1>(keys, of_k, i);
+      rows.template scores<1>(keys, of_k, f, s, [](int) __attribute__((always_inline)) {});
+      reads_done();
+      load_k(step + 1);
       rows.template mask<1>(it.seg, at, lane, s);
       float top = s[0][0];
 #pragma unroll
@@ -825,115 +832,97 @@ __global__ __launch_bounds__(kThreads, Few<D>::kBlocks) void few_rows_kernel(Att
       rows.template weights<1>(p, 0, 16, rows.subtracted(), s, w);
       wait_loads<F::kLoads>();
       if (rows.template partly<1>(it.seg, at)) {
-        take_out<T, D>(mine + F::kHalf, at, it.seg.lo, bad, lane);
-        take_out<T, D>(mine + F::kHalf + 32 * D, at + 16, it.seg.lo, bad, lane);
+        if (!searched) bad.clear(lane, 64);
+        searched = true;
+        take_out<T, D>(values, at, it.seg.lo, bad, lane);
+        take_out<T, D>(values + 32 * D, at + 16, it.seg.lo, bad, lane);
       }
 #pragma unroll
-      for (int i = 0; i < Rows<T, D>::kAhead; ++i) f[i] = Rows<T, D>::template value<1>(mine + F::kHalf, of_v, i);
-      rows.template values<1>(mine + F::kHalf, of_v, f, w, [](int) {});
+      for (int i = 0; i < R::kAhead; ++i) f[i] = R::template value<1>(values, of_v, i);
+      rows.template values<1>(values, of_v, f, w, [](int) __attribute__((always_inline)) {});
       reads_done();
-      load_v(step + 4);
+      load_v(step + 1);
     }
-    wait_loads<0>();  // those past the end too, before the sums take their place
-    float l = rows.l + other_half(rows.l);
-    if (lane < 32) stats[wave][lane] = make_float2(rows.m, l);
-    lds_barrier();
-    float m = -INFINITY;
-#pragma unroll
-    for (int w = 0; w < 4; ++w) m = fmaxf(m, stats[w][lane & 31].x);
-    const float mine_to = weight_of(rows.m, l, m);
-    // [D / 4][32 rows][4 channels]: lanes side by side
-#pragma unroll
-    for (int d = 0; d < D / 32; ++d)
-#pragma unroll
-      for (int e = 0; e < 16; e += 4) {
-        const int quad = 8 * d + 2 * (e >> 2) + (lane >> 5);
-        *reinterpret_cast<float4*>(mine + (quad * 32 + (lane & 31)) * 16) =
-            make_float4(rows.o[d][e] * mine_to, rows.o[d][e + 1] * mine_to, rows.o[d][e + 2] * mine_to,
-                        rows.o[d][e + 3] * mine_to);
-      }
-    lds_barrier();
-    const int count = it.seg.tokens * p.per;
-    for (int i = threadIdx.x; i < count * (D / 4); i += kThreads) {
-      const int r = i / (D / 4), quad = i % (D / 4);
-      float y[4] = {0.f, 0.f, 0.f, 0.f};
-      float top = -INFINITY, sum = 0.f;
-#pragma unroll
-      for (int w = 0; w < 4; ++w) {
-        const float4 part = *reinterpret_cast<const float4*>(lds + w * F::kWave + (quad * 32 + r) * 16);
-        y[0] += part.x, y[1] += part.y, y[2] += part.z, y[3] += part.w;
-        top = fmaxf(top, stats[w][r].x);
-      }
-#pragma unroll
-      for (int w = 0; w < 4; ++w) sum += stats[w][r].y * weight_of(stats[w][r].x, stats[w][r].y, top);
-      if (bad.found) {
-#pragma unroll
-        for (int e = 0; e < 4; ++e) y[e] += bad.added(4 * quad + e, limits[r]);
-      }
-      if (whole(it)) {
-        const int in = r / p.per, token = it.seg.token + in, head = it.head * p.per + r - in * p.per;
-        const float inverse = sum > 0.f || sum != sum ? 1.0f / sum : 0.f;
-#pragma unroll
-        for (int e = 0; e < 4; ++e) y[e] *= inverse;
-        put4<T>(p, token, head, 4 * quad, y);
-        if (p.lse && quad == 0) p.lse[static_cast<int64_t>(token) * p.heads + head] = lse_of(top, sum);
-      } else {
-        const int64_t at = static_cast<int64_t>(item) * kFew + r;
-        *reinterpret_cast<float4*>(p.sums[0] + at * D + 4 * quad) = make_float4(y[0], y[1], y[2], y[3]);
-        if (quad == 0) p.stats[0][at] = make_float2(top, sum);
-      }
-    }
+    if (searched && uniform(bad.found)) rows.add_not_finite(bad, lane);
+    rows.put(p, it, lane & 31, 0, static_cast<int64_t>(item) * kFew + (lane & 31), lane);
+    wait_loads<0>();  // those past the end too
   }
 }
 
 // ------------------------------------------------------------------ join
-// WAVES waves a row: the pieces of the row's shared and own segments by turns.
+// WAVES waves a row: the pieces of the row's shared and own segments by turns, 64 of
+// a wave's at a time: a lane looks up one piece, then all lanes add the pieces.
 template <class T, int D, int WAVES>
 __global__ __launch_bounds__(kThreads) void join_kernel(Attend p) {
   constexpr int kRowsABlock = kThreads / (64 * WAVES), kLane = D / 64;  // channels a lane
   __shared__ float sums[4][D];
   __shared__ float2 stats[4];
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6);
   const int64_t at = static_cast<int64_t>(blockIdx.x) * kRowsABlock + (WAVES == 1 ? wave : 0);
-  const int64_t rows = static_cast<int64_t>(p.tokens) * p.heads;
-  const bool there = at < rows;
-  const int token = there ? static_cast<int>(at / p.heads) : 0, head = there ? static_cast<int>(at % p.heads) : 0;
+  if (at >= static_cast<int64_t>(p.tokens) * p.heads) return;  // whole waves, and no barrier behind it then
+  const int token = static_cast<int>(at / p.heads), head = static_cast<int>(at % p.heads);
   const int request = p.cu ? static_cast<int>(find_sequence(p.cu, p.cu_is64, p.requests, token)) : token;
-  const int group = group_of(p, request), shared = p.shared ? p.num_groups : 0;
-  float m = -INFINITY, l = 0.f, y[kLane];
-#pragma unroll
-  for (int e = 0; e < kLane; ++e) y[e] = 0.f;
   // tokens behind the last request (or before the first) are nobody's: left as they were
-  bool done = !there || token < token_of(p, request) || token >= token_of(p, request + 1);
+  if (token < token_of(p, request) || token >= token_of(p, request + 1)) return;
+  const int group = group_of(p, request), shared = p.shared ? p.num_groups : 0;
+  // pieces of the shared segment, then of the own one
+  int many[2], first[2], tiles[2], count[2], row[2];
 #pragma unroll
   for (int which = 0; which < 2; ++which) {
     const int s = which ? shared + request : group;
-    if (s < 0 || done) continue;
+    count[which] = 0;
+    if (s < 0) continue;
     const Segment seg = segment(p, s);
-    const int row = (token - seg.token) * p.per + head % p.per;
-    if (row < 0 || row >= seg.tokens * p.per || seg.hi <= seg.lo) continue;
-    const int many = seg.tokens * p.per > kFew, tile_rows = many ? Many<D>::kRows : kFew;
-    const int tiles = (seg.tokens * p.per + tile_rows - 1) / tile_rows;
     const int2 place = p.places[s];
-    if (which && place.y == 1 && seg.lo == 0) {  // the item wrote the row itself
-      done = true;
-      continue;
+    const int in = (token - seg.token) * p.per + head % p.per, rows = seg.tokens * p.per;
+    if (in < 0 || in >= rows || seg.hi <= seg.lo) continue;
+    if (which && place.y == 1 && seg.lo == 0) return;  // the item wrote the row itself
+    many[which] = rows > kFew;
+    const int tile_rows = many[which] ? Many<D>::kRows : kFew;
+    tiles[which] = (rows + tile_rows - 1) / tile_rows;
+    first[which] = place.x + head / p.per * place.y * tiles[which] + in / tile_rows;
+    row[which] = in % tile_rows;
+    count[which] = place.y;
+  }
+  const int pieces = count[0] + count[1];
+  float m = -INFINITY, l = 0.f, y[kLane];
+#pragma unroll
+  for (int e = 0; e < kLane; ++e) y[e] = 0.f;
+  for (int base = 0; base < pieces; base += 64 * WAVES) {
+    const int piece = base + lane * WAVES + (WAVES == 1 ? 0 : wave);
+    float2 st = make_float2(-INFINITY, 0.f);
+    uint64_t from = 0;
+    if (piece < pieces) {
+      const int which = piece >= count[0], kind = which ? many[1] : many[0];
+      const int item = which ? first[1] + (piece - count[0]) * tiles[1] : first[0] + piece * tiles[0];
+      if (item >= 0 && item < p.items_max[kind]) {
+        const int64_t to = static_cast<int64_t>(item) * (kind ? Many<D>::kRows : kFew) + (which ? row[1] : row[0]);
+        st = p.stats[kind][to];
+        from = reinterpret_cast<uint64_t>(p.sums[kind] + to * D);
+      }
     }
-    const int first = place.x + head / p.per * place.y * tiles + row / tile_rows;
-    for (int i = WAVES == 1 ? 0 : wave; i < place.y; i += WAVES) {
-      const int item = first + i * tiles;
-      if (item >= p.items_max[many]) break;
-      const int64_t from = static_cast<int64_t>(item) * tile_rows + row % tile_rows;
-      const float2 st = p.stats[many][from];
-      const float* part = p.sums[many] + from * D + lane * kLane;
-      float x[kLane];
+    float top = st.x;
 #pragma unroll
-      for (int e = 0; e < kLane; ++e) x[e] = part[e];
-      const float top = fmaxf(m, st.x), a = weight_of(m, l, top), b = weight_of(st.x, st.y, top);
-      l = l * a + st.y * b;
+    for (int off = 32; off > 0; off >>= 1) top = fmaxf(top, __shfl_xor(top, off, 64));
+    top = fmaxf(top, m);
+    const float old = weight_of(m, l, top), mine = weight_of(st.x, st.y, top);
+    float sum = st.y * mine;
 #pragma unroll
-      for (int e = 0; e < kLane; ++e) y[e] = y[e] * a + x[e] * b;
-      m = top;
+    for (int off = 32; off > 0; off >>= 1) sum += __shfl_xor(sum, off, 64);
+    l = l * old + sum;
+    m = top;
+#pragma unroll
+    for (int e = 0; e < kLane; ++e) y[e] *= old;
+    const int here = (min(pieces - base, 64 * WAVES) + WAVES - 1 - (WAVES == 1 ? 0 : wave)) / WAVES;
+#pragma unroll 8
+    for (int i = 0; i < here; ++i) {
+      const float weight = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(mine), i));
+      const uint64_t of = static_cast<uint64_t>(static_cast<uint32_t>(__builtin_amdgcn_readlane(static_cast<int>(from >> 32), i))) << 32 |
+                          static_cast<uint32_t>(__builtin_amdgcn_readlane(static_cast<int>(from), i));
+      if (of == 0) continue;
+      const float* part = reinterpret_cast<const float*>(of) + lane * kLane;
+#pragma unroll
+      for (int e = 0; e < kLane; ++e) y[e] += part[e] * weight;
     }
   }
   if constexpr (WAVES > 1) {
@@ -955,7 +944,6 @@ __global__ __launch_bounds__(kThreads) void join_kernel(Attend p) {
       for (int e = 0; e < kLane; ++e) y[e] += sums[w][lane * kLane + e] * b;
     }
   }
-  if (done) return;
   const float inverse = l > 0.f || l != l ? 1.0f / l : 0.f;
   T* to = static_cast<T*>(p.out) + token * p.out_token + head * p.out_head + lane * kLane;
 #pragma unroll
@@ -982,8 +970,8 @@ Sizes sizes_of(int64_t tokens, int64_t requests, int64_t groups, int64_t heads, 
   const int64_t per = heads / kv_heads, rows = tokens * per, sets = groups > 0 ? 2 : 1;
   z.few = per <= kFew;
   z.many = rows > kFew && (varlen || per > kFew || groups > 0);
-  z.target[0] = 2 * kCus * (dim == 256 ? 1 : 2);
-  z.target[1] = 2 * kCus;
+  z.target[0] = 4 * kCus * (dim == 256 ? 1 : dim == 128 ? 2 : 3);  // waves that run at once
+  z.target[1] = kCus * (dim == 256 ? 1 : 2);                       // blocks
   const int64_t few_tiles = requests + groups, many_tiles = sets * (rows / 128 + std::min(requests + groups, rows / kFew + 1));
   z.items[0] = z.few ? z.target[0] + few_tiles * kv_heads : 0;
   z.items[1] = z.many ? z.target[1] + many_tiles * kv_heads : 0;
@@ -1005,9 +993,9 @@ Sizes sizes_of(int64_t tokens, int64_t requests, int64_t groups, int64_t heads, 
 
 template <class T, int D>
 int launch_attend(const Attend& p, const Sizes& z, hipStream_t stream) {
-  if (z.many) many_rows_kernel<T, D><<<2 * kCus, kThreads, 0, stream>>>(p);
+  if (z.many) many_rows_kernel<T, D><<<static_cast<uint32_t>(z.target[1]), kThreads, 0, stream>>>(p);
   if (z.few)
-    few_rows_kernel<T, D><<<static_cast<uint32_t>(std::min(z.items[0], z.target[0])), kThreads, 0, stream>>>(p);
+    few_rows_kernel<T, D><<<static_cast<uint32_t>(ceil_div(std::min(z.items[0], z.target[0]), 4)), kThreads, 0, stream>>>(p);
   const int64_t rows = static_cast<int64_t>(p.tokens) * p.heads;
   if (rows <= 16 * kCus)
     join_kernel<T, D, 4><<<static_cast<uint32_t>(rows), kThreads, 0, stream>>>(p);
