@@ -66,7 +66,14 @@ struct Attend {
   float* sums[2];
   float2* stats[2];
   int items_max[2], target[2], min_units[2];
-  int2* places;
+  struct Place* places;  // of each segment, for the joining kernel
+};
+// Where the items of a segment lie, and what it is.
+struct Place {
+  int item, ranges;  // first item; ranges of keys
+  int token, tokens, lo, hi;
+  int group;  // of a request (-1: none)
+  int unused;
 };
 
 // ------------------------------------------------------------------ segments
@@ -75,6 +82,7 @@ struct Segment {
   int lo, hi;         // positions
   int request;        // whose row of the table is read
   int length;         // of the request, as given (a group's: unused)
+  int group;          // of the request, or -1
 };
 
 __device__ __forceinline__ int uniform(int v) { return __builtin_amdgcn_readfirstlane(v); }
@@ -100,10 +108,6 @@ __device__ __forceinline__ int group_of(const Attend& p, int request) {
   }
   return group_start(p, lo) <= request && request < group_start(p, lo + 1) ? lo : -1;
 }
-__device__ __forceinline__ int shared_before(const Attend& p, int request) {
-  const int g = group_of(p, request);
-  return g < 0 ? 0 : shared_of(p, g);
-}
 __device__ __forceinline__ int segments_of(const Attend& p) { return p.requests + (p.shared ? p.num_groups : 0); }
 
 __device__ __forceinline__ Segment segment(const Attend& p, int s) {
@@ -117,11 +121,13 @@ __device__ __forceinline__ Segment segment(const Attend& p, int s) {
     seg.hi = shared_of(p, s);
     seg.request = min(r0, p.requests - 1);
     seg.length = 0;
+    seg.group = -1;
   } else {
     const int r = s - shared;
     seg.token = token_of(p, r);
     seg.tokens = max(0, token_of(p, r + 1) - seg.token);
-    seg.lo = shared_before(p, r);
+    seg.group = group_of(p, r);
+    seg.lo = seg.group < 0 ? 0 : shared_of(p, seg.group);
     seg.length = static_cast<int>(load_index(p.lens, r, p.lens_is64));
     seg.hi = clampi(seg.length, 0, p.capacity);
     seg.request = r;
@@ -204,7 +210,7 @@ __device__ int schedule(const Attend& p, Plan& plan) {
       const Segment seg = s == from ? first : segment(p, s);
       const Cut c = cut_of<MANY, ROWS, UNIT>(p, seg);
       const int ranges = (c.units + range - 1) / range;
-      if ((seg.tokens * p.per > kFew) == MANY) p.places[s] = make_int2(before, ranges);
+      if ((seg.tokens * p.per > kFew) == MANY) p.places[s] = {before, ranges, seg.token, seg.tokens, seg.lo, seg.hi, seg.group, 0};
       before += c.tiles * p.kv_heads * ranges;
     }
   __syncthreads();
@@ -237,7 +243,7 @@ __device__ Item item_of(const Attend& p, const Plan& plan, int item) {
     if (at < items || s >= last) {
       Item it;
       it.seg = {uniform(seg.token), uniform(seg.tokens), uniform(seg.lo),
-                uniform(seg.hi),    uniform(seg.request), uniform(seg.length)};
+                uniform(seg.hi),    uniform(seg.request), uniform(seg.length), uniform(seg.group)};
       it.ranges = ranges;
       it.own = s >= segments_of(p) - p.requests;
       const int across = uniform(at / max(1, tiles));
@@ -850,39 +856,50 @@ __global__ __launch_bounds__(kThreads, Few<D>::kBlocks) void few_rows_kernel(Att
 }
 
 // ------------------------------------------------------------------ join
+// The request of a token: the last that starts at or before it, found by a whole wave.
+__device__ __forceinline__ int request_of(const Attend& p, int token, int lane) {
+  int first = 0, count = p.requests;
+  while (count > 1) {
+    const int each = (count + 63) / 64, at = first + lane * each;
+    const bool before = lane * each < count && load_index(p.cu, at, p.cu_is64) <= token;
+    const int found = max(1, __popcll(__ballot(before)));
+    first += (found - 1) * each;
+    count = min(each, count - (found - 1) * each);
+  }
+  return first;
+}
 // WAVES waves a row: the pieces of the row's shared and own segments by turns, 64 of
 // a wave's at a time: a lane looks up one piece, then all lanes add the pieces.
 template <class T, int D, int WAVES>
 __global__ __launch_bounds__(kThreads) void join_kernel(Attend p) {
-  constexpr int kRowsABlock = kThreads / (64 * WAVES), kLane = D / 64;  // channels a lane
+  constexpr int kRowsABlock = kThreads / (64 * WAVES), kLane = D / 64, kBatch = 8;  // channels a lane
+  typedef float Channels __attribute__((ext_vector_type(kLane)));
   __shared__ float sums[4][D];
   __shared__ float2 stats[4];
   const int lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6);
   const int64_t at = static_cast<int64_t>(blockIdx.x) * kRowsABlock + (WAVES == 1 ? wave : 0);
   if (at >= static_cast<int64_t>(p.tokens) * p.heads) return;  // whole waves, and no barrier behind it then
   const int token = static_cast<int>(at / p.heads), head = static_cast<int>(at % p.heads);
-  const int request = p.cu ? static_cast<int>(find_sequence(p.cu, p.cu_is64, p.requests, token)) : token;
+  const int request = p.cu ? request_of(p, token, lane) : token, shared = p.shared ? p.num_groups : 0;
+  const Place own = p.places[shared + request];
   // tokens behind the last request (or before the first) are nobody's: left as they were
   if (token < token_of(p, request) || token >= token_of(p, request + 1)) return;
-  const int group = group_of(p, request), shared = p.shared ? p.num_groups : 0;
   // pieces of the shared segment, then of the own one
   int many[2], first[2], tiles[2], count[2], row[2];
 #pragma unroll
   for (int which = 0; which < 2; ++which) {
-    const int s = which ? shared + request : group;
     count[which] = 0;
-    if (s < 0) continue;
-    const Segment seg = segment(p, s);
-    const int2 place = p.places[s];
-    const int in = (token - seg.token) * p.per + head % p.per, rows = seg.tokens * p.per;
-    if (in < 0 || in >= rows || seg.hi <= seg.lo) continue;
-    if (which && place.y == 1 && seg.lo == 0) return;  // the item wrote the row itself
+    if (!which && own.group < 0) continue;
+    const Place place = which ? own : p.places[own.group];
+    const int in = (token - place.token) * p.per + head % p.per, rows = place.tokens * p.per;
+    if (in < 0 || in >= rows || place.hi <= place.lo) continue;
+    if (which && place.ranges == 1 && place.lo == 0) return;  // the item wrote the row itself
     many[which] = rows > kFew;
     const int tile_rows = many[which] ? Many<D>::kRows : kFew;
     tiles[which] = (rows + tile_rows - 1) / tile_rows;
-    first[which] = place.x + head / p.per * place.y * tiles[which] + in / tile_rows;
+    first[which] = place.item + head / p.per * place.ranges * tiles[which] + in / tile_rows;
     row[which] = in % tile_rows;
-    count[which] = place.y;
+    count[which] = place.ranges;
   }
   const int pieces = count[0] + count[1];
   float m = -INFINITY, l = 0.f, y[kLane];
@@ -895,11 +912,10 @@ __global__ __launch_bounds__(kThreads) void join_kernel(Attend p) {
     if (piece < pieces) {
       const int which = piece >= count[0], kind = which ? many[1] : many[0];
       const int item = which ? first[1] + (piece - count[0]) * tiles[1] : first[0] + piece * tiles[0];
-      if (item >= 0 && item < p.items_max[kind]) {
-        const int64_t to = static_cast<int64_t>(item) * (kind ? Many<D>::kRows : kFew) + (which ? row[1] : row[0]);
-        st = p.stats[kind][to];
-        from = reinterpret_cast<uint64_t>(p.sums[kind] + to * D);
-      }
+      const int64_t to = static_cast<int64_t>(clampi(item, 0, p.items_max[kind] - 1)) * (kind ? Many<D>::kRows : kFew) +
+                         (which ? row[1] : row[0]);
+      st = p.stats[kind][to];
+      from = reinterpret_cast<uint64_t>(p.sums[kind] + to * D);
     }
     float top = st.x;
 #pragma unroll
@@ -914,15 +930,23 @@ __global__ __launch_bounds__(kThreads) void join_kernel(Attend p) {
 #pragma unroll
     for (int e = 0; e < kLane; ++e) y[e] *= old;
     const int here = (min(pieces - base, 64 * WAVES) + WAVES - 1 - (WAVES == 1 ? 0 : wave)) / WAVES;
-#pragma unroll 8
-    for (int i = 0; i < here; ++i) {
-      const float weight = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(mine), i));
-      const uint64_t of = static_cast<uint64_t>(static_cast<uint32_t>(__builtin_amdgcn_readlane(static_cast<int>(from >> 32), i))) << 32 |
-                          static_cast<uint32_t>(__builtin_amdgcn_readlane(static_cast<int>(from), i));
-      if (of == 0) continue;
-      const float* part = reinterpret_cast<const float*>(of) + lane * kLane;
+    for (int i = 0; i < here; i += kBatch) {
+      Channels part[kBatch];
+      float weight[kBatch];
 #pragma unroll
-      for (int e = 0; e < kLane; ++e) y[e] += part[e] * weight;
+      for (int j = 0; j < kBatch; ++j) {  // past the last: that one again, unused
+        const int k = min(i + j, here - 1);
+        const uint32_t low = __builtin_amdgcn_readlane(static_cast<int>(from), k),
+                       high = __builtin_amdgcn_readlane(static_cast<int>(from >> 32), k);
+        part[j] = reinterpret_cast<const Channels*>(static_cast<uint64_t>(high) << 32 | low)[lane];
+        weight[j] = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(mine), k));
+      }
+#pragma unroll
+      for (int j = 0; j < kBatch; ++j)
+        if (i + j < here) {
+#pragma unroll
+          for (int e = 0; e < kLane; ++e) y[e] = fmaf(part[j][e], weight[j], y[e]);
+        }
     }
   }
   if constexpr (WAVES > 1) {
@@ -986,7 +1010,7 @@ Sizes sizes_of(int64_t tokens, int64_t requests, int64_t groups, int64_t heads, 
     z.sums[kind] = take(n * dim * 4);
     z.stats[kind] = take(n * 8);
   }
-  z.places = take((requests + groups) * 8);
+  z.places = take((requests + groups) * static_cast<int64_t>(sizeof(Place)));
   z.bytes = at;
   return z;
 }
@@ -1086,7 +1110,7 @@ extern "C" int gdn_paged_attention(const void* q, int64_t q_token_stride, int64_
     p.target[kind] = static_cast<int>(z.target[kind]);
     p.min_units[kind] = 1;
   }
-  p.places = reinterpret_cast<int2*>(ws + z.places);
+  p.places = reinterpret_cast<Place*>(ws + z.places);
   auto go = [&](auto type) {
     using T = decltype(type);
     const hipStream_t on = static_cast<hipStream_t>(stream);
