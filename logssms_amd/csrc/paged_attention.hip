@@ -55,6 +55,7 @@ struct Attend {
   const void *lens, *shared, *groups, *cu;  // shared NULL: nothing shared; groups NULL: one; cu NULL: a token each
   int table_is64, lens_is64, shared_is64, groups_is64, cu_is64;
   int tokens, requests, num_groups, heads, kv_heads, per;
+  Div32 by_per, by_heads;
   int pages, capacity;  // of the cache; positions of a row of the table
   Div32 page;
   float factor;  // scale log2 e
@@ -65,7 +66,8 @@ struct Attend {
   // the first item and the number of key ranges of each segment
   float* sums[2];
   float2* stats[2];
-  int items_max[2], target[2], min_units[2];
+  int items_max[2], min_units[2];
+  float per_target[2];  // key heads over the number of items wanted
   struct Place* places;  // of each segment, for the joining kernel
 };
 // Where the items of a segment lie, and what it is.
@@ -150,13 +152,23 @@ __device__ __forceinline__ Cut cut_of(const Attend& p, const Segment& seg) {
 struct Plan {
   int base[kThreads];  // items before each thread's segments
   Segment segments[kThreads];  // each thread's first one: all, of up to kThreads
-  int64_t units[kThreads / 64];
+  float units[kThreads / 64];
   int count[kThreads / 64];
   int each, range;     // segments of a thread; units of a range of keys
 };
 // One LDS array holds it all in a kernel with direct loads: beside a second one, the
 // compiler waits for every load in flight in front of each read.
 static_assert(sizeof(Plan) % 8 == 0, "what lies behind it is aligned");
+
+// n / d for d > 0 where the quotient is below 2^22: shorter than the exact division,
+// and what a launch runs once it has to fetch first.
+__device__ __forceinline__ int short_div(int n, int d) {
+  int q = static_cast<int>(static_cast<float>(n) * __builtin_amdgcn_rcpf(static_cast<float>(d)));
+  const int r = n - q * d;
+  q += r >= d ? 1 : r < 0 ? -1 : 0;
+  return q;
+}
+__device__ __forceinline__ int ranges_of(int units, int range) { return short_div(units + range - 1, range); }
 
 // Counts the items of the launch: thread i answers for `each` consecutive
 // segments.  A range of keys is as long as it has to be for `target` items.
@@ -166,53 +178,55 @@ __device__ int schedule(const Attend& p, Plan& plan) {
   const int n = segments_of(p), lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const int each = (n + kThreads - 1) / kThreads;
   const int from = threadIdx.x * each, to = min(n, from + each);
-  int64_t units = 0;
+  float units = 0.f;  // the same in all blocks; its rounding is in the bound of the items
+  int items = 0, before = 0, total = 0, range = 1;
   Segment first{};
-  for (int s = from; s < to; ++s) {
-    const Segment seg = segment(p, s);
-    const Cut c = cut_of<MANY, ROWS, UNIT>(p, seg);
-    if (s == from) first = seg;
-    units += static_cast<int64_t>(c.tiles) * c.units;
-  }
-  plan.segments[threadIdx.x] = first;
-#pragma unroll
-  for (int off = 32; off > 0; off >>= 1) units += __shfl_xor(units, off, 64);
-  if (lane == 0) plan.units[wave] = units;
-  __syncthreads();
-  units = 0;
-#pragma unroll
-  for (int w = 0; w < kThreads / 64; ++w) units += plan.units[w];
-  const int64_t wanted = (units * p.kv_heads + p.target[MANY] - 1) / p.target[MANY];
-  const int range = static_cast<int>(wanted < p.min_units[MANY] ? p.min_units[MANY] : wanted);
-  int items = 0;
-  for (int s = from; s < to; ++s) {
-    const Cut c = cut_of<MANY, ROWS, UNIT>(p, s == from ? first : segment(p, s));
-    items += c.tiles * p.kv_heads * ((c.units + range - 1) / range);
-  }
-  int sum = items;
-#pragma unroll
-  for (int off = 1; off < 64; off <<= 1) {
-    const int below = __shfl_up(sum, off, 64);
-    if (lane >= off) sum += below;
-  }
-  if (lane == 63) plan.count[wave] = sum;
-  __syncthreads();
-  int before = sum - items, total = 0;
-#pragma unroll
-  for (int w = 0; w < kThreads / 64; ++w) {
-    if (w < wave) before += plan.count[w];
-    total += plan.count[w];
-  }
-  plan.base[threadIdx.x] = before;
-  if (threadIdx.x == 0) plan.each = each, plan.range = range;
-  if (blockIdx.x == 0)
+  // units, items, places: one loop, so that the code of segment() is there once
+#pragma unroll 1
+  for (int pass = 0; pass < 3; ++pass) {
+#pragma unroll 1
     for (int s = from; s < to; ++s) {
-      const Segment seg = s == from ? first : segment(p, s);
+      const Segment seg = pass > 0 && s == from ? first : segment(p, s);
       const Cut c = cut_of<MANY, ROWS, UNIT>(p, seg);
-      const int ranges = (c.units + range - 1) / range;
-      if ((seg.tokens * p.per > kFew) == MANY) p.places[s] = {before, ranges, seg.token, seg.tokens, seg.lo, seg.hi, seg.group, 0};
-      before += c.tiles * p.kv_heads * ranges;
+      const int ranges = ranges_of(c.units, range);
+      if (pass == 0) {
+        if (s == from) first = seg;
+        units += static_cast<float>(c.tiles) * static_cast<float>(c.units);
+      } else if (pass == 1) {
+        items += c.tiles * p.kv_heads * ranges;
+      } else {
+        if ((seg.tokens * p.per > kFew) == MANY)
+          p.places[s] = {before, ranges, seg.token, seg.tokens, seg.lo, seg.hi, seg.group, 0};
+        before += c.tiles * p.kv_heads * ranges;
+      }
     }
+    if (pass == 0) {
+      plan.segments[threadIdx.x] = first;
+      units = head_sum<64>(units);
+      if (lane == 0) plan.units[wave] = units;
+      __syncthreads();
+      units = plan.units[0] + plan.units[1] + plan.units[2] + plan.units[3];
+      range = max(p.min_units[MANY], static_cast<int>(fminf(units * p.per_target[MANY], 1.0e9f)) + 1);
+    } else if (pass == 1) {
+      int sum = items;
+#pragma unroll
+      for (int off = 1; off < 64; off <<= 1) {
+        const int below = __shfl_up(sum, off, 64);
+        if (lane >= off) sum += below;
+      }
+      if (lane == 63) plan.count[wave] = sum;
+      __syncthreads();
+      before = sum - items;
+#pragma unroll
+      for (int w = 0; w < kThreads / 64; ++w) {
+        if (w < wave) before += plan.count[w];
+        total += plan.count[w];
+      }
+      plan.base[threadIdx.x] = before;
+      if (threadIdx.x == 0) plan.each = each, plan.range = range;
+      if (blockIdx.x > 0) break;
+    }
+  }
   __syncthreads();
   return min(total, p.items_max[MANY]);
 }
@@ -239,16 +253,16 @@ __device__ Item item_of(const Attend& p, const Plan& plan, int item) {
   for (int s = thread * each;; ++s) {
     const Segment seg = s == thread * each ? plan.segments[thread] : segment(p, s);
     const Cut c = cut_of<MANY, ROWS, UNIT>(p, seg);
-    const int ranges = uniform((c.units + range - 1) / range), tiles = uniform(c.tiles), items = tiles * p.kv_heads * ranges;
+    const int ranges = uniform(ranges_of(c.units, range)), tiles = uniform(c.tiles), items = tiles * p.kv_heads * ranges;
     if (at < items || s >= last) {
       Item it;
       it.seg = {uniform(seg.token), uniform(seg.tokens), uniform(seg.lo),
                 uniform(seg.hi),    uniform(seg.request), uniform(seg.length), uniform(seg.group)};
       it.ranges = ranges;
       it.own = s >= segments_of(p) - p.requests;
-      const int across = uniform(at / max(1, tiles));
+      const int across = uniform(short_div(at, max(1, tiles)));
       it.tile = at - across * max(1, tiles);
-      it.head = uniform(across / max(1, ranges));
+      it.head = uniform(short_div(across, max(1, ranges)));
       it.from = (it.seg.lo & ~15) + (across - it.head * max(1, ranges)) * range * UNIT;
       it.to = min(it.seg.hi, it.from + range * UNIT);
       return it;
@@ -478,7 +492,7 @@ struct Rows {
   // Row `row` of the segment: its token and head, its queries, the positions visible to it.
   __device__ __forceinline__ void load(const Attend& p, const Item& it, int row, int lane) {
     const bool there = row < it.seg.tokens * p.per;
-    const int in = there ? row / p.per : 0, token = it.seg.token + in;
+    const int in = there ? p.by_per.div(row) : 0, token = it.seg.token + in;
     const int head = it.head * p.per + (there ? row - in * p.per : 0);
     const T* from = static_cast<const T*>(p.q) + token * p.q_token + head * p.q_head + 8 * (lane >> 5);
 #pragma unroll
@@ -605,7 +619,7 @@ struct Rows {
     const float sum = l + other_half(l);
     if (row >= it.seg.tokens * p.per) return;
     if (whole(it)) {
-      const int in = row / p.per, token = it.seg.token + in, head = it.head * p.per + row - in * p.per;
+      const int in = p.by_per.div(row), token = it.seg.token + in, head = it.head * p.per + row - in * p.per;
       const float inverse = sum > 0.f || sum != sum ? 1.0f / sum : 0.f;
 #pragma unroll
       for (int d = 0; d < D / 32; ++d)
@@ -661,7 +675,7 @@ __global__ __launch_bounds__(kThreads, D == 256 ? 1 : 2) void many_rows_kernel(A
     rows.load(p, it, row, lane);
     rows.clear();
     // nothing behind the last position that a row of the tile sees
-    const int last_token = min(it.seg.tokens - 1, (it.tile * M::kRows + M::kRows - 1) / p.per);
+    const int last_token = min(it.seg.tokens - 1, static_cast<int>(p.by_per.div(it.tile * M::kRows + M::kRows - 1)));
     int to = it.to;
     if (it.own) to = uniform(clampi(static_cast<int64_t>(it.seg.length) - (it.seg.tokens - 1 - last_token), 0, to));
     const int end = it.seg.hi, steps = to > it.from ? (to - it.from + M::kKeys - 1) / M::kKeys : 0;
@@ -877,13 +891,14 @@ __global__ __launch_bounds__(kThreads) void join_kernel(Attend p) {
   __shared__ float sums[4][D];
   __shared__ float2 stats[4];
   const int lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6);
-  const int64_t at = static_cast<int64_t>(blockIdx.x) * kRowsABlock + (WAVES == 1 ? wave : 0);
-  if (at >= static_cast<int64_t>(p.tokens) * p.heads) return;  // whole waves, and no barrier behind it then
-  const int token = static_cast<int>(at / p.heads), head = static_cast<int>(at % p.heads);
+  const uint32_t at = blockIdx.x * kRowsABlock + (WAVES == 1 ? wave : 0);
+  if (at >= static_cast<uint32_t>(p.tokens) * p.heads) return;  // whole waves, and no barrier behind it then
+  const int token = p.by_heads.div(at), head = at - token * p.heads;
   const int request = p.cu ? request_of(p, token, lane) : token, shared = p.shared ? p.num_groups : 0;
   const Place own = p.places[shared + request];
   // tokens behind the last request (or before the first) are nobody's: left as they were
   if (token < token_of(p, request) || token >= token_of(p, request + 1)) return;
+  const int kv_head = p.by_per.div(head);
   // pieces of the shared segment, then of the own one
   int many[2], first[2], tiles[2], count[2], row[2];
 #pragma unroll
@@ -891,13 +906,13 @@ __global__ __launch_bounds__(kThreads) void join_kernel(Attend p) {
     count[which] = 0;
     if (!which && own.group < 0) continue;
     const Place place = which ? own : p.places[own.group];
-    const int in = (token - place.token) * p.per + head % p.per, rows = place.tokens * p.per;
+    const int in = (token - place.token) * p.per + head - kv_head * p.per, rows = place.tokens * p.per;
     if (in < 0 || in >= rows || place.hi <= place.lo) continue;
     if (which && place.ranges == 1 && place.lo == 0) return;  // the item wrote the row itself
     many[which] = rows > kFew;
     const int tile_rows = many[which] ? Many<D>::kRows : kFew;
     tiles[which] = (rows + tile_rows - 1) / tile_rows;
-    first[which] = place.item + head / p.per * place.ranges * tiles[which] + in / tile_rows;
+    first[which] = place.item + kv_head * place.ranges * tiles[which] + in / tile_rows;
     row[which] = in % tile_rows;
     count[which] = place.ranges;
   }
@@ -987,7 +1002,8 @@ struct Sizes {
 };
 
 // Bounds from what the host knows.  Each of a kind's items is one of `target` (a
-// range of keys is at least all units over it) or the last range of a tile.
+// range of keys is at least all units over it, but for the rounding of that sum) or
+// the last range of a tile.
 Sizes sizes_of(int64_t tokens, int64_t requests, int64_t groups, int64_t heads, int64_t kv_heads, int64_t dim,
                bool varlen) {
   Sizes z{};
@@ -997,8 +1013,8 @@ Sizes sizes_of(int64_t tokens, int64_t requests, int64_t groups, int64_t heads, 
   z.target[0] = 4 * kCus * (dim == 256 ? 1 : dim == 128 ? 2 : 3);  // waves that run at once
   z.target[1] = kCus * (dim == 256 ? 1 : 2);                       // blocks
   const int64_t few_tiles = requests + groups, many_tiles = sets * (rows / 128 + std::min(requests + groups, rows / kFew + 1));
-  z.items[0] = z.few ? z.target[0] + few_tiles * kv_heads : 0;
-  z.items[1] = z.many ? z.target[1] + many_tiles * kv_heads : 0;
+  z.items[0] = z.few ? z.target[0] + z.target[0] / 64 + few_tiles * kv_heads : 0;
+  z.items[1] = z.many ? z.target[1] + z.target[1] / 64 + many_tiles * kv_heads : 0;
   int64_t at = 0;
   auto take = [&](int64_t bytes) {
     const int64_t from = at;
@@ -1064,8 +1080,8 @@ extern "C" int gdn_paged_attention(const void* q, int64_t q_token_stride, int64_
     return GDN_ERR_UNSUPPORTED;
   }
   if (tokens * heads >= (int64_t{1} << 31) || requests + groups >= (int64_t{1} << 24) ||
-      table_width * page_size > (int64_t{1} << 30) || pages >= (int64_t{1} << 31)) {
-    set_error("up to 2^31 rows, 2^24 requests, 2^30 positions and 2^31 pages");
+      table_width * page_size > (int64_t{1} << 30) || pages >= (int64_t{1} << 31) || kv_heads > (1 << 16)) {
+    set_error("up to 2^31 rows, 2^24 requests, 2^30 positions, 2^31 pages and 2^16 key heads");
     return GDN_ERR_UNSUPPORTED;
   }
   if (tokens == 0 || requests == 0) return GDN_OK;
@@ -1097,6 +1113,7 @@ extern "C" int gdn_paged_attention(const void* q, int64_t q_token_stride, int64_
   p.cu = cu_seqlens, p.cu_is64 = cu_dtype == GDN_I64;
   p.tokens = static_cast<int>(tokens), p.requests = static_cast<int>(requests), p.num_groups = static_cast<int>(groups);
   p.heads = static_cast<int>(heads), p.kv_heads = static_cast<int>(kv_heads), p.per = static_cast<int>(heads / kv_heads);
+  p.by_per = make_div32(p.per), p.by_heads = make_div32(heads);
   p.pages = static_cast<int>(pages), p.capacity = static_cast<int>(table_width * page_size);
   p.page = make_div32(page_size);
   p.factor = scale * kLog2e;
@@ -1107,7 +1124,7 @@ extern "C" int gdn_paged_attention(const void* q, int64_t q_token_stride, int64_
     p.sums[kind] = reinterpret_cast<float*>(ws + z.sums[kind]);
     p.stats[kind] = reinterpret_cast<float2*>(ws + z.stats[kind]);
     p.items_max[kind] = static_cast<int>(z.items[kind]);
-    p.target[kind] = static_cast<int>(z.target[kind]);
+    p.per_target[kind] = static_cast<float>(static_cast<double>(kv_heads) / static_cast<double>(z.target[kind]));
     p.min_units[kind] = 1;
   }
   p.places = reinterpret_cast<Place*>(ws + z.places);
