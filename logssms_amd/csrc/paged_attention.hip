@@ -38,6 +38,7 @@ typedef __attribute__((address_space(3))) void lds_void;
 
 constexpr int kFew = 32;        // rows of a segment up to which its waves split the keys instead of the rows
 constexpr int kThreads = 256;   // of every kernel here
+constexpr float kItem = 8.f;    // what an item of many rows costs beside its steps, in steps
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 constexpr float kLater = 8.0f;  // a maximum may lag by 2^8 before the sums are rescaled
 
@@ -140,12 +141,15 @@ __device__ __forceinline__ Segment segment(const Attend& p, int s) {
 // Cut of a segment: tiles of `rows` rows and units of `unit` positions from a multiple of 16 on.
 struct Cut {
   int tiles, units;
+  int least;  // units of the tile that sees the fewest: its tokens come first
 };
 template <bool MANY, int ROWS, int UNIT>
-__device__ __forceinline__ Cut cut_of(const Attend& p, const Segment& seg) {
+__device__ __forceinline__ Cut cut_of(const Attend& p, const Segment& seg, bool own) {
   const int rows = seg.tokens * p.per, from = seg.lo & ~15;
-  if (rows == 0 || (rows > kFew) != MANY || seg.hi <= seg.lo) return {0, 0};
-  return {(rows + ROWS - 1) / ROWS, (seg.hi - from + UNIT - 1) / UNIT};
+  if (rows == 0 || (rows > kFew) != MANY || seg.hi <= seg.lo) return {0, 0, 0};
+  const int units = (seg.hi - from + UNIT - 1) / UNIT;
+  const int seen = clampi(static_cast<int64_t>(seg.length) - seg.tokens - from, 0, seg.hi) / UNIT + 1;
+  return {(rows + ROWS - 1) / ROWS, units, own && seen < units ? seen : units};
 }
 
 // ------------------------------------------------------------------ schedule
@@ -155,6 +159,8 @@ struct Plan {
   float units[kThreads / 64];
   int count[kThreads / 64];
   int each, range;     // segments of a thread; units of a range of keys
+  // of each candidate for the range: items, those that are not empty, the longest
+  int items[8], filled[8], longest[8];
 };
 // One LDS array holds it all in a kernel with direct loads: beside a second one, the
 // compiler waits for every load in flight in front of each read.
@@ -170,8 +176,19 @@ __device__ __forceinline__ int short_div(int n, int d) {
 }
 __device__ __forceinline__ int ranges_of(int units, int range) { return short_div(units + range - 1, range); }
 
+// The range of keys for items of many rows, of eight candidates the one under which the
+// last block should end first: items are taken in rounds, a block one of each round,
+// and each costs kItem units to begin and to store.  (Equal parts of one line of all
+// the work, whatever tiles they cut, balance better, but then no two blocks read the
+// same keys at a time, and the L2 no longer serves them: six prompts behind 8192 shared
+// positions took 431 us so, 320 in ranges of one length that all the work gives.)
+__device__ __forceinline__ int candidate(float units_a_block, int i) {
+  constexpr float kShares[8] = {0.f, 1.f, 0.8f, 0.667f, 0.5f, 0.4f, 0.333f, 0.25f};
+  return i == 0 ? 1 << 30 : static_cast<int>(units_a_block * kShares[i]) + 1;
+}
+
 // Counts the items of the launch: thread i answers for `each` consecutive
-// segments.  A range of keys is as long as it has to be for `target` items.
+// segments.  A range of keys of few rows is as long as it has to be for `target` items.
 // Block 0 notes for the joining kernel where each segment's items lie.
 template <bool MANY, int ROWS, int UNIT>
 __device__ int schedule(const Attend& p, Plan& plan) {
@@ -183,15 +200,26 @@ __device__ int schedule(const Attend& p, Plan& plan) {
   Segment first{};
   // units, items, places: one loop, so that the code of segment() is there once
 #pragma unroll 1
-  for (int pass = 0; pass < 3; ++pass) {
+  for (int pass = MANY ? -1 : 0; pass < 3; ++pass) {
 #pragma unroll 1
     for (int s = from; s < to; ++s) {
-      const Segment seg = pass > 0 && s == from ? first : segment(p, s);
-      const Cut c = cut_of<MANY, ROWS, UNIT>(p, seg);
-      const int ranges = ranges_of(c.units, range);
-      if (pass == 0) {
+      const Segment seg = pass > (MANY ? -1 : 0) && s == from ? first : segment(p, s);
+      const Cut c = cut_of<MANY, ROWS, UNIT>(p, seg, s >= segments_of(p) - p.requests);
+      const int ranges = ranges_of(c.units, MANY ? min(range, max(1, c.units)) : range);
+      if (pass == (MANY ? -1 : 0)) {
         if (s == from) first = seg;
-        units += static_cast<float>(c.tiles) * static_cast<float>(c.units);
+        units += static_cast<float>(c.tiles) * static_cast<float>(c.units + c.least) * 0.5f;
+      } else if (pass == 0) {
+        if (c.tiles > 0)
+#pragma unroll 1
+          for (int i = 0; i < 8; ++i) {
+            const int cut = ranges_of(c.units, min(c.units, candidate(units, i))), length = ranges_of(c.units, cut);
+            atomicAdd(&plan.items[i], c.tiles * p.kv_heads * cut);
+            // on average a tile sees half of the units between the fewest and all
+            const float mean = c.tiles * p.kv_heads * (static_cast<float>(c.units + c.least) / (2 * length) + (c.least < c.units ? 0.5f : 0.f));
+            atomicAdd(&plan.filled[i], max(c.tiles * p.kv_heads, min(c.tiles * p.kv_heads * cut, static_cast<int>(mean + 0.5f))));
+            atomicMax(&plan.longest[i], length);
+          }
       } else if (pass == 1) {
         items += c.tiles * p.kv_heads * ranges;
       } else {
@@ -200,13 +228,26 @@ __device__ int schedule(const Attend& p, Plan& plan) {
         before += c.tiles * p.kv_heads * ranges;
       }
     }
-    if (pass == 0) {
+    if (pass == (MANY ? -1 : 0)) {
       plan.segments[threadIdx.x] = first;
       units = head_sum<64>(units);
       if (lane == 0) plan.units[wave] = units;
+      if (MANY && threadIdx.x < 8) plan.items[threadIdx.x] = plan.filled[threadIdx.x] = plan.longest[threadIdx.x] = 0;
       __syncthreads();
-      units = plan.units[0] + plan.units[1] + plan.units[2] + plan.units[3];
-      range = max(p.min_units[MANY], static_cast<int>(fminf(units * p.per_target[MANY], 1.0e9f)) + 1);
+      units = (plan.units[0] + plan.units[1] + plan.units[2] + plan.units[3]) * p.per_target[MANY];
+    }
+    if (MANY && pass == 0) {
+      __syncthreads();
+      float best = INFINITY;
+#pragma unroll 1
+      for (int i = 0; i < 8; ++i) {
+        const float a_block = plan.filled[i] / static_cast<float>(gridDim.x);
+        // rounds of items of the mean length, at least the longest
+        const float time = fmaxf(ceilf(a_block) * units / fmaxf(a_block, 1e-9f), plan.longest[i]) + ceilf(a_block) * kItem;
+        if (plan.items[i] <= p.items_max[1] && time < best) best = time, range = candidate(units, i);
+      }
+    } else if (pass == 0) {
+      range = max(p.min_units[MANY], static_cast<int>(fminf(units, 1.0e9f)) + 1);
     } else if (pass == 1) {
       int sum = items;
 #pragma unroll
@@ -231,6 +272,24 @@ __device__ int schedule(const Attend& p, Plan& plan) {
   return min(total, p.items_max[MANY]);
 }
 
+// The order of a segment's tiles of many rows: the last first, since in prompts it sees
+// the most, and in eight runs of every eighth tile, so that each XCD, which takes a run of
+// items, gets its share of long and short ones.
+__device__ __forceinline__ int tile_at(int place, int tiles) {
+  const int each = tiles >> 3, more = tiles & 7, longer = more * (each + 1);
+  int run, in;
+  if (place < longer) {
+    run = short_div(place, each + 1), in = place - run * (each + 1);
+  } else {
+    run = short_div(place - longer, max(1, each)), in = place - longer - run * each, run += more;
+  }
+  return tiles - 1 - (8 * in + run);
+}
+__device__ __forceinline__ int place_of(int tile, int tiles) {
+  const int back = tiles - 1 - tile, run = back & 7;
+  return run * (tiles >> 3) + min(run, tiles & 7) + (back >> 3);
+}
+
 struct Item {
   Segment seg;
   int head, tile;  // key head, tile of rows
@@ -252,19 +311,20 @@ __device__ Item item_of(const Attend& p, const Plan& plan, int item) {
   const int last = min(segments_of(p), (thread + 1) * each) - 1;
   for (int s = thread * each;; ++s) {
     const Segment seg = s == thread * each ? plan.segments[thread] : segment(p, s);
-    const Cut c = cut_of<MANY, ROWS, UNIT>(p, seg);
-    const int ranges = uniform(ranges_of(c.units, range)), tiles = uniform(c.tiles), items = tiles * p.kv_heads * ranges;
+    const Cut c = cut_of<MANY, ROWS, UNIT>(p, seg, s >= segments_of(p) - p.requests);
+    const int ranges = uniform(ranges_of(c.units, MANY ? min(range, max(1, c.units)) : range)), tiles = uniform(c.tiles), items = tiles * p.kv_heads * ranges;
     if (at < items || s >= last) {
       Item it;
       it.seg = {uniform(seg.token), uniform(seg.tokens), uniform(seg.lo),
                 uniform(seg.hi),    uniform(seg.request), uniform(seg.length), uniform(seg.group)};
       it.ranges = ranges;
       it.own = s >= segments_of(p) - p.requests;
-      const int across = uniform(short_div(at, max(1, tiles)));
+      const int across = uniform(short_div(at, max(1, tiles))), length = MANY ? uniform(ranges_of(c.units, max(1, ranges))) : range;
       it.tile = at - across * max(1, tiles);
+      if (MANY) it.tile = uniform(tile_at(it.tile, tiles));
       it.head = uniform(short_div(across, max(1, ranges)));
-      it.from = (it.seg.lo & ~15) + (across - it.head * max(1, ranges)) * range * UNIT;
-      it.to = min(it.seg.hi, it.from + range * UNIT);
+      it.from = (it.seg.lo & ~15) + (across - it.head * max(1, ranges)) * length * UNIT;
+      it.to = min(it.seg.hi, it.from + length * UNIT);
       return it;
     }
     at -= items;
@@ -667,8 +727,12 @@ __global__ __launch_bounds__(kThreads, D == 256 ? 1 : 2) void many_rows_kernel(A
   const int total = schedule<true, M::kRows, M::kKeys>(p, plan);
   // blocks with the same index modulo 8 share an XCD and its L2: neighbours in the order of items, which share keys
   const int xcd = blockIdx.x & 7, last = static_cast<int>(static_cast<int64_t>(total) * (xcd + 1) / 8);
-  for (int item = static_cast<int>(static_cast<int64_t>(total) * xcd / 8) + (blockIdx.x >> 3); item < last;
-       item += gridDim.x >> 3) {
+  // to and fro: a block that has had a long one of a round's items gets a short one of the next
+  const int across = gridDim.x >> 3, mine = blockIdx.x >> 3;
+  int round = static_cast<int>(static_cast<int64_t>(total) * xcd / 8);
+  for (bool back = false; round < last; round += across, back = !back) {
+    const int item = round + (back ? across - 1 - mine : mine);
+    if (item >= last) continue;  // whole block
     const Item it = item_of<true, M::kRows, M::kKeys>(p, plan, item);
     R rows;
     const int row = it.tile * M::kRows + 32 * wave + (lane & 31);
@@ -912,7 +976,8 @@ __global__ __launch_bounds__(kThreads) void join_kernel(Attend p) {
     many[which] = rows > kFew;
     const int tile_rows = many[which] ? Many<D>::kRows : kFew;
     tiles[which] = (rows + tile_rows - 1) / tile_rows;
-    first[which] = place.item + kv_head * place.ranges * tiles[which] + in / tile_rows;
+    const int tile = in / tile_rows;
+    first[which] = place.item + kv_head * place.ranges * tiles[which] + (many[which] ? place_of(tile, tiles[which]) : tile);
     row[which] = in % tile_rows;
     count[which] = place.ranges;
   }
