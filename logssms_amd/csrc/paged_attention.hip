@@ -38,7 +38,7 @@ typedef __attribute__((address_space(3))) void lds_void;
 
 constexpr int kFew = 32;        // rows of a segment up to which its waves split the keys instead of the rows
 constexpr int kThreads = 256;   // of every kernel here
-constexpr float kItem = 8.f;    // what an item of many rows costs beside its steps, in steps
+constexpr float kItem = 24.f;   // what an item of many rows costs beside its steps, in steps
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 constexpr float kLater = 8.0f;  // a maximum may lag by 2^8 before the sums are rescaled
 
@@ -113,31 +113,43 @@ __device__ __forceinline__ int group_of(const Attend& p, int request) {
 }
 __device__ __forceinline__ int segments_of(const Attend& p) { return p.requests + (p.shared ? p.num_groups : 0); }
 
+// Its loads do not wait for each other, but for those behind a search among groups and
+// a group's first and last token.
 __device__ __forceinline__ Segment segment(const Attend& p, int s) {
   Segment seg;
   const int shared = p.shared ? p.num_groups : 0;
-  if (s < shared) {
-    const int r0 = group_start(p, s), r1 = max(r0, group_start(p, s + 1));
-    seg.token = token_of(p, r0);
-    seg.tokens = max(0, token_of(p, r1) - seg.token);
-    seg.lo = 0;
-    seg.hi = shared_of(p, s);
-    seg.request = min(r0, p.requests - 1);
-    seg.length = 0;
-    seg.group = -1;
-  } else {
-    const int r = s - shared;
-    seg.token = token_of(p, r);
-    seg.tokens = max(0, token_of(p, r + 1) - seg.token);
-    seg.group = group_of(p, r);
-    seg.lo = seg.group < 0 ? 0 : shared_of(p, seg.group);
-    seg.length = static_cast<int>(load_index(p.lens, r, p.lens_is64));
-    seg.hi = clampi(seg.length, 0, p.capacity);
-    seg.request = r;
+  const bool own = s >= shared;
+  const int request = own ? s - shared : 0, g = !own ? s : p.num_groups > 1 ? group_of(p, request) : 0;
+  const int64_t length = load_index(p.lens, request, p.lens_is64);
+  int r0 = 0, r1 = p.requests, common = 0;
+  if (shared > 0 && g >= 0) {
+    r0 = group_start(p, g), r1 = group_start(p, g + 1);
+    common = shared_of(p, g);
   }
+  const bool in = shared > 0 && g >= 0 && r0 <= request && request < r1;
+  const int first = own ? request : r0, last = own ? request + 1 : max(r0, r1);
+  seg.token = token_of(p, first);
+  seg.tokens = max(0, token_of(p, last) - seg.token);
+  seg.lo = own && in ? common : 0;
+  seg.hi = own ? clampi(length, 0, p.capacity) : common;
+  seg.request = own ? request : min(r0, p.requests - 1);
+  seg.length = own ? static_cast<int>(length) : 0;
+  seg.group = own && in ? g : -1;
   return seg;
 }
 
+// The request of a token: the last that starts at or before it, found by a whole wave.
+__device__ __forceinline__ int request_of(const Attend& p, int token, int lane) {
+  int first = 0, count = p.requests;
+  while (count > 1) {
+    const int each = (count + 63) / 64, at = first + lane * each;
+    const bool before = lane * each < count && load_index(p.cu, at, p.cu_is64) <= token;
+    const int found = max(1, __popcll(__ballot(before)));
+    first += (found - 1) * each;
+    count = min(each, count - (found - 1) * each);
+  }
+  return first;
+}
 // Cut of a segment: tiles of `rows` rows and units of `unit` positions from a multiple of 16 on.
 struct Cut {
   int tiles, units;
@@ -153,14 +165,19 @@ __device__ __forceinline__ Cut cut_of(const Attend& p, const Segment& seg, bool 
 }
 
 // ------------------------------------------------------------------ schedule
-struct Plan {
+constexpr int kCandidates = 8;
+struct alignas(16) Plan {
   int base[kThreads];  // items before each thread's segments
   Segment segments[kThreads];  // each thread's first one: all, of up to kThreads
   float units[kThreads / 64];
   int count[kThreads / 64];
-  int each, range;     // segments of a thread; units of a range of keys
-  // of each candidate for the range: items, those that are not empty, the longest
-  int items[8], filled[8], longest[8];
+  int range;           // units of a range of keys
+};
+// What the choice of the range looks at: segments (their tiles in all heads, units, least
+// units); of each candidate the items, those that are not empty, the longest.
+struct Choice {
+  int segments, items[kCandidates], filled[kCandidates], longest[kCandidates];
+  int cuts[kThreads][3];
 };
 // One LDS array holds it all in a kernel with direct loads: beside a second one, the
 // compiler waits for every load in flight in front of each read.
@@ -183,43 +200,76 @@ __device__ __forceinline__ int ranges_of(int units, int range) { return short_di
 // same keys at a time, and the L2 no longer serves them: six prompts behind 8192 shared
 // positions took 431 us so, 320 in ranges of one length that all the work gives.)
 __device__ __forceinline__ int candidate(float units_a_block, int i) {
-  constexpr float kShares[8] = {0.f, 1.f, 0.8f, 0.667f, 0.5f, 0.4f, 0.333f, 0.25f};
-  return i == 0 ? 1 << 30 : static_cast<int>(units_a_block * kShares[i]) + 1;
+  // none is split; otherwise this part of what a block gets
+  const float share = i == 1 ? 1.f : i == 2 ? 0.8f : i == 3 ? 0.667f : i == 4 ? 0.5f : i == 5 ? 0.4f : i == 6 ? 0.333f : 0.25f;
+  return i == 0 ? 1 << 30 : static_cast<int>(units_a_block * share) + 1;
+}
+struct Outcome {
+  int items, filled, longest;
+  // one more segment, `tiles` in all heads, under a range
+  __device__ __forceinline__ void add(int tiles, int units, int least, int range) {
+    const int ranges = ranges_of(units, min(units, range)), length = ranges_of(units, ranges);
+    // on average a tile sees half of the units between the fewest and all, and half of its last range
+    const float mean = static_cast<float>(units + least) / static_cast<float>(2 * length) + (least < units ? 0.5f : 0.f);
+    items += tiles * ranges;
+    filled += max(tiles, min(tiles * ranges, static_cast<int>(static_cast<float>(tiles) * mean + 0.5f)));
+    longest = max(longest, length);
+  }
+  __device__ __forceinline__ void put(Choice& to, int i) const {
+    atomicAdd(&to.items[i], items);
+    atomicAdd(&to.filled[i], filled);
+    atomicMax(&to.longest[i], longest);
+  }
+};
+__device__ __forceinline__ int choose(const Attend& p, const Choice& choice, float units, int lane) {
+  int best = lane & (kCandidates - 1);
+  const float a_block = static_cast<float>(choice.filled[best]) / static_cast<float>(gridDim.x), rounds = ceilf(a_block);
+  // rounds of items of the mean length, at least the longest
+  float time = fmaxf(rounds * units / fmaxf(a_block, 1e-9f), static_cast<float>(choice.longest[best])) + rounds * kItem;
+  if (choice.items[best] > p.items_max[1] && best > 0) time = INFINITY;
+#pragma unroll
+  for (int off = 1; off < kCandidates; off <<= 1) {
+    const float other = __shfl_xor(time, off, 64);
+    const int which = __shfl_xor(best, off, 64);
+    if (other < time || (other == time && which < best)) time = other, best = which;
+  }
+  return candidate(units, best);
 }
 
-// Counts the items of the launch: thread i answers for `each` consecutive
-// segments.  A range of keys of few rows is as long as it has to be for `target` items.
-// Block 0 notes for the joining kernel where each segment's items lie.
+// Counts the items of the launch: thread i answers for the segments i, i + kThreads, ...,
+// and the items lie thread by thread.  A range of keys of few rows is as long as it has
+// to be for so many items as waves run at once.  Block 0 notes for the joining kernel
+// where each segment's items lie.
 template <bool MANY, int ROWS, int UNIT>
-__device__ int schedule(const Attend& p, Plan& plan) {
+__device__ int schedule(const Attend& p, Plan& plan, Choice* choice) {
   const int n = segments_of(p), lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const int each = (n + kThreads - 1) / kThreads;
-  const int from = threadIdx.x * each, to = min(n, from + each);
   float units = 0.f;  // the same in all blocks; its rounding is in the bound of the items
   int items = 0, before = 0, total = 0, range = 1;
-  Segment first{};
+  Segment first{}, second{};  // of this thread
+  if (MANY) {
+    if (threadIdx.x < sizeof(Choice) / 4 - 3 * kThreads) reinterpret_cast<int*>(choice)[threadIdx.x] = 0;
+    __syncthreads();
+  }
   // units, items, places: one loop, so that the code of segment() is there once
 #pragma unroll 1
-  for (int pass = MANY ? -1 : 0; pass < 3; ++pass) {
+  for (int pass = 0; pass < 3; ++pass) {
 #pragma unroll 1
-    for (int s = from; s < to; ++s) {
-      const Segment seg = pass > (MANY ? -1 : 0) && s == from ? first : segment(p, s);
+    for (int s = threadIdx.x; s < n; s += kThreads) {
+      const int which = s / kThreads;
+      Segment seg = which == 0 ? first : second;
+      if (pass == 0 || which > 1) seg = segment(p, s);
       const Cut c = cut_of<MANY, ROWS, UNIT>(p, seg, s >= segments_of(p) - p.requests);
       const int ranges = ranges_of(c.units, MANY ? min(range, max(1, c.units)) : range);
-      if (pass == (MANY ? -1 : 0)) {
-        if (s == from) first = seg;
+      if (pass == 0) {
+        if (which == 0) first = seg;
+        if (which == 1) second = seg;
         units += static_cast<float>(c.tiles) * static_cast<float>(c.units + c.least) * 0.5f;
-      } else if (pass == 0) {
-        if (c.tiles > 0)
-#pragma unroll 1
-          for (int i = 0; i < 8; ++i) {
-            const int cut = ranges_of(c.units, min(c.units, candidate(units, i))), length = ranges_of(c.units, cut);
-            atomicAdd(&plan.items[i], c.tiles * p.kv_heads * cut);
-            // on average a tile sees half of the units between the fewest and all
-            const float mean = c.tiles * p.kv_heads * (static_cast<float>(c.units + c.least) / (2 * length) + (c.least < c.units ? 0.5f : 0.f));
-            atomicAdd(&plan.filled[i], max(c.tiles * p.kv_heads, min(c.tiles * p.kv_heads * cut, static_cast<int>(mean + 0.5f))));
-            atomicMax(&plan.longest[i], length);
+        if (MANY && c.tiles > 0) {
+          const int to = atomicAdd(&choice->segments, 1);
+          if (to < kThreads) {
+            choice->cuts[to][0] = c.tiles * p.kv_heads, choice->cuts[to][1] = c.units, choice->cuts[to][2] = c.least;
           }
+        }
       } else if (pass == 1) {
         items += c.tiles * p.kv_heads * ranges;
       } else {
@@ -228,26 +278,28 @@ __device__ int schedule(const Attend& p, Plan& plan) {
         before += c.tiles * p.kv_heads * ranges;
       }
     }
-    if (pass == (MANY ? -1 : 0)) {
+    if (pass == 0) {
       plan.segments[threadIdx.x] = first;
       units = head_sum<64>(units);
       if (lane == 0) plan.units[wave] = units;
-      if (MANY && threadIdx.x < 8) plan.items[threadIdx.x] = plan.filled[threadIdx.x] = plan.longest[threadIdx.x] = 0;
       __syncthreads();
       units = (plan.units[0] + plan.units[1] + plan.units[2] + plan.units[3]) * p.per_target[MANY];
-    }
-    if (MANY && pass == 0) {
-      __syncthreads();
-      float best = INFINITY;
-#pragma unroll 1
-      for (int i = 0; i < 8; ++i) {
-        const float a_block = plan.filled[i] / static_cast<float>(gridDim.x);
-        // rounds of items of the mean length, at least the longest
-        const float time = fmaxf(ceilf(a_block) * units / fmaxf(a_block, 1e-9f), plan.longest[i]) + ceilf(a_block) * kItem;
-        if (plan.items[i] <= p.items_max[1] && time < best) best = time, range = candidate(units, i);
+      if constexpr (MANY) {
+        // of more segments than that, every one is split alike
+        if (choice->segments <= kThreads) {
+          const int i = threadIdx.x & (kCandidates - 1);
+          Outcome outcome{0, 0, 0};
+          for (int e = threadIdx.x / kCandidates; e < choice->segments; e += kThreads / kCandidates)
+            outcome.add(choice->cuts[e][0], choice->cuts[e][1], choice->cuts[e][2], candidate(units, i));
+          if (outcome.items > 0) outcome.put(*choice, i);
+          __syncthreads();
+          range = choose(p, *choice, units, lane);
+        } else {
+          range = candidate(units, 1);
+        }
+      } else {
+        range = max(p.min_units[MANY], static_cast<int>(fminf(units, 1.0e9f)) + 1);
       }
-    } else if (pass == 0) {
-      range = max(p.min_units[MANY], static_cast<int>(fminf(units, 1.0e9f)) + 1);
     } else if (pass == 1) {
       int sum = items;
 #pragma unroll
@@ -264,7 +316,7 @@ __device__ int schedule(const Attend& p, Plan& plan) {
         total += plan.count[w];
       }
       plan.base[threadIdx.x] = before;
-      if (threadIdx.x == 0) plan.each = each, plan.range = range;
+      if (threadIdx.x == 0) plan.range = range;
       if (blockIdx.x > 0) break;
     }
   }
@@ -302,23 +354,22 @@ struct Item {
 template <bool MANY, int ROWS, int UNIT>
 __device__ Item item_of(const Attend& p, const Plan& plan, int item) {
   static_assert(kThreads == 256, "four bases a lane");
-  const int lane = threadIdx.x & 63, each = uniform(plan.each), range = uniform(plan.range);
+  const int lane = threadIdx.x & 63, range = uniform(plan.range), n = segments_of(p);
   int thread = -1;  // the last whose base is at most `item`
 #pragma unroll
   for (int i = 0; i < 4; ++i) thread += __popcll(__ballot(plan.base[4 * lane + i] <= item));
   thread = uniform(thread);
   int at = item - uniform(plan.base[thread]);
-  const int last = min(segments_of(p), (thread + 1) * each) - 1;
-  for (int s = thread * each;; ++s) {
-    const Segment seg = s == thread * each ? plan.segments[thread] : segment(p, s);
+  for (int s = thread;; s += kThreads) {
+    const Segment seg = s == thread ? plan.segments[thread] : segment(p, s);
     const Cut c = cut_of<MANY, ROWS, UNIT>(p, seg, s >= segments_of(p) - p.requests);
     const int ranges = uniform(ranges_of(c.units, MANY ? min(range, max(1, c.units)) : range)), tiles = uniform(c.tiles), items = tiles * p.kv_heads * ranges;
-    if (at < items || s >= last) {
+    if (at < items || s + kThreads >= n) {
       Item it;
       it.seg = {uniform(seg.token), uniform(seg.tokens), uniform(seg.lo),
                 uniform(seg.hi),    uniform(seg.request), uniform(seg.length), uniform(seg.group)};
       it.ranges = ranges;
-      it.own = s >= segments_of(p) - p.requests;
+      it.own = s >= n - p.requests;
       const int across = uniform(short_div(at, max(1, tiles))), length = MANY ? uniform(ranges_of(c.units, max(1, ranges))) : range;
       it.tile = at - across * max(1, tiles);
       if (MANY) it.tile = uniform(tile_at(it.tile, tiles));
@@ -539,7 +590,7 @@ struct Rows {
   f32x16 o[D / 32];
   float m, l;    // maximum of the scaled scores (base 2), and this lane's part of the sum
   int limit;     // positions before it are visible to the row
-  int least, most;  // of the wave's rows
+  int least;     // of the wave's rows
 
   __device__ __forceinline__ void clear() {
 #pragma unroll
@@ -549,8 +600,8 @@ struct Rows {
     m = -INFINITY, l = 0.f;
   }
 
-  // Row `row` of the segment: its token and head, its queries, the positions visible to it.
-  __device__ __forceinline__ void load(const Attend& p, const Item& it, int row, int lane) {
+  // Row `row` of the segment: its queries.
+  __device__ __forceinline__ void fetch(const Attend& p, const Item& it, int row, int lane) {
     const bool there = row < it.seg.tokens * p.per;
     const int in = there ? p.by_per.div(row) : 0, token = it.seg.token + in;
     const int head = it.head * p.per + (there ? row - in * p.per : 0);
@@ -560,20 +611,38 @@ struct Rows {
       const uint4 raw = there ? *reinterpret_cast<const uint4*>(from + 16 * i) : make_uint4(0, 0, 0, 0);
       q[i] = __builtin_bit_cast(Frag, raw);
     }
-    limit = 0;
-    if (there) {
-      int length = it.seg.length, behind = it.seg.tokens - 1 - in;  // tokens of the request behind this one
-      if (!it.own) {
-        const int r = p.cu ? static_cast<int>(find_sequence(p.cu, p.cu_is64, p.requests, token)) : token;
-        length = static_cast<int>(load_index(p.lens, r, p.lens_is64));
-        behind = token_of(p, r + 1) - 1 - token;
-      }
-      limit = clampi(static_cast<int64_t>(length) - behind, 0, it.seg.hi);
-    }
-    int a = there ? limit : INT32_MAX, b = limit;
+  }
+  // The positions visible to it.
+  __device__ __forceinline__ void see(const Attend& p, const Item& it, int row, int lane) {
+    const bool there = row < it.seg.tokens * p.per;
+    const int in = there ? p.by_per.div(row) : 0, token = it.seg.token + in;
+    int length = it.seg.length, behind = it.seg.tokens - 1 - in;  // tokens of the request behind this one
+    if (!it.own) {  // uniform
+      int r = token, next = token + 1;
+      if (p.cu) {
+        // the requests of the wave's tokens lie behind that of its first one: their ends in the lanes, searched there
+        const int first = request_of(p, uniform(token), lane);
+        const int end = token_of(p, min(first + 1 + lane, p.requests));
+        int at = 0;
 #pragma unroll
-    for (int off = 16; off > 0; off >>= 1) a = min(a, __shfl_xor(a, off, 64)), b = max(b, __shfl_xor(b, off, 64));
-    least = uniform(a), most = uniform(b);
+        for (int half = 32; half > 0; half >>= 1)
+          if (__shfl(end, at + half - 1, 64) <= token) at += half;
+        r = first + at, next = __shfl(end, at, 64);
+        if (__any(next <= token)) {  // more requests than lanes (most of them empty)
+          r = static_cast<int>(find_sequence(p.cu, p.cu_is64, p.requests, token));
+          next = token_of(p, r + 1);
+        }
+      }
+      r = min(r, p.requests - 1);
+      length = static_cast<int>(load_index(p.lens, r, p.lens_is64));
+      behind = next - 1 - token;
+    }
+    const int seen = clampi(static_cast<int64_t>(length) - behind, 0, it.seg.hi);
+    limit = there ? seen : 0;
+    int a = there ? limit : INT32_MAX;
+#pragma unroll
+    for (int off = 16; off > 0; off >>= 1) a = min(a, __shfl_xor(a, off, 64));
+    least = uniform(a);
   }
 
   // The i-th fragment of 32 TILES positions.
@@ -723,8 +792,9 @@ __global__ __launch_bounds__(kThreads, D == 256 ? 1 : 2) void many_rows_kernel(A
   NotFinite<D>& bad = *reinterpret_cast<NotFinite<D>*>(lds + M::kLds);
   Plan& plan = *reinterpret_cast<Plan*>(lds + M::kLds + sizeof(bad));
   int* least = reinterpret_cast<int*>(lds + M::kLds + sizeof(bad) + sizeof(Plan));  // of each wave's rows
+  static_assert(sizeof(Choice) <= M::kLds, "in the place of the rings, before they are used");
   const int lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6);
-  const int total = schedule<true, M::kRows, M::kKeys>(p, plan);
+  const int total = schedule<true, M::kRows, M::kKeys>(p, plan, reinterpret_cast<Choice*>(lds));
   // blocks with the same index modulo 8 share an XCD and its L2: neighbours in the order of items, which share keys
   const int xcd = blockIdx.x & 7, last = static_cast<int>(static_cast<int64_t>(total) * (xcd + 1) / 8);
   // to and fro: a block that has had a long one of a round's items gets a short one of the next
@@ -736,8 +806,7 @@ __global__ __launch_bounds__(kThreads, D == 256 ? 1 : 2) void many_rows_kernel(A
     const Item it = item_of<true, M::kRows, M::kKeys>(p, plan, item);
     R rows;
     const int row = it.tile * M::kRows + 32 * wave + (lane & 31);
-    rows.load(p, it, row, lane);
-    rows.clear();
+    rows.fetch(p, it, row, lane);
     // nothing behind the last position that a row of the tile sees
     const int last_token = min(it.seg.tokens - 1, static_cast<int>(p.by_per.div(it.tile * M::kRows + M::kRows - 1)));
     int to = it.to;
@@ -760,8 +829,6 @@ __global__ __launch_bounds__(kThreads, D == 256 ? 1 : 2) void many_rows_kernel(A
     auto key_at = [](int tile) __attribute__((always_inline)) { return tile % M::kKeyRing * M::kTile; };
     auto value_at = [](int slot) __attribute__((always_inline)) { return (M::kKeyRing + slot) * M::kTile; };
     lds_barrier();  // the last item's rings are free
-    bad.clear(threadIdx.x, kThreads);
-    if (lane == 0) least[wave] = rows.least;
 #pragma unroll
     for (int tile = 0; tile < M::kKeyRing; ++tile) {  // keys of tiles 0 to 3, beside the last two values of 0 and 1
       if (!of_values) {
@@ -773,6 +840,10 @@ __global__ __launch_bounds__(kThreads, D == 256 ? 1 : 2) void many_rows_kernel(A
         feed[kBoth ? 1 : 0].load_all(share + value_at(tile - 2));
       }
     }
+    bad.clear(threadIdx.x, kThreads);
+    rows.clear();
+    rows.see(p, it, row, lane);
+    if (lane == 0) least[wave] = rows.least;
     wait_loads<2 * M::kLoads>();
     lds_barrier();  // the keys of tiles 0 and 1 are there
     const int all_see = uniform(min(min(least[0], least[1]), min(least[2], least[3])));
@@ -864,17 +935,16 @@ __global__ __launch_bounds__(kThreads, Few<D>::kBlocks) void few_rows_kernel(Att
   char* const values = keys + F::kHalf;
   NotFinite<D>& bad = reinterpret_cast<NotFinite<D>*>(lds + 4 * F::kWave)[wave];
   Plan& plan = *reinterpret_cast<Plan*>(lds + 4 * (F::kWave + sizeof(bad)));
-  const int total = schedule<false, kFew, 32>(p, plan);
+  const int total = schedule<false, kFew, 32>(p, plan, nullptr);
   const int of_k = lane_k<D>(lane), of_v = lane_v<D>(lane);
   // neighbours in the order of items share keys or a table: side by side in a block
   for (int item = blockIdx.x * 4 + wave; item < total; item += gridDim.x * 4) {
     const Item it = item_of<false, kFew, 32>(p, plan, item);
     const int end = it.seg.hi, steps = (it.to - it.from + 31) / 32;
     Pages pages;
-    pages.find(p, it.seg.request, it.from + 16 * lane, end);
     R rows;
-    rows.load(p, it, lane & 31, lane);
-    rows.clear();
+    rows.fetch(p, it, lane & 31, lane);
+    pages.find(p, it.seg.request, it.from + 16 * lane, end);
     Feed<D> k_feed, v_feed;
     k_feed.start(p.k, it.head, false, lane);
     v_feed.start(p.v, it.head, true, lane);
@@ -896,6 +966,8 @@ __global__ __launch_bounds__(kThreads, Few<D>::kBlocks) void few_rows_kernel(Att
     };
     load_k(0);
     load_v(0);
+    rows.clear();
+    rows.see(p, it, lane & 31, lane);
     bool searched = false;
     for (int step = 0; step < steps; ++step) {
       f32x16 s[1];
@@ -934,18 +1006,6 @@ __global__ __launch_bounds__(kThreads, Few<D>::kBlocks) void few_rows_kernel(Att
 }
 
 // ------------------------------------------------------------------ join
-// The request of a token: the last that starts at or before it, found by a whole wave.
-__device__ __forceinline__ int request_of(const Attend& p, int token, int lane) {
-  int first = 0, count = p.requests;
-  while (count > 1) {
-    const int each = (count + 63) / 64, at = first + lane * each;
-    const bool before = lane * each < count && load_index(p.cu, at, p.cu_is64) <= token;
-    const int found = max(1, __popcll(__ballot(before)));
-    first += (found - 1) * each;
-    count = min(each, count - (found - 1) * each);
-  }
-  return first;
-}
 // WAVES waves a row: the pieces of the row's shared and own segments by turns, 64 of
 // a wave's at a time: a lane looks up one piece, then all lanes add the pieces.
 template <class T, int D, int WAVES>
@@ -1066,9 +1126,9 @@ struct Sizes {
   int64_t sums[2], stats[2], places, bytes;  // offsets
 };
 
-// Bounds from what the host knows.  Each of a kind's items is one of `target` (a
-// range of keys is at least all units over it, but for the rounding of that sum) or
-// the last range of a tile.
+// Bounds from what the host knows.  Each item of few rows is one of `target` (a range
+// of keys is at least all units over it, but for the rounding of that sum) or the
+// last range of a tile; those of many rows may be cut into four times as many.
 Sizes sizes_of(int64_t tokens, int64_t requests, int64_t groups, int64_t heads, int64_t kv_heads, int64_t dim,
                bool varlen) {
   Sizes z{};
@@ -1079,7 +1139,7 @@ Sizes sizes_of(int64_t tokens, int64_t requests, int64_t groups, int64_t heads, 
   z.target[1] = kCus * (dim == 256 ? 1 : 2);                       // blocks
   const int64_t few_tiles = requests + groups, many_tiles = sets * (rows / 128 + std::min(requests + groups, rows / kFew + 1));
   z.items[0] = z.few ? z.target[0] + z.target[0] / 64 + few_tiles * kv_heads : 0;
-  z.items[1] = z.many ? z.target[1] + z.target[1] / 64 + many_tiles * kv_heads : 0;
+  z.items[1] = z.many ? 4 * z.target[1] + many_tiles * kv_heads : 0;
   int64_t at = 0;
   auto take = [&](int64_t bytes) {
     const int64_t from = at;
