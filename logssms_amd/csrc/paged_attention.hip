@@ -165,7 +165,7 @@ __device__ __forceinline__ Cut cut_of(const Attend& p, const Segment& seg, bool 
 }
 
 // ------------------------------------------------------------------ schedule
-constexpr int kCandidates = 8;
+constexpr int kCandidates = 16;
 struct alignas(16) Plan {
   int base[kThreads];  // items before each thread's segments
   Segment segments[kThreads];  // each thread's first one: all, of up to kThreads
@@ -193,16 +193,16 @@ __device__ __forceinline__ int short_div(int n, int d) {
 }
 __device__ __forceinline__ int ranges_of(int units, int range) { return short_div(units + range - 1, range); }
 
-// The range of keys for items of many rows, of eight candidates the one under which the
+// The range of keys for items of many rows, of sixteen candidates the one under which the
 // last block should end first: items are taken in rounds, a block one of each round,
 // and each costs kItem units to begin and to store.  (Equal parts of one line of all
 // the work, whatever tiles they cut, balance better, but then no two blocks read the
 // same keys at a time, and the L2 no longer serves them: six prompts behind 8192 shared
 // positions took 431 us so, 320 in ranges of one length that all the work gives.)
 __device__ __forceinline__ int candidate(float units_a_block, int i) {
-  // none is split; otherwise this part of what a block gets
-  const float share = i == 1 ? 1.f : i == 2 ? 0.8f : i == 3 ? 0.667f : i == 4 ? 0.5f : i == 5 ? 0.4f : i == 6 ? 0.333f : 0.25f;
-  return i == 0 ? 1 << 30 : static_cast<int>(units_a_block * share) + 1;
+  // none is split; otherwise 2, 1.71, 1.5, 1.33, 1.2 .. 0.25 times what a block gets
+  const float shares = i < 6 ? 0.5f + (i - 1) / 12.f : 0.91f + (i - 6) * (i - 6) * 0.038f;
+  return i == 0 ? 1 << 30 : static_cast<int>(units_a_block / shares) + 1;
 }
 struct Outcome {
   int items, filled, longest;
