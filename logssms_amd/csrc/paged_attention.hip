@@ -399,20 +399,25 @@ template <> struct Op<f16> {
   }
 };
 
-// Where 64 subtiles of 16 positions lie, one in each lane, looked up together so
-// that the steps' loads wait for no table.
-struct Pages {
-  int id, in;  // page (-1: none), first position inside it
-  // lane l: the positions from `at` on (a multiple of 16) of a request's row of the table
-  __device__ __forceinline__ void find(const Attend& p, int request, int at, int end) {
-    id = -1, in = 0;
-    if (at < end) {
-      const uint32_t index = p.page.div(at);
-      in = at - static_cast<int>(index * p.page.d);
-      const int64_t entry = static_cast<int64_t>(request) * p.table_row + index;
-      id = static_cast<int>(load_index(p.table, entry, p.table_is64));
-      if (id < 0 || id >= p.pages) id = -1;
-    }
+// Where 16 positions from `at` on (a multiple of 16) lie: page (-1: none) and place inside it.
+struct Spot {
+  int page, in;
+};
+__device__ __forceinline__ Spot find(const Attend& p, int request, int at, int end) {
+  if (at >= end) return {-1, 0};
+  const uint32_t index = p.page.div(at);
+  const int64_t entry = static_cast<int64_t>(request) * p.table_row + index;
+  const int id = static_cast<int>(load_index(p.table, entry, p.table_is64));
+  return {id < 0 || id >= p.pages ? -1 : id, at - static_cast<int>(index * p.page.d)};
+}
+// The same of 64 times 16 positions, one in each lane, in bytes of a cache, looked up
+// together so that the steps' loads wait for no table.
+struct Spots {
+  int low, high;  // high kNone: nowhere
+  static constexpr int kNone = INT32_MIN;
+  __device__ __forceinline__ void set(Spot spot, int64_t page, int64_t token) {
+    const int64_t bytes = spot.page * page + spot.in * token;
+    low = static_cast<int>(bytes), high = spot.page < 0 ? kNone : static_cast<int>(bytes >> 32);
   }
 };
 
@@ -448,6 +453,7 @@ struct Feed {
   uint32_t from[kLoads];  // the lane's piece of each load, bytes behind the first position's
   const char* at;        // what aim() has found: the first position, the bytes that may be read
   uint32_t bytes;
+  int valid;
 
   __device__ __forceinline__ void start(const Cache& c, int of, bool values, int lane) {
     using L = Tile<D>;
@@ -460,13 +466,20 @@ struct Feed {
       from[i] = r * static_cast<uint32_t>(token) + 16 * (piece ^ (values ? L::swizzle_v(r) : L::swizzle_k(r)));
     }
   }
-  // The subtile in lane `which` of `pages`, of which `there` positions (or more than 16)
-  // may be read: zeros behind them, and for a page outside of the cache.
-  __device__ __forceinline__ void aim(const Pages& pages, int which, int there) {
-    const int id = __builtin_amdgcn_readlane(pages.id, which), in = __builtin_amdgcn_readlane(pages.in, which);
-    const int valid = id < 0 ? 0 : there < 16 ? there : 16;
-    at = head + id * page + in * token;
-    bytes = valid > 0 ? (valid - 1) * static_cast<uint32_t>(token) + Tile<D>::kRow : 0;
+  // The 16 positions in lane `which` of `spots`, of which `there` (or more than 16) may
+  // be read: zeros behind them, and for a page outside of the cache.
+  // In two halves, to stand between matrix instructions.
+  __device__ __forceinline__ void aim_at(const Spots& spots, int which, int there) {
+    const int low = __builtin_amdgcn_readlane(spots.low, which), high = __builtin_amdgcn_readlane(spots.high, which);
+    at = head + (static_cast<int64_t>(high) << 32 | static_cast<uint32_t>(low));
+    valid = high == Spots::kNone ? 0 : there;
+  }
+  __device__ __forceinline__ void aim_bytes() {
+    bytes = valid > 0 ? ((valid < 16 ? valid : 16) - 1) * static_cast<uint32_t>(token) + Tile<D>::kRow : 0;
+  }
+  __device__ __forceinline__ void aim(const Spots& spots, int which, int there) {
+    aim_at(spots, which, there);
+    aim_bytes();
   }
   __device__ __forceinline__ void load(int i, char* lds) const {
     dma16(at, bytes, from[i], lds + 1024 * i);
@@ -519,7 +532,15 @@ template <class V> __device__ __forceinline__ V here(V v) {
 // Instructions stay on their side of it.
 __device__ __forceinline__ void in_order() { __builtin_amdgcn_sched_barrier(0); }
 
-__device__ __forceinline__ float other_half(float v) { return __shfl_xor(v, 32, 64); }
+// Of this lane's value and that of the lane 32 before or behind it.
+__device__ __forceinline__ float max_of_halves(float v) {
+  const auto halves = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  return fmaxf(__uint_as_float(halves[0]), __uint_as_float(halves[1]));
+}
+__device__ __forceinline__ float sum_of_halves(float v) {
+  const auto halves = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  return __uint_as_float(halves[0]) + __uint_as_float(halves[1]);
+}
 
 // A weight of zero does not silence a value that is not finite.  Where rows of an
 // item do not see all of a tile's positions, such values are taken out of it, and
@@ -691,7 +712,7 @@ struct Rows {
   }
   // The row's largest score (base 2) from the largest of the lane's own.
   __device__ __forceinline__ float of_row(const Attend& p, float top) const {
-    return fmaxf(top, other_half(top)) * p.factor;
+    return max_of_halves(top) * p.factor;
   }
   // The maximum raised to `top`, where that is more than 2^8 above it: fp32 sums have room for less.
   __device__ __forceinline__ void raise(float top) {
@@ -713,13 +734,16 @@ struct Rows {
     for (int i = first; i < last; ++i) {
       float& x = reinterpret_cast<float*>(&s[i / 16])[i % 16];
       x = fast_exp2(fmaf(x, p.factor, -less));
-      l += x;
       if (i & 1) {
         const uint32_t pair = out_pack2<T>(reinterpret_cast<float*>(&s[i / 16])[i % 16 - 1], x);
         reinterpret_cast<uint32_t*>(&w[i / 8])[i % 8 / 2] = here(pair);
       }
     }
-    l = here(l);
+  }
+  // Their sum, unrounded.
+  template <int TILES> __device__ __forceinline__ void add(int first, int last, const f32x16 (&s)[TILES]) {
+#pragma unroll
+    for (int i = first; i < last; ++i) l += s[i / 16][i % 16];
   }
   __device__ __forceinline__ float subtracted() const { return m == -INFINITY ? 0.f : m; }
   // O^T += V^T P^T of 32 TILES positions, as above.
@@ -745,7 +769,7 @@ struct Rows {
   }
   // Row `row` of the segment out: finished, or as a piece to be joined, row `to` of its kind's sums.
   __device__ __forceinline__ void put(const Attend& p, const Item& it, int row, int kind, int64_t to, int lane) {
-    const float sum = l + other_half(l);
+    const float sum = sum_of_halves(l);
     if (row >= it.seg.tokens * p.per) return;
     if (whole(it)) {
       const int in = p.by_per.div(row), token = it.seg.token + in, head = it.head * p.per + row - in * p.per;
@@ -818,12 +842,20 @@ __global__ __launch_bounds__(kThreads, D == 256 ? 1 : 2) void many_rows_kernel(A
     const bool of_values = !kBoth && wave >= 2;
     const int sub = kBoth ? wave : wave & 1;
     Feed<D> feed[kBoth ? 2 : 1];
-    Pages pages[kBoth ? 2 : 1];
+    Spots spots[kBoth ? 2 : 1];
     feed[0].start(of_values ? p.v : p.k, it.head, of_values, lane);
     if constexpr (kBoth) feed[1].start(p.v, it.head, true, lane);
+    auto spot = [&](int which, int tile) __attribute__((always_inline)) {
+      if ((tile & 63) == 0)
+        spots[which].set(find(p, it.seg.request, it.from + (tile + lane) * M::kKeys + 16 * sub, end), feed[which].page,
+                         feed[which].token);
+    };
+    auto there = [&](int tile) __attribute__((always_inline)) {
+      return tile < steps ? end - (it.from + tile * M::kKeys + 16 * sub) : 0;
+    };
     auto aim = [&](int which, int tile) __attribute__((always_inline)) {
-      if ((tile & 63) == 0) pages[which].find(p, it.seg.request, it.from + (tile + lane) * M::kKeys + 16 * sub, end);
-      feed[which].aim(pages[which], tile & 63, tile < steps ? end - (it.from + tile * M::kKeys + 16 * sub) : 0);
+      spot(which, tile);
+      feed[which].aim(spots[which], tile & 63, there(tile));
     };
     char* const share = lds + sub * 32 * D;
     auto key_at = [](int tile) __attribute__((always_inline)) { return tile % M::kKeyRing * M::kTile; };
@@ -882,18 +914,22 @@ __global__ __launch_bounds__(kThreads, D == 256 ? 1 : 2) void many_rows_kernel(A
       const int later = slot == 0 ? 2 : slot - 1;
       char* to0 = share + (of_values ? value_at(later) : key_at(step));
       char* to1 = share + value_at(later);
-      aim(0, of_values ? step + 2 : step + 4);
-      if constexpr (kBoth) aim(1, step + 2);
+      const int ahead = of_values ? step + 2 : step + 4;
+      spot(0, ahead);
+      if constexpr (kBoth) spot(1, step + 2);
       const int k_next = key_at(step + 2) + of_k;
       top = -INFINITY;
       rows.template values<kTiles>(lds, v_at, values, w, [&](int i) __attribute__((always_inline)) {
         // behind the first quarter: the scores' last matrix instruction is done by then
         constexpr int kFrom = kMmas / 4, kEach = (kScores + kMmas - kFrom - 1) / (kMmas - kFrom);
-        constexpr int kIssue = M::kLoads;
-        if (i < kIssue) {
-          if (!kBoth || i < kIssue / 2) feed[0].load(i, to0);
-          else feed[kBoth ? 1 : 0].load(i - kIssue / 2, to1);
-        }
+        constexpr int kIssue = M::kLoads, kHalf = kBoth ? kIssue / 2 : kIssue;
+        if (i == 0) feed[0].aim_at(spots[0], ahead & 63, there(ahead));
+        if (i == 1) feed[0].aim_bytes();
+        if (kBoth && i == 2) feed[kBoth].aim_at(spots[kBoth], (step + 2) & 63, there(step + 2));
+        if (kBoth && i == 3) feed[kBoth].aim_bytes();
+        if (i >= 2 && i < 2 + kHalf) feed[0].load(i - 2, to0);
+        if (kBoth && i >= 4 && i < 4 + kHalf) feed[kBoth].load(i - 4, to1);
+        rows.template add<kTiles>(i * kScores / kMmas, (i + 1) * kScores / kMmas, now);
 #pragma unroll
         for (int e = 0; e < kEach; ++e)
           if (i >= kFrom && (i - kFrom) * kEach + e < kScores) larger(next, (i - kFrom) * kEach + e);
@@ -941,27 +977,31 @@ __global__ __launch_bounds__(kThreads, Few<D>::kBlocks) void few_rows_kernel(Att
   for (int item = blockIdx.x * 4 + wave; item < total; item += gridDim.x * 4) {
     const Item it = item_of<false, kFew, 32>(p, plan, item);
     const int end = it.seg.hi, steps = (it.to - it.from + 31) / 32;
-    Pages pages;
     R rows;
     rows.fetch(p, it, lane & 31, lane);
-    pages.find(p, it.seg.request, it.from + 16 * lane, end);
+    Spot spot = find(p, it.seg.request, it.from + 16 * lane, end);
     Feed<D> k_feed, v_feed;
     k_feed.start(p.k, it.head, false, lane);
     v_feed.start(p.v, it.head, true, lane);
+    Spots k_spots, v_spots;
     // 32 steps to a lookup; a step's keys are loaded before its values
     auto load_k = [&](int step) __attribute__((always_inline)) {
-      if ((step & 31) == 0 && step > 0) pages.find(p, it.seg.request, it.from + 32 * step + 16 * lane, end);
+      if ((step & 31) == 0) {
+        if (step > 0) spot = find(p, it.seg.request, it.from + 32 * step + 16 * lane, end);
+        k_spots.set(spot, k_feed.page, k_feed.token);
+        v_spots.set(spot, v_feed.page, v_feed.token);
+      }
       const int there = step < steps ? end - (it.from + 32 * step) : 0, which = 2 * (step & 31);
-      k_feed.aim(pages, which, there);
+      k_feed.aim(k_spots, which, there);
       k_feed.load_all(keys);
-      k_feed.aim(pages, which + 1, there - 16);
+      k_feed.aim(k_spots, which + 1, there - 16);
       k_feed.load_all(keys + 32 * D);
     };
     auto load_v = [&](int step) __attribute__((always_inline)) {
       const int there = step < steps ? end - (it.from + 32 * step) : 0, which = 2 * (step & 31);
-      v_feed.aim(pages, which, there);
+      v_feed.aim(v_spots, which, there);
       v_feed.load_all(values);
-      v_feed.aim(pages, which + 1, there - 16);
+      v_feed.aim(v_spots, which + 1, there - 16);
       v_feed.load_all(values + 32 * D);
     };
     load_k(0);
@@ -986,6 +1026,7 @@ __global__ __launch_bounds__(kThreads, Few<D>::kBlocks) void few_rows_kernel(Att
       for (int e = 1; e < 16; ++e) top = fmaxf(top, s[0][e]);
       rows.raise(rows.of_row(p, top));
       rows.template weights<1>(p, 0, 16, rows.subtracted(), s, w);
+      rows.template add<1>(0, 16, s);
       wait_loads<F::kLoads>();
       if (rows.template partly<1>(it.seg, at)) {
         if (!searched) bad.clear(lane, 64);
