@@ -38,7 +38,8 @@ typedef __attribute__((address_space(3))) void lds_void;
 
 constexpr int kFew = 32;        // rows of a segment up to which its waves split the keys instead of the rows
 constexpr int kThreads = 256;   // of every kernel here
-constexpr float kItem = 24.f;   // what an item of many rows costs beside its steps, in steps
+// what an item of many rows costs beside its steps, in steps; what a piece to be joined costs more
+constexpr float kItem = 10.f, kPiece = 16.f;
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 constexpr float kLater = 8.0f;  // a maximum may lag by 2^8 before the sums are rescaled
 
@@ -174,10 +175,11 @@ struct alignas(16) Plan {
   int range;           // units of a range of keys
 };
 // What the choice of the range looks at: segments (their tiles in all heads, units, least
-// units); of each candidate the items, those that are not empty, the longest.
+// units, whether nothing is to be joined if they are not split); of each candidate the
+// items, those that are not empty, those of them to be joined, the longest.
 struct Choice {
-  int segments, items[kCandidates], filled[kCandidates], longest[kCandidates];
-  int cuts[kThreads][3];
+  int segments, items[kCandidates], filled[kCandidates], pieces[kCandidates], longest[kCandidates];
+  int cuts[kThreads][4];
 };
 // One LDS array holds it all in a kernel with direct loads: beside a second one, the
 // compiler waits for every load in flight in front of each read.
@@ -195,7 +197,7 @@ __device__ __forceinline__ int ranges_of(int units, int range) { return short_di
 
 // The range of keys for items of many rows, of sixteen candidates the one under which the
 // last block should end first: items are taken in rounds, a block one of each round,
-// and each costs kItem units to begin and to store.  (Equal parts of one line of all
+// and each costs kItem units to begin and to store, kPiece more if its sums are joined.  (Equal parts of one line of all
 // the work, whatever tiles they cut, balance better, but then no two blocks read the
 // same keys at a time, and the L2 no longer serves them: six prompts behind 8192 shared
 // positions took 431 us so, 320 in ranges of one length that all the work gives.)
@@ -205,19 +207,22 @@ __device__ __forceinline__ int candidate(float units_a_block, int i) {
   return i == 0 ? 1 << 30 : static_cast<int>(units_a_block / shares) + 1;
 }
 struct Outcome {
-  int items, filled, longest;
+  int items, filled, pieces, longest;
   // one more segment, `tiles` in all heads, under a range
-  __device__ __forceinline__ void add(int tiles, int units, int least, int range) {
+  __device__ __forceinline__ void add(int tiles, int units, int least, int alone, int range) {
     const int ranges = ranges_of(units, min(units, range)), length = ranges_of(units, ranges);
     // on average a tile sees half of the units between the fewest and all, and half of its last range
     const float mean = static_cast<float>(units + least) / static_cast<float>(2 * length) + (least < units ? 0.5f : 0.f);
     items += tiles * ranges;
-    filled += max(tiles, min(tiles * ranges, static_cast<int>(static_cast<float>(tiles) * mean + 0.5f)));
+    const int here = max(tiles, min(tiles * ranges, static_cast<int>(static_cast<float>(tiles) * mean + 0.5f)));
+    filled += here;
+    pieces += alone && ranges == 1 ? 0 : here;
     longest = max(longest, length);
   }
   __device__ __forceinline__ void put(Choice& to, int i) const {
     atomicAdd(&to.items[i], items);
     atomicAdd(&to.filled[i], filled);
+    atomicAdd(&to.pieces[i], pieces);
     atomicMax(&to.longest[i], longest);
   }
 };
@@ -225,7 +230,8 @@ __device__ __forceinline__ int choose(const Attend& p, const Choice& choice, flo
   int best = lane & (kCandidates - 1);
   const float a_block = static_cast<float>(choice.filled[best]) / static_cast<float>(gridDim.x), rounds = ceilf(a_block);
   // rounds of items of the mean length, at least the longest
-  float time = fmaxf(rounds * units / fmaxf(a_block, 1e-9f), static_cast<float>(choice.longest[best])) + rounds * kItem;
+  float time = fmaxf(rounds * units / fmaxf(a_block, 1e-9f), static_cast<float>(choice.longest[best])) + rounds * kItem +
+               ceilf(static_cast<float>(choice.pieces[best]) / static_cast<float>(gridDim.x)) * kPiece;
   if (choice.items[best] > p.items_max[1] && best > 0) time = INFINITY;
 #pragma unroll
   for (int off = 1; off < kCandidates; off <<= 1) {
@@ -247,7 +253,7 @@ __device__ int schedule(const Attend& p, Plan& plan, Choice* choice) {
   int items = 0, before = 0, total = 0, range = 1;
   Segment first{}, second{};  // of this thread
   if (MANY) {
-    if (threadIdx.x < sizeof(Choice) / 4 - 3 * kThreads) reinterpret_cast<int*>(choice)[threadIdx.x] = 0;
+    if (threadIdx.x < sizeof(Choice) / 4 - 4 * kThreads) reinterpret_cast<int*>(choice)[threadIdx.x] = 0;
     __syncthreads();
   }
   // units, items, places: one loop, so that the code of segment() is there once
@@ -268,6 +274,7 @@ __device__ int schedule(const Attend& p, Plan& plan, Choice* choice) {
           const int to = atomicAdd(&choice->segments, 1);
           if (to < kThreads) {
             choice->cuts[to][0] = c.tiles * p.kv_heads, choice->cuts[to][1] = c.units, choice->cuts[to][2] = c.least;
+            choice->cuts[to][3] = s >= n - p.requests && seg.lo == 0;
           }
         }
       } else if (pass == 1) {
@@ -288,9 +295,10 @@ __device__ int schedule(const Attend& p, Plan& plan, Choice* choice) {
         // of more segments than that, every one is split alike
         if (choice->segments <= kThreads) {
           const int i = threadIdx.x & (kCandidates - 1);
-          Outcome outcome{0, 0, 0};
+          Outcome outcome{0, 0, 0, 0};
           for (int e = threadIdx.x / kCandidates; e < choice->segments; e += kThreads / kCandidates)
-            outcome.add(choice->cuts[e][0], choice->cuts[e][1], choice->cuts[e][2], candidate(units, i));
+            outcome.add(choice->cuts[e][0], choice->cuts[e][1], choice->cuts[e][2], choice->cuts[e][3],
+                        candidate(units, i));
           if (outcome.items > 0) outcome.put(*choice, i);
           __syncthreads();
           range = choose(p, *choice, units, lane);
