@@ -38,6 +38,7 @@ typedef __attribute__((address_space(3))) void lds_void;
 
 constexpr int kFew = 32;        // rows of a segment up to which its waves split the keys instead of the rows
 constexpr int kThreads = 256;   // of every kernel here
+constexpr int kCus = 256;
 // what an item of many rows costs beside its steps, in steps; what a piece to be joined costs more
 constexpr float kItem = 10.f, kPiece = 16.f;
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
@@ -226,12 +227,12 @@ struct Outcome {
     atomicMax(&to.longest[i], longest);
   }
 };
-__device__ __forceinline__ int choose(const Attend& p, const Choice& choice, float units, int lane) {
+__device__ __forceinline__ int choose(const Attend& p, const Choice& choice, float units, int lane, int blocks) {
   int best = lane & (kCandidates - 1);
-  const float a_block = static_cast<float>(choice.filled[best]) / static_cast<float>(gridDim.x), rounds = ceilf(a_block);
+  const float a_block = static_cast<float>(choice.filled[best]) / static_cast<float>(blocks), rounds = ceilf(a_block);
   // rounds of items of the mean length, at least the longest
   float time = fmaxf(rounds * units / fmaxf(a_block, 1e-9f), static_cast<float>(choice.longest[best])) + rounds * kItem +
-               ceilf(static_cast<float>(choice.pieces[best]) / static_cast<float>(gridDim.x)) * kPiece;
+               ceilf(static_cast<float>(choice.pieces[best]) / static_cast<float>(blocks)) * kPiece;
   if (choice.items[best] > p.items_max[1] && best > 0) time = INFINITY;
 #pragma unroll
   for (int off = 1; off < kCandidates; off <<= 1) {
@@ -247,7 +248,7 @@ __device__ __forceinline__ int choose(const Attend& p, const Choice& choice, flo
 // to be for so many items as waves run at once.  Block 0 notes for the joining kernel
 // where each segment's items lie.
 template <bool MANY, int ROWS, int UNIT>
-__device__ int schedule(const Attend& p, Plan& plan, Choice* choice) {
+__device__ __forceinline__ int schedule(const Attend& p, Plan& plan, Choice* choice, int block, int blocks) {
   const int n = segments_of(p), lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   float units = 0.f;  // the same in all blocks; its rounding is in the bound of the items
   int items = 0, before = 0, total = 0, range = 1;
@@ -301,7 +302,7 @@ __device__ int schedule(const Attend& p, Plan& plan, Choice* choice) {
                         candidate(units, i));
           if (outcome.items > 0) outcome.put(*choice, i);
           __syncthreads();
-          range = choose(p, *choice, units, lane);
+          range = choose(p, *choice, units, lane, blocks);
         } else {
           range = candidate(units, 1);
         }
@@ -325,7 +326,7 @@ __device__ int schedule(const Attend& p, Plan& plan, Choice* choice) {
       }
       plan.base[threadIdx.x] = before;
       if (threadIdx.x == 0) plan.range = range;
-      if (blockIdx.x > 0) break;
+      if (block > 0) break;
     }
   }
   __syncthreads();
@@ -813,24 +814,27 @@ template <int D> struct Many {
   static constexpr int kRows = 128, kTiles = D == 64 ? 2 : 1, kKeys = 32 * kTiles;
   static constexpr int kTile = kKeys * 2 * D, kKeyRing = 4, kValueRing = 3, kLds = (kKeyRing + kValueRing) * kTile;
   static constexpr int kLoads = 2 * kTile / 1024 / 4;  // of a wave and step
+  static constexpr int kShared = kLds + static_cast<int>(sizeof(NotFinite<D>) + sizeof(Plan)) + 16;
+  static constexpr int kBlocks = D == 256 ? 1 : 2;  // of a CU
+  static_assert(kBlocks * kShared <= 160 * 1024, "fits");
 };
 
+// Block `block` of `blocks` of them.
 template <class T, int D>
-__global__ __launch_bounds__(kThreads, D == 256 ? 1 : 2) void many_rows_kernel(Attend p) {
+__device__ __forceinline__ void many_rows(const Attend& p, char* lds, int block, int blocks) {
   using M = Many<D>;
   using R = Rows<T, D>;
   constexpr int kTiles = M::kTiles, kScores = 16 * kTiles, kMmas = D / 16 * kTiles, kAhead = R::kAhead;
-  __shared__ __align__(1024) char lds[M::kLds + sizeof(NotFinite<D>) + sizeof(Plan) + 16];
   NotFinite<D>& bad = *reinterpret_cast<NotFinite<D>*>(lds + M::kLds);
   Plan& plan = *reinterpret_cast<Plan*>(lds + M::kLds + sizeof(bad));
   int* least = reinterpret_cast<int*>(lds + M::kLds + sizeof(bad) + sizeof(Plan));  // of each wave's rows
   static_assert(sizeof(Choice) <= M::kLds, "in the place of the rings, before they are used");
   const int lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6);
-  const int total = schedule<true, M::kRows, M::kKeys>(p, plan, reinterpret_cast<Choice*>(lds));
+  const int total = schedule<true, M::kRows, M::kKeys>(p, plan, reinterpret_cast<Choice*>(lds), block, blocks);
   // blocks with the same index modulo 8 share an XCD and its L2: neighbours in the order of items, which share keys
-  const int xcd = blockIdx.x & 7, last = static_cast<int>(static_cast<int64_t>(total) * (xcd + 1) / 8);
+  const int xcd = block & 7, last = static_cast<int>(static_cast<int64_t>(total) * (xcd + 1) / 8);
   // to and fro: a block that has had a long one of a round's items gets a short one of the next
-  const int across = gridDim.x >> 3, mine = blockIdx.x >> 3;
+  const int across = blocks >> 3, mine = block >> 3;
   int round = static_cast<int>(static_cast<int64_t>(total) * xcd / 8);
   for (bool back = false; round < last; round += across, back = !back) {
     const int item = round + (back ? across - 1 - mine : mine);
@@ -970,19 +974,18 @@ template <int D> struct Few {
 };
 
 template <class T, int D>
-__global__ __launch_bounds__(kThreads, Few<D>::kBlocks) void few_rows_kernel(Attend p) {
+__device__ __forceinline__ void few_rows(const Attend& p, char* lds, int block, int blocks) {
   using F = Few<D>;
   using R = Rows<T, D>;
-  __shared__ __align__(1024) char lds[F::kLds];
   const int lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6);
   char* const keys = lds + wave * F::kWave;
   char* const values = keys + F::kHalf;
   NotFinite<D>& bad = reinterpret_cast<NotFinite<D>*>(lds + 4 * F::kWave)[wave];
   Plan& plan = *reinterpret_cast<Plan*>(lds + 4 * (F::kWave + sizeof(bad)));
-  const int total = schedule<false, kFew, 32>(p, plan, nullptr);
+  const int total = schedule<false, kFew, 32>(p, plan, nullptr, block, blocks);
   const int of_k = lane_k<D>(lane), of_v = lane_v<D>(lane);
   // neighbours in the order of items share keys or a table: side by side in a block
-  for (int item = blockIdx.x * 4 + wave; item < total; item += gridDim.x * 4) {
+  for (int item = block * 4 + wave; item < total; item += blocks * 4) {
     const Item it = item_of<false, kFew, 32>(p, plan, item);
     const int end = it.seg.hi, steps = (it.to - it.from + 31) / 32;
     R rows;
@@ -1052,6 +1055,31 @@ __global__ __launch_bounds__(kThreads, Few<D>::kBlocks) void few_rows_kernel(Att
     rows.put(p, it, lane & 31, 0, static_cast<int64_t>(item) * kFew + (lane & 31), lane);
     wait_loads<0>();  // those past the end too
   }
+}
+
+// ------------------------------------------------------------------ kernels
+template <class T, int D>
+__global__ __launch_bounds__(kThreads, Few<D>::kBlocks) void few_rows_kernel(Attend p) {
+  __shared__ __align__(1024) char lds[Few<D>::kLds];
+  few_rows<T, D>(p, lds, blockIdx.x, gridDim.x);
+}
+template <class T, int D>
+__global__ __launch_bounds__(kThreads, Many<D>::kBlocks) void many_rows_kernel(Attend p) {
+  __shared__ __align__(1024) char lds[Many<D>::kShared];
+  many_rows<T, D>(p, lds, blockIdx.x, gridDim.x);
+}
+// Both in one launch, kCus blocks of one and kCus of the other by turns: the first is
+// bound by the matrix cores, the second by memory, and where a CU has room for two
+// blocks it runs one of each.
+template <class T, int D>
+__global__ __launch_bounds__(kThreads, Many<D>::kBlocks) void both_kernel(Attend p) {
+  constexpr int kShared = Many<D>::kShared > Few<D>::kLds ? Many<D>::kShared : Few<D>::kLds;
+  __shared__ __align__(1024) char lds[kShared];
+  const int block = (blockIdx.x / (2 * kCus)) * kCus + blockIdx.x % kCus;
+  if (blockIdx.x / kCus % 2 == 0)
+    many_rows<T, D>(p, lds, block, kCus * Many<D>::kBlocks);
+  else
+    few_rows<T, D>(p, lds, block, kCus * Many<D>::kBlocks);
 }
 
 // ------------------------------------------------------------------ join
@@ -1165,7 +1193,6 @@ __global__ __launch_bounds__(kThreads) void join_kernel(Attend p) {
 }
 
 // ------------------------------------------------------------------ host
-constexpr int kCus = 256;
 inline int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
 inline int64_t aligned(int64_t n) { return (n + 255) / 256 * 256; }
 
@@ -1184,7 +1211,7 @@ Sizes sizes_of(int64_t tokens, int64_t requests, int64_t groups, int64_t heads, 
   const int64_t per = heads / kv_heads, rows = tokens * per, sets = groups > 0 ? 2 : 1;
   z.few = per <= kFew;
   z.many = rows > kFew && (varlen || per > kFew || groups > 0);
-  z.target[0] = 4 * kCus * (dim == 256 ? 1 : dim == 128 ? 2 : 3);  // waves that run at once
+  z.target[0] = 4 * kCus * (dim == 256 ? 1 : dim == 128 || z.many ? 2 : 3);  // waves that run at once
   z.target[1] = kCus * (dim == 256 ? 1 : 2);                       // blocks
   const int64_t few_tiles = requests + groups, many_tiles = sets * (rows / 128 + std::min(requests + groups, rows / kFew + 1));
   z.items[0] = z.few ? z.target[0] + z.target[0] / 64 + few_tiles * kv_heads : 0;
@@ -1207,8 +1234,12 @@ Sizes sizes_of(int64_t tokens, int64_t requests, int64_t groups, int64_t heads, 
 
 template <class T, int D>
 int launch_attend(const Attend& p, const Sizes& z, hipStream_t stream) {
-  if (z.many) many_rows_kernel<T, D><<<static_cast<uint32_t>(z.target[1]), kThreads, 0, stream>>>(p);
-  if (z.few)
+  const uint32_t many = kCus * Many<D>::kBlocks;
+  if (z.many && z.few)
+    both_kernel<T, D><<<2 * many, kThreads, 0, stream>>>(p);
+  else if (z.many)
+    many_rows_kernel<T, D><<<many, kThreads, 0, stream>>>(p);
+  else
     few_rows_kernel<T, D><<<static_cast<uint32_t>(ceil_div(std::min(z.items[0], z.target[0]), 4)), kThreads, 0, stream>>>(p);
   const int64_t rows = static_cast<int64_t>(p.tokens) * p.heads;
   if (rows <= 16 * kCus)
