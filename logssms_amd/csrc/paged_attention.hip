@@ -292,6 +292,7 @@ __device__ __forceinline__ int schedule(const Attend& p, Plan& plan, Choice* cho
       if (lane == 0) plan.units[wave] = units;
       __syncthreads();
       units = (plan.units[0] + plan.units[1] + plan.units[2] + plan.units[3]) * p.per_target[MANY];
+      if (units == 0.f && block > 0) return 0;  // nothing of this kind; block 0 notes the places
       if constexpr (MANY) {
         // of more segments than that, every one is split alike
         if (choice->segments <= kThreads) {
@@ -1242,7 +1243,7 @@ int launch_attend(const Attend& p, const Sizes& z, hipStream_t stream) {
   else
     few_rows_kernel<T, D><<<static_cast<uint32_t>(ceil_div(std::min(z.items[0], z.target[0]), 4)), kThreads, 0, stream>>>(p);
   const int64_t rows = static_cast<int64_t>(p.tokens) * p.heads;
-  if (rows <= 16 * kCus)
+  if (rows <= 4 * kCus)
     join_kernel<T, D, 4><<<static_cast<uint32_t>(rows), kThreads, 0, stream>>>(p);
   else
     join_kernel<T, D, 1><<<static_cast<uint32_t>(ceil_div(rows, 4)), kThreads, 0, stream>>>(p);
