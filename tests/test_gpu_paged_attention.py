@@ -390,3 +390,93 @@ def test_pool_appends_and_attention_together():
         step([0, 1, 2], [prefix + n + i for n in own], [1, 1, 1], prefix)
     assert (pool.storage[:, list(held)].view(2, len(held), -1) != 0).any()
     assert (pool.recurrent_state[pool._starts(state)[0]] == 3).all()
+
+
+@pytest.mark.parametrize("io", ["bf16", "f16"])
+@pytest.mark.parametrize("heads,kv_heads,dim", [(16, 1, 256), (16, 1, 128), (32, 2, 64)])
+def test_prompts_of_many_tiles(io, heads, kv_heads, dim):
+    """Tiles of rows that are no multiple of eight, their last ones in part, behind keys in several ranges."""
+    b = Batch(40 + dim, heads, kv_heads, dim, 64, [75, 2900, 73 + 5], new=[75, 140, 73], io=io)
+    out, lse = b.run(return_lse=True)
+    b.check(out, lse)
+
+
+@pytest.mark.parametrize("dim", [64, 256])
+def test_prompts_behind_a_shared_prefix(dim):
+    """All of their tokens are rows of the shared part; one of them ends inside it."""
+    b = Batch(41, 16, 2, dim, 64, [640 + 50, 640 + 33, 640 + 1, 600], new=[50, 30, 1, 20], shared=[640])
+    out, lse = b.run(return_lse=True)
+    b.check(out, lse)
+
+
+def requests_over(b, n):
+    """n requests over the pages of the only one of `b`, in another order each."""
+    b.table = torch.stack([b.table[0].roll(3 * r) for r in range(n)])
+    b.lens = [b.lens[0] - 5 * r for r in range(n)]
+    b.q = randn(n, *b.q.shape[1:], g=gen(n)).to(b.io)
+    return b
+
+
+@pytest.mark.parametrize("heads,kv_heads,dim,n", [(8, 8, 256, 128), (320, 8, 256, 32), (320, 8, 64, 64)])
+def test_long_ranges_of_keys(heads, kv_heads, dim, n):
+    """A block's or wave's keys go on past what one lookup in the table serves; the first and the last
+    request stand for all."""
+    b = requests_over(Batch(42, heads, kv_heads, dim, 16, [4096 + 5 * n]), n)
+    out, lse = b.run(return_lse=True)
+    q, table, lens = b.q, b.table, b.lens
+    for r in (0, n - 1):
+        b.q, b.table, b.lens = q[r:r + 1], table[r:r + 1], lens[r:r + 1]
+        b.check(out[r:r + 1], lse[r:r + 1])
+
+
+def test_more_segments_of_many_rows_than_threads():
+    lens = [48 + (r * 29) % 90 for r in range(300)]
+    b = Batch(43, 36, 1, 64, 16, lens, shared=[48, 48, 0], groups=[0, 120, 121, 290])
+    out, lse = b.run(return_lse=True)
+    b.check(out, lse)
+
+
+@pytest.mark.parametrize("heads", [2, 16])
+def test_many_empty_requests_in_a_group(heads):
+    """Few and many rows of a shared part, the tokens' requests far apart."""
+    new = [0] * 150
+    new[0], new[1], new[90], new[149] = 2, 1, 3, 1
+    lens = [64 + (7 * r) % 40 for r in range(150)]
+    b = Batch(44, heads, 1, 128, 16, lens, new=new, shared=[64])
+    out, lse = b.run(return_lse=True)
+    b.check(out, lse)
+
+
+def test_thousands_of_requests():
+    new = [int(r % 3 != 1) for r in range(5000)]
+    lens = [16 + r % 23 for r in range(5000)]
+    b = Batch(45, 1, 1, 64, 16, lens, new=new, shared=[16, 16], groups=[7, 4500, 4990])
+    out, lse = b.run(return_lse=True)
+    b.check(out, lse)
+
+
+def test_two_streams_at_once():
+    """Each call has a workspace of its own."""
+    batches = [Batch(46, 16, 2, 256, 64, [900, 4000, 30], new=[3, 200, 1]), Batch(47, 8, 8, 128, 16, [700] * 40)]
+    want = [b.run() for b in batches]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in batches]
+    got = [[], []]
+    for _ in range(5):
+        for b, stream, results in zip(batches, streams, got):
+            with torch.cuda.stream(stream):
+                results.append(b.run())
+    torch.cuda.synchronize()
+    for w, results in zip(want, got):
+        assert all(torch.equal(w, x) for x in results)
+
+
+def test_tables_and_lengths_that_are_views():
+    from logssms_amd.kernel import paged_attention
+    b = Batch(48, 8, 2, 128, 16, [100, 333, 7])
+    want = b.run()
+    wide = torch.full((6, b.width + 5), 10 ** 6, device=DEV)
+    wide[::2, 2:2 + b.width] = b.table.to(DEV)
+    lens = torch.tensor(b.lens, device=DEV)
+    got = paged_attention(b.q.to(DEV), *b.caches(), wide[::2, 2:2 + b.width], lens)
+    assert torch.equal(got, want)
