@@ -40,7 +40,7 @@ constexpr int kFew = 32;        // rows of a segment up to which its waves split
 constexpr int kThreads = 256;   // of every kernel here
 constexpr int kCus = 256;
 // what an item of many rows costs beside its steps, in steps; what a piece to be joined costs more
-constexpr float kItem = 10.f, kPiece = 16.f;
+constexpr float kItem = 10.f, kPiece = 32.f;
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 constexpr float kLater = 8.0f;  // a maximum may lag by 2^8 before the sums are rescaled
 
@@ -542,6 +542,10 @@ template <class V> __device__ __forceinline__ V here(V v) {
 // Instructions stay on their side of it.
 __device__ __forceinline__ void in_order() { __builtin_amdgcn_sched_barrier(0); }
 
+// The lane, found anew.
+__device__ __forceinline__ int lane_again() {
+  return here(static_cast<int>(__builtin_amdgcn_mbcnt_hi(~0u, __builtin_amdgcn_mbcnt_lo(~0u, 0u))));
+}
 // Of this lane's value and that of the lane 32 before or behind it.
 __device__ __forceinline__ float max_of_halves(float v) {
   const auto halves = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
@@ -830,7 +834,7 @@ __device__ __forceinline__ void many_rows(const Attend& p, char* lds, int block,
   Plan& plan = *reinterpret_cast<Plan*>(lds + M::kLds + sizeof(bad));
   int* least = reinterpret_cast<int*>(lds + M::kLds + sizeof(bad) + sizeof(Plan));  // of each wave's rows
   static_assert(sizeof(Choice) <= M::kLds, "in the place of the rings, before they are used");
-  const int lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6);
+  const int wave = uniform(threadIdx.x >> 6);
   const int total = schedule<true, M::kRows, M::kKeys>(p, plan, reinterpret_cast<Choice*>(lds), block, blocks);
   // blocks with the same index modulo 8 share an XCD and its L2: neighbours in the order of items, which share keys
   const int xcd = block & 7, last = static_cast<int>(static_cast<int64_t>(total) * (xcd + 1) / 8);
@@ -840,6 +844,7 @@ __device__ __forceinline__ void many_rows(const Attend& p, char* lds, int block,
   for (bool back = false; round < last; round += across, back = !back) {
     const int item = round + (back ? across - 1 - mine : mine);
     if (item >= last) continue;  // whole block
+    const int lane = lane_again();  // what follows from it is not kept in registers from item to item
     const Item it = item_of<true, M::kRows, M::kKeys>(p, plan, item);
     R rows;
     const int row = it.tile * M::kRows + 32 * wave + (lane & 31);
