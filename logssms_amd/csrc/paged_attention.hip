@@ -69,7 +69,7 @@ struct Attend {
   // the first item and the number of key ranges of each segment
   float* sums[2];
   float2* stats[2];
-  int items_max[2], min_units[2];
+  int items_max[2];
   float per_target[2];  // key heads over the number of items wanted
   struct Place* places;  // of each segment, for the joining kernel
 };
@@ -308,7 +308,11 @@ __device__ __forceinline__ int schedule(const Attend& p, Plan& plan, Choice* cho
           range = candidate(units, 1);
         }
       } else {
-        range = max(p.min_units[MANY], static_cast<int>(fminf(units, 1.0e9f)) + 1);
+        // Where half of the waves get by with two steps each, they take them: the other half
+        // may have to wait for blocks of the other kind to end, and there are half as many
+        // pieces to join (37 short requests, 8 heads of 64: 19 -> 15 us; one request of 4096
+        // positions, 2 heads of 256, stays at one step: 20 us, 20.4 with three, 22 with four).
+        range = static_cast<int>(fminf(units >= 1.f ? units : 2.f * units, 1.0e9f)) + 1;
       }
     } else if (pass == 1) {
       int sum = items;
@@ -1093,7 +1097,7 @@ __global__ __launch_bounds__(kThreads, Many<D>::kBlocks) void both_kernel(Attend
 // a wave's at a time: a lane looks up one piece, then all lanes add the pieces.
 template <class T, int D, int WAVES>
 __global__ __launch_bounds__(kThreads) void join_kernel(Attend p) {
-  constexpr int kRowsABlock = kThreads / (64 * WAVES), kLane = D / 64, kBatch = 8;  // channels a lane
+  constexpr int kRowsABlock = kThreads / (64 * WAVES), kLane = D / 64, kBatch = WAVES > 1 ? 16 : 8;  // channels a lane
   typedef float Channels __attribute__((ext_vector_type(kLane)));
   __shared__ float sums[4][D];
   __shared__ float2 stats[4];
@@ -1336,7 +1340,6 @@ extern "C" int gdn_paged_attention(const void* q, int64_t q_token_stride, int64_
     p.stats[kind] = reinterpret_cast<float2*>(ws + z.stats[kind]);
     p.items_max[kind] = static_cast<int>(z.items[kind]);
     p.per_target[kind] = static_cast<float>(static_cast<double>(kv_heads) / static_cast<double>(z.target[kind]));
-    p.min_units[kind] = 1;
   }
   p.places = reinterpret_cast<Place*>(ws + z.places);
   auto go = [&](auto type) {
