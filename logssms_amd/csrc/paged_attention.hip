@@ -20,7 +20,15 @@
 // another lane the other half of its keys), so that a row's statistics take one
 // exchange between two lanes, and the accumulators of S^T are the right operand
 // of the second product as they stand, with the keys of each 16 in the order
-// 0-3, 8-11 | 4-7, 12-15, in which V is read as well.
+// 0-3, 8-11 | 4-7, 12-15, in which V is read as well.  The weights are rounded to the
+// io type for it (their sum is not); maxima, sums and outputs stay in fp32, the pieces
+// too.
+//
+// Many rows are bound by the matrix cores and what feeds them, few rows by memory.
+// Measured on an MI355X (copies 4.9 TB/s, bf16 products of 8192^3 1205 TFLOP/s):
+// a prompt of 8192 tokens 840-900 TFLOP/s (dims 256, 128; 64: 680), 1024 requests
+// behind 16384 shared positions 780-840, 64 and 256 requests of 4096 and 1024
+// positions with nothing shared 5.0-5.7 TB/s.
 #include <algorithm>
 
 #include "common.hpp"
@@ -36,10 +44,17 @@ typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
 typedef __attribute__((address_space(3))) void lds_void;
 
-constexpr int kFew = 32;        // rows of a segment up to which its waves split the keys instead of the rows
-constexpr int kThreads = 256;   // of every kernel here
+// Rows of a segment up to which its waves split the keys instead of the rows: a
+// matrix instruction's.  (With 16, 64 requests of 8 drafts, 32/8 heads of 128: alone
+// behind 2048 positions 116 us instead of 129, since fewer pieces are joined, but 169
+// instead of 155 for 512 requests behind 256, and 119 instead of 115 behind prompts that
+// are shared.)
+constexpr int kFew = 32;
+constexpr int kThreads = 256;  // of every kernel here
 constexpr int kCus = 256;
-// what an item of many rows costs beside its steps, in steps; what a piece to be joined costs more
+// What an item of many rows costs beside its steps, in steps, and what a piece to be joined
+// costs more.  (A prompt of 1024 tokens, 16/2 heads of 256: 46 us, 58 with kPiece 16; one
+// of 2048 77 us, 112 with kItem 5 and kPiece 8; kItem 20 changes neither.)
 constexpr float kItem = 10.f, kPiece = 32.f;
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 constexpr float kLater = 8.0f;  // a maximum may lag by 2^8 before the sums are rescaled
@@ -74,11 +89,10 @@ struct Attend {
   struct Place* places;  // of each segment, for the joining kernel
 };
 // Where the items of a segment lie, and what it is.
-struct Place {
+struct alignas(16) Place {
   int item, ranges;  // first item; ranges of keys
   int token, tokens, lo, hi;
   int group;  // of a request (-1: none)
-  int unused;
 };
 
 // ------------------------------------------------------------------ segments
@@ -186,7 +200,8 @@ struct Choice {
 // compiler waits for every load in flight in front of each read.
 static_assert(sizeof(Plan) % 8 == 0, "what lies behind it is aligned");
 
-// n / d for d > 0 where the quotient is below 2^22: shorter than the exact division,
+// n / d for d > 0 where the quotient is at most 2^22 (there are up to 2^27 positions, 2^22
+// steps): shorter than the exact division,
 // and what a launch runs once it has to fetch first.
 __device__ __forceinline__ int short_div(int n, int d) {
   int q = static_cast<int>(static_cast<float>(n) * __builtin_amdgcn_rcpf(static_cast<float>(d)));
@@ -196,12 +211,13 @@ __device__ __forceinline__ int short_div(int n, int d) {
 }
 __device__ __forceinline__ int ranges_of(int units, int range) { return short_div(units + range - 1, range); }
 
-// The range of keys for items of many rows, of sixteen candidates the one under which the
-// last block should end first: items are taken in rounds, a block one of each round,
-// and each costs kItem units to begin and to store, kPiece more if its sums are joined.  (Equal parts of one line of all
-// the work, whatever tiles they cut, balance better, but then no two blocks read the
-// same keys at a time, and the L2 no longer serves them: six prompts behind 8192 shared
-// positions took 431 us so, 320 in ranges of one length that all the work gives.)
+// The range of keys for items of many rows: of sixteen candidates the one under which
+// the last block should end first, where a block takes one item of each round, and an
+// item costs its steps, kItem, and kPiece if its sums are joined.  Six prompts behind
+// 8192 shared positions, 16/2 heads of 256: 200 us, 272 in ranges of the length that
+// all the work gives a block.  (Equal parts of one line of all the work, whatever
+// tiles they cut, balance better still, but then no two blocks read the same keys at a
+// time, the L2 no longer serves them, and it took a third longer than equal ranges.)
 __device__ __forceinline__ int candidate(float units_a_block, int i) {
   // none is split; otherwise 2, 1.71, 1.5, 1.33, 1.2 .. 0.25 times what a block gets
   const float shares = i < 6 ? 0.5f + (i - 1) / 12.f : 0.91f + (i - 6) * (i - 6) * 0.038f;
@@ -282,7 +298,7 @@ __device__ __forceinline__ int schedule(const Attend& p, Plan& plan, Choice* cho
         items += c.tiles * p.kv_heads * ranges;
       } else {
         if ((seg.tokens * p.per > kFew) == MANY)
-          p.places[s] = {before, ranges, seg.token, seg.tokens, seg.lo, seg.hi, seg.group, 0};
+          p.places[s] = {before, ranges, seg.token, seg.tokens, seg.lo, seg.hi, seg.group};
         before += c.tiles * p.kv_heads * ranges;
       }
     }
@@ -377,14 +393,16 @@ __device__ Item item_of(const Attend& p, const Plan& plan, int item) {
   for (int s = thread;; s += kThreads) {
     const Segment seg = s == thread ? plan.segments[thread] : segment(p, s);
     const Cut c = cut_of<MANY, ROWS, UNIT>(p, seg, s >= segments_of(p) - p.requests);
-    const int ranges = uniform(ranges_of(c.units, MANY ? min(range, max(1, c.units)) : range)), tiles = uniform(c.tiles), items = tiles * p.kv_heads * ranges;
+    const int ranges = uniform(ranges_of(c.units, MANY ? min(range, max(1, c.units)) : range));
+    const int tiles = uniform(c.tiles), items = tiles * p.kv_heads * ranges;
     if (at < items || s + kThreads >= n) {
       Item it;
       it.seg = {uniform(seg.token), uniform(seg.tokens), uniform(seg.lo),
                 uniform(seg.hi),    uniform(seg.request), uniform(seg.length), uniform(seg.group)};
       it.ranges = ranges;
       it.own = s >= n - p.requests;
-      const int across = uniform(short_div(at, max(1, tiles))), length = MANY ? uniform(ranges_of(c.units, max(1, ranges))) : range;
+      const int across = uniform(short_div(at, max(1, tiles)));
+      const int length = MANY ? uniform(ranges_of(c.units, max(1, ranges))) : range;
       it.tile = at - across * max(1, tiles);
       if (MANY) it.tile = uniform(tile_at(it.tile, tiles));
       it.head = uniform(short_div(across, max(1, ranges)));
@@ -819,6 +837,17 @@ struct Rows {
 // j + 2; so keys lie in a ring of four tiles, values in one of three, and a load has
 // a step and a half to arrive.  The first fragments of each product are read during
 // the last matrix instructions of the one before it.
+//
+// Of 256 channels a step takes 1.12 us on all CUs at once (955 TFLOP/s), some 20 us of
+// a call are outside of the steps.  What bounds a step is LDS beside the matrix cores:
+// a wave of 32 rows reads each fragment for one matrix instruction, which takes LDS
+// as long as that takes the matrix core.  (64 rows a wave, its sums in the upper 256
+// registers, read them for two: 1053 TFLOP/s in long runs of steps, but tiles twice as
+// high mean twice the pieces to store and to join: 256 requests behind 32768 shared
+// positions 193-203 us against 193-201, prompts of 1024 to 4096 tokens 90, 144 and 326
+// against 62, 85 and 176.)  Of 64 channels, where a product has too few instructions
+// to hide one step's weights and a barrier, a step is 64 keys: eight prompts of 512
+// tokens 117 us, in steps of 32 126.
 template <int D> struct Many {
   static constexpr int kRows = 128, kTiles = D == 64 ? 2 : 1, kKeys = 32 * kTiles;
   static constexpr int kTile = kKeys * 2 * D, kKeyRing = 4, kValueRing = 3, kLds = (kKeyRing + kValueRing) * kTile;
@@ -975,7 +1004,10 @@ __device__ __forceinline__ void many_rows(const Attend& p, char* lds, int block,
 // A segment of at most 32 rows: what bounds it is how fast its keys come in.  Each
 // wave takes items of its own, in LDS of its own for 32 positions' keys and values;
 // the next keys are loaded when these have become scores, the next values when
-// these have been summed.  There is no barrier among the waves.
+// these have been summed.  There is no barrier among the waves.  One request of 4096
+// positions, 16/2 heads of 256, is bound by what follows one another: 3 us to the
+// schedule, 3 to the first loads, 3.5 for a step and its piece, 2 to the joining kernel's
+// launch and 6 in it.
 template <int D> struct Few {
   static constexpr int kHalf = 32 * 2 * D, kWave = 2 * kHalf, kLoads = kHalf / 1024;
   static constexpr int kLds = 4 * (kWave + static_cast<int>(sizeof(NotFinite<D>))) + static_cast<int>(sizeof(Plan));
@@ -1080,7 +1112,8 @@ __global__ __launch_bounds__(kThreads, Many<D>::kBlocks) void many_rows_kernel(A
 }
 // Both in one launch, kCus blocks of one and kCus of the other by turns: the first is
 // bound by the matrix cores, the second by memory, and where a CU has room for two
-// blocks it runs one of each.
+// blocks it runs one of each (64 requests of 8 drafts behind four shared prompts,
+// 32/8 heads of 128: 116 us, 141 in two launches, one after the other).
 template <class T, int D>
 __global__ __launch_bounds__(kThreads, Many<D>::kBlocks) void both_kernel(Attend p) {
   constexpr int kShared = Many<D>::kShared > Few<D>::kLds ? Many<D>::kShared : Few<D>::kLds;
@@ -1094,7 +1127,11 @@ __global__ __launch_bounds__(kThreads, Many<D>::kBlocks) void both_kernel(Attend
 
 // ------------------------------------------------------------------ join
 // WAVES waves a row: the pieces of the row's shared and own segments by turns, 64 of
-// a wave's at a time: a lane looks up one piece, then all lanes add the pieces.
+// a wave's at a time: a lane looks up one piece, then all lanes add the pieces.  What
+// bounds it is the pieces' bytes, or for few rows one load after another: four waves a
+// row up to 1024 rows (64 rows of one request of 4096 positions 20.1 us for the call,
+// with one wave 23.9; 256 rows 33.0 and 34.7), one from there on (2048 rows 193.9 us with
+// four, 192.1 with one).
 template <class T, int D, int WAVES>
 __global__ __launch_bounds__(kThreads) void join_kernel(Attend p) {
   constexpr int kRowsABlock = kThreads / (64 * WAVES), kLane = D / 64, kBatch = WAVES > 1 ? 16 : 8;  // channels a lane
@@ -1295,8 +1332,8 @@ extern "C" int gdn_paged_attention(const void* q, int64_t q_token_stride, int64_
     return GDN_ERR_UNSUPPORTED;
   }
   if (tokens * heads >= (int64_t{1} << 31) || requests + groups >= (int64_t{1} << 24) ||
-      table_width * page_size > (int64_t{1} << 30) || pages >= (int64_t{1} << 31) || kv_heads > (1 << 16)) {
-    set_error("up to 2^31 rows, 2^24 requests, 2^30 positions, 2^31 pages and 2^16 key heads");
+      table_width * page_size > (int64_t{1} << 27) || pages >= (int64_t{1} << 31) || kv_heads > (1 << 16)) {
+    set_error("up to 2^31 rows, 2^24 requests, 2^27 positions, 2^31 pages and 2^16 key heads");
     return GDN_ERR_UNSUPPORTED;
   }
   if (tokens == 0 || requests == 0) return GDN_OK;
