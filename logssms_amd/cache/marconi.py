@@ -13,7 +13,8 @@ implementation is this library's own:
   state slots are recycled lowest id first; the lane-strided
   ``recurrent_state`` / ``conv_state`` views the kernels index with
   (start block, lane); ``copy_state`` / ``zero_state`` / ``copy_blocks`` are
-  one gfx950 launch each (``gdn_copy_rows`` / ``gdn_zero_rows``), and
+  one gfx950 launch each (``gdn_copy_rows`` / ``gdn_zero_rows``),
+  ``kv_cache`` gives a full-attention layer's keys and values as pages, and
   ``map_metadata`` is one device gather per slot table through a column
   that ends in a -1 sentinel.
 * ``MarconiRequestState`` / ``MarconiCheckpointer`` -- where a prefill writes

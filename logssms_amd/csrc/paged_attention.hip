@@ -839,15 +839,14 @@ struct Rows {
 // the last matrix instructions of the one before it.
 //
 // Of 256 channels a step takes 1.12 us on all CUs at once (955 TFLOP/s), some 20 us of
-// a call are outside of the steps.  What bounds a step is LDS beside the matrix cores:
-// a wave of 32 rows reads each fragment for one matrix instruction, which takes LDS
-// as long as that takes the matrix core.  (64 rows a wave, its sums in the upper 256
-// registers, read them for two: 1053 TFLOP/s in long runs of steps, but tiles twice as
-// high mean twice the pieces to store and to join: 256 requests behind 32768 shared
-// positions 193-203 us against 193-201, prompts of 1024 to 4096 tokens 90, 144 and 326
-// against 62, 85 and 176.)  Of 64 channels, where a product has too few instructions
-// to hide one step's weights and a barrier, a step is 64 keys: eight prompts of 512
-// tokens 117 us, in steps of 32 126.
+// a call are outside of the steps.  Matrix cores are busy for 43 % of the cycles, and LDS,
+// which a wave of 32 rows reads for each matrix instruction, as long.  (64 rows a wave, its
+// sums in the upper 256 registers, read it half as often: 1053 TFLOP/s in long runs of
+// steps, but tiles twice as high mean twice the pieces to store and to join: 256 requests
+// behind 32768 shared positions 193-203 us against 197-201, prompts of 1024 to 4096 tokens
+// 90, 144 and 326 against 62, 85 and 176.)  Of 64 channels, where a product has too few
+// instructions to hide one step's weights and a barrier, a step is 64 keys: eight prompts
+// of 512 tokens 117 us, in steps of 32 126.
 template <int D> struct Many {
   static constexpr int kRows = 128, kTiles = D == 64 ? 2 : 1, kKeys = 32 * kTiles;
   static constexpr int kTile = kKeys * 2 * D, kKeyRing = 4, kValueRing = 3, kLds = (kKeyRing + kValueRing) * kTile;

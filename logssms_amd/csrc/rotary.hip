@@ -10,7 +10,9 @@
 // Bound by memory: 16 bytes a lane, each value read and written once.  A block takes a
 // few tokens and some or all of their heads: its cosines and sines are computed once
 // into LDS, each thread keeps those of its pairs and walks over the heads, the
-// loads of four of them in flight.
+// loads of four of them in flight.  16384 tokens, 16/2 heads of 256, a quarter of them
+// turned: 72 us, 4.2 TB/s (copies reach 4.9); appended 76 us, 4.4 TB/s; a token 5.5 us, a
+// launch and a call from Python.
 #include <algorithm>
 
 #include "common.hpp"
@@ -68,7 +70,8 @@ __device__ __forceinline__ void turn_pair(float2 cs, float& a, float& b) {
 
 // WIDE: rows in pieces of 16 bytes; a unit of work is a pair of pieces (half
 // layout), a piece of pairs (interleaved), or a piece behind the rotated ones.
-// Otherwise a unit is one pair, or one value.
+// Otherwise (rows at odd addresses, odd dims) a unit is one pair, or one value: 16384
+// tokens of 16 heads of 256 46 us and, one value further on, 151.
 template <class T, bool WIDE>
 __global__ __launch_bounds__(kThreads) void rotary_kernel(Turn p) {
   constexpr int V = WIDE ? Vec16<T>::n : 1, kHeads = 4;

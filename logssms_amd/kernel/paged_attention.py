@@ -48,8 +48,9 @@ def paged_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
 
     The requests ``group_offsets[g]`` .. ``group_offsets[g + 1] - 1`` of group g (all of
     them without ``group_offsets``) share their first ``shared_lens[g]`` positions: the
-    same pages in each of their rows.  These are attended once for the group, and
-    nothing else depends on it.
+    same pages in each of their rows, of which the first request's is read (an empty
+    request's too).  These are attended once for the group, and nothing else depends on
+    it.
 
     A token that sees no position gives zeros; tokens that no request owns are left as
     they were in ``out``.  ``return_lse``: also the logarithm of each row's sum of
