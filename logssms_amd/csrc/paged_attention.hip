@@ -45,10 +45,9 @@ typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
 typedef __attribute__((address_space(3))) void lds_void;
 
 // Rows of a segment up to which its waves split the keys instead of the rows: a
-// matrix instruction's.  (With 16, 64 requests of 8 drafts, 32/8 heads of 128: alone
-// behind 2048 positions 116 us instead of 129, since fewer pieces are joined, but 169
-// instead of 155 for 512 requests behind 256, and 119 instead of 115 behind prompts that
-// are shared.)
+// matrix instruction's.  (With 16, so that 24 and 32 rows are many, 32/8 heads of 128: 64
+// requests of 6 drafts behind 2048 positions 115 us for 113, two of 8 behind 32768 56
+// for 59, 512 of 8 behind 256 169 for 153, 64 of 8 behind shared prompts 119 for 112.)
 constexpr int kFew = 32;
 constexpr int kThreads = 256;  // of every kernel here
 constexpr int kCus = 256;
@@ -260,8 +259,8 @@ __device__ __forceinline__ int choose(const Attend& p, const Choice& choice, flo
 }
 
 // Counts the items of the launch: thread i answers for the segments i, i + kThreads, ...,
-// and the items lie thread by thread.  A range of keys of few rows is as long as it has
-// to be for so many items as waves run at once.  Block 0 notes for the joining kernel
+// and the items lie thread by thread.  A range of keys of few rows is as long as all of
+// their work gives to each of three waves a CU.  Block 0 notes for the joining kernel
 // where each segment's items lie.
 template <bool MANY, int ROWS, int UNIT>
 __device__ __forceinline__ int schedule(const Attend& p, Plan& plan, Choice* choice, int block, int blocks) {
@@ -324,11 +323,7 @@ __device__ __forceinline__ int schedule(const Attend& p, Plan& plan, Choice* cho
           range = candidate(units, 1);
         }
       } else {
-        // Where half of the waves get by with two steps each, they take them: the other half
-        // may have to wait for blocks of the other kind to end, and there are half as many
-        // pieces to join (37 short requests, 8 heads of 64: 19 -> 15 us; one request of 4096
-        // positions, 2 heads of 256, stays at one step: 20 us, 20.4 with three, 22 with four).
-        range = static_cast<int>(fminf(units >= 1.f ? units : 2.f * units, 1.0e9f)) + 1;
+        range = static_cast<int>(fminf(units, 1.0e9f)) + 1;
       }
     } else if (pass == 1) {
       int sum = items;
@@ -838,15 +833,17 @@ struct Rows {
 // a step and a half to arrive.  The first fragments of each product are read during
 // the last matrix instructions of the one before it.
 //
-// Of 256 channels a step takes 1.12 us on all CUs at once (955 TFLOP/s), some 20 us of
-// a call are outside of the steps.  Matrix cores are busy for 43 % of the cycles, and LDS,
-// which a wave of 32 rows reads for each matrix instruction, as long.  (64 rows a wave, its
-// sums in the upper 256 registers, read it half as often: 1053 TFLOP/s in long runs of
-// steps, but tiles twice as high mean twice the pieces to store and to join: 256 requests
-// behind 32768 shared positions 193-203 us against 197-201, prompts of 1024 to 4096 tokens
-// 90, 144 and 326 against 62, 85 and 176.)  Of 64 channels, where a product has too few
-// instructions to hide one step's weights and a barrier, a step is 64 keys: eight prompts
-// of 512 tokens 117 us, in steps of 32 126.
+// Of 256 channels a step takes 1.1 us on all CUs at once (955 to 985 TFLOP/s), some 20 us
+// of a call are outside of the steps.  What bounds the steps is the clock that power
+// leaves: on keys and values of zeros the same call runs at 1247 TFLOP/s (128 channels:
+// 1303 for 942).  Without its loads to LDS it ran at 1206, with half of its LDS reads at
+// 1033, without exponentials at 1010.  (64 rows a wave, its sums in the upper 256
+// registers, halve the loads and the reads: 1053 in long runs of steps, but tiles twice as
+// high mean twice the pieces to store and to join: 256 requests behind 32768 shared
+// positions 193-203 us against 197-201, prompts of 1024 to 4096 tokens 90, 144 and 326
+// against 62, 85 and 176.)  Of 64 channels, where a product has too few instructions to
+// hide one step's weights and a barrier, a step is 64 keys: eight prompts of 512 tokens
+// 117 us, in steps of 32 126.
 template <int D> struct Many {
   static constexpr int kRows = 128, kTiles = D == 64 ? 2 : 1, kKeys = 32 * kTiles;
   static constexpr int kTile = kKeys * 2 * D, kKeyRing = 4, kValueRing = 3, kLds = (kKeyRing + kValueRing) * kTile;
@@ -1000,12 +997,12 @@ __device__ __forceinline__ void many_rows(const Attend& p, char* lds, int block,
 }
 
 // ------------------------------------------------------------------ few rows
-// A segment of at most 32 rows: what bounds it is how fast its keys come in.  Each
-// wave takes items of its own, in LDS of its own for 32 positions' keys and values;
+// A segment of at most 32 rows: what bounds it is how fast its keys come in, for which
+// three waves a CU are about enough.  Each wave takes items of its own, in LDS of its own for 32 positions' keys and values;
 // the next keys are loaded when these have become scores, the next values when
 // these have been summed.  There is no barrier among the waves.  One request of 4096
 // positions, 16/2 heads of 256, is bound by what follows one another: 3 us to the
-// schedule, 3 to the first loads, 3.5 for a step and its piece, 2 to the joining kernel's
+// schedule, 3 to the first loads, 3 for a step and its piece, 2 to the joining kernel's
 // launch and 6 in it.
 template <int D> struct Few {
   static constexpr int kHalf = 32 * 2 * D, kWave = 2 * kHalf, kLoads = kHalf / 1024;
@@ -1025,8 +1022,12 @@ __device__ __forceinline__ void few_rows(const Attend& p, char* lds, int block, 
   Plan& plan = *reinterpret_cast<Plan*>(lds + 4 * (F::kWave + sizeof(bad)));
   const int total = schedule<false, kFew, 32>(p, plan, nullptr, block, blocks);
   const int of_k = lane_k<D>(lane), of_v = lane_v<D>(lane);
-  // neighbours in the order of items share keys or a table: side by side in a block
-  for (int item = block * 4 + wave; item < total; item += blocks * 4) {
+  // neighbours in the order of items share keys or a table, or lie side by side: in one
+  // block (64 requests of 4096 positions, 32/8 heads of 128: 188 us, 215 with a block's
+  // waves far apart); few items on as many CUs as there are (eight requests of 1000, 16/2
+  // heads of 256: 16.3 us, 18.3 with four to a block)
+  const int each = min(4, (total + kCus - 1) / kCus);
+  for (int item = wave < each ? block * each + wave : total; item < total; item += blocks * each) {
     const Item it = item_of<false, kFew, 32>(p, plan, item);
     const int end = it.seg.hi, steps = (it.to - it.from + 31) / 32;
     R rows;
@@ -1244,7 +1245,7 @@ inline int64_t aligned(int64_t n) { return (n + 255) / 256 * 256; }
 
 struct Sizes {
   bool few, many;  // whether segments of that kind can be there
-  int64_t items[2], target[2];
+  int64_t items[2], target[2], waves;
   int64_t sums[2], stats[2], places, bytes;  // offsets
 };
 
@@ -1257,8 +1258,13 @@ Sizes sizes_of(int64_t tokens, int64_t requests, int64_t groups, int64_t heads, 
   const int64_t per = heads / kv_heads, rows = tokens * per, sets = groups > 0 ? 2 : 1;
   z.few = per <= kFew;
   z.many = rows > kFew && (varlen || per > kFew || groups > 0);
-  z.target[0] = 4 * kCus * (dim == 256 ? 1 : dim == 128 || z.many ? 2 : 3);  // waves that run at once
-  z.target[1] = kCus * (dim == 256 ? 1 : 2);                       // blocks
+  // Of few rows, fewer than run at once: more bring the keys no faster and leave more pieces
+  // (64 requests of 4096 positions, 32/8 heads of 128: 188 us, 190 with 4 a CU, 203 with 8;
+  // 64 x 8 drafts behind shared prompts 112, 117, 114; on average over 54 batches 2 % less
+  // than with 4, 6 % less than with all that run)
+  z.target[0] = 3 * kCus;
+  z.target[1] = kCus * (dim == 256 ? 1 : 2);  // blocks
+  z.waves = 4 * kCus * (dim == 256 ? 1 : dim == 128 || z.many ? 2 : 3);  // of few rows, that run at once
   const int64_t few_tiles = requests + groups, many_tiles = sets * (rows / 128 + std::min(requests + groups, rows / kFew + 1));
   z.items[0] = z.few ? z.target[0] + z.target[0] / 64 + few_tiles * kv_heads : 0;
   z.items[1] = z.many ? 4 * z.target[1] + many_tiles * kv_heads : 0;
@@ -1286,7 +1292,9 @@ int launch_attend(const Attend& p, const Sizes& z, hipStream_t stream) {
   else if (z.many)
     many_rows_kernel<T, D><<<many, kThreads, 0, stream>>>(p);
   else
-    few_rows_kernel<T, D><<<static_cast<uint32_t>(ceil_div(std::min(z.items[0], z.target[0]), 4)), kThreads, 0, stream>>>(p);
+    few_rows_kernel<T, D><<<static_cast<uint32_t>(std::max(ceil_div(std::min(z.items[0], z.waves), 4),
+                                                           std::min<int64_t>(z.items[0], kCus))),
+                            kThreads, 0, stream>>>(p);
   const int64_t rows = static_cast<int64_t>(p.tokens) * p.heads;
   if (rows <= 4 * kCus)
     join_kernel<T, D, 4><<<static_cast<uint32_t>(rows), kThreads, 0, stream>>>(p);
