@@ -65,6 +65,12 @@ __device__ __forceinline__ int64_t load_index(const void* p, int64_t i, int is64
   return static_cast<int64_t>(static_cast<const int32_t*>(p)[is64 ? 2 * i : i]);
 }
 
+// The same, all 64 bits of it: for indices that only the device checks.
+__device__ __forceinline__ int64_t load_index64(const void* p, int64_t i, int is64) {
+  if (is64) return static_cast<const int64_t*>(p)[i];
+  return static_cast<const int32_t*>(p)[i];
+}
+
 // x / d and x % d for 0 <= x < 2^32: a shift and a mask when d is a power of
 // two (frame sizes, granularities), a 32-bit division otherwise -- never the
 // long 64-bit division sequence.  The host checks that the offsets fit.

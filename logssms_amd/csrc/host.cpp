@@ -616,6 +616,9 @@ PyObject* append_paged_kv(PyObject*, PyObject* const* args, Py_ssize_t n) {
     check_cache(k_cache, k, heads, dim);
     check_cache(v_cache, k, heads, dim);
     require(v_cache.size(0) == k_cache.size(0) && v_cache.size(1) == k_cache.size(1), "caches of one size");
+    for (const at::Tensor* cache : {&k_cache, &v_cache})
+      for (int64_t d = 0; d < 3; ++d)
+        require(cache->size(d) <= 1 || cache->stride(d) >= dim, "a cache's rows must not overlap");
     const at::Tensor slots = indices(tensor(args[4]), tokens, k, "slots must be [tokens]");
     Turns t;
     require((args[5] == Py_None) == (args[6] == Py_None), "positions go with a rotation");

@@ -84,6 +84,7 @@ struct Attend {
   float* sums[2];
   float2* stats[2];
   int items_max[2];
+  int few_rows;         // rows kept of an item of few: no segment has more
   float per_target[2];  // key heads over the number of items wanted
   struct Place* places;  // of each segment, for the joining kernel
 };
@@ -106,6 +107,10 @@ struct Segment {
 __device__ __forceinline__ int uniform(int v) { return __builtin_amdgcn_readfirstlane(v); }
 __device__ __forceinline__ int clampi(int64_t v, int lo, int hi) {
   return static_cast<int>(v < lo ? lo : v > hi ? hi : v);
+}
+// A length as it is given, which may be behind the end of the table or below zero.
+__device__ __forceinline__ int length_of(const Attend& p, int request) {
+  return clampi(load_index64(p.lens, request, p.lens_is64), INT32_MIN / 2, INT32_MAX);
 }
 __device__ __forceinline__ int token_of(const Attend& p, int request) {
   return p.cu ? clampi(load_index(p.cu, request, p.cu_is64), 0, p.tokens) : request;
@@ -135,7 +140,7 @@ __device__ __forceinline__ Segment segment(const Attend& p, int s) {
   const int shared = p.shared ? p.num_groups : 0;
   const bool own = s >= shared;
   const int request = own ? s - shared : 0, g = !own ? s : p.num_groups > 1 ? group_of(p, request) : 0;
-  const int64_t length = load_index(p.lens, request, p.lens_is64);
+  const int length = length_of(p, request);
   int r0 = 0, r1 = p.requests, common = 0;
   if (shared > 0 && g >= 0) {
     r0 = group_start(p, g), r1 = group_start(p, g + 1);
@@ -148,7 +153,7 @@ __device__ __forceinline__ Segment segment(const Attend& p, int s) {
   seg.lo = own && in ? common : 0;
   seg.hi = own ? clampi(length, 0, p.capacity) : common;
   seg.request = own ? request : min(r0, p.requests - 1);
-  seg.length = own ? static_cast<int>(length) : 0;
+  seg.length = own ? length : 0;
   seg.group = own && in ? g : -1;
   return seg;
 }
@@ -296,7 +301,7 @@ __device__ __forceinline__ int schedule(const Attend& p, Plan& plan, Choice* cho
       } else if (pass == 1) {
         items += c.tiles * p.kv_heads * ranges;
       } else {
-        if ((seg.tokens * p.per > kFew) == MANY)
+        if ((seg.tokens * p.per > kFew) == MANY || p.items_max[0] == 0)  // the kind's, or all in a launch of one kind
           p.places[s] = {before, ranges, seg.token, seg.tokens, seg.lo, seg.hi, seg.group};
         before += c.tiles * p.kv_heads * ranges;
       }
@@ -434,8 +439,8 @@ __device__ __forceinline__ Spot find(const Attend& p, int request, int at, int e
   if (at >= end) return {-1, 0};
   const uint32_t index = p.page.div(at);
   const int64_t entry = static_cast<int64_t>(request) * p.table_row + index;
-  const int id = static_cast<int>(load_index(p.table, entry, p.table_is64));
-  return {id < 0 || id >= p.pages ? -1 : id, at - static_cast<int>(index * p.page.d)};
+  const int64_t id = load_index64(p.table, entry, p.table_is64);
+  return {id < 0 || id >= p.pages ? -1 : static_cast<int>(id), at - static_cast<int>(index * p.page.d)};
 }
 // The same of 64 times 16 positions, one in each lane, in bytes of a cache, looked up
 // together so that the steps' loads wait for no table.
@@ -686,7 +691,7 @@ struct Rows {
         }
       }
       r = min(r, p.requests - 1);
-      length = static_cast<int>(load_index(p.lens, r, p.lens_is64));
+      length = length_of(p, r);
       behind = next - 1 - token;
     }
     const int seen = clampi(static_cast<int64_t>(length) - behind, 0, it.seg.hi);
@@ -1094,7 +1099,7 @@ __device__ __forceinline__ void few_rows(const Attend& p, char* lds, int block, 
       load_v(step + 1);
     }
     if (searched && uniform(bad.found)) rows.add_not_finite(bad, lane);
-    rows.put(p, it, lane & 31, 0, static_cast<int64_t>(item) * kFew + (lane & 31), lane);
+    rows.put(p, it, lane & 31, 0, static_cast<int64_t>(item) * p.few_rows + (lane & 31), lane);
     wait_loads<0>();  // those past the end too
   }
 }
@@ -1176,7 +1181,7 @@ __global__ __launch_bounds__(kThreads) void join_kernel(Attend p) {
     if (piece < pieces) {
       const int which = piece >= count[0], kind = which ? many[1] : many[0];
       const int item = which ? first[1] + (piece - count[0]) * tiles[1] : first[0] + piece * tiles[0];
-      const int64_t to = static_cast<int64_t>(clampi(item, 0, p.items_max[kind] - 1)) * (kind ? Many<D>::kRows : kFew) +
+      const int64_t to = static_cast<int64_t>(clampi(item, 0, p.items_max[kind] - 1)) * (kind ? Many<D>::kRows : p.few_rows) +
                          (which ? row[1] : row[0]);
       st = p.stats[kind][to];
       from = reinterpret_cast<uint64_t>(p.sums[kind] + to * D);
@@ -1245,7 +1250,7 @@ inline int64_t aligned(int64_t n) { return (n + 255) / 256 * 256; }
 
 struct Sizes {
   bool few, many;  // whether segments of that kind can be there
-  int64_t items[2], target[2], waves;
+  int64_t items[2], target[2], waves, few_rows;
   int64_t sums[2], stats[2], places, bytes;  // offsets
 };
 
@@ -1265,7 +1270,8 @@ Sizes sizes_of(int64_t tokens, int64_t requests, int64_t groups, int64_t heads, 
   z.target[0] = 3 * kCus;
   z.target[1] = kCus * (dim == 256 ? 1 : 2);  // blocks
   z.waves = 4 * kCus * (dim == 256 ? 1 : dim == 128 || z.many ? 2 : 3);  // of few rows, that run at once
-  const int64_t few_tiles = requests + groups, many_tiles = sets * (rows / 128 + std::min(requests + groups, rows / kFew + 1));
+  z.few_rows = varlen || groups > 0 ? kFew : std::min<int64_t>(per, kFew);
+  const int64_t few_tiles = std::min(requests, tokens) + std::min(groups, tokens), many_tiles = sets * (rows / 128 + std::min(requests + groups, rows / kFew + 1));
   z.items[0] = z.few ? z.target[0] + z.target[0] / 64 + few_tiles * kv_heads : 0;
   z.items[1] = z.many ? 4 * z.target[1] + many_tiles * kv_heads : 0;
   int64_t at = 0;
@@ -1275,7 +1281,7 @@ Sizes sizes_of(int64_t tokens, int64_t requests, int64_t groups, int64_t heads, 
     return from;
   };
   for (int kind = 0; kind < 2; ++kind) {
-    const int64_t n = z.items[kind] * (kind ? 128 : kFew);
+    const int64_t n = z.items[kind] * (kind ? 128 : z.few_rows);
     z.sums[kind] = take(n * dim * 4);
     z.stats[kind] = take(n * 8);
   }
@@ -1338,9 +1344,10 @@ extern "C" int gdn_paged_attention(const void* q, int64_t q_token_stride, int64_
     set_error("head dims 64, 128 and 256");
     return GDN_ERR_UNSUPPORTED;
   }
-  if (tokens * heads >= (int64_t{1} << 31) || requests + groups >= (int64_t{1} << 24) ||
+  // 64 threads a row in a launch
+  if (tokens * heads >= (int64_t{1} << 26) || requests + groups >= (int64_t{1} << 24) ||
       table_width * page_size > (int64_t{1} << 27) || pages >= (int64_t{1} << 31) || kv_heads > (1 << 16)) {
-    set_error("up to 2^31 rows, 2^24 requests, 2^27 positions, 2^31 pages and 2^16 key heads");
+    set_error("up to 2^26 rows, 2^24 requests, 2^27 positions, 2^31 pages and 2^16 key heads");
     return GDN_ERR_UNSUPPORTED;
   }
   if (tokens == 0 || requests == 0) return GDN_OK;
@@ -1386,6 +1393,7 @@ extern "C" int gdn_paged_attention(const void* q, int64_t q_token_stride, int64_
     p.per_target[kind] = static_cast<float>(static_cast<double>(kv_heads) / static_cast<double>(z.target[kind]));
   }
   p.places = reinterpret_cast<Place*>(ws + z.places);
+  p.few_rows = static_cast<int>(z.few_rows);
   auto go = [&](auto type) {
     using T = decltype(type);
     const hipStream_t on = static_cast<hipStream_t>(stream);

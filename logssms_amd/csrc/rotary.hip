@@ -82,7 +82,7 @@ __global__ __launch_bounds__(kThreads) void rotary_kernel(Turn p) {
   const int half = p.rotated / 2;
   for (int i = threadIdx.x; i < count * half; i += kThreads) {
     const int t = i / half, pair = i - t * half;
-    const double position = static_cast<double>(load_index(p.positions, t0 + t, p.positions_is64));
+    const double position = static_cast<double>(load_index64(p.positions, t0 + t, p.positions_is64));
     double turns = position * p.turns[pair];
     turns -= rint(turns);
     float s, c;
@@ -91,7 +91,7 @@ __global__ __launch_bounds__(kThreads) void rotary_kernel(Turn p) {
   }
   if (p.slots)
     for (int t = threadIdx.x; t < count; t += kThreads) {
-      const int64_t slot = load_index(p.slots, t0 + t, p.slots_is64);
+      const int64_t slot = load_index64(p.slots, t0 + t, p.slots_is64);
       const bool in = slot >= 0 && slot < p.capacity;
       place[t][0] = in ? static_cast<int64_t>(p.page.div(static_cast<uint32_t>(slot))) : int64_t{-1};
       place[t][1] = in ? static_cast<int64_t>(p.page.mod(static_cast<uint32_t>(slot))) : int64_t{0};
@@ -188,12 +188,12 @@ int launch_turn(Turn& p, int dtype, hipStream_t stream) {
   const int v = wide ? vec : 1, turned = wide && p.interleaved ? p.rotated / v : p.rotated / 2 / v;
   const int units = turned + (p.dim - p.rotated) / v;
   p.per_block = std::max(1, kThreads / units);
-  const int64_t blocks = (p.tokens + p.per_block - 1) / p.per_block;
+  const int64_t blocks = (static_cast<int64_t>(p.tokens) + p.per_block - 1) / p.per_block;
   const int64_t heads = p.first[3], share = (heads * blocks + 4095) / 4096 * 4;
   p.heads_a_block = static_cast<int>(std::min<int64_t>(heads, share));
   const dim3 grid(static_cast<uint32_t>(blocks), static_cast<uint32_t>((heads + p.heads_a_block - 1) / p.heads_a_block));
-  if (grid.y > 65535) {
-    set_error("too many heads");
+  if (grid.y > 65535 || blocks >= (int64_t{1} << 24)) {  // 2^32 threads of a launch
+    set_error("too many heads or tokens");
     return GDN_ERR_UNSUPPORTED;
   }
   auto go = [&](auto kernel) { kernel<<<grid, kThreads, 0, stream>>>(p); };

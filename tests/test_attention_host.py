@@ -250,3 +250,24 @@ def test_c_entries_refuse_without_launching():
     assert turn(tokens=0, q=None) == 0 and turn(heads=0) == 0
     assert lib.gdn_paged_attention_workspace_bytes(0, 3, 0, 4, 2, 64, 0) == 0
     assert lib.gdn_paged_attention_workspace_bytes(3, 3, 0, 4, 2, 64, 0) > 0
+
+
+def test_append_refuses_caches_on_top_of_themselves():
+    from logssms_amd.kernel import append_paged_kv
+    _built()
+    k, cache, slots = torch.zeros(4, 2, 32), torch.zeros(5, 8, 2, 32), torch.arange(4)
+    for view in (cache[:1].expand(5, 8, 2, 32), cache[:, :1].expand(5, 8, 2, 32), cache[:, :, :1].expand(5, 8, 2, 32),
+                 torch.zeros(5 * 8 * 2 * 32).as_strided((5, 8, 2, 32), (512, 64, 16, 1))):
+        for caches in ((view, cache), (cache, view)):
+            with pytest.raises(AssertionError, match="overlap"):
+                append_paged_kv(k, k, *caches, slots)
+
+
+def test_more_rows_than_a_launch_has_threads_for():
+    lib = _built()
+    assert _attend(lib, tokens=1 << 24, requests=1 << 24) == 2  # 2^26 rows
+    d = 0x10000
+    turn = dict(q=d, qt=64, qh=32, heads=2, k=None, kt=0, kh=0, k_heads=0, dtype=1, tokens=3, dim=32, pos=d, pd=0, turns=d,
+                rotated=16, inter=0, scale=1.0, qo=d, qot=64, qoh=32, ko=None, kot=0, koh=0, stream=None)
+    turn.update(dim=4096, tokens=1 << 24)
+    assert lib.gdn_apply_rotary(*turn.values()) == 2

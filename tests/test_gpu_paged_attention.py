@@ -480,3 +480,30 @@ def test_tables_and_lengths_that_are_views():
     lens = torch.tensor(b.lens, device=DEV)
     got = paged_attention(b.q.to(DEV), *b.caches(), wide[::2, 2:2 + b.width], lens)
     assert torch.equal(got, want)
+
+
+def test_indices_past_32_bits():
+    """Pages and lengths whose low halves would be others."""
+    b = Batch(49, 8, 2, 128, 16, [100, 64, 200, 33], new=[2, 40, 1, 3], shared=[32])
+    b.k, b.v = b.k.nan_to_num(0.5), b.v.nan_to_num(0.5, 0.5, 0.5)
+    b.table[:, 1] += 2 ** 32
+    b.table[2, 9] -= 2 ** 40
+    b.lens[0], b.lens[3] = 2 ** 32 + 5, -(2 ** 33) + 9
+    out, lse = b.run(index=torch.int64, return_lse=True)
+    b.check(out, lse)
+
+
+@pytest.mark.parametrize("heads", [3, 40])
+def test_empty_requests_and_tokens_of_nobody(heads):
+    """Few and many heads to a key head, requests without tokens among the others, at the start and the end."""
+    b = Batch(50, heads, 1, 64, 16, [20, 30, 9, 70, 64, 5], new=[0, 2, 0, 1, 3, 0], shared=[16, 64], groups=[1, 3, 5])
+    b.table[2, 0] = b.table[1, 0]
+    b.cu = b.cu + 2
+    b.q = torch.cat([b.q[:2], b.q, b.q[:1]])
+    for _ in range(3):
+        out = torch.full(b.q.shape, 7.0, dtype=b.io, device=DEV)
+        b.run(out=out)
+        out = out.cpu()
+        assert (out[:2] == 7).all() and (out[8:] == 7).all()
+        want, _, bound, _ = ref.attention(b.q, b.k, b.v, b.table, b.lens, b.cu, 0.125)
+        assert ((out.double() - want).abs() <= ref.attention_bound(want, bound, b.io))[2:8].all()

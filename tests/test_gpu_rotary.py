@@ -194,3 +194,22 @@ def test_append_in_a_graph_follows_its_slots():
         want_q = append_paged_kv(k, v, k_cache, v_cache, slots, positions=positions, rotary=rotary, q=k)
         assert torch.equal(got[0], k_cache) and torch.equal(got[1], v_cache) and torch.equal(got[2], want_q)
         torch.cuda.synchronize()
+
+
+def test_positions_and_slots_past_32_bits():
+    """Whose low halves would be others."""
+    from logssms_amd.kernel import append_paged_kv
+    rotary = _rotary(32)
+    positions = torch.tensor([2 ** 32 + 3, 2 ** 40 + 1, -(2 ** 33), 2 ** 31, 7])
+    slots = torch.tensor([2 ** 32 + 1, 3, -(2 ** 33) + 2, 2 ** 40, 0])
+    k, v, q = randn(3, 5, 2, 64, g=gen(11), dtype=torch.bfloat16).unbind(0)
+    _, k_cache, v_cache = _cache(4, 16, 2, 64, torch.bfloat16, True)
+    got = append_paged_kv(k.to(DEV), v.to(DEV), k_cache, v_cache, slots.to(DEV), positions=positions.to(DEV),
+                          rotary=_on(rotary), q=q.to(DEV))
+    _check(got, q, positions, rotary)
+    flat_k, flat_v = k_cache.cpu().reshape(-1, 2, 64), v_cache.cpu().reshape(-1, 2, 64)
+    _check(flat_k[[3, 0]], k[[1, 4]], positions[[1, 4]], rotary)
+    assert torch.equal(flat_v[[3, 0]], v[[1, 4]])
+    others = torch.ones(64, dtype=torch.bool)
+    others[[3, 0]] = False
+    assert (flat_k[others] == 7).all() and (flat_v[others] == 7).all()
