@@ -756,8 +756,10 @@ int gdn_fp8_linear(const void* x, int64_t x_row_stride, const float* x_scales, i
  *   q [tokens, q_heads, dim] and k [tokens, k_heads, dim] (NULL with no heads),
  *     unit channel stride, of `dtype` (f32, bf16, f16); q_out, k_out like them,
  *     or the operand itself, whole, in place.
- *   positions [tokens]; turns [rotated / 2] in 64 bits on the device.
- * GDN_ERR_UNSUPPORTED from 2^24 channels a token on and for dim above 4096.
+ *   positions [tokens], all 64 bits of them read where there are as many;
+ *   turns [rotated / 2] in 64 bits on the device.
+ * GDN_ERR_UNSUPPORTED from 2^24 channels a token on, for dim above 4096 and from
+ * 2^24 thread blocks on (256 threads, on pieces of 16 bytes of a head).
  */
 int gdn_apply_rotary(const void* q, int64_t q_token_stride, int64_t q_head_stride, int64_t q_heads, const void* k,
                      int64_t k_token_stride, int64_t k_head_stride, int64_t k_heads, int dtype, int64_t tokens,
@@ -768,7 +770,8 @@ int gdn_apply_rotary(const void* q, int64_t q_token_stride, int64_t q_head_strid
 /*
  * k_cache[slot / page_size, slot % page_size] = k turned as above, v_cache[...] = v,
  * for slot = slots[token]; nothing is written for a slot below 0 or from pages *
- * page_size on.  The slots of one call differ.  q (q_heads 0: none) is turned to q_out.
+ * page_size on (all 64 bits of int64 slots count).  The slots of one call differ.  q
+ * (q_heads 0: none) is turned to q_out.
  *   k, v [tokens, kv_heads, dim]; caches [pages, page_size, kv_heads, dim] with
  *   unit channel stride.  rotated 0 (positions and turns unused): k and q as they are.
  */
@@ -798,7 +801,10 @@ int gdn_append_paged_kv(const void* k, int64_t k_token_stride, int64_t k_head_st
  *   q, out [tokens, heads, dim] bf16 or f16, caches [pages, page_size, kv_heads,
  *   dim] alike, unit channel stride, rows at multiples of 16 bytes (out: 8);
  *   page_size a multiple of 16; lse fp32 [tokens, heads] (natural logarithm) or NULL.
- * dim 64, 128 or 256 (GDN_ERR_UNSUPPORTED beyond).  Sums and statistics are fp32;
+ * dim 64, 128 or 256, fewer than 2^26 rows (tokens x heads), requests and groups
+ * fewer than 2^24, up to 2^27 positions and 2^16 key heads (GDN_ERR_UNSUPPORTED
+ * beyond).  All 64 bits of int64 pages and lengths count; the offsets and shared
+ * lengths lie in the int32 range.  Sums and statistics are fp32;
  * the softmax's weights are rounded to the io type in front of the product with v.
  * workspace: gdn_paged_attention_workspace_bytes, varlen 1 with cu_seqlens.
  */
