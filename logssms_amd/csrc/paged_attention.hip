@@ -414,6 +414,53 @@ __device__ Item item_of(const Attend& p, const Plan& plan, int item) {
   }
 }
 
+// Up to 64 segments of few rows: every wave counts the same items for itself, a segment a
+// lane, without barriers and LDS (one request of 4096 positions, 16/2 heads of 256: 17.0
+// us, 18.0 by the general way; 40 of 700, 8/8 heads of 64: 18.2 and 19.8).
+struct Lane {
+  Segment seg;
+  int base, ranges, range;  // items before it, its ranges, units of a range of all
+};
+template <int ROWS, int UNIT>
+__device__ __forceinline__ int count_few(const Attend& p, Lane& mine, bool notes, int lane) {
+  const int n = segments_of(p);
+  Cut c{0, 0, 0};
+  if (lane < n) {
+    mine.seg = segment(p, lane);
+    c = cut_of<false, ROWS, UNIT>(p, mine.seg, lane >= n - p.requests);
+  }
+  const float here = static_cast<float>(c.tiles) * static_cast<float>(c.units + c.least) * 0.5f;
+  const float units = head_sum<64>(here) * p.per_target[0];
+  mine.range = static_cast<int>(fminf(units, 1.0e9f)) + 1;
+  mine.ranges = ranges_of(c.units, mine.range);
+  const int items = c.tiles * p.kv_heads * mine.ranges;
+  int sum = items;
+#pragma unroll
+  for (int off = 1; off < 64; off <<= 1) {
+    const int below = __shfl_up(sum, off, 64);
+    if (lane >= off) sum += below;
+  }
+  mine.base = sum - items;
+  if (notes && lane < n && mine.seg.tokens * p.per <= kFew)
+    p.places[lane] = {mine.base, mine.ranges, mine.seg.token, mine.seg.tokens, mine.seg.lo, mine.seg.hi, mine.seg.group};
+  return min(__builtin_amdgcn_readlane(sum, 63), p.items_max[0]);
+}
+template <int UNIT> __device__ __forceinline__ Item item_of_few(const Attend& p, const Lane& mine, int item) {
+  const int s = __popcll(__ballot(mine.base <= item)) - 1;  // the last whose base is at most `item`
+  auto of = [&](int v) __attribute__((always_inline)) { return __builtin_amdgcn_readlane(v, s); };
+  Item it;
+  it.seg = {of(mine.seg.token),   of(mine.seg.tokens), of(mine.seg.lo),   of(mine.seg.hi),
+            of(mine.seg.request), of(mine.seg.length), of(mine.seg.group)};
+  it.ranges = of(mine.ranges);
+  it.own = s >= segments_of(p) - p.requests;
+  it.tile = 0;
+  const int across = item - of(mine.base), range = uniform(mine.range);
+  it.head = uniform(short_div(across, max(1, it.ranges)));
+  it.from = (it.seg.lo & ~15) + (across - it.head * max(1, it.ranges)) * range * UNIT;
+  it.to = min(it.seg.hi, it.from + range * UNIT);
+  return it;
+}
+
 // ------------------------------------------------------------------ matrix instructions and loads
 template <class T> struct Op;
 template <> struct Op<bf16> {
@@ -1006,8 +1053,8 @@ __device__ __forceinline__ void many_rows(const Attend& p, char* lds, int block,
 // three waves a CU are about enough.  Each wave takes items of its own, in LDS of its own for 32 positions' keys and values;
 // the next keys are loaded when these have become scores, the next values when
 // these have been summed.  There is no barrier among the waves.  One request of 4096
-// positions, 16/2 heads of 256, is bound by what follows one another: 3 us to the
-// schedule, 3 to the first loads, 3 for a step and its piece, 2 to the joining kernel's
+// positions, 16/2 heads of 256, is bound by what follows one another: 2 us to count the
+// items, 3 to the first loads, 3 for a step and its piece, 2 to the joining kernel's
 // launch and 6 in it.
 template <int D> struct Few {
   static constexpr int kHalf = 32 * 2 * D, kWave = 2 * kHalf, kLoads = kHalf / 1024;
@@ -1025,7 +1072,10 @@ __device__ __forceinline__ void few_rows(const Attend& p, char* lds, int block, 
   char* const values = keys + F::kHalf;
   NotFinite<D>& bad = reinterpret_cast<NotFinite<D>*>(lds + 4 * F::kWave)[wave];
   Plan& plan = *reinterpret_cast<Plan*>(lds + 4 * (F::kWave + sizeof(bad)));
-  const int total = schedule<false, kFew, 32>(p, plan, nullptr, block, blocks);
+  const bool small = segments_of(p) <= 64;  // the same in all blocks
+  Lane mine{};
+  const int total = small ? count_few<kFew, 32>(p, mine, block == 0 && wave == 0, lane)
+                          : schedule<false, kFew, 32>(p, plan, nullptr, block, blocks);
   const int of_k = lane_k<D>(lane), of_v = lane_v<D>(lane);
   // neighbours in the order of items share keys or a table, or lie side by side: in one
   // block (64 requests of 4096 positions, 32/8 heads of 128: 188 us, 215 with a block's
@@ -1033,7 +1083,7 @@ __device__ __forceinline__ void few_rows(const Attend& p, char* lds, int block, 
   // heads of 256: 16.3 us, 18.3 with four to a block)
   const int each = min(4, (total + kCus - 1) / kCus);
   for (int item = wave < each ? block * each + wave : total; item < total; item += blocks * each) {
-    const Item it = item_of<false, kFew, 32>(p, plan, item);
+    const Item it = small ? item_of_few<32>(p, mine, item) : item_of<false, kFew, 32>(p, plan, item);
     const int end = it.seg.hi, steps = (it.to - it.from + 31) / 32;
     R rows;
     rows.fetch(p, it, lane & 31, lane);
