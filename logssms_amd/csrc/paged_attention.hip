@@ -205,8 +205,8 @@ struct Choice {
 static_assert(sizeof(Plan) % 8 == 0, "what lies behind it is aligned");
 
 // n / d for d > 0 where the quotient is at most 2^22 (there are up to 2^27 positions, 2^22
-// steps): shorter than the exact division,
-// and what a launch runs once it has to fetch first.
+// steps): shorter than the exact division, and what a launch runs once it has to fetch
+// first.
 __device__ __forceinline__ int short_div(int n, int d) {
   int q = static_cast<int>(static_cast<float>(n) * __builtin_amdgcn_rcpf(static_cast<float>(d)));
   const int r = n - q * d;

@@ -507,3 +507,14 @@ def test_empty_requests_and_tokens_of_nobody(heads):
         assert (out[:2] == 7).all() and (out[8:] == 7).all()
         want, _, bound, _ = ref.attention(b.q, b.k, b.v, b.table, b.lens, b.cu, 0.125)
         assert ((out.double() - want).abs() <= ref.attention_bound(want, bound, b.io))[2:8].all()
+
+
+@pytest.mark.parametrize("requests", [1, 62, 63, 64, 65, 255, 256])
+@pytest.mark.parametrize("new", [1, 4])
+def test_as_many_segments_as_lanes_and_threads(requests, new):
+    """One more or fewer than are counted at once; a group, and tokens of nobody's group."""
+    lens = [32 + (5 * r) % 40 + new for r in range(requests)]
+    b = Batch(51 + requests, 4, 2, 64, 16, lens, new=None if new == 1 else [new] * requests, shared=[32],
+              groups=[requests // 3, requests])
+    out, lse = b.run(return_lse=True)
+    b.check(out, lse)
