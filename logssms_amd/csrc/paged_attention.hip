@@ -51,10 +51,11 @@ typedef __attribute__((address_space(3))) void lds_void;
 constexpr int kFew = 32;
 constexpr int kThreads = 256;  // of every kernel here
 constexpr int kCus = 256;
-// What an item of many rows costs beside its steps, in steps, and what a piece to be joined
-// costs more.  (A prompt of 1024 tokens, 16/2 heads of 256: 46 us, 58 with kPiece 16; one
-// of 2048 77 us, 112 with kItem 5 and kPiece 8; kItem 20 changes neither.)
-constexpr float kItem = 10.f, kPiece = 32.f;
+// What an item of many rows costs beside its steps, in steps, what a piece to be joined
+// costs more, and what it costs that there are any.  (A prompt of 1024 tokens, 16/2 heads
+// of 256, is not split so: 47 us; 58 where it was, at a price of pieces that was half of
+// theirs.  One of 2048 77 us, 112 with half of all of them.)
+constexpr float kItem = 10.f, kPiece = 16.f, kJoin = 12.f;
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 constexpr float kLater = 8.0f;  // a maximum may lag by 2^8 before the sums are rescaled
 
@@ -185,19 +186,22 @@ __device__ __forceinline__ Cut cut_of(const Attend& p, const Segment& seg, bool 
 }
 
 // ------------------------------------------------------------------ schedule
-constexpr int kCandidates = 16;
+constexpr int kCandidates = 32;
 struct alignas(16) Plan {
   int base[kThreads];  // items before each thread's segments
   Segment segments[kThreads];  // each thread's first one: all, of up to kThreads
   float units[kThreads / 64];
   int count[kThreads / 64];
-  int range;           // units of a range of keys
+  int range[2];        // units of a range of shared keys, of a request's own
+  int alike;           // one segment of many rows: its items lie in the order of their lengths
 };
-// What the choice of the range looks at: segments (their tiles in all heads, units, least
-// units, whether nothing is to be joined if they are not split); of each candidate the
-// items, those that are not empty, those of them to be joined, the longest.
+// What the choice of the ranges looks at: segments (their tiles in all heads, units, least
+// units; 1: own, 2: nothing is to be joined if it is not split); of each candidate the
+// items, those that are not empty, those of them to be joined, the shared ones, the
+// longest of the shared and of the own.
 struct Choice {
-  int segments, items[kCandidates], filled[kCandidates], pieces[kCandidates], longest[kCandidates];
+  int segments, items[kCandidates], filled[kCandidates], pieces[kCandidates], shared[kCandidates];
+  int longest[2][kCandidates];
   int cuts[kThreads][4];
 };
 // One LDS array holds it all in a kernel with direct loads: beside a second one, the
@@ -215,22 +219,28 @@ __device__ __forceinline__ int short_div(int n, int d) {
 }
 __device__ __forceinline__ int ranges_of(int units, int range) { return short_div(units + range - 1, range); }
 
-// The range of keys for items of many rows: of sixteen candidates the one under which
-// the last block should end first, where a block takes one item of each round, and an
-// item costs its steps, kItem, and kPiece if its sums are joined.  Six prompts behind
-// 8192 shared positions, 16/2 heads of 256: 200 us, 272 in ranges of the length that
-// all the work gives a block.  (Equal parts of one line of all the work, whatever
-// tiles they cut, balance better still, but then no two blocks read the same keys at a
-// time, the L2 no longer serves them, and it took a third longer than equal ranges.)
-__device__ __forceinline__ int candidate(float units_a_block, int i) {
-  // none is split; otherwise 2, 1.71, 1.5, 1.33, 1.2 .. 0.25 times what a block gets
-  const float shares = i < 6 ? 0.5f + (i - 1) / 12.f : 0.91f + (i - 6) * (i - 6) * 0.038f;
-  return i == 0 ? 1 << 30 : static_cast<int>(units_a_block / shares) + 1;
+// The ranges of keys for items of many rows: of 32 candidates the one under which the
+// last block should end first.  Shared items come first and are alike, a block takes
+// one of each round; a request's own ones fill what these leave, but for half of their
+// longest.  An item costs its steps, kItem, and kPiece if its sums are joined.  (Six
+// prompts behind 8192 shared positions, 16/2 heads of 256: 272 us in ranges of the
+// length that all the work gives a block.  Equal parts of one line of all the work,
+// whatever tiles they cut, balance better still, but then no two blocks read the same
+// keys at a time, the L2 no longer serves them, and it took a third longer than equal
+// ranges.)
+__device__ __forceinline__ int2 candidate(float units_a_block, int i) {
+  // none is split; otherwise 2, 1.71, 1.5, 1.33, 1.2 .. 0.25 times what a block gets; own ones alike or in eighths
+  const int which = i & 15;
+  const float shares = which < 6 ? 0.5f + (which - 1) / 12.f : 0.91f + (which - 6) * (which - 6) * 0.038f;
+  const int range = which == 0 ? 1 << 30 : static_cast<int>(units_a_block / shares) + 1;
+  return make_int2(range, i < 16 ? range : (range >> 3) + 1);
 }
 struct Outcome {
-  int items, filled, pieces, longest;
+  int items, filled, pieces, shared, longest, longest_own;
   // one more segment, `tiles` in all heads, under a range
-  __device__ __forceinline__ void add(int tiles, int units, int least, int alone, int range) {
+  __device__ __forceinline__ void add(int tiles, int units, int least, int kind, int2 limit) {
+    const bool own = kind & 1, alone = kind & 2;
+    const int range = own ? limit.y : limit.x;
     const int ranges = ranges_of(units, min(units, range)), length = ranges_of(units, ranges);
     // on average a tile sees half of the units between the fewest and all, and half of its last range
     const float mean = static_cast<float>(units + least) / static_cast<float>(2 * length) + (least < units ? 0.5f : 0.f);
@@ -238,22 +248,26 @@ struct Outcome {
     const int here = max(tiles, min(tiles * ranges, static_cast<int>(static_cast<float>(tiles) * mean + 0.5f)));
     filled += here;
     pieces += alone && ranges == 1 ? 0 : here;
-    longest = max(longest, length);
+    shared += own ? 0 : here;
+    longest = max(longest, own ? 0 : length), longest_own = max(longest_own, own ? length : 0);
   }
   __device__ __forceinline__ void put(Choice& to, int i) const {
     atomicAdd(&to.items[i], items);
     atomicAdd(&to.filled[i], filled);
     atomicAdd(&to.pieces[i], pieces);
-    atomicMax(&to.longest[i], longest);
+    atomicAdd(&to.shared[i], shared);
+    atomicMax(&to.longest[0][i], longest);
+    atomicMax(&to.longest[1][i], longest_own);
   }
 };
-__device__ __forceinline__ int choose(const Attend& p, const Choice& choice, float units, int lane, int blocks) {
+__device__ __forceinline__ int2 choose(const Attend& p, const Choice& choice, float units, int lane, int blocks) {
   int best = lane & (kCandidates - 1);
-  const float a_block = static_cast<float>(choice.filled[best]) / static_cast<float>(blocks), rounds = ceilf(a_block);
-  // rounds of items of the mean length, at least the longest
-  float time = fmaxf(rounds * units / fmaxf(a_block, 1e-9f), static_cast<float>(choice.longest[best])) + rounds * kItem +
-               ceilf(static_cast<float>(choice.pieces[best]) / static_cast<float>(blocks)) * kPiece;
-  if (choice.items[best] > p.items_max[1] && best > 0) time = INFINITY;
+  const float each = 1.f / static_cast<float>(blocks), own = static_cast<float>(choice.longest[1][best]);
+  float time = units + static_cast<float>(choice.filled[best]) * each * kItem + (own > 0.f ? 0.5f * (own + kItem) : 0.f);
+  time = fmaxf(time, own + kItem);
+  time = fmaxf(time, ceilf(static_cast<float>(choice.shared[best]) * each) * (static_cast<float>(choice.longest[0][best]) + kItem));
+  if (choice.pieces[best] > 0) time += kJoin + static_cast<float>(choice.pieces[best]) * each * kPiece;
+  if (choice.items[best] > p.items_max[1] && (best & 15) > 0) time = INFINITY;
 #pragma unroll
   for (int off = 1; off < kCandidates; off <<= 1) {
     const float other = __shfl_xor(time, off, 64);
@@ -271,9 +285,11 @@ template <bool MANY, int ROWS, int UNIT>
 __device__ __forceinline__ int schedule(const Attend& p, Plan& plan, Choice* choice, int block, int blocks) {
   const int n = segments_of(p), lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   float units = 0.f;  // the same in all blocks; its rounding is in the bound of the items
-  int items = 0, before = 0, total = 0, range = 1;
+  int items = 0, before = 0, total = 0;
+  int2 range = make_int2(1, 1);  // shared, own
   Segment first{}, second{};  // of this thread
   if (MANY) {
+    static_assert(sizeof(Choice) / 4 - 4 * kThreads <= kThreads, "a word a thread");
     if (threadIdx.x < sizeof(Choice) / 4 - 4 * kThreads) reinterpret_cast<int*>(choice)[threadIdx.x] = 0;
     __syncthreads();
   }
@@ -286,7 +302,8 @@ __device__ __forceinline__ int schedule(const Attend& p, Plan& plan, Choice* cho
       Segment seg = which == 0 ? first : second;
       if (pass == 0 || which > 1) seg = segment(p, s);
       const Cut c = cut_of<MANY, ROWS, UNIT>(p, seg, s >= segments_of(p) - p.requests);
-      const int ranges = ranges_of(c.units, MANY ? min(range, max(1, c.units)) : range);
+      const int limit = s >= n - p.requests ? range.y : range.x;
+      const int ranges = ranges_of(c.units, MANY ? min(limit, max(1, c.units)) : limit);
       if (pass == 0) {
         if (which == 0) first = seg;
         if (which == 1) second = seg;
@@ -295,7 +312,7 @@ __device__ __forceinline__ int schedule(const Attend& p, Plan& plan, Choice* cho
           const int to = atomicAdd(&choice->segments, 1);
           if (to < kThreads) {
             choice->cuts[to][0] = c.tiles * p.kv_heads, choice->cuts[to][1] = c.units, choice->cuts[to][2] = c.least;
-            choice->cuts[to][3] = s >= n - p.requests && seg.lo == 0;
+            choice->cuts[to][3] = s < n - p.requests ? 0 : seg.lo == 0 ? 3 : 1;
           }
         }
       } else if (pass == 1) {
@@ -317,7 +334,7 @@ __device__ __forceinline__ int schedule(const Attend& p, Plan& plan, Choice* cho
         // of more segments than that, every one is split alike
         if (choice->segments <= kThreads) {
           const int i = threadIdx.x & (kCandidates - 1);
-          Outcome outcome{0, 0, 0, 0};
+          Outcome outcome{0, 0, 0, 0, 0, 0};
           for (int e = threadIdx.x / kCandidates; e < choice->segments; e += kThreads / kCandidates)
             outcome.add(choice->cuts[e][0], choice->cuts[e][1], choice->cuts[e][2], choice->cuts[e][3],
                         candidate(units, i));
@@ -328,7 +345,7 @@ __device__ __forceinline__ int schedule(const Attend& p, Plan& plan, Choice* cho
           range = candidate(units, 1);
         }
       } else {
-        range = static_cast<int>(fminf(units, 1.0e9f)) + 1;
+        range.x = range.y = static_cast<int>(fminf(units, 1.0e9f)) + 1;
       }
     } else if (pass == 1) {
       int sum = items;
@@ -346,30 +363,15 @@ __device__ __forceinline__ int schedule(const Attend& p, Plan& plan, Choice* cho
         total += plan.count[w];
       }
       plan.base[threadIdx.x] = before;
-      if (threadIdx.x == 0) plan.range = range;
+      if (threadIdx.x == 0) {
+        plan.range[0] = range.x, plan.range[1] = range.y;
+        if (MANY) plan.alike = choice->segments <= 1;
+      }
       if (block > 0) break;
     }
   }
   __syncthreads();
   return min(total, p.items_max[MANY]);
-}
-
-// The order of a segment's tiles of many rows: the last first, since in prompts it sees
-// the most, and in eight runs of every eighth tile, so that each XCD, which takes a run of
-// items, gets its share of long and short ones.
-__device__ __forceinline__ int tile_at(int place, int tiles) {
-  const int each = tiles >> 3, more = tiles & 7, longer = more * (each + 1);
-  int run, in;
-  if (place < longer) {
-    run = short_div(place, each + 1), in = place - run * (each + 1);
-  } else {
-    run = short_div(place - longer, max(1, each)), in = place - longer - run * each, run += more;
-  }
-  return tiles - 1 - (8 * in + run);
-}
-__device__ __forceinline__ int place_of(int tile, int tiles) {
-  const int back = tiles - 1 - tile, run = back & 7;
-  return run * (tiles >> 3) + min(run, tiles & 7) + (back >> 3);
 }
 
 struct Item {
@@ -380,38 +382,58 @@ struct Item {
   bool own;        // of a request, not of a group
 };
 
-// Called by whole waves: what it finds is the same in all lanes, and kept in scalar registers.
+// The item that is `at` among those of a thread's segments.  Items of many rows lie with the
+// last tiles, which see the most, first; of each tile the ranges of keys, of each
+// range the heads.
 template <bool MANY, int ROWS, int UNIT>
-__device__ Item item_of(const Attend& p, const Plan& plan, int item) {
-  static_assert(kThreads == 256, "four bases a lane");
-  const int lane = threadIdx.x & 63, range = uniform(plan.range), n = segments_of(p);
-  int thread = -1;  // the last whose base is at most `item`
-#pragma unroll
-  for (int i = 0; i < 4; ++i) thread += __popcll(__ballot(plan.base[4 * lane + i] <= item));
-  thread = uniform(thread);
-  int at = item - uniform(plan.base[thread]);
+__device__ __forceinline__ Item item_at(const Attend& p, const Plan& plan, int thread, int at) {
+  const int n = segments_of(p);
   for (int s = thread;; s += kThreads) {
     const Segment seg = s == thread ? plan.segments[thread] : segment(p, s);
-    const Cut c = cut_of<MANY, ROWS, UNIT>(p, seg, s >= segments_of(p) - p.requests);
-    const int ranges = uniform(ranges_of(c.units, MANY ? min(range, max(1, c.units)) : range));
-    const int tiles = uniform(c.tiles), items = tiles * p.kv_heads * ranges;
+    const bool own = s >= n - p.requests;
+    const Cut c = cut_of<MANY, ROWS, UNIT>(p, seg, own);
+    const int limit = plan.range[own];
+    const int ranges = ranges_of(c.units, MANY ? min(limit, max(1, c.units)) : limit), items = c.tiles * p.kv_heads * ranges;
     if (at < items || s + kThreads >= n) {
       Item it;
-      it.seg = {uniform(seg.token), uniform(seg.tokens), uniform(seg.lo),
-                uniform(seg.hi),    uniform(seg.request), uniform(seg.length), uniform(seg.group)};
-      it.ranges = ranges;
-      it.own = s >= n - p.requests;
-      const int across = uniform(short_div(at, max(1, tiles)));
-      const int length = MANY ? uniform(ranges_of(c.units, max(1, ranges))) : range;
-      it.tile = at - across * max(1, tiles);
-      if (MANY) it.tile = uniform(tile_at(it.tile, tiles));
-      it.head = uniform(short_div(across, max(1, ranges)));
-      it.from = (it.seg.lo & ~15) + (across - it.head * max(1, ranges)) * length * UNIT;
-      it.to = min(it.seg.hi, it.from + length * UNIT);
+      it.seg = seg, it.ranges = ranges, it.own = own;
+      const int each = max(1, ranges), length = MANY ? ranges_of(c.units, each) : limit;
+      int range;
+      if (MANY) {
+        const int rest = short_div(at, p.kv_heads), back = short_div(rest, each);
+        it.head = at - rest * p.kv_heads, range = rest - back * each, it.tile = max(0, c.tiles - 1 - back);
+      } else {
+        it.head = short_div(at, each), range = at - it.head * each, it.tile = 0;
+      }
+      it.from = (seg.lo & ~15) + range * length * UNIT;
+      it.to = min(seg.hi, it.from + length * UNIT);
       return it;
     }
     at -= items;
   }
+}
+// Called by whole waves: what it finds is the same in all lanes, and kept in scalar registers.
+template <bool MANY, int ROWS, int UNIT>
+__device__ Item item_of(const Attend& p, const Plan& plan, int item) {
+  static_assert(kThreads == 256, "four bases a lane");
+  const int lane = threadIdx.x & 63;
+  int thread = -1;  // the last whose base is at most `item`
+#pragma unroll
+  for (int i = 0; i < 4; ++i) thread += __popcll(__ballot(plan.base[4 * lane + i] <= item));
+  thread = uniform(thread);
+  const Item it = item_at<MANY, ROWS, UNIT>(p, plan, thread, item - uniform(plan.base[thread]));
+  return {{uniform(it.seg.token), uniform(it.seg.tokens), uniform(it.seg.lo), uniform(it.seg.hi),
+           uniform(it.seg.request), uniform(it.seg.length), uniform(it.seg.group)},
+          uniform(it.head), uniform(it.tile), uniform(it.from), uniform(it.to), uniform(it.ranges), it.own};
+}
+// Steps of an item of many rows: nothing behind the last position that a row of its tile sees.
+template <int ROWS, int UNIT> __device__ __forceinline__ int steps_of(const Attend& p, const Item& it) {
+  int to = it.to;
+  if (it.own) {
+    const int last_token = min(it.seg.tokens - 1, static_cast<int>(p.by_per.div(it.tile * ROWS + ROWS - 1)));
+    to = clampi(static_cast<int64_t>(it.seg.length) - (it.seg.tokens - 1 - last_token), 0, to);
+  }
+  return to > it.from ? (to - it.from + UNIT - 1) / UNIT : 0;
 }
 
 // Up to 64 segments of few rows: every wave counts the same items for itself, a segment a
@@ -614,6 +636,31 @@ __device__ __forceinline__ void in_order() { __builtin_amdgcn_sched_barrier(0); 
 // The lane, found anew.
 __device__ __forceinline__ int lane_again() {
   return here(static_cast<int>(__builtin_amdgcn_mbcnt_hi(~0u, __builtin_amdgcn_mbcnt_lo(~0u, 0u))));
+}
+// The value of the lane 32 before or behind this one.
+__device__ __forceinline__ uint32_t other_half(uint32_t v) {
+  const auto halves = __builtin_amdgcn_permlane32_swap(v, v, false, false);
+  return halves[0] == v ? halves[1] : halves[0];
+}
+// How many lanes of the wave hold less.
+__device__ __forceinline__ int place_among(int v) {
+  int n = 0;
+#pragma unroll 8
+  for (int k = 0; k < 64; ++k) n += __builtin_amdgcn_readlane(v, k) < v ? 1 : 0;
+  return n;
+}
+// The least of a wave's lanes.
+__device__ __forceinline__ uint32_t min_of_wave(uint32_t v) {
+  auto step = [](uint32_t x, auto ctrl) __attribute__((always_inline)) {
+    return min(x, static_cast<uint32_t>(__builtin_amdgcn_update_dpp(-1, static_cast<int>(x), decltype(ctrl)::value, 0xf, 0xf, false)));
+  };
+  v = step(v, std::integral_constant<int, 0xB1>{});   // quad_perm [1,0,3,2]
+  v = step(v, std::integral_constant<int, 0x4E>{});   // quad_perm [2,3,0,1]
+  v = step(v, std::integral_constant<int, 0x141>{});  // row_half_mirror
+  v = step(v, std::integral_constant<int, 0x128>{});  // row_ror:8
+  const uint32_t a = __builtin_amdgcn_readlane(v, 0), b = __builtin_amdgcn_readlane(v, 16);
+  const uint32_t c = __builtin_amdgcn_readlane(v, 32), d = __builtin_amdgcn_readlane(v, 48);
+  return min(min(a, b), min(c, d));
 }
 // Of this lane's value and that of the lane 32 before or behind it.
 __device__ __forceinline__ float max_of_halves(float v) {
@@ -917,24 +964,84 @@ __device__ __forceinline__ void many_rows(const Attend& p, char* lds, int block,
   static_assert(sizeof(Choice) <= M::kLds, "in the place of the rings, before they are used");
   const int wave = uniform(threadIdx.x >> 6);
   const int total = schedule<true, M::kRows, M::kKeys>(p, plan, reinterpret_cast<Choice*>(lds), block, blocks);
-  // blocks with the same index modulo 8 share an XCD and its L2: neighbours in the order of items, which share keys
-  const int xcd = block & 7, last = static_cast<int>(static_cast<int64_t>(total) * (xcd + 1) / 8);
-  // to and fro: a block that has had a long one of a round's items gets a short one of the next
-  const int across = blocks >> 3, mine = block >> 3;
-  int round = static_cast<int>(static_cast<int64_t>(total) * xcd / 8);
-  for (bool back = false; round < last; round += across, back = !back) {
-    const int item = round + (back ? across - 1 - mine : mine);
-    if (item >= last) continue;  // whole block
+  // Blocks with the same index modulo 8 share an XCD and its L2.  It takes every eighth item
+  // (of one head, then, and often of one range of keys).  Of one segment they lie in the
+  // order of their lengths, and the blocks take them to and fro; of several each goes to the
+  // block that is free first: 64 at a time their steps are looked up, a lane each, put in
+  // order and given out.  (Three prompts of 700 tokens behind 4096 shared positions, 16/2
+  // heads of 256, 247 us, 407 where each XCD took a run of items and its blocks took them
+  // to and fro; six ragged ones behind 8192 194 to 198, 205; one prompt of 3000 tokens 108,
+  // 148.  Given out one after the other throughout, four prompts of 1000 tokens, 32/8
+  // heads of 128, took 101 us instead of 88, to and fro 82.)
+  constexpr bool kTwo = M::kBlocks == 2;
+  constexpr uint32_t kNoBlock = (1u << 25) - 1;
+  const int across = blocks >> 3, mine = block >> 3, xcd = block & 7, locals = (total + 7 - xcd) >> 3;
+  const bool alike = locals <= across || uniform(plan.alike);
+  uint32_t load = lane_again() < across ? 0 : kNoBlock;  // of a block: steps
+  uint64_t todo = 0;
+  bool back = false;
+  for (int base = alike ? -across : -64;;) {
+    while (todo == 0 && (base += alike ? across : 64) < locals) {
+      if (alike) {
+        const int at = back ? across - 1 - mine : mine;
+        if (base + at < locals) todo = uint64_t{1} << at;
+        back = !back;
+        continue;
+      }
+      const int id = lane_again(), count = min(64, locals - base);
+      int key = 63 - id;
+      if (id < count) {
+        const int item = 8 * (base + id) + xcd;
+        int thread = 0;  // the last whose base is at most the item
+#pragma unroll
+        for (int half = kThreads / 2; half > 0; half >>= 1)
+          if (plan.base[thread + half] <= item) thread += half;
+        const Item it = item_at<true, M::kRows, M::kKeys>(p, plan, thread, item - plan.base[thread]);
+        key |= (steps_of<M::kRows, M::kKeys>(p, it) + static_cast<int>(kItem)) << 6;
+      }
+      // the longest first, places behind the last item at the end
+      key = __builtin_amdgcn_ds_permute(4 * (63 - place_among(key)), key);
+      int k = 0;
+      if (base == 0) {  // the first round: one each; of a CU's two, a short one to the long one
+        k = across;
+        const int at = kTwo && id >= 32 ? 95 - id : id;
+        const int given = __shfl(key, at, 64);
+        if (id < k) load += given >> 6;
+        todo = uint64_t{1} << (63 - (__builtin_amdgcn_readlane(given, mine) & 63));
+      }
+      while (k < count) {
+        if (k % across == 0 && count - k >= across) {
+          // one each, the longest to the one with the least, if that evens them out
+          const int place = place_among(static_cast<int>(load << 6 | id));
+          const int given = __shfl(key, id < across ? k + place : 0, 64);
+          const uint32_t then = min(load + (given >> 6), kNoBlock - 1);
+          const float most = static_cast<float>(~min_of_wave(id < across ? ~then : ~0u));
+          const float all = head_sum<64>(id < across ? static_cast<float>(then) : 0.f);
+          if (most * static_cast<float>(across) <= 1.03f * all) {
+            if (id < across) load = then;
+            todo |= uint64_t{1} << (63 - (__builtin_amdgcn_readlane(given, mine) & 63));
+            k += across;
+            continue;
+          }
+        }
+        // two blocks of a CU go on at half the rate each until one is done
+        const uint32_t other = kTwo ? other_half(load) : load;
+        const int who = min_of_wave((load <= other ? 2 * load : load + other) << 6 | id) & 63;
+        const int next = __builtin_amdgcn_readlane(key, k);
+        if (id == who) load = min(load + (next >> 6), kNoBlock - 1);
+        if (who == mine) todo |= uint64_t{1} << (63 - (next & 63));
+        ++k;
+      }
+    }
+    if (todo == 0) break;
+    const int item = 8 * (base + __builtin_ctzll(todo)) + xcd;
+    todo &= todo - 1;
     const int lane = lane_again();  // what follows from it is not kept in registers from item to item
     const Item it = item_of<true, M::kRows, M::kKeys>(p, plan, item);
     R rows;
     const int row = it.tile * M::kRows + 32 * wave + (lane & 31);
     rows.fetch(p, it, row, lane);
-    // nothing behind the last position that a row of the tile sees
-    const int last_token = min(it.seg.tokens - 1, static_cast<int>(p.by_per.div(it.tile * M::kRows + M::kRows - 1)));
-    int to = it.to;
-    if (it.own) to = uniform(clampi(static_cast<int64_t>(it.seg.length) - (it.seg.tokens - 1 - last_token), 0, to));
-    const int end = it.seg.hi, steps = to > it.from ? (to - it.from + M::kKeys - 1) / M::kKeys : 0;
+    const int end = it.seg.hi, steps = uniform(steps_of<M::kRows, M::kKeys>(p, it));
     // A wave brings 16 positions of a step: of the keys or of the values, or (steps of 64) of both.  A
     // feed's loads of steps past the end are issued as well, with nothing in range, so that every step counts alike.
     constexpr bool kBoth = kTiles == 2;
@@ -1203,7 +1310,7 @@ __global__ __launch_bounds__(kThreads) void join_kernel(Attend p) {
   if (token < token_of(p, request) || token >= token_of(p, request + 1)) return;
   const int kv_head = p.by_per.div(head);
   // pieces of the shared segment, then of the own one
-  int many[2], first[2], tiles[2], count[2], row[2];
+  int many[2], first[2], apart[2], count[2], row[2];
 #pragma unroll
   for (int which = 0; which < 2; ++which) {
     count[which] = 0;
@@ -1214,9 +1321,9 @@ __global__ __launch_bounds__(kThreads) void join_kernel(Attend p) {
     if (which && place.ranges == 1 && place.lo == 0) return;  // the item wrote the row itself
     many[which] = rows > kFew;
     const int tile_rows = many[which] ? Many<D>::kRows : kFew;
-    tiles[which] = (rows + tile_rows - 1) / tile_rows;
-    const int tile = in / tile_rows;
-    first[which] = place.item + kv_head * place.ranges * tiles[which] + (many[which] ? place_of(tile, tiles[which]) : tile);
+    apart[which] = many[which] ? p.kv_heads : 1;
+    const int tile = in / tile_rows, back = (rows + tile_rows - 1) / tile_rows - 1 - tile;
+    first[which] = place.item + (many[which] ? back * place.ranges * p.kv_heads + kv_head : kv_head * place.ranges);
     row[which] = in % tile_rows;
     count[which] = place.ranges;
   }
@@ -1230,7 +1337,7 @@ __global__ __launch_bounds__(kThreads) void join_kernel(Attend p) {
     uint64_t from = 0;
     if (piece < pieces) {
       const int which = piece >= count[0], kind = which ? many[1] : many[0];
-      const int item = which ? first[1] + (piece - count[0]) * tiles[1] : first[0] + piece * tiles[0];
+      const int item = which ? first[1] + (piece - count[0]) * apart[1] : first[0] + piece * apart[0];
       const int64_t to = static_cast<int64_t>(clampi(item, 0, p.items_max[kind] - 1)) * (kind ? Many<D>::kRows : p.few_rows) +
                          (which ? row[1] : row[0]);
       st = p.stats[kind][to];
