@@ -518,3 +518,21 @@ def test_as_many_segments_as_lanes_and_threads(requests, new):
               groups=[requests // 3, requests])
     out, lse = b.run(return_lse=True)
     b.check(out, lse)
+
+
+@pytest.mark.parametrize("heads,kv_heads,dim,io", [(48, 16, 64, "f16"), (48, 16, 128, "bf16"), (16, 4, 256, "bf16")])
+def test_ragged_prompts_in_several_rounds(heads, kv_heads, dim, io):
+    """More tiles than run at once, of all lengths."""
+    new = [300, 40, 200, 1, 150, 60]
+    lens = [512 + n + 17 * i for i, n in enumerate(new)]
+    b = Batch(60 + dim, heads, kv_heads, dim, 64, lens, new=new, shared=[512], io=io)
+    out, lse = b.run(return_lse=True)
+    b.check(out, lse)
+
+
+def test_many_segments_in_several_rounds():
+    """More of many rows than threads, several to a block."""
+    lens = [20 + (r * 37) % 60 for r in range(300)]
+    b = Batch(61, 66, 2, 256, 16, lens)
+    out, lse = b.run(return_lse=True)
+    b.check(out, lse)
