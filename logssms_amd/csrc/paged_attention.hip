@@ -26,8 +26,8 @@
 //
 // Many rows are bound by the matrix cores and what feeds them, few rows by memory.
 // Measured on an MI355X (copies 4.9 TB/s, bf16 products of 8192^3 1205 TFLOP/s):
-// a prompt of 8192 tokens 840-900 TFLOP/s (dims 256, 128; 64: 680), 1024 requests
-// behind 16384 shared positions 780-840, 64 and 256 requests of 4096 and 1024
+// a prompt of 8192 tokens 900-1010 TFLOP/s (dims 256, 128; 64: 650-680), 1024 requests
+// behind 16384 shared positions 780-860, 64 and 256 requests of 4096 and 1024
 // positions with nothing shared 5.0-5.7 TB/s.
 #include <algorithm>
 
