@@ -190,7 +190,7 @@ constexpr int kCandidates = 32;
 struct alignas(16) Plan {
   int base[kThreads];  // items before each thread's segments
   Segment segments[kThreads];  // each thread's first one: all, of up to kThreads
-  float units[kThreads / 64];
+  float units[kThreads / 64], few[kThreads / 64];
   int count[kThreads / 64];
   int range[2];        // units of a range of shared keys, of a request's own
   int alike;           // one segment of many rows: its items lie in the order of their lengths
@@ -284,7 +284,7 @@ __device__ __forceinline__ int2 choose(const Attend& p, const Choice& choice, fl
 template <bool MANY, int ROWS, int UNIT>
 __device__ __forceinline__ int schedule(const Attend& p, Plan& plan, Choice* choice, int block, int blocks) {
   const int n = segments_of(p), lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  float units = 0.f;  // the same in all blocks; its rounding is in the bound of the items
+  float units = 0.f, few = 0.f;  // the same in all blocks; its rounding is in the bound of the items
   int items = 0, before = 0, total = 0;
   int2 range = make_int2(1, 1);  // shared, own
   Segment first{}, second{};  // of this thread
@@ -308,6 +308,7 @@ __device__ __forceinline__ int schedule(const Attend& p, Plan& plan, Choice* cho
         if (which == 0) first = seg;
         if (which == 1) second = seg;
         units += static_cast<float>(c.tiles) * static_cast<float>(c.units + c.least) * 0.5f;
+        if (MANY && c.tiles == 0) few += static_cast<float>(cut_of<false, kFew, UNIT>(p, seg, false).units);
         if (MANY && c.tiles > 0) {
           const int to = atomicAdd(&choice->segments, 1);
           if (to < kThreads) {
@@ -326,11 +327,18 @@ __device__ __forceinline__ int schedule(const Attend& p, Plan& plan, Choice* cho
     if (pass == 0) {
       plan.segments[threadIdx.x] = first;
       units = head_sum<64>(units);
-      if (lane == 0) plan.units[wave] = units;
+      if (MANY) few = head_sum<64>(few);
+      if (lane == 0) plan.units[wave] = units, plan.few[wave] = few;
       __syncthreads();
       units = (plan.units[0] + plan.units[1] + plan.units[2] + plan.units[3]) * p.per_target[MANY];
       if (units == 0.f && block > 0) return 0;  // nothing of this kind; block 0 notes the places
       if constexpr (MANY) {
+        // Where a CU has two blocks and its few rows take longer to read than its many to
+        // multiply, half as many ranges leave fewer pieces and are done as soon (64 x 8 drafts
+        // behind shared prompts 118 -> 112 us; 256 requests behind 16384 shared positions
+        // with few of their own would take 110 instead of 103).
+        few = (plan.few[0] + plan.few[1] + plan.few[2] + plan.few[3]) * p.per_target[1];
+        if (blocks > kCus && p.items_max[0] > 0 && few > 0.66f * units) units *= 2.f, blocks /= 2;
         // of more segments than that, every one is split alike
         if (choice->segments <= kThreads) {
           const int i = threadIdx.x & (kCandidates - 1);
