@@ -801,7 +801,7 @@ int gdn_append_paged_kv(const void* k, int64_t k_token_stride, int64_t k_head_st
  *   q, out [tokens, heads, dim] bf16 or f16, caches [pages, page_size, kv_heads,
  *   dim] alike, unit channel stride, rows at multiples of 16 bytes (out: 8);
  *   page_size a multiple of 16; lse fp32 [tokens, heads] (natural logarithm) or NULL.
- * dim 64, 128 or 256, fewer than 2^26 rows (tokens x heads), requests and groups
+ * dim 64, 128 or 256, up to 2^26 - 4 rows (tokens x heads), requests and groups
  * fewer than 2^24, up to 2^27 positions and 2^16 key heads (GDN_ERR_UNSUPPORTED
  * beyond).  All 64 bits of int64 pages and lengths count; the offsets and shared
  * lengths lie in the int32 range.  Sums and statistics are fp32;

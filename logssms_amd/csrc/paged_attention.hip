@@ -1509,10 +1509,10 @@ extern "C" int gdn_paged_attention(const void* q, int64_t q_token_stride, int64_
     set_error("head dims 64, 128 and 256");
     return GDN_ERR_UNSUPPORTED;
   }
-  // 64 threads a row in a launch
-  if (tokens * heads >= (int64_t{1} << 26) || requests + groups >= (int64_t{1} << 24) ||
+  // the joining kernel's blocks of 256 threads for four rows each: fewer than 2^32 threads
+  if (tokens * heads > (int64_t{1} << 26) - 4 || requests + groups >= (int64_t{1} << 24) ||
       table_width * page_size > (int64_t{1} << 27) || pages >= (int64_t{1} << 31) || kv_heads > (1 << 16)) {
-    set_error("up to 2^26 rows, 2^24 requests, 2^27 positions, 2^31 pages and 2^16 key heads");
+    set_error("up to 2^26 - 4 rows, fewer than 2^24 requests, 2^27 positions, 2^31 pages and 2^16 key heads");
     return GDN_ERR_UNSUPPORTED;
   }
   if (tokens == 0 || requests == 0) return GDN_OK;

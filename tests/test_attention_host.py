@@ -271,3 +271,13 @@ def test_more_rows_than_a_launch_has_threads_for():
                 rotated=16, inter=0, scale=1.0, qo=d, qot=64, qoh=32, ko=None, kot=0, koh=0, stream=None)
     turn.update(dim=4096, tokens=1 << 24)
     assert lib.gdn_apply_rotary(*turn.values()) == 2
+
+
+def test_the_largest_launch_that_joins_pieces():
+    """A block of 256 threads joins four rows, and a launch has up to 2^32 - 1 threads."""
+    lib = _built()
+    one = dict(heads=1, kv_heads=1, requests=1, cu=0x10000)
+    for rows in ((1 << 26) - 3, (1 << 26) - 1):
+        assert _attend(lib, tokens=rows, **one) == 2, rows
+    assert _attend(lib, tokens=((1 << 26) - 1) // 3, **{**one, "heads": 3}) == 2
+    assert _attend(lib, tokens=(1 << 26) - 4, **one) == 1  # not its size: no room in the workspace
