@@ -500,17 +500,34 @@ PyObject* fp8_linear(PyObject*, PyObject* const* args, Py_ssize_t n) {
 }
 
 // ---------------------------------------------------------------- full attention
-int64_t span(const at::Tensor& t, int64_t d) { return t.size(d) > 1 ? t.stride(d) * (t.size(d) - 1) : 0; }
-// Rows [tokens, heads, dim] of unit channel stride, none on top of another.
+// The axes of a view that its rows (the last axis) are walked along, the widest step first.
+struct Axes {
+  int64_t stride[3], size[3];
+  int n = 0;
+  explicit Axes(const at::Tensor& t) {
+    for (int64_t d = 0; d + 1 < t.dim(); ++d) {
+      if (t.size(d) <= 1) continue;
+      int at = n++;
+      for (; at > 0 && stride[at - 1] < t.stride(d); --at) stride[at] = stride[at - 1], size[at] = size[at - 1];
+      stride[at] = t.stride(d), size[at] = t.size(d);
+    }
+  }
+  // Elements from the first to the last of what lies inside axis `from`, in rows of `dim`.
+  int64_t span(int from, int64_t dim) const {
+    for (int i = from; i < n; ++i) dim += stride[i] * (size[i] - 1);
+    return dim;
+  }
+};
+// Rows [.., dim] (up to four axes) of unit channel stride, none on top of another: every
+// axis steps over what lies inside it.
 bool apart(const at::Tensor& t) {
   if (t.numel() == 0) return true;
-  const int64_t dim = t.size(2);
-  if (dim > 1 && t.stride(2) != 1) return false;
-  auto nested = [&](int64_t inner, int64_t outer) {
-    return (t.size(inner) == 1 || t.stride(inner) >= dim) &&
-           (t.size(outer) == 1 || t.stride(outer) >= span(t, inner) + dim);
-  };
-  return nested(1, 0) || nested(0, 1);
+  const int64_t dim = t.size(t.dim() - 1);
+  if (dim > 1 && t.stride(t.dim() - 1) != 1) return false;
+  const Axes axes(t);
+  for (int i = 0; i < axes.n; ++i)
+    if (axes.stride[i] < axes.span(i + 1, dim)) return false;
+  return true;
 }
 // A stride that is walked: 0 along an axis of one, whatever the view says.
 int64_t step(const at::Tensor& t, int64_t d) { return t.size(d) > 1 ? t.stride(d) : 0; }
@@ -616,9 +633,7 @@ PyObject* append_paged_kv(PyObject*, PyObject* const* args, Py_ssize_t n) {
     check_cache(k_cache, k, heads, dim);
     check_cache(v_cache, k, heads, dim);
     require(v_cache.size(0) == k_cache.size(0) && v_cache.size(1) == k_cache.size(1), "caches of one size");
-    for (const at::Tensor* cache : {&k_cache, &v_cache})
-      for (int64_t d = 0; d < 3; ++d)
-        require(cache->size(d) <= 1 || cache->stride(d) >= dim, "a cache's rows must not overlap");
+    require(apart(k_cache) && apart(v_cache), "a cache's rows must not overlap");
     const at::Tensor slots = indices(tensor(args[4]), tokens, k, "slots must be [tokens]");
     Turns t;
     require((args[5] == Py_None) == (args[6] == Py_None), "positions go with a rotation");

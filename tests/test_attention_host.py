@@ -281,3 +281,37 @@ def test_the_largest_launch_that_joins_pieces():
         assert _attend(lib, tokens=rows, **one) == 2, rows
     assert _attend(lib, tokens=((1 << 26) - 1) // 3, **{**one, "heads": 3}) == 2
     assert _attend(lib, tokens=(1 << 26) - 4, **one) == 1  # not its size: no room in the workspace
+
+
+@pytest.mark.parametrize("strides", [
+    (512, 32, 32, 1),  # a head is the next token's first
+    (64, 256, 32, 1),  # pages inside tokens: the last page is the first one's next token
+    (512, 512, 32, 1),  # a page's second token is the next page's first
+    (480, 64, 32, 1),  # half of a page's last token is the next page's
+    (64, 160, 32, 1), (32, 160, 768, 1)])
+def test_append_refuses_caches_whose_axes_coincide(strides):
+    """Every stride is a row or more, and rows lie on top of each other all the same."""
+    from logssms_amd.kernel import append_paged_kv
+    _built()
+    k, cache, slots = torch.zeros(4, 2, 32), torch.zeros(5, 8, 2, 32), torch.arange(4)
+    view = torch.zeros(5 * 8 * 1024).as_strided((5, 8, 2, 32), strides)
+    at = torch.arange(view.untyped_storage().nbytes() // 4).as_strided(view.shape, strides)
+    assert at.unique().numel() < view.numel()
+    for caches in ((view, cache), (cache, view)):
+        with pytest.raises(AssertionError, match="overlap"):
+            append_paged_kv(k, k, *caches, slots)
+
+
+@pytest.mark.parametrize("strides", [
+    (1024, 64, 32, 1),  # the pool's: keys, then values
+    (512, 32, 256, 1), (1024, 32, 256, 1),  # heads first
+    (64, 320, 32, 1), (32, 320, 160, 1),  # pages inside tokens
+    (600, 70, 33, 1)])
+def test_append_takes_caches_in_any_order(strides):
+    from logssms_amd.kernel import append_paged_kv
+    _built()
+    k, cache, slots = torch.zeros(4, 2, 32), torch.zeros(5, 8, 2, 32), torch.arange(4)
+    view = torch.zeros(5 * 8 * 1024).as_strided((5, 8, 2, 32), strides)
+    for caches in ((view, cache), (cache, view)):
+        with pytest.raises(RuntimeError, match="ROCm"):  # no other objection
+            append_paged_kv(k, k, *caches, slots)
