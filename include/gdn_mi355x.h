@@ -773,7 +773,8 @@ int gdn_apply_rotary(const void* q, int64_t q_token_stride, int64_t q_head_strid
  * page_size on (all 64 bits of int64 slots count).  The slots of one call differ.  q
  * (q_heads 0: none) is turned to q_out.
  *   k, v [tokens, kv_heads, dim]; caches [pages, page_size, kv_heads, dim] with
- *   unit channel stride.  rotated 0 (positions and turns unused): k and q as they are.
+ *   unit channel stride, no two of whose rows overlap, and neither those of k_cache and
+ *   v_cache.  rotated 0 (positions and turns unused): k and q as they are.
  */
 int gdn_append_paged_kv(const void* k, int64_t k_token_stride, int64_t k_head_stride, const void* v,
                         int64_t v_token_stride, int64_t v_head_stride, int64_t kv_heads, int dtype, int64_t tokens,

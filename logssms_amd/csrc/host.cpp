@@ -529,6 +529,24 @@ bool apart(const at::Tensor& t) {
     if (axes.stride[i] < axes.span(i + 1, dim)) return false;
   return true;
 }
+// Whether rows of a (its axes from i on) from 0 on and rows of b (from j on) from `at` on
+// keep clear of each other, as far as their axes tell; each of them is apart() by itself.
+bool clear_of(const Axes& a, int i, const Axes& b, int j, int64_t at, int64_t dim) {
+  if (at >= a.span(i, dim) || -at >= b.span(j, dim)) return true;
+  if (i == a.n || j == b.n || a.stride[i] != b.stride[j]) return false;
+  // What lies inside an axis is no longer than its step: an entry of a meets the entries of
+  // b that are `steps` and `steps + 1` before it, where there are such.
+  const int64_t step = a.stride[i], behind = (at % step + step) % step, steps = (at - behind) / step;
+  auto clear = [&](int64_t before, int64_t off) {
+    return before <= -b.size[j] || before >= a.size[i] || clear_of(a, i + 1, b, j + 1, off, dim);
+  };
+  return clear(steps, behind) && clear(steps + 1, behind - step);
+}
+bool clear_of(const at::Tensor& a, const at::Tensor& b) {
+  if (a.numel() == 0 || b.numel() == 0) return true;
+  const int64_t bytes = static_cast<const char*>(b.data_ptr()) - static_cast<const char*>(a.data_ptr());
+  return clear_of(Axes(a), 0, Axes(b), 0, bytes / a.element_size(), a.size(a.dim() - 1));
+}
 // A stride that is walked: 0 along an axis of one, whatever the view says.
 int64_t step(const at::Tensor& t, int64_t d) { return t.size(d) > 1 ? t.stride(d) : 0; }
 at::Tensor unit_channels(const at::Tensor& t) { return t.size(2) == 1 || t.stride(2) == 1 ? t : t.contiguous(); }
@@ -652,6 +670,7 @@ PyObject* append_paged_kv(PyObject*, PyObject* const* args, Py_ssize_t n) {
       require(args[10] == Py_None, "q_out without q");
     }
     require_device(k);
+    require(clear_of(k_cache, v_cache), "the caches must not overlap");
     const bool with_q = q.defined();
     launch("gdn_append_paged_kv", lib::gdn_append_paged_kv, k, k.data_ptr(), step(k, 0), step(k, 1), v.data_ptr(),
            step(v, 0), step(v, 1), heads, code, tokens, dim, slots.data_ptr(), index_code(slots), k_cache.data_ptr(),

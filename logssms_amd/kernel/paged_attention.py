@@ -24,8 +24,8 @@ def append_paged_kv(k: torch.Tensor, v: torch.Tensor, k_cache: torch.Tensor, v_c
                     slots: torch.Tensor, *, positions: torch.Tensor | None = None, rotary: Rotary | None = None,
                     q: torch.Tensor | None = None, q_out: torch.Tensor | None = None) -> torch.Tensor | None:
     """``k`` and ``v`` [tokens, kv heads, dim] to the slots [tokens] (int32 or int64,
-    no two alike) of the caches, ``k`` rotated by ``positions`` where a ``rotary``
-    is given.  A slot below 0, or past the cache, takes no write.  ``q`` [tokens,
+    no two alike) of the caches, which may not overlap, ``k`` rotated by ``positions``
+    where a ``rotary`` is given.  A slot below 0, or past the cache, takes no write.  ``q`` [tokens,
     heads, dim] is rotated in the same launch and returned (``q_out``, which may be
     ``q`` itself, or a new tensor).  fp32, bf16 or f16, one dtype for all."""
     turns, interleaved, scale = (None, False, 1.0) if rotary is None else rotary

@@ -213,3 +213,56 @@ def test_positions_and_slots_past_32_bits():
     others = torch.ones(64, dtype=torch.bool)
     others[[3, 0]] = False
     assert (flat_k[others] == 7).all() and (flat_v[others] == 7).all()
+
+
+def _two(storage, k_at, v_at, k_strides, v_strides, shape=(5, 8, 2, 32)):
+    return storage.as_strided(shape, k_strides, k_at), storage.as_strided(shape, v_strides, v_at)
+
+
+@pytest.mark.parametrize("k_at,v_at,k_strides,v_strides", [
+    (0, 0, (512, 64, 32, 1), (512, 64, 32, 1)),  # the same tensor twice
+    (0, 512, (512, 64, 32, 1), (512, 64, 32, 1)),  # a page further on
+    (0, 2560 - 32, (512, 64, 32, 1), (512, 64, 32, 1)),  # the last head of the one, the first of the other
+    (0, 480, (1024, 64, 32, 1), (1024, 64, 32, 1)),  # a page's values from its last key on
+    (0, 544, (1024, 64, 32, 1), (1024, 64, 32, 1)),  # its last value the next page's first key
+    (0, 16, (1024, 128, 64, 1), (1024, 128, 64, 1)),  # by heads, from half a row on
+    (0, 64, (1024, 64, 512, 1), (1024, 64, 512, 1)),  # heads first, a token further on
+    (0, 512, (2048, 128, 32, 1), (2048, 64, 32, 1))])  # layouts of their own, in one block
+def test_caches_on_top_of_each_other_are_refused(k_at, v_at, k_strides, v_strides):
+    from logssms_amd.kernel import append_paged_kv
+    k_cache, v_cache = _two(torch.zeros(20000, device=DEV), k_at, v_at, k_strides, v_strides)
+    held = torch.arange(20000)
+    a, b = _two(held, k_at, v_at, k_strides, v_strides)
+    assert torch.isin(a, b).any()
+    k, slots = torch.ones(4, 2, 32, device=DEV), torch.arange(4, device=DEV)
+    for caches in ((k_cache, v_cache), (v_cache, k_cache)):
+        with pytest.raises(AssertionError, match="overlap"):
+            append_paged_kv(k, k, *caches, slots)
+
+
+@pytest.mark.parametrize("k_at,v_at,k_strides,v_strides", [
+    (0, 512, (1024, 64, 32, 1), (1024, 64, 32, 1)),  # the pool's
+    (0, 64, (1024, 128, 32, 1), (1024, 128, 32, 1)), (0, 32, (1024, 128, 64, 1), (1024, 128, 64, 1)),  # by tokens, by heads
+    (512, 0, (1024, 32, 256, 1), (1024, 32, 256, 1)),  # heads first, values in front
+    (0, 512, (1024, 64, 32, 1), (1024, 32, 256, 1)),  # keys by tokens, values by heads
+    (0, 3000, (512, 64, 32, 1), (600, 70, 33, 1)),  # one behind the other
+    (0, 320, (32, 640, 160, 1), (32, 640, 160, 1)),  # pages inside tokens and heads
+    (0, 5 * 512 + 7, (512, 64, 32, 1), (512, 32, 256, 1))])
+def test_caches_beside_each_other(k_at, v_at, k_strides, v_strides):
+    """Layouts of their own, in one storage: each takes its rows, and nothing else changes."""
+    from logssms_amd.kernel import append_paged_kv
+    rotary = _rotary(16)
+    storage = torch.full((20000,), 7.0, device=DEV)
+    k_cache, v_cache = _two(storage, k_at, v_at, k_strides, v_strides)
+    k, v = randn(2, 6, 2, 32, g=gen(21)).unbind(0)
+    positions, slots = torch.arange(6) * 1000, torch.tensor([39, 0, 17, -1, 8, 40])
+    append_paged_kv(k.to(DEV), v.to(DEV), k_cache, v_cache, slots.to(DEV), positions=positions.to(DEV),
+                    rotary=_on(rotary))
+    there = [0, 1, 2, 4]
+    at = slots[there]
+    _check(k_cache[at // 8, at % 8].cpu(), k[there], positions[there], rotary)
+    assert torch.equal(v_cache[at // 8, at % 8].cpu(), v[there])
+    a, b = _two(torch.arange(20000), k_at, v_at, k_strides, v_strides)
+    others = torch.ones(20000, dtype=torch.bool)
+    others[torch.cat([a[at // 8, at % 8], b[at // 8, at % 8]]).flatten()] = False
+    assert (storage.cpu()[others] == 7).all()
