@@ -4,8 +4,9 @@
 // Pair i of a head's first R channels, (x[i], x[i + R/2]) in the half layout or
 // (x[2i], x[2i + 1]) interleaved, is turned by the angle 2 pi turns[i] position
 // and multiplied by `scale`; the channels behind them pass through.  Angles are
-// products in 64 bits of which only the fraction of a revolution is kept, so that
-// a position of any size costs no precision and there is no table to outgrow.
+// products in 64 bits of which only the fraction of a revolution is kept: off by at
+// most |position turns| 2^-53 revolutions, less than fp32 holds up to positions of some
+// 2^30, and there is no table to outgrow.
 //
 // Bound by memory: 16 bytes a lane, each value read and written once.  A block takes a
 // few tokens and some or all of their heads: its cosines and sines are computed once
