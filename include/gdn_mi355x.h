@@ -795,7 +795,8 @@ int gdn_append_paged_kv(const void* k, int64_t k_token_stride, int64_t k_head_st
  * all, each one before it one less.  Position p of it lies in page
  * page_table[r, p / page_size]; an entry outside of the cache stands for zero keys
  * and values; positions past the table are not there.  A token that sees nothing
- * gives zeros (lse -infinity); tokens that no request owns are left as they were.
+ * gives zeros (lse -infinity), one all of whose scores are -infinity NaN (lse -infinity), as
+ * their softmax is; tokens that no request owns are left as they were.
  *   Group g holds the requests group_offsets[g] .. group_offsets[g + 1] - 1 (all of
  *   them without offsets); their first shared_lens[g] positions have to lie in
  *   the same pages: they are read through the first request's row.

@@ -738,6 +738,9 @@ __device__ __forceinline__ void put4(const Attend& p, int token, int head, int c
 // The factor of a piece with maximum m and sum l under the joint maximum; 0 where the
 // piece saw nothing (a NaN stays one).
 __device__ __forceinline__ float weight_of(float m, float l, float top) { return l == 0.f ? 0.f : fast_exp2(m - top); }
+// One over a row's sum of weights.  There are none where it sees nothing: zeros; and where
+// all that it sees scores -infinity: NaN, as the softmax of it.
+__device__ __forceinline__ float inverse_of(float l, bool sees) { return l != 0.f ? 1.0f / l : sees ? NAN : 0.f; }
 __device__ __forceinline__ float lse_of(float m, float l) { return l > 0.f || l != l ? (m + log2f(l)) * kLn2 : -INFINITY; }
 
 // One wave's rows: 32 of them, a lane and its partner 32 lanes on share one.
@@ -911,7 +914,7 @@ struct Rows {
     if (row >= it.seg.tokens * p.per) return;
     if (whole(it)) {
       const int in = p.by_per.div(row), token = it.seg.token + in, head = it.head * p.per + row - in * p.per;
-      const float inverse = sum > 0.f || sum != sum ? 1.0f / sum : 0.f;
+      const float inverse = inverse_of(sum, limit > 0);
 #pragma unroll
       for (int d = 0; d < D / 32; ++d)
 #pragma unroll
@@ -1402,7 +1405,9 @@ __global__ __launch_bounds__(kThreads) void join_kernel(Attend p) {
       for (int e = 0; e < kLane; ++e) y[e] += sums[w][lane * kLane + e] * b;
     }
   }
-  const float inverse = l > 0.f || l != l ? 1.0f / l : 0.f;
+  bool sees = false;
+  if (l == 0.f) sees = own.hi > 0 && length_of(p, request) > own.tokens - 1 - (token - own.token);
+  const float inverse = inverse_of(l, sees);
   T* to = static_cast<T*>(p.out) + token * p.out_token + head * p.out_head + lane * kLane;
 #pragma unroll
   for (int e = 0; e < kLane; ++e) to[e] = from_f32<T>(y[e] * inverse);

@@ -25,9 +25,9 @@ def append_paged_kv(k: torch.Tensor, v: torch.Tensor, k_cache: torch.Tensor, v_c
                     q: torch.Tensor | None = None, q_out: torch.Tensor | None = None) -> torch.Tensor | None:
     """``k`` and ``v`` [tokens, kv heads, dim] to the slots [tokens] (int32 or int64,
     no two alike) of the caches, which may not overlap, ``k`` rotated by ``positions``
-    where a ``rotary`` is given.  A slot below 0, or past the cache, takes no write.  ``q`` [tokens,
-    heads, dim] is rotated in the same launch and returned (``q_out``, which may be
-    ``q`` itself, or a new tensor).  fp32, bf16 or f16, one dtype for all."""
+    where a ``rotary`` is given.  A slot below 0, or past the cache, takes no write.
+    ``q`` [tokens, heads, dim] is rotated in the same launch and returned (``q_out``,
+    which may be ``q`` itself, or a new tensor).  fp32, bf16 or f16, one dtype for all."""
     turns, interleaved, scale = (None, False, 1.0) if rotary is None else rotary
     return _lib.host().append_paged_kv(k, v, k_cache, v_cache, slots, positions, turns, interleaved, scale, q, q_out)
 
@@ -52,10 +52,11 @@ def paged_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
     request's too).  These are attended once for the group, and nothing else depends on
     it.
 
-    A token that sees no position gives zeros; tokens that no request owns are left as
-    they were in ``out``.  ``return_lse``: also the logarithm of each row's sum of
-    exponentials, fp32 [tokens, heads], -inf where nothing is seen.  Lengths, offsets
-    and tables are read on the device: a captured call follows them at each replay."""
+    A token that sees no position gives zeros, one all of whose scores are -inf NaN;
+    tokens that no request owns are left as they were in ``out`` (a new one holds
+    anything there).  ``return_lse``: also the logarithm of each row's sum of exponentials,
+    fp32 [tokens, heads], -inf where nothing is seen.  Lengths, offsets and tables are read
+    on the device: a captured call follows them at each replay."""
     if scale is None:
         scale = q.shape[-1] ** -0.5
     result, lse = _lib.host().paged_attention(q, k_cache, v_cache, page_table, seq_lens, shared_lens, group_offsets,

@@ -536,3 +536,52 @@ def test_many_segments_in_several_rounds():
     b = Batch(61, 66, 2, 256, 16, lens)
     out, lse = b.run(return_lse=True)
     b.check(out, lse)
+
+
+@pytest.mark.parametrize("io", ["bf16", "f16"])
+@pytest.mark.parametrize("heads,kv_heads,dim", [(4, 2, 64), (16, 2, 256), (80, 2, 128)])
+@pytest.mark.parametrize("lens,new,shared", [
+    ([90, 16, 40, 9], None, None), ([5000, 3000, 4001], None, None), ([90, 3, 70, 40], [40, 5, 70, 1], None),
+    ([160 + 20, 160 + 7, 160 + 30], [20, 3, 1], [160])])
+def test_scores_of_minus_infinity(io, heads, kv_heads, dim, lens, new, shared):
+    """A token all of whose scores are so gives NaN, as their softmax is, also where it is put together
+    from pieces; weights of some of them are zero; a token that sees nothing gives zeros all the same."""
+    b = Batch(53, heads, kv_heads, dim, 16, lens, new=new, shared=shared, io=io)
+    b.q[..., 5] = b.q[..., 5].abs() + 1
+    cu = b.cu if b.cu is not None else torch.arange(len(lens) + 1)
+    clean, k = b.run().cpu(), b.k.clone()
+    per = heads // kv_heads
+    # all of request 1's
+    own = torch.zeros(b.q.shape[0], heads, dtype=torch.bool)
+    own[cu[1]:cu[2], per:] = True
+    for p in range(lens[1]):
+        b.k[b.table[1, p // 16], p % 16, 1, 5] = -math.inf
+    hit = own.clone()
+    if shared is None:
+        for t in range(int(cu[1]), int(cu[2])):  # those before its first position
+            hit[t] &= lens[1] - (int(cu[2]) - 1 - t) > 0
+    out, lse = b.run(return_lse=True)
+    out, lse = out.cpu(), lse.cpu()
+    assert out[hit].isnan().all() and (lse[hit] == -math.inf).all()
+    assert (out[own & ~hit] == 0).all()
+    if shared is None:
+        assert torch.equal(out[~own], clean[~own])
+        # every other one of request 2's, the first among them: as good as scores that are far below the others
+        results = []
+        for value in (-math.inf, -3.0e4):
+            b.k = k.clone()
+            for p in range(0, lens[2], 2):
+                b.k[b.table[2, p // 16], p % 16, 1, 5] = value
+            results.append(b.run(return_lse=True))
+        seen = torch.ones(b.q.shape[0], heads, dtype=torch.bool)  # more than the first position
+        for t in range(int(cu[2]), int(cu[3])):
+            if lens[2] - (int(cu[3]) - 1 - t) == 1:
+                seen[t, per:] = False
+                assert results[0][0].cpu()[t, per:].isnan().all()
+        assert torch.equal(results[0][0].cpu()[seen], results[1][0].cpu()[seen])
+        assert torch.equal(results[0][1].cpu()[seen], results[1][1].cpu()[seen])
+    else:  # whoever shares them sees some others as well, or none
+        others = torch.zeros_like(own)
+        others[:, per:] = True
+        assert torch.equal(out[~others], clean[~others])
+        assert out[~own].isfinite().all()
