@@ -585,3 +585,43 @@ def test_scores_of_minus_infinity(io, heads, kv_heads, dim, lens, new, shared):
         others[:, per:] = True
         assert torch.equal(out[~others], clean[~others])
         assert out[~own].isfinite().all()
+
+
+def test_neighbours_of_other_lengths():
+    """A row's last bits may follow where the keys are cut, which the lengths beside it decide: it stays
+    within its bound."""
+    b = Batch(54, 16, 2, 256, 64, [200, 6000, 900, 70], shared=[64])
+    for others in ((6000, 900, 70), (64, 64, 64), (6000, 0, 1), (70, 900, 0), (0, 0, 0)):
+        b.lens = [200, *others]
+        out, lse = b.run(return_lse=True)
+        b.check(out, lse)
+
+
+@pytest.mark.parametrize("heads,kv_heads,dim,lens,new,shared", [
+    (8, 2, 128, [500, 33, 70], None, None), (16, 2, 256, [400, 90, 130], [60, 1, 9], [64]),
+    (12, 4, 64, [64 + 3, 64 + 40, 64], [3, 40, 1], [64])])
+def test_caches_of_other_layouts(heads, kv_heads, dim, lens, new, shared):
+    """Heads first, tokens of all pages side by side, room between rows and pages, keys and values each
+    in a layout of its own."""
+    from logssms_amd.kernel import paged_attention
+    page = 32
+    b = Batch(55, heads, kv_heads, dim, page, lens, new=new, shared=shared)
+    want, want_lse = b.run(return_lse=True)
+    b.check(want, want_lse)
+
+    def laid_out(x, order, pad):
+        """`x` with its axes in this order in memory, `pad` more elements behind each row."""
+        at = x.permute(order)
+        room = torch.full((*at.shape[:-1], at.shape[-1] + pad), math.nan, dtype=x.dtype, device=DEV)
+        view = room[..., :at.shape[-1]]
+        view.copy_(at)
+        return view.permute([order.index(d) for d in range(4)])
+
+    layouts = [((0, 2, 1, 3), 0), ((2, 0, 1, 3), 0), ((1, 0, 2, 3), 8), ((0, 1, 2, 3), 24)]
+    on = lambda t: None if t is None else t.to(DEV)  # noqa: E731
+    for k_layout, v_layout in zip(layouts + [((0, 1, 2, 3), 0)], layouts[::-1] + [((0, 2, 1, 3), 0)]):
+        k, v = laid_out(b.k, *k_layout), laid_out(b.v, *v_layout)
+        assert torch.equal(k.cpu().nan_to_num(), b.k.nan_to_num())
+        out, lse = paged_attention(b.q.to(DEV), k, v, b.table.to(DEV), torch.tensor(lens).to(DEV),
+                                   shared_lens=on(b.shared), cu_seqlens=on(b.cu), return_lse=True)
+        assert torch.equal(out, want) and torch.equal(lse, want_lse), (k_layout, v_layout)
