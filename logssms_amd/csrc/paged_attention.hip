@@ -56,6 +56,9 @@ constexpr int kCus = 256;
 // of 256, is not split so: 47 us; 58 where it was, at a price of pieces that was half of
 // theirs.  One of 2048 77 us, 112 with half of all of them.)
 constexpr float kItem = 10.f, kPiece = 16.f, kJoin = 12.f;
+// Steps of the longest segment, 2^27 positions in steps of 32: no range is longer, so that its
+// end in positions fits an int however much work there is.
+constexpr float kLongest = 4194304.f;
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 constexpr float kLater = 8.0f;  // a maximum may lag by 2^8 before the sums are rescaled
 
@@ -232,7 +235,7 @@ __device__ __forceinline__ int2 candidate(float units_a_block, int i) {
   // none is split; otherwise 2, 1.71, 1.5, 1.33, 1.2 .. 0.25 times what a block gets; own ones alike or in eighths
   const int which = i & 15;
   const float shares = which < 6 ? 0.5f + (which - 1) / 12.f : 0.91f + (which - 6) * (which - 6) * 0.038f;
-  const int range = which == 0 ? 1 << 30 : static_cast<int>(units_a_block / shares) + 1;
+  const int range = which == 0 ? 1 << 30 : static_cast<int>(fminf(units_a_block / shares, kLongest)) + 1;
   return make_int2(range, i < 16 ? range : (range >> 3) + 1);
 }
 struct Outcome {
@@ -353,7 +356,7 @@ __device__ __forceinline__ int schedule(const Attend& p, Plan& plan, Choice* cho
           range = candidate(units, 1);
         }
       } else {
-        range.x = range.y = static_cast<int>(fminf(units, 1.0e9f)) + 1;
+        range.x = range.y = static_cast<int>(fminf(units, kLongest)) + 1;
       }
     } else if (pass == 1) {
       int sum = items;
@@ -461,7 +464,7 @@ __device__ __forceinline__ int count_few(const Attend& p, Lane& mine, bool notes
   }
   const float here = static_cast<float>(c.tiles) * static_cast<float>(c.units + c.least) * 0.5f;
   const float units = head_sum<64>(here) * p.per_target[0];
-  mine.range = static_cast<int>(fminf(units, 1.0e9f)) + 1;
+  mine.range = static_cast<int>(fminf(units, kLongest)) + 1;
   mine.ranges = ranges_of(c.units, mine.range);
   const int items = c.tiles * p.kv_heads * mine.ranges;
   int sum = items;
