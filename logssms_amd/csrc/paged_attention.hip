@@ -21,14 +21,16 @@
 // exchange between two lanes, and the accumulators of S^T are the right operand
 // of the second product as they stand, with the keys of each 16 in the order
 // 0-3, 8-11 | 4-7, 12-15, in which V is read as well.  The weights are rounded to the
-// io type for it (their sum is not); maxima, sums and outputs stay in fp32, the pieces
-// too.
+// io type for it, since the matrix instructions take no wider ones (their sum is not):
+// half a step of each at most, as much again as the rounding of the result (bf16: 2.3e-3
+// off 64 bits in all, 1.7e-3 if only the result is rounded).  Maxima, sums and outputs
+// stay in fp32, the pieces too.
 //
 // Many rows are bound by the matrix cores and what feeds them, few rows by memory.
-// Measured on an MI355X (copies 4.9 TB/s, bf16 products of 8192^3 1205 TFLOP/s):
-// a prompt of 8192 tokens 900-1010 TFLOP/s (dims 256, 128; 64: 650-680), 1024 requests
-// behind 16384 shared positions 780-860, 64 and 256 requests of 4096 and 1024
-// positions with nothing shared 5.0-5.7 TB/s.
+// Measured on an MI355X (reads of long rows 6.2 TB/s, bf16 products of 8192^3 1370
+// TFLOP/s): a prompt of 8192 tokens 890-1010 TFLOP/s (dims 256, 128; 64: 650-680), 1024
+// requests behind 16384 shared positions 780-860, 64 and 256 requests of 4096 and 1024
+// positions with nothing shared 4.9-5.8 TB/s.
 #include <algorithm>
 
 #include "common.hpp"
@@ -225,7 +227,9 @@ __device__ __forceinline__ int ranges_of(int units, int range) { return short_di
 // The ranges of keys for items of many rows: of 32 candidates the one under which the
 // last block should end first.  Shared items come first and are alike, a block takes
 // one of each round; a request's own ones fill what these leave, but for half of their
-// longest.  An item costs its steps, kItem, and kPiece if its sums are joined.  (Six
+// longest.  An item costs its steps, kItem, and kPiece if its sums are joined; one that
+// sees nothing is priced at nothing, though it starts, and its piece is stored and joined
+// like the others.  (Six
 // prompts behind 8192 shared positions, 16/2 heads of 256: 272 us in ranges of the
 // length that all the work gives a block.  Equal parts of one line of all the work,
 // whatever tiles they cut, balance better still, but then no two blocks read the same
@@ -339,7 +343,9 @@ __device__ __forceinline__ int schedule(const Attend& p, Plan& plan, Choice* cho
         // Where a CU has two blocks and its few rows take longer to read than its many to
         // multiply, half as many ranges leave fewer pieces and are done as soon (64 x 8 drafts
         // behind shared prompts 118 -> 112 us; 256 requests behind 16384 shared positions
-        // with few of their own would take 110 instead of 103).
+        // with few of their own would take 110 instead of 103.  64 channels, 32/8 heads, 64 x 8
+        // drafts behind 16384: 171 us for 189 with as many of their own each, 143 for 125
+        // with a sixteenth).
         few = (plan.few[0] + plan.few[1] + plan.few[2] + plan.few[3]) * p.per_target[1];
         if (blocks > kCus && p.items_max[0] > 0 && few > 0.66f * units) units *= 2.f, blocks /= 2;
         // of more segments than that, every one is split alike
@@ -729,7 +735,8 @@ __device__ __forceinline__ void take_out(char* v, int at, int lo, NotFinite<D>& 
   }
 }
 
-// Whether an item holds all that its rows see: nothing has to be joined.
+// Whether an item holds all that its rows see, as the only range of its segment (a tile that
+// ends in the first of several is joined all the same): nothing has to be joined.
 __device__ __forceinline__ bool whole(const Item& it) { return it.own && it.ranges == 1 && it.seg.lo == 0; }
 
 // Four channels of a finished row.
@@ -947,10 +954,13 @@ struct Rows {
 // the last matrix instructions of the one before it.
 //
 // Of 256 channels a step takes 1.1 us on all CUs at once (955 to 985 TFLOP/s), some 20 us
-// of a call are outside of the steps.  What bounds the steps is the clock that power
-// leaves: on keys and values of zeros the same call runs at 1247 TFLOP/s (128 channels:
-// 1303 for 942).  Without its loads to LDS it ran at 1206, with half of its LDS reads at
-// 1033, without exponentials at 1010.  (64 rows a wave, its sums in the upper 256
+// of a call are outside of the steps.  The matrix cores are busy for 43 % of a step's
+// cycles, vector instructions for 28 % (128 channels: 43 and 52; 64: 29 and 62), LDS reads
+// for 22 %: one hardly goes on beside the other.  How long a cycle is, power decides: on
+// keys and values of zeros the same call takes as many of them, at 2.27 GHz for 2.03 (128
+// channels 2.22 for 1.99), and long runs of steps reach 1247 TFLOP/s (1303 for 942).
+// Without its loads to LDS it ran at 1206, with half of its LDS reads at 1033, without
+// exponentials at 1010.  (64 rows a wave, its sums in the upper 256
 // registers, halve the loads and the reads: 1053 in long runs of steps, but tiles twice as
 // high mean twice the pieces to store and to join: 256 requests behind 32768 shared
 // positions 193-203 us against 197-201, prompts of 1024 to 4096 tokens 90, 144 and 326
