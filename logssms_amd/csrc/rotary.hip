@@ -73,7 +73,8 @@ __device__ __forceinline__ void turn_pair(float2 cs, float& a, float& b) {
 // layout), a piece of pairs (interleaved), or a piece behind the rotated ones.
 // Otherwise (rows at odd addresses, odd dims) a unit is one pair, or one value: 16384
 // tokens of 16 heads of 256 46 us and, one value further on, 151, bound by instructions for
-// two bytes a lane.  Heads of whole 16-byte pieces, as models have them, do not come here.
+// two bytes a lane.  Heads whose rotated part and rest are whole pieces, as most models'
+// are, do not come here.
 template <class T, bool WIDE>
 __global__ __launch_bounds__(kThreads) void rotary_kernel(Turn p) {
   constexpr int V = WIDE ? Vec16<T>::n : 1, kHeads = 4;
